@@ -152,6 +152,35 @@ PAIA_API int paia_gemv_batch_int4(const void* Wq, const void* scales, const void
 PAIA_API int paia_gemv_batch_int4_zp(const void* Wq, const void* scales, const void* zeros, const void* x,
                                      const void* bias, void* y, int M, int N, int K, int variant, void* stream);
 
+/* ---- between and beside the projections of a decode step (no reference counterpart: the reference ends at the
+ *      projections): rotation + cache write, attention over the paged cache, low-rank adapters. Same conventions; where
+ *      an entry point takes a workspace, the caller owns it, its contents need no preparation and nothing is kept in it
+ *      from one call to the next. -------------------------------------------------------------------------------- */
+
+/* A paged key-value cache: pages of page_size positions for each of kv_heads heads of head_dim values. Element (page,
+ * head, position, i) of k lies at k + page * k_strides[0] + head * k_strides[1] + position * k_strides[2] + i (in
+ * elements), so heads and positions may come in either order. fp8 = 0: bf16; 1: e4m3fn codes, which stand for code *
+ * k_scale[head] (fp32 [kv_heads], NULL = 1). head_dim 64, 128 or 256; k and v 16-byte aligned, strides >= 0 and multiples
+ * of 16 bytes; page_size >= 1 of any size. Slot s is position s % page_size of page s / page_size. */
+typedef struct {
+    void *k, *v;
+    const float *k_scale, *v_scale;
+    long long k_strides[3], v_strides[3];
+    int pages, page_size, kv_heads, head_dim, fp8;
+} paia_kv_cache;
+
+/* One token's fused projection q|k|v (qkv bf16, row m at qkv + m * qkv_stride, (heads + 2 kv_heads) * head_dim values) ->
+ * q_out bf16 [M][heads][head_dim] and, at slot slots[m], k and v in the cache. q and k heads: x *= rsqrt(mean(x^2) + eps)
+ * * norm weight where a weight (bf16 [head_dim]) is given, then the first `rotary` dims turn by row positions[m] of cos_sin
+ * (fp32 [context][rotary]: rotary/2 cosines, then the sines): dims i and i + rotary/2, or 2i and 2i+1 (interleaved).
+ * Everything in fp32, rounded once to bf16 (nearest even) or, divided by the head's scale and clamped to +-448, to e4m3.
+ * A slot outside [0, pages * page_size) is not written; a position outside [0, context) gives NaN in its rotated dims. Two
+ * tokens of a call must not share a slot. rotary % 16 == 0, 0 < rotary <= head_dim; qkv, cos_sin, q_out, norm weights
+ * 16-byte aligned, qkv_stride % 8 == 0; positions and slots are int64. M = 0 does nothing. */
+PAIA_API int paia_rope_append(const void* qkv, long long qkv_stride, const void* positions, const void* cos_sin,
+                              int context, int rotary, int interleaved, const void* q_norm, const void* k_norm, float eps,
+                              const void* slots, const paia_kv_cache* cache, void* q_out, int M, int heads, void* stream);
+
 /* no reference counterpart: a human-readable build tag */
 PAIA_API const char* paia_gemv_build_info(void);
 

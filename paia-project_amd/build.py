@@ -43,7 +43,9 @@ HIP_FLAGS = [
 ]
 HIP_SOURCES = ["gemv_runtime.hip", "gemv_bf16.hip", "gemv_fp8.hip", "gemv_int4.hip", "gemv_dequant.hip",
                "gemv_select.hip", "quantize.hip", "gemv_batch.hip",
-               "gemv_tile.hip"]
+               "gemv_tile.hip", "rope_append.hip"]
+
+TORCH_SOURCES = ["torch_ops.cpp", "torch_decode_ops.cpp"]
 
 
 def _run(cmd, quiet_warn=True):
@@ -136,7 +138,7 @@ def build_torch_ext() -> Path:
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=paia_gemv_torch",
            *[f"-I{p}" for p in ce.include_paths()], f"-I{ROCM / 'include'}", f"-I{INCLUDE}",
-           str(CSRC / "torch_ops.cpp"),
+           *[str(CSRC / s) for s in TORCH_SOURCES],
            f"-L{tdir / 'lib'}", "-lc10", "-ltorch", "-ltorch_cpu", "-lc10_hip", "-ltorch_hip",
            f"-L{BUILD}", "-lpaia_gemv", f"-L{ROCM / 'lib'}", "-lamdhip64",
            "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tdir / 'lib'}",

@@ -1,0 +1,607 @@
+// Attention of a sequence's newest tokens over a paged key-value cache, split over the cache's length and joined.
+//
+//   s_p = scale k_scale[h] <q, k_p>,  o = v_scale[h] sum_p exp(s_p - m) v_p / sum_p exp(s_p - m),  m = max_p s_p
+//   token t of T sees positions p < len - (T-1-t), the last `window` of them where there is a window, on valid pages.
+//
+// Each cache byte is used for T G products a value (G query heads share a kv head), a few operations per byte: bound by
+// reading the cache once. The pieces of the design:
+//   * Work: a unit is one piece of one sequence for one kv head and up to 16 columns (token, query head of the group). The
+//     lengths are on the device and the grid is fixed by the host, so each block derives the split from the lengths
+//     itself (find_piece): about as many equal pieces as blocks fit the chip, whatever the lengths are. A captured call
+//     stays balanced as the sequences grow. Pieces of one sequence leave (m, l, o) in the workspace, joined by a second
+//     kernel; a sequence of one piece is written by its block.
+//   * A block's four waves take its 32-position tiles in turn, each with its own running maximum, sum and output (no
+//     barrier until the end), and one tile of K and V loads in flight ahead of the one in work.
+//   * S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_bf16. Both leave a column (token, head) on the same lane, so
+//     P goes from the first product's result to the second's operand in registers, and the rescaling is per lane.
+//   * K rows are loaded contiguously and brought to the matrix layout through a wave-private piece of LDS (XOR swizzle).
+//     V rows are loaded contiguously too, D/16 dims of eight positions per lane: 16 lanes are the 16 rows of the V^T
+//     operand, whose eight contraction values are the eight positions; one v_perm_b32 per register pairs them up.
+//   * e4m3 codes become bf16 exactly (v_cvt_scalef32_pk_bf16_fp8); the heads' factors go to the scores and the output.
+// Scores, statistics and sums are fp32. P is rounded to bf16 for the second product (2^-9 of each weight, independent of
+// each other, against the output's own rounding of the same size); the sum l is that of the unrounded weights.
+// What no token sees (positions past the end, before the window, on a page outside the cache) contributes nothing, whatever
+// its bytes are: scores are replaced, V rows zeroed, and where tokens differ in what they see, each takes its own product.
+#include <hip/hip_runtime.h>
+#include <limits.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "gemv_kernel.h"
+#include "kv_cache.h"
+#include "paia_gemv.h"
+
+namespace paia {
+
+constexpr int kTile = 32;            // positions a wave takes at a time
+constexpr int kCols = 16;            // columns (token, head) of a unit
+constexpr int kAttnWaves = 4, kAttnBlock = kAttnWaves * kWave;
+constexpr int kMinTiles = 8;         // a piece is at least this many tiles, where the sequence has them
+
+struct AttnParams {
+    const uint8_t* q;
+    int64_t qb, qt, qh;              // bytes between sequences, tokens, heads
+    uint16_t* out;                   // bf16 [B][T][heads][D]
+    float* lse;                      // fp32 [B][T][heads] or null
+    const int32_t *table, *lens;
+    int64_t table_stride;
+    CacheView cache;
+    float *part_o, *part_ml;         // [item][kv head][column][D], [item][kv head][column][2]
+    float scale;                     // scale * log2(e)
+    int B, T, heads, group, cols, col_groups;
+    int window, max_len;             // positions the table can hold
+    int target;                      // pieces aimed at per kv head and column group
+    int units;                       // items * kv heads
+};
+
+// ---- the split of the sequences into pieces -------------------------------------------------------------------------
+struct Span {
+    int len, tile0, tiles;           // positions, first tile seen by any token, number of tiles
+};
+__device__ __forceinline__ Span span_of(const AttnParams& p, int b)
+{
+    Span s;
+    s.len = min(max(p.lens[b], 0), p.max_len);
+    const int first = p.window > 0 ? max(0, s.len - (p.T - 1) - p.window) : 0;
+    s.tile0 = first / kTile;
+    s.tiles = (int)(((int64_t)s.len + kTile - 1) / kTile) - s.tile0;
+    return s;
+}
+__device__ __forceinline__ int64_t wave_sum_i64(int64_t v)
+{
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) v += __shfl_xor(v, d);
+    return v;
+}
+// Tiles a piece takes at most: the sequences' tiles over the pieces aimed at, less one a sequence for its last, shorter
+// piece. With pieces of this size there are at most max(target, target / 2 + B).
+__device__ __forceinline__ int piece_tiles(const AttnParams& p, const Span& first_chunk)
+{
+    const int lane = lane_id();
+    int64_t total = lane < p.B ? first_chunk.tiles : 0;
+    for (int b = kWave + lane; b < p.B; b += kWave) total += span_of(p, b).tiles;
+    total = wave_sum_i64(total);
+    const int aim = max(p.target - p.B, (p.target + 1) / 2);
+    const int64_t n = (total + aim - 1) / aim;
+    return (int)min((int64_t)(1 << 27), (max(n, (int64_t)kMinTiles) + kAttnWaves - 1) / kAttnWaves * kAttnWaves);
+}
+// Pieces of a sequence, at least one, and tiles of each but the last.
+__device__ __forceinline__ int pieces_of(int tiles, int most, int* each)
+{
+    const int n = max(1, (tiles + most - 1) / most);
+    *each = max(1, (tiles + n - 1) / n);
+    return max(1, (tiles + *each - 1) / *each);
+}
+__device__ __forceinline__ int wave_scan(int v)      // inclusive
+{
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const int o = __shfl_up(v, d);
+        if (lane_id() >= d) v += o;
+    }
+    return v;
+}
+struct Piece {
+    int b, len, tile0, tile1, count;     // sequence, its length, the piece's tiles, pieces of the sequence
+};
+__device__ __forceinline__ bool find_piece(const AttnParams& p, int item, Piece* r)
+{
+    const int lane = lane_id();
+    Span s{0, 0, 0};
+    if (lane < p.B) s = span_of(p, lane);
+    const int most = piece_tiles(p, s);
+    for (int b0 = 0, before = 0; b0 < p.B; b0 += kWave) {
+        const int b = b0 + lane;
+        if (b0 > 0 && b < p.B) s = span_of(p, b);
+        int each = 1;
+        const int n = b < p.B ? pieces_of(s.tiles, most, &each) : 0;
+        const int end = before + wave_scan(n);
+        const uint64_t here = __ballot(item < end && item >= end - n);
+        if (here != 0) {
+            const int src = __builtin_ctzll(here);
+            const int j = item - __builtin_amdgcn_readlane(end - n, src);
+            const int tiles = __builtin_amdgcn_readlane(s.tiles, src), t0 = __builtin_amdgcn_readlane(s.tile0, src);
+            each = __builtin_amdgcn_readlane(each, src);
+            r->b = b0 + src;
+            r->len = __builtin_amdgcn_readlane(s.len, src);
+            r->tile0 = t0 + min(tiles, j * each);
+            r->tile1 = t0 + min(tiles, (j + 1) * each);
+            r->count = __builtin_amdgcn_readlane(n, src);
+            return true;
+        }
+        before = __builtin_amdgcn_readlane(end, kWave - 1);
+    }
+    return false;
+}
+
+// ---- lanes l, l^16, l^32, l^48 ---------------------------------------------------------------------------------------
+__device__ __forceinline__ float col_max(float v)
+{
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float col_sum(float v)
+{
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ void lds_order()      // a wave's LDS operations stay in order; the compiler has to keep them so
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+__device__ __forceinline__ f32x4 mfma(const u32x4 a, const u32x4 b, const f32x4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <int N> struct Words { uint32_t w[N]; };
+template <int N>
+__device__ __forceinline__ Words<N> load_words(const uint8_t* p)
+{
+    Words<N> r;
+    if constexpr (N >= 4) {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            const u32x4 v = reinterpret_cast<const u32x4*>(p)[i];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r.w[4 * i + e] = v[e];
+        }
+    } else if constexpr (N == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        r.w[0] = v.x, r.w[1] = v.y;
+    } else {
+        r.w[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+    return r;
+}
+
+// P8: pages are multiples of eight positions, so eight aligned positions lie on one page
+template <int D, bool FP8, bool P8>
+struct Layout {
+    static constexpr int kRow = D * (FP8 ? 1 : 2);           // bytes of a cache row
+    static constexpr int kRowLanes = kRow / 16;              // lanes that load a K row, 16 bytes each
+    static constexpr int kKLoads = kRowLanes / 2;            // K loads (and consecutive positions) per lane and tile
+    static constexpr int kVWords = D / 32 / (FP8 ? 2 : 1);   // registers of a V row per lane (D/16 dims)
+    static constexpr int kKStep = P8 ? (kKLoads < 8 ? kKLoads : 8) : 1;    // positions per page lookup
+    static constexpr int kVStep = P8 ? 8 : 1;
+    static constexpr int kKPages = kKLoads / kKStep, kVPages = 8 / kVStep;
+    static constexpr int kOutStride = D + 4;                 // floats between the columns of a wave's output in LDS
+    static constexpr int kWaveLds = kCols * kOutStride * 4 > kTile * kRow ? kCols * kOutStride * 4 : kTile * kRow;
+    // Row r of a tile, 16-byte piece c, lies at piece c ^ swizzle(r): the 16 rows that one read takes (four of every
+    // eight) then cover all banks.
+    static __device__ __forceinline__ int swizzle(int r)
+    {
+        const int m = (r >> 3) * 4 + (r & 3);
+        return kRow >= 256 ? m : kRow == 128 ? (m >> 1) & 7 : (m >> 2) & 3;
+    }
+};
+
+template <int D, bool FP8, bool P8>
+__global__ void __launch_bounds__(kAttnBlock) paged_attention_kernel(const AttnParams p)
+{
+    using L = Layout<D, FP8, P8>;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[kAttnWaves * L::kWaveLds];
+    __shared__ float stats[kAttnWaves][2][kCols];
+    // the column groups of a unit on one XCD, next to each other: they read the same cache rows
+    const int cg = (int)(blockIdx.x / 8) % p.col_groups;
+    const int unit = (int)(blockIdx.x / 8 / p.col_groups) * 8 + (int)(blockIdx.x % 8);
+    if (unit >= p.units) return;
+    const int hkv = p.cache.kv_heads, item = unit / hkv, h = unit % hkv;
+    Piece pc;
+    if (!find_piece(p, item, &pc)) return;
+
+    const int lane = lane_id(), wave = wave_id(), n = lane & 15, g = lane >> 4;
+    const int c0 = cg * kCols, col = c0 + n;
+    const bool live = col < p.cols;
+    const int tok = live ? col / p.group : 0, head = h * p.group + (live ? col % p.group : 0);
+    const int hi = pc.len - (p.T - 1 - tok), lo = p.window > 0 ? hi - p.window : 0;   // positions this column sees
+    const int t_first = c0 / p.group, t_last = min(c0 + kCols, p.cols) - 1 >= 0 ? (min(c0 + kCols, p.cols) - 1) / p.group : 0;
+    // positions that every token of the block sees
+    const int all_hi = pc.len - (p.T - 1 - t_first), all_lo = p.window > 0 ? pc.len - (p.T - 1 - t_last) - p.window : 0;
+
+    u32x4 q[D / 32];
+    {
+        const uint8_t* src = p.q + pc.b * p.qb + tok * p.qt + head * p.qh + 16 * g;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) q[j] = live ? *reinterpret_cast<const u32x4*>(src + 64 * j) : u32x4{0, 0, 0, 0};
+    }
+    const float score_scale = p.scale * (p.cache.k_scale != nullptr ? p.cache.k_scale[h] : 1.0f);
+    const int32_t* table = p.table + pc.b * p.table_stride;
+    const int kpiece = lane % L::kRowLanes, krow = lane / L::kRowLanes * L::kKLoads;
+    const uint8_t* kbase = p.cache.k + h * p.cache.kh + 16 * kpiece;
+    const uint8_t* vbase = p.cache.v + h * p.cache.vh + 4 * L::kVWords * n;
+    const uint32_t last = (uint32_t)pc.len - 1;
+    uint8_t* mine = smem + wave * L::kWaveLds;
+
+    int kpage[L::kKPages], vpage[L::kVPages];
+    // Page numbers of a tile's rows. Rows past the end take the last row's page (its bytes are there), and are masked.
+    auto position = [&](uint32_t pos, uint32_t step) { return min(pos, last & ~(step - 1)); };
+    auto lookup = [&](int tile) {
+        const uint32_t p0 = (uint32_t)tile * kTile;
+#pragma unroll
+        for (int i = 0; i < L::kKPages; ++i)
+            kpage[i] = table[p.cache.page_of(position(p0 + krow + i * L::kKStep, L::kKStep))];
+#pragma unroll
+        for (int i = 0; i < L::kVPages; ++i)
+            vpage[i] = table[p.cache.page_of(position(p0 + 8 * g + i * L::kVStep, L::kVStep))];
+    };
+    auto in_cache = [&](int page) { return (uint32_t)page < (uint32_t)p.cache.pages; };
+    Words<4> k[L::kKLoads];
+    Words<L::kVWords> v[8];
+    auto load_k = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < L::kKPages; ++i) {
+            const uint32_t pos = position((uint32_t)tile * kTile + krow + i * L::kKStep, L::kKStep);
+            const uint32_t at = pos - p.cache.page_of(pos) * (uint32_t)p.cache.page_size;
+            const uint8_t* row = kbase + (in_cache(kpage[i]) ? kpage[i] : 0) * p.cache.kp + at * p.cache.kr;
+#pragma unroll
+            for (int e = 0; e < L::kKStep; ++e) k[i * L::kKStep + e] = load_words<4>(row + e * p.cache.kr);
+        }
+    };
+    const uint8_t* vrow[L::kVPages];
+    uint32_t vok = 0;                  // bit i: the page of row 8 g + i is in the cache
+    auto address_v = [&](int tile) {
+        uint32_t ok = 0;
+#pragma unroll
+        for (int i = 0; i < L::kVPages; ++i) {
+            const uint32_t pos = position((uint32_t)tile * kTile + 8 * g + i * L::kVStep, L::kVStep);
+            const uint32_t at = pos - p.cache.page_of(pos) * (uint32_t)p.cache.page_size;
+            const bool in = in_cache(vpage[i]);
+            vrow[i] = vbase + (in ? vpage[i] : 0) * p.cache.vp + at * p.cache.vr;
+            if (in) ok |= (P8 ? 0xFFu : 1u) << i;
+        }
+        return ok;
+    };
+    auto load_v = [&]() {
+#pragma unroll
+        for (int i = 0; i < L::kVPages; ++i)
+#pragma unroll
+            for (int e = 0; e < L::kVStep; ++e)
+                v[i * L::kVStep + e] = load_words<L::kVWords>(vrow[i] + e * p.cache.vr);
+    };
+
+    float m = -INFINITY, l = 0.0f;
+    f32x4 o[D / 16];
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    int tile = pc.tile0 + wave;
+    if (tile < pc.tile1) {
+        lookup(tile);
+        vok = address_v(tile);
+        load_k(tile);
+        load_v();
+        if (tile + kAttnWaves < pc.tile1) lookup(tile + kAttnWaves);
+    }
+    for (; tile < pc.tile1; tile += kAttnWaves) {
+        const int next = tile + kAttnWaves;
+        const bool more = next < pc.tile1;
+#pragma unroll
+        for (int i = 0; i < L::kKLoads; ++i) {
+            const int r = krow + i;
+            *reinterpret_cast<u32x4*>(mine + r * L::kRow + 16 * (kpiece ^ L::swizzle(r))) =
+                u32x4{k[i].w[0], k[i].w[1], k[i].w[2], k[i].w[3]};
+        }
+        lds_order();
+        uint32_t vok_next = 0;
+        if (more) {
+            load_k(next);
+            vok_next = address_v(next);
+            if (next + kAttnWaves < pc.tile1) lookup(next + kAttnWaves);
+        }
+        // S^T: row m of half `half` is position 8 (m / 4) + 4 half + m % 4 of the tile, so a lane ends with positions
+        // 8 g + 4 half + i, i = 0..3, of its column
+        f32x4 s[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int r = (n >> 2) * 8 + half * 4 + (n & 3);
+            const uint8_t* row = mine + r * L::kRow;
+            s[half] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+                u32x4 a;
+                if constexpr (FP8) {
+                    const uint2 w = *reinterpret_cast<const uint2*>(row + 16 * ((2 * j + (g >> 1)) ^ L::swizzle(r)) + 8 * (g & 1));
+                    a = u32x4{fp8x2_to_bf16x2<false>(w.x), fp8x2_to_bf16x2<true>(w.x), fp8x2_to_bf16x2<false>(w.y),
+                              fp8x2_to_bf16x2<true>(w.y)};
+                } else {
+                    a = *reinterpret_cast<const u32x4*>(row + 16 * ((4 * j + g) ^ L::swizzle(r)));
+                }
+                s[half] = mfma(a, q[j], s[half]);
+            }
+        }
+        lds_order();
+        const int p0 = tile * kTile;
+        const bool masked = p0 + kTile > all_hi || p0 < all_lo || __ballot(vok != 0xFFu) != 0;
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float x = s[i / 4][i % 4] * score_scale;
+            if (masked) {
+                const int pos = p0 + 8 * g + i;
+                x = pos < hi && pos >= lo && (vok >> i & 1u) ? x : -INFINITY;
+            }
+            s[i / 4][i % 4] = x;
+            top = fmaxf(top, x);
+        }
+        top = fmaxf(m, col_max(top));
+        const float base = top == -INFINITY ? 0.0f : top;
+        if (__ballot(top > m) != 0) {
+            const float fade = __builtin_amdgcn_exp2f(m - base);
+            l *= fade;
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) o[j] *= fade;
+            m = top;
+        }
+        float w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            w[i] = __builtin_amdgcn_exp2f(s[i / 4][i % 4] - base);
+            l += w[i];
+        }
+        const u32x4 pw = {pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3]), pack_bf16x2(w[4], w[5]), pack_bf16x2(w[6], w[7])};
+        // O^T += V^T P^T: rows 8 g + i, i = 0..7, of the tile against the lane's own eight weights. `see`: bit i keeps row
+        // i; `take`: the product is this lane's (of its token), or nobody's business.
+        auto add_pv = [&](uint32_t see, bool all, bool take) {
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) {
+                uint32_t x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if constexpr (FP8)
+                        x[i] = d % 2 ? fp8x2_to_bf16x2<true>(v[i].w[d / 2]) : fp8x2_to_bf16x2<false>(v[i].w[d / 2]);
+                    else
+                        x[i] = v[i].w[d];
+                    if (!all) x[i] = see >> i & 1u ? x[i] : 0u;
+                }
+                const u32x4 even = {__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u),
+                                    __builtin_amdgcn_perm(x[5], x[4], 0x05040100u), __builtin_amdgcn_perm(x[7], x[6], 0x05040100u)};
+                const u32x4 odd = {__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u),
+                                   __builtin_amdgcn_perm(x[5], x[4], 0x07060302u), __builtin_amdgcn_perm(x[7], x[6], 0x07060302u)};
+                const f32x4 a = mfma(even, pw, o[2 * d]), b = mfma(odd, pw, o[2 * d + 1]);
+                if (all) {
+                    o[2 * d] = a, o[2 * d + 1] = b;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        o[2 * d][e] = take ? a[e] : o[2 * d][e];
+                        o[2 * d + 1][e] = take ? b[e] : o[2 * d + 1][e];
+                    }
+                }
+            }
+        };
+        if (!masked) {
+            add_pv(0xFFu, true, true);
+        } else {
+            for (int t = t_first; t <= t_last; ++t) {
+                const int thi = pc.len - (p.T - 1 - t), tlo = p.window > 0 ? thi - p.window : 0;
+                uint32_t see = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int pos = p0 + 8 * g + i;
+                    if (pos < thi && pos >= tlo) see |= 1u << i;
+                }
+                add_pv(see & vok, false, tok == t);
+            }
+        }
+        vok = vok_next;
+        if (more) load_v();
+    }
+    l = col_sum(l);
+
+    // join the block's waves: column n of a wave's O^T lies at [n][dim], dims (4 g + i) D/16 + j
+    float* part = reinterpret_cast<float*>(mine);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < D / 16; j += 4)
+            *reinterpret_cast<f32x4*>(part + n * L::kOutStride + (4 * g + i) * (D / 16) + j) =
+                f32x4{o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]};
+    if (g == 0) stats[wave][0][n] = m, stats[wave][1][n] = l;
+    __syncthreads();
+    const float v_scale = p.cache.v_scale != nullptr ? p.cache.v_scale[h] : 1.0f;
+    for (int e = (int)threadIdx.x; e < kCols * (D / 4); e += kAttnBlock) {
+        const int cn = e / (D / 4), d = e % (D / 4) * 4, c = c0 + cn;
+        if (c >= p.cols) break;
+        float all = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kAttnWaves; ++w) all = fmaxf(all, stats[w][0][cn]);
+        const float base = all == -INFINITY ? 0.0f : all;
+        f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < kAttnWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(stats[w][0][cn] - base);
+            sum += f * stats[w][1][cn];
+            acc += f * *reinterpret_cast<const f32x4*>(smem + w * L::kWaveLds + 4 * (cn * L::kOutStride + d));
+        }
+        if (pc.count > 1) {
+            const int64_t at = (int64_t)unit * p.cols + c;
+            *reinterpret_cast<f32x4*>(p.part_o + at * D + d) = acc;
+            if (d == 0) p.part_ml[2 * at] = all, p.part_ml[2 * at + 1] = sum;
+            continue;
+        }
+        const int64_t row = ((int64_t)pc.b * p.T + c / p.group) * p.heads + h * p.group + c % p.group;
+        const float f = sum == 0.0f ? 0.0f : v_scale / sum;
+        const uint2 y = {pack_bf16x2(acc[0] * f, acc[1] * f), pack_bf16x2(acc[2] * f, acc[3] * f)};
+        *reinterpret_cast<uint2*>(p.out + row * D + d) = y;
+        if (d == 0 && p.lse != nullptr) p.lse[row] = (all + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+    }
+}
+
+// Joins the pieces of the sequences that have several: a block per sequence, kv head and column; D/4 lanes hold the output,
+// the block's groups of them take the pieces in turn.
+template <int D>
+__global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
+{
+    constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
+    __shared__ f32x4 acc_of[kGroups][kLanes];
+    __shared__ float m_of[kGroups], l_of[kGroups];
+    const int hkv = p.cache.kv_heads;
+    const int c = (int)(blockIdx.x % (uint32_t)p.cols), h = (int)(blockIdx.x / (uint32_t)p.cols) % hkv;
+    const int b = (int)(blockIdx.x / ((uint32_t)p.cols * (uint32_t)hkv));
+    const int lane = lane_id();
+    Span s{0, 0, 0};
+    if (lane < p.B) s = span_of(p, lane);
+    const int most = piece_tiles(p, s);
+    // pieces of this sequence and of all before it
+    int count, each, before = 0;
+    count = pieces_of(span_of(p, b).tiles, most, &each);
+    if (count == 1) return;
+    for (int i = lane; i < b; i += kWave) before += pieces_of(span_of(p, i).tiles, most, &each);
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) before += __shfl_xor(before, d);
+
+    const int grp = (int)threadIdx.x / kLanes, i4 = (int)threadIdx.x % kLanes;
+    float m = -INFINITY, l = 0.0f;
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = grp; j < count; j += kGroups) {
+        const int64_t at = ((int64_t)(before + j) * hkv + h) * p.cols + c;
+        const f32x4 x = *reinterpret_cast<const f32x4*>(p.part_o + at * D + 4 * i4);
+        const float pm = p.part_ml[2 * at], pl = p.part_ml[2 * at + 1];
+        const float top = fmaxf(m, pm), base = top == -INFINITY ? 0.0f : top;
+        const float fa = __builtin_amdgcn_exp2f(m - base), fb = __builtin_amdgcn_exp2f(pm - base);
+        acc = acc * fa + x * fb;
+        l = l * fa + pl * fb;
+        m = top;
+    }
+    acc_of[grp][i4] = acc;
+    if (i4 == 0) m_of[grp] = m, l_of[grp] = l;
+    __syncthreads();
+    if (grp != 0) return;
+    float all = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kGroups; ++w) all = fmaxf(all, m_of[w]);
+    const float base = all == -INFINITY ? 0.0f : all;
+    acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kGroups; ++w) {
+        const float f = __builtin_amdgcn_exp2f(m_of[w] - base);
+        sum += f * l_of[w];
+        acc += f * acc_of[w][i4];
+    }
+    const int64_t row = ((int64_t)b * p.T + c / p.group) * p.heads + h * p.group + c % p.group;
+    const float f = sum == 0.0f ? 0.0f : (p.cache.v_scale != nullptr ? p.cache.v_scale[h] : 1.0f) / sum;
+    const uint2 y = {pack_bf16x2(acc[0] * f, acc[1] * f), pack_bf16x2(acc[2] * f, acc[3] * f)};
+    *reinterpret_cast<uint2*>(p.out + row * D + 4 * i4) = y;
+    if (i4 == 0 && p.lse != nullptr) p.lse[row] = (all + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+constexpr int kBlocksPerCu = 3;
+
+// The launch's plan; false where its sizes leave the contract.
+static bool attention_plan(const paia_kv_cache* c, int table_width, int B, int T, int heads, AttnParams* p, int64_t* bytes)
+{
+    if (!cache_view(c, &p->cache) || table_width < 0 || B < 0 || T <= 0 || heads <= 0 || heads % c->kv_heads) return false;
+    p->B = B, p->T = T, p->heads = heads;
+    p->group = heads / c->kv_heads;
+    const int64_t cols = (int64_t)T * p->group, max_len = (int64_t)table_width * c->page_size;
+    // tile numbers times 32, with a tile to spare, stay within 31 bits
+    p->max_len = (int)(max_len < INT_MAX - 4096 ? max_len : INT_MAX - 4096);
+    if (cols > INT_MAX / 2) return false;
+    p->cols = (int)cols;
+    p->col_groups = (p->cols + kCols - 1) / kCols;
+    const int64_t wide = (int64_t)c->kv_heads * p->col_groups, slots = (int64_t)device_facts().cus * kBlocksPerCu;
+    int64_t target = slots / wide;
+    target = target < 1 ? 1 : target;
+    // pieces per sequence that the table's width allows, and the bound of piece_tiles
+    const int64_t per_seq = ((int64_t)p->max_len / kTile + 1 + kMinTiles - 1) / kMinTiles;
+    int64_t items = target > (target + 1) / 2 + B ? target : (target + 1) / 2 + B;
+    if (items > per_seq * B) items = per_seq * B;
+    p->target = (int)target;
+    const int64_t units = items * c->kv_heads, blocks = (units + 7) / 8 * 8 * p->col_groups;
+    if (blocks > INT_MAX || (int64_t)B * c->kv_heads * p->cols > INT_MAX) return false;
+    p->units = (int)units;
+    // one piece a sequence at most: nothing is joined
+    *bytes = per_seq <= 1 ? 0 : units * p->cols * (c->head_dim + 2) * (int64_t)sizeof(float);
+    return true;
+}
+
+template <int D>
+static int launch_attention(const AttnParams& p, bool fp8, bool join, hipStream_t st)
+{
+    const dim3 grid((uint32_t)((p.units + 7) / 8 * 8 * p.col_groups));
+    const bool p8 = p.cache.page_size % 8 == 0;
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kAttnBlock), 0, st, p); };
+    if (fp8) p8 ? go(paged_attention_kernel<D, true, true>) : go(paged_attention_kernel<D, true, false>);
+    else p8 ? go(paged_attention_kernel<D, false, true>) : go(paged_attention_kernel<D, false, false>);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return (int)e;
+    if (join) {
+        hipLaunchKernelGGL((attention_join_kernel<D>), dim3((uint32_t)(p.B * p.cache.kv_heads * p.cols)), dim3(256), 0, st, p);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return (int)e;
+    }
+    return 0;
+}
+
+}  // namespace paia
+
+extern "C" {
+
+long long paia_paged_attention_workspace(const paia_kv_cache* cache, int table_width, int B, int T, int heads)
+{
+    paia::AttnParams p;
+    int64_t bytes = 0;
+    return paia::attention_plan(cache, table_width, B, T, heads, &p, &bytes) ? bytes : -2;
+}
+
+int paia_paged_attention(const void* q, const long long* q_strides, const paia_kv_cache* cache, const void* block_table,
+                         long long table_stride, int table_width, const void* lens, float scale, int window, void* out,
+                         void* lse, int B, int T, int heads, void* workspace, long long workspace_bytes, void* stream)
+{
+    using namespace paia;
+    AttnParams p;
+    int64_t bytes = 0;
+    if (!attention_plan(cache, table_width, B, T, heads, &p, &bytes) || window < 0 || table_stride < 0) return -2;
+    if (B == 0) return 0;
+    if (q == nullptr || q_strides == nullptr || lens == nullptr || out == nullptr || (block_table == nullptr && table_width > 0))
+        return -2;
+    if (!aligned(q, 16) || !aligned(block_table, 4) || !aligned(lens, 4) || !aligned(out, 16) || !aligned(lse, 4)) return -2;
+    for (int i = 0; i < 3; ++i)
+        if (q_strides[i] < 0 || q_strides[i] % 8) return -2;
+    if (bytes > 0 && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < bytes)) return -2;
+    p.q = static_cast<const uint8_t*>(q);
+    p.qb = q_strides[0] * 2, p.qt = q_strides[1] * 2, p.qh = q_strides[2] * 2;
+    p.out = static_cast<uint16_t*>(out);
+    p.lse = static_cast<float*>(lse);
+    p.table = static_cast<const int32_t*>(block_table);
+    p.lens = static_cast<const int32_t*>(lens);
+    p.table_stride = table_stride;
+    p.scale = scale * 1.4426950408889634f;
+    p.window = window;
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = p.part_o + (int64_t)p.units * p.cols * cache->head_dim;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    switch (cache->head_dim) {
+    case 64: return launch_attention<64>(p, cache->fp8, bytes > 0, st);
+    case 128: return launch_attention<128>(p, cache->fp8, bytes > 0, st);
+    default: return launch_attention<256>(p, cache->fp8, bytes > 0, st);
+    }
+}
+
+}  // extern "C"

@@ -7,7 +7,8 @@ torch's current stream, so calls can be captured into a HIP graph (torch.cuda.CU
 
 Additions for the gfx950 build: `bf16_bias`, `fp8_bias`, `int4_zp` (asymmetric INT4 with optional bias),
 `dequant_fp8`, `dequant_int4`, `dequant_int4_zp`, `quantize_fp8_rowwise`, `quantize_int4_g128`,
-`quantize_int4_zp_g128`, `pick_variant`, `launch_kind`, `build_info`.
+`quantize_int4_zp_g128`, `pick_variant`, `launch_kind`, `build_info`, and between the projections of a decode step
+`rope_append` (on a `KVCache` description of the paged cache).
 """
 from __future__ import annotations
 
@@ -39,7 +40,22 @@ def current_raw_stream():
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
+_L = ctypes.c_longlong
+_F = ctypes.c_float
 KINDS = {"bf16": 0, "fp8": 1, "int4": 2, "int4zp": 3}
+
+
+class KVCache(ctypes.Structure):
+    """paia_kv_cache: device addresses (k_scale, v_scale fp32 [kv_heads] or None) and the strides, in elements, of page,
+    head and position. Positions of one head are together by default: [pages, kv_heads, page_size, head_dim]."""
+    _fields_ = [("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P), ("k_strides", _L * 3), ("v_strides", _L * 3),
+                ("pages", _I), ("page_size", _I), ("kv_heads", _I), ("head_dim", _I), ("fp8", _I)]
+
+    def __init__(self, k_ptr, v_ptr, pages, page_size, kv_heads, head_dim, fp8=False, k_scale_ptr=None, v_scale_ptr=None,
+                 k_strides=None, v_strides=None):
+        plain = (kv_heads * page_size * head_dim, page_size * head_dim, head_dim)
+        super().__init__(k_ptr, v_ptr, k_scale_ptr, v_scale_ptr, (_L * 3)(*(k_strides or plain)),
+                         (_L * 3)(*(v_strides or plain)), pages, page_size, kv_heads, head_dim, int(fp8))
 
 
 class GemvLib:
@@ -75,6 +91,7 @@ class GemvLib:
             "paia_gemv_batch_fp8": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
             "paia_gemv_batch_int4": [_P, _P, _P, _P, _I, _I, _I, _I, _P],
             "paia_gemv_batch_int4_zp": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
+            "paia_rope_append": [_P, _L, _P, _P, _I, _I, _I, _P, _P, _F, _P, ctypes.POINTER(KVCache), _P, _I, _I, _P],
         }
         for name, argtypes in sig.items():
             fn = getattr(lib, name)
@@ -236,6 +253,16 @@ class GemvLib:
     def batch_int4_zp(self, Wq_ptr, scales_ptr, zeros_ptr, x_ptr, bias_ptr, y_ptr, M, N, K, variant=-1, stream=None):
         self._check(self._lib.paia_gemv_batch_int4_zp(Wq_ptr, scales_ptr, zeros_ptr, x_ptr, bias_ptr, y_ptr, M, N, K,
                                                       variant, self._st(stream)), "paia_gemv_batch_int4_zp")
+
+    # ---- between the projections of a decode step -------------------------------------------------------------
+    def rope_append(self, qkv_ptr, qkv_stride, positions_ptr, cos_sin_ptr, context, rotary, slots_ptr, cache, q_ptr, M,
+                    heads, q_norm_ptr=None, k_norm_ptr=None, eps=1e-6, interleaved=False, stream=None):
+        """Head norms, rotation and cache write of M tokens' q|k|v rows (bf16, qkv_stride elements apart): rotated q
+        [M, heads, head_dim] to q_ptr, k and v to their slots (int64) of `cache` (a KVCache)."""
+        self._check(self._lib.paia_rope_append(qkv_ptr, qkv_stride, positions_ptr, cos_sin_ptr, context, rotary,
+                                               int(interleaved), q_norm_ptr, k_norm_ptr, eps, slots_ptr,
+                                               ctypes.byref(cache), q_ptr, M, heads, self._st(stream)),
+                    "paia_rope_append")
 
     def build_info(self):
         return self._lib.paia_gemv_build_info().decode()

@@ -107,3 +107,29 @@ def quantize_int4_zp_g128(W):
     """fp32 W [N,K] on the device -> asymmetric INT4 (packed [N,K/2], scales bf16 [N,G], zeros [N,ceil(G/2)])."""
     load()
     return torch.ops.paia_gemv.quantize_int4_zp_g128(W)
+
+
+def rope_append(qkv, positions, cos_sin, k_cache, v_cache, slots, num_heads, q_norm=None, k_norm=None, eps=1e-6,
+                interleaved=False, k_scale=None, v_scale=None, out=None):
+    """Head norms, position rotation and cache write of M tokens in one pass over the fused projection's output.
+
+    qkv bf16 [M, (heads + 2 kv_heads) * head_dim] (rows may be strided) -> rotated q, bf16 [M, heads, head_dim]; k and v
+    go to slot slots[m] (int64; negative or past the end: not written) of the cache, in place. The first cos_sin.shape[1]
+    dims of each q and k head turn by row positions[m] (int64) of cos_sin (fp32 [context, rotary]: cosines, then sines;
+    `rope_table` makes one). q_norm, k_norm: bf16 [head_dim] weights of an RMS norm ahead of the rotation.
+    Caches: [pages, kv_heads, page_size, head_dim], bf16, or e4m3 with fp32 [kv_heads] k_scale and v_scale."""
+    load()
+    args = (qkv, positions, cos_sin, k_cache, v_cache, slots, num_heads, q_norm, k_norm, eps, interleaved, k_scale, v_scale)
+    if out is None:
+        return torch.ops.paia_gemv.rope_append(*args)
+    torch.ops.paia_gemv.rope_append_out(*args, out)
+    return out
+
+
+def rope_table(context, rotary, base=500000.0, inverse_frequencies=None, device=None):
+    """The cos_sin argument of rope_append: fp32 [context, rotary], row p = cos(p f), then sin(p f), in 64 bits before the
+    rounding. f_i = base^(-2i/rotary), or `inverse_frequencies` [rotary/2] where a model scales them."""
+    f = (base ** (-torch.arange(0, rotary, 2, dtype=torch.float64) / rotary) if inverse_frequencies is None
+         else torch.as_tensor(inverse_frequencies, dtype=torch.float64).cpu())
+    angle = torch.arange(context, dtype=torch.float64)[:, None] * f
+    return torch.cat([angle.cos(), angle.sin()], dim=1).float().to(device)

@@ -1,0 +1,72 @@
+"""Host-side checks of the entry points between and beside the projections: every call below returns from them, nothing is
+launched (no GPU needed)."""
+import ctypes
+
+import pytest
+import torch
+
+from paia_gemv.loader import KVCache
+
+A = 1 << 20      # a 16-byte-aligned address, never dereferenced
+
+
+def cache(**change):
+    c = KVCache(A, A, 10, 16, 8, 128, change.pop("fp8", False))
+    for k, v in change.items():
+        if k in ("k_strides", "v_strides"):
+            getattr(c, k)[:] = v
+        else:
+            setattr(c, k, v)
+    return c
+
+
+BAD_CACHES = [dict(k=None), dict(v=A + 8), dict(pages=0), dict(page_size=0), dict(kv_heads=0), dict(head_dim=96),
+              dict(fp8=2), dict(k_scale=A + 2), dict(k_strides=(16384, 2048, 132)), dict(v_strides=(-16384, 2048, 128)),
+              dict(fp8=True, v_strides=(16384, 2048, 136))]
+
+
+def rope(lib, c, **change):
+    a = dict(qkv=A, stride=48 * 128, positions=A, cos_sin=A, context=100, rotary=128, q_norm=None, k_norm=None, slots=A,
+             q=A, M=4, heads=32)
+    a.update(change)
+    return lib._lib.paia_rope_append(a["qkv"], a["stride"], a["positions"], a["cos_sin"], a["context"], a["rotary"], 0,
+                                     a["q_norm"], a["k_norm"], 1e-6, a["slots"], ctypes.byref(c) if c else None, a["q"],
+                                     a["M"], a["heads"], None)
+
+
+def test_rope_append_refusals(gemv_lib):
+    for bad in BAD_CACHES:
+        assert rope(gemv_lib, cache(**bad)) == -2, bad
+    assert rope(gemv_lib, None) == -2
+    for bad in (dict(qkv=A + 8), dict(qkv=None), dict(stride=6148), dict(positions=A + 4), dict(cos_sin=A + 4),
+                dict(context=0), dict(rotary=0), dict(rotary=136), dict(rotary=144), dict(rotary=24), dict(q_norm=A + 8),
+                dict(k_norm=A + 2), dict(slots=None), dict(q=A + 4), dict(M=-1), dict(heads=0)):
+        assert rope(gemv_lib, cache(), **bad) == -2, bad
+    assert rope(gemv_lib, cache(), M=0) == 0
+
+
+def test_rope_append_meta_shape():
+    from paia_gemv import ops
+    ops.load()
+    m = torch.device("meta")
+    kc = torch.empty(4, 2, 16, 64, dtype=torch.bfloat16, device=m)
+    q = torch.ops.paia_gemv.rope_append(torch.empty(3, 8 * 64, dtype=torch.bfloat16, device=m), torch.empty(3, device=m),
+                                        torch.empty(9, 64, device=m), kc, kc.clone(), torch.empty(3, device=m), 4)
+    assert q.shape == (3, 4, 64) and q.dtype == torch.bfloat16
+
+
+def test_rope_table():
+    from paia_gemv import ops
+    t = ops.rope_table(50, 16, base=100.0)
+    assert t.shape == (50, 16) and t.dtype == torch.float32
+    f = 100.0 ** (-2.0 * 3 / 16)
+    assert abs(float(t[37, 3]) - float(torch.tensor(37 * f, dtype=torch.float64).cos())) <= 2.0 ** -24
+    assert abs(float(t[37, 8 + 3]) - float(torch.tensor(37 * f, dtype=torch.float64).sin())) <= 2.0 ** -24
+    assert torch.equal(ops.rope_table(50, 16, inverse_frequencies=[0.5] * 8)[2, :8], torch.full((8,), 1.0, dtype=torch.float64).cos().float())
+
+
+@pytest.mark.parametrize("bad", [dict(context=-5, rotary=16)])
+def test_rope_table_refuses(bad):
+    from paia_gemv import ops
+    with pytest.raises(RuntimeError):
+        ops.rope_table(**bad)
