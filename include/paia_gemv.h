@@ -181,6 +181,24 @@ PAIA_API int paia_rope_append(const void* qkv, long long qkv_stride, const void*
                               int context, int rotary, int interleaved, const void* q_norm, const void* k_norm, float eps,
                               const void* slots, const paia_kv_cache* cache, void* q_out, int M, int heads, void* stream);
 
+/* Attention of each sequence's T newest tokens over the cache. q bf16, element (b, t, head, i) at q + b * q_strides[0] +
+ * t * q_strides[1] + head * q_strides[2] + i (elements, multiples of 8; q 16-byte aligned); heads % kv_heads == 0, query
+ * head j reads kv head j / (heads / kv_heads). lens int32 [B]: positions of sequence b in the cache, the T tokens' own
+ * included; block_table int32, row b at block_table + b * table_stride: table_width page numbers, position p on page
+ * number p / page_size. Token t sees positions p < lens[b] - (T-1-t), of these the last `window` where window > 0, and none
+ * on a page number outside [0, pages) (lengths beyond the table's width end there). With s_p = scale * k_scale[head] *
+ * <q, k_p>: out bf16 [B][T][heads][head_dim] (16-byte aligned) = v_scale[head] * sum softmax(s)_p v_p, lse fp32
+ * [B][T][heads] or NULL = log(sum exp(s_p)); a token that sees nothing has out 0, lse -inf. Scores, statistics and sums in
+ * fp32; the weights are rounded to bf16 for their product with v. Nothing a token does not see reaches its output, NaN and
+ * infinities included. The lengths are read on the device: a captured call serves sequences as they grow.
+ * workspace: device memory, 16-byte aligned, of at least paia_paged_attention_workspace() bytes (for the same cache, width,
+ * B, T and heads; 0 = NULL will do, -2 = outside the contract). Calls that overlap need a workspace each. */
+PAIA_API long long paia_paged_attention_workspace(const paia_kv_cache* cache, int table_width, int B, int T, int heads);
+PAIA_API int paia_paged_attention(const void* q, const long long* q_strides, const paia_kv_cache* cache,
+                                  const void* block_table, long long table_stride, int table_width, const void* lens,
+                                  float scale, int window, void* out, void* lse, int B, int T, int heads, void* workspace,
+                                  long long workspace_bytes, void* stream);
+
 /* no reference counterpart: a human-readable build tag */
 PAIA_API const char* paia_gemv_build_info(void);
 

@@ -36,6 +36,8 @@ namespace paia {
 constexpr int kTile = 32;            // positions a wave takes at a time
 constexpr int kCols = 16;            // columns (token, head) of a unit
 constexpr int kAttnWaves = 4, kAttnBlock = kAttnWaves * kWave;
+// Blocks that a CU holds at the registers a wave takes (one wave of a block on each SIMD).
+constexpr int blocks_per_cu(int dim) { return dim <= 64 ? 3 : dim <= 128 ? 2 : 1; }
 constexpr int kMinTiles = 8;         // a piece is at least this many tiles, where the sequence has them
 
 struct AttnParams {
@@ -203,7 +205,7 @@ struct Layout {
 };
 
 template <int D, bool FP8, bool P8>
-__global__ void __launch_bounds__(kAttnBlock) paged_attention_kernel(const AttnParams p)
+__global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_kernel(const AttnParams p)
 {
     using L = Layout<D, FP8, P8>;
     __shared__ __attribute__((aligned(16))) uint8_t smem[kAttnWaves * L::kWaveLds];
@@ -513,8 +515,6 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
-constexpr int kBlocksPerCu = 3;
-
 // The launch's plan; false where its sizes leave the contract.
 static bool attention_plan(const paia_kv_cache* c, int table_width, int B, int T, int heads, AttnParams* p, int64_t* bytes)
 {
@@ -527,7 +527,7 @@ static bool attention_plan(const paia_kv_cache* c, int table_width, int B, int T
     if (cols > INT_MAX / 2) return false;
     p->cols = (int)cols;
     p->col_groups = (p->cols + kCols - 1) / kCols;
-    const int64_t wide = (int64_t)c->kv_heads * p->col_groups, slots = (int64_t)device_facts().cus * kBlocksPerCu;
+    const int64_t wide = (int64_t)c->kv_heads * p->col_groups, slots = (int64_t)device_facts().cus * blocks_per_cu(c->head_dim);
     int64_t target = slots / wide;
     target = target < 1 ? 1 : target;
     // pieces per sequence that the table's width allows, and the bound of piece_tiles
@@ -593,7 +593,7 @@ int paia_paged_attention(const void* q, const long long* q_strides, const paia_k
     p.lens = static_cast<const int32_t*>(lens);
     p.table_stride = table_stride;
     p.scale = scale * 1.4426950408889634f;
-    p.window = window;
+    p.window = window >= (int64_t)p.max_len + T ? 0 : window;    // it hides nothing
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = p.part_o + (int64_t)p.units * p.cols * cache->head_dim;
     const hipStream_t st = static_cast<hipStream_t>(stream);

@@ -10,8 +10,10 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
+#include <cmath>
 #include <cstdint>
 #include <optional>
+#include <tuple>
 
 #include "paia_gemv.h"
 
@@ -132,6 +134,104 @@ at::Tensor rope_append(const at::Tensor& qkv, const at::Tensor& positions, const
     return out;
 }
 
+// -------------------------------------------------------------------------------------------------------------
+// q [B, heads, D] (one token a sequence) or [B, T, heads, D]: its sizes as the C ABI takes them.
+struct Query {
+    int64_t B, T, heads;
+    long long strides[3];
+};
+Query query_of(const at::Tensor& q)
+{
+    TORCH_CHECK((q.dim() == 3 || q.dim() == 4) && q.scalar_type() == at::kBFloat16,
+                "q must be bfloat16 [B, heads, head_dim] or [B, T, heads, head_dim]");
+    TORCH_CHECK(q.numel() == 0 || q.stride(-1) == 1, "q's last dimension must be contiguous");
+    const int64_t d = q.dim();
+    return {q.size(0), d == 4 ? q.size(1) : 1, q.size(d - 2), {q.stride(0), d == 4 ? q.stride(1) : 0, q.stride(d - 2)}};
+}
+
+// lse may be an undefined tensor: not wanted.
+void paged_attention_run(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                         const at::Tensor& block_table, const at::Tensor& lens, std::optional<double> scale, int64_t window,
+                         const std::optional<at::Tensor>& k_scale, const std::optional<at::Tensor>& v_scale,
+                         const at::Tensor& out, const at::Tensor& lse, const std::optional<at::Tensor>& workspace)
+{
+    TORCH_CHECK(q.is_cuda(), "q must be on a GPU, found ", q.device());
+    const Query y = query_of(q);
+    const paia_kv_cache c = cache_of(k_cache, v_cache, k_scale, v_scale, q);
+    TORCH_CHECK(q.size(-1) == c.head_dim, "q and the cache must have the same head_dim");
+    TORCH_CHECK(y.T > 0 && y.heads > 0 && y.heads % c.kv_heads == 0, "q's heads (", y.heads,
+                ") must be a multiple of the cache's (", c.kv_heads, "), its tokens at least one");
+    check_index(lens, at::kInt, y.B, q, "lens");
+    TORCH_CHECK(block_table.dim() == 2 && block_table.scalar_type() == at::kInt && block_table.size(0) == y.B &&
+                    (block_table.numel() == 0 || block_table.stride(1) == 1),
+                "block_table must be int32 [B, pages of a sequence] with contiguous rows");
+    on_device_of(q, block_table, "block_table");
+    TORCH_CHECK(out.scalar_type() == at::kBFloat16 && out.is_contiguous() && out.numel() == y.B * y.T * y.heads * c.head_dim,
+                "out must be a contiguous bfloat16 tensor of q's shape");
+    on_device_of(q, out, "out");
+    TORCH_CHECK(window >= 0, "window must not be negative");
+    const int B = to_int(y.B, "B"), T = to_int(y.T, "T"), heads = to_int(y.heads, "heads");
+    const int width = to_int(block_table.size(1), "the block table's width");
+    c10::DeviceGuard g(q.device());
+    const long long need = paia_paged_attention_workspace(&c, width, B, T, heads);
+    check_rc(need < 0 ? (int)need : 0, "paia_paged_attention");
+    at::Tensor space;
+    if (workspace.has_value()) {
+        TORCH_CHECK(workspace->is_contiguous() && (int64_t)workspace->nbytes() >= need,
+                    "workspace must be contiguous and hold ", need, " bytes");
+        on_device_of(q, *workspace, "workspace");
+        space = *workspace;
+    } else if (need > 0) {
+        space = at::empty({need}, q.options().dtype(at::kByte));
+    }
+    const double s = scale.has_value() ? *scale : 1.0 / std::sqrt((double)c.head_dim);
+    check_rc(paia_paged_attention(q.data_ptr(), y.strides, &c, block_table.data_ptr(), block_table.stride(0), width,
+                                  lens.data_ptr(), (float)s, to_int(window, "window"), out.data_ptr(),
+                                  lse.defined() ? lse.data_ptr() : nullptr, B, T, heads,
+                                  space.defined() ? space.data_ptr() : nullptr,
+                                  space.defined() ? (long long)space.nbytes() : 0, stream_of(q)),
+             "paia_paged_attention");
+}
+at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                           const at::Tensor& block_table, const at::Tensor& lens, std::optional<double> scale,
+                           int64_t window, const std::optional<at::Tensor>& k_scale,
+                           const std::optional<at::Tensor>& v_scale, const std::optional<at::Tensor>& workspace)
+{
+    at::Tensor out = at::empty(q.sizes(), q.options());
+    paged_attention_run(q, k_cache, v_cache, block_table, lens, scale, window, k_scale, v_scale, out, {}, workspace);
+    return out;
+}
+at::Tensor new_lse(const at::Tensor& q)
+{
+    return at::empty(q.sizes().slice(0, q.dim() > 0 ? q.dim() - 1 : 0), q.options().dtype(at::kFloat));
+}
+std::tuple<at::Tensor, at::Tensor> paged_attention_lse(const at::Tensor& q, const at::Tensor& k_cache,
+                                                       const at::Tensor& v_cache, const at::Tensor& block_table,
+                                                       const at::Tensor& lens, std::optional<double> scale, int64_t window,
+                                                       const std::optional<at::Tensor>& k_scale,
+                                                       const std::optional<at::Tensor>& v_scale,
+                                                       const std::optional<at::Tensor>& workspace)
+{
+    at::Tensor out = at::empty(q.sizes(), q.options()), lse = new_lse(q);
+    paged_attention_run(q, k_cache, v_cache, block_table, lens, scale, window, k_scale, v_scale, out, lse, workspace);
+    return {out, lse};
+}
+void paged_attention_out(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                         const at::Tensor& block_table, const at::Tensor& lens, std::optional<double> scale, int64_t window,
+                         const std::optional<at::Tensor>& k_scale, const std::optional<at::Tensor>& v_scale,
+                         const std::optional<at::Tensor>& workspace, at::Tensor& out)
+{
+    paged_attention_run(q, k_cache, v_cache, block_table, lens, scale, window, k_scale, v_scale, out, {}, workspace);
+}
+int64_t paged_attention_workspace(const at::Tensor& k_cache, int64_t table_width, int64_t B, int64_t T, int64_t num_heads)
+{
+    const paia_kv_cache c = cache_of(k_cache, k_cache, {}, {}, k_cache);
+    const long long need = paia_paged_attention_workspace(&c, to_int(table_width, "table_width"), to_int(B, "B"),
+                                                          to_int(T, "T"), to_int(num_heads, "num_heads"));
+    check_rc(need < 0 ? (int)need : 0, "paia_paged_attention_workspace");
+    return need;
+}
+
 // ---- Meta (shape-only) kernels ------------------------------------------------------------------------------
 at::Tensor rope_append_meta(const at::Tensor& qkv, const at::Tensor&, const at::Tensor&, at::Tensor& k_cache, at::Tensor&,
                             const at::Tensor&, int64_t num_heads, const std::optional<at::Tensor>&,
@@ -144,6 +244,24 @@ void rope_append_out_meta(const at::Tensor&, const at::Tensor&, const at::Tensor
                           const at::Tensor&, int64_t, const std::optional<at::Tensor>&, const std::optional<at::Tensor>&,
                           double, bool, const std::optional<at::Tensor>&, const std::optional<at::Tensor>&, at::Tensor&) {}
 
+at::Tensor paged_attention_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                const at::Tensor&, std::optional<double>, int64_t, const std::optional<at::Tensor>&,
+                                const std::optional<at::Tensor>&, const std::optional<at::Tensor>&)
+{
+    return at::empty(q.sizes(), q.options());
+}
+std::tuple<at::Tensor, at::Tensor> paged_attention_lse_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&,
+                                                            const at::Tensor&, const at::Tensor&, std::optional<double>,
+                                                            int64_t, const std::optional<at::Tensor>&,
+                                                            const std::optional<at::Tensor>&,
+                                                            const std::optional<at::Tensor>&)
+{
+    return {at::empty(q.sizes(), q.options()), new_lse(q)};
+}
+void paged_attention_out_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                              std::optional<double>, int64_t, const std::optional<at::Tensor>&,
+                              const std::optional<at::Tensor>&, const std::optional<at::Tensor>&, at::Tensor&) {}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(paia_gemv, m)
@@ -154,16 +272,31 @@ TORCH_LIBRARY_FRAGMENT(paia_gemv, m)
     m.def("rope_append_out(Tensor qkv, Tensor positions, Tensor cos_sin, Tensor(a!) k_cache, Tensor(b!) v_cache, "
           "Tensor slots, int num_heads, Tensor? q_norm, Tensor? k_norm, float eps, bool interleaved, Tensor? k_scale, "
           "Tensor? v_scale, Tensor(c!) out) -> ()");
+    m.def("paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor lens, float? scale=None, "
+          "int window=0, Tensor? k_scale=None, Tensor? v_scale=None, Tensor(a!)? workspace=None) -> Tensor");
+    m.def("paged_attention_lse(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor lens, "
+          "float? scale=None, int window=0, Tensor? k_scale=None, Tensor? v_scale=None, Tensor(a!)? workspace=None) "
+          "-> (Tensor, Tensor)");
+    m.def("paged_attention_out(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor lens, float? scale, "
+          "int window, Tensor? k_scale, Tensor? v_scale, Tensor(a!)? workspace, Tensor(b!) out) -> ()");
+    m.def("paged_attention_workspace(Tensor k_cache, int table_width, int B, int T, int num_heads) -> int");
 }
 
 TORCH_LIBRARY_IMPL(paia_gemv, CUDA, m)
 {
     m.impl("rope_append", &rope_append);
     m.impl("rope_append_out", &rope_append_out);
+    m.impl("paged_attention", &paged_attention);
+    m.impl("paged_attention_lse", &paged_attention_lse);
+    m.impl("paged_attention_out", &paged_attention_out);
+    m.impl("paged_attention_workspace", &paged_attention_workspace);
 }
 
 TORCH_LIBRARY_IMPL(paia_gemv, Meta, m)
 {
     m.impl("rope_append", &rope_append_meta);
     m.impl("rope_append_out", &rope_append_out_meta);
+    m.impl("paged_attention", &paged_attention_meta);
+    m.impl("paged_attention_lse", &paged_attention_lse_meta);
+    m.impl("paged_attention_out", &paged_attention_out_meta);
 }

@@ -8,7 +8,7 @@ torch's current stream, so calls can be captured into a HIP graph (torch.cuda.CU
 Additions for the gfx950 build: `bf16_bias`, `fp8_bias`, `int4_zp` (asymmetric INT4 with optional bias),
 `dequant_fp8`, `dequant_int4`, `dequant_int4_zp`, `quantize_fp8_rowwise`, `quantize_int4_g128`,
 `quantize_int4_zp_g128`, `pick_variant`, `launch_kind`, `build_info`, and between the projections of a decode step
-`rope_append` (on a `KVCache` description of the paged cache).
+`rope_append` and `paged_attention` (on a `KVCache` description of the paged cache).
 """
 from __future__ import annotations
 
@@ -92,11 +92,15 @@ class GemvLib:
             "paia_gemv_batch_int4": [_P, _P, _P, _P, _I, _I, _I, _I, _P],
             "paia_gemv_batch_int4_zp": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
             "paia_rope_append": [_P, _L, _P, _P, _I, _I, _I, _P, _P, _F, _P, ctypes.POINTER(KVCache), _P, _I, _I, _P],
+            "paia_paged_attention": [_P, ctypes.POINTER(_L), ctypes.POINTER(KVCache), _P, _L, _I, _P, _F, _I, _P, _P, _I,
+                                     _I, _I, _P, _L, _P],
         }
         for name, argtypes in sig.items():
             fn = getattr(lib, name)
             fn.restype = _I
             fn.argtypes = argtypes
+        lib.paia_paged_attention_workspace.restype = _L
+        lib.paia_paged_attention_workspace.argtypes = [ctypes.POINTER(KVCache), _I, _I, _I, _I]
         lib.paia_gemv_build_info.restype = ctypes.c_char_p
         lib.paia_gemv_build_info.argtypes = []
         self.variants_fp8 = self._qvariants(lib, "fp8")
@@ -263,6 +267,24 @@ class GemvLib:
                                                int(interleaved), q_norm_ptr, k_norm_ptr, eps, slots_ptr,
                                                ctypes.byref(cache), q_ptr, M, heads, self._st(stream)),
                     "paia_rope_append")
+
+    def paged_attention_workspace(self, cache, table_width, B, T, heads):
+        """Bytes of device memory that paged_attention takes as its workspace."""
+        need = self._lib.paia_paged_attention_workspace(ctypes.byref(cache), table_width, B, T, heads)
+        self._check(min(need, 0), "paia_paged_attention_workspace")
+        return need
+
+    def paged_attention(self, q_ptr, cache, table_ptr, table_width, lens_ptr, out_ptr, B, T, heads, scale, window=0,
+                        lse_ptr=None, workspace_ptr=None, workspace_bytes=0, q_strides=None, table_stride=None,
+                        stream=None):
+        """Attention of each sequence's T newest tokens (q bf16 [B, T, heads, head_dim], or strides in elements) over
+        `cache` (a KVCache) through the int32 block table and lens."""
+        D = cache.head_dim
+        strides = (_L * 3)(*(q_strides or (T * heads * D, heads * D, D)))
+        self._check(self._lib.paia_paged_attention(q_ptr, strides, ctypes.byref(cache), table_ptr,
+                                                   table_width if table_stride is None else table_stride, table_width,
+                                                   lens_ptr, scale, window, out_ptr, lse_ptr, B, T, heads, workspace_ptr,
+                                                   workspace_bytes, self._st(stream)), "paia_paged_attention")
 
     def build_info(self):
         return self._lib.paia_gemv_build_info().decode()

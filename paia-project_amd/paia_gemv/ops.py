@@ -133,3 +133,36 @@ def rope_table(context, rotary, base=500000.0, inverse_frequencies=None, device=
          else torch.as_tensor(inverse_frequencies, dtype=torch.float64).cpu())
     angle = torch.arange(context, dtype=torch.float64)[:, None] * f
     return torch.cat([angle.cos(), angle.sin()], dim=1).float().to(device)
+
+
+def paged_attention(q, k_cache, v_cache, block_table, lens, scale=None, window=0, k_scale=None, v_scale=None,
+                    return_lse=False, out=None, workspace=None):
+    """Attention of each sequence's newest tokens over the paged cache: out of q's shape, bf16, and with return_lse also
+    log sum exp of the scores, fp32 [B, (T,) heads].
+
+    q bf16 [B, heads, head_dim], or [B, T, heads, head_dim] for the T newest tokens (a draft to verify); strided views are
+    taken. lens int32 [B] counts each sequence's positions in the cache, the tokens' own included (append first, then
+    attend); block_table int32 [B, width] lists its pages, position p on entry p // page_size. Token t sees positions below
+    lens[b] - (T-1-t), with a window only the last `window` of them, and none on a page number outside the cache (-1 for
+    pages given back); what sees nothing gives 0 (lse -inf). scale defaults to head_dim ** -0.5. Caches as rope_append
+    writes them.
+
+    The work is split by the lengths as the GPU finds them, so a captured call may be replayed as they grow.
+    `workspace` (any contiguous tensor of `paged_attention_workspace` bytes) avoids an allocation; not to be shared by calls
+    that overlap."""
+    load()
+    args = (q, k_cache, v_cache, block_table, lens, scale, window, k_scale, v_scale, workspace)
+    if return_lse:
+        if out is not None:
+            raise ValueError("paged_attention: out goes without return_lse")
+        return torch.ops.paia_gemv.paged_attention_lse(*args)
+    if out is None:
+        return torch.ops.paia_gemv.paged_attention(*args)
+    torch.ops.paia_gemv.paged_attention_out(*args, out)
+    return out
+
+
+def paged_attention_workspace(k_cache, table_width, B, T, num_heads):
+    """Bytes that paged_attention's workspace takes for these sizes."""
+    load()
+    return torch.ops.paia_gemv.paged_attention_workspace(k_cache, table_width, B, T, num_heads)

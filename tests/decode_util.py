@@ -68,30 +68,37 @@ def rope64(qkv, positions, cos_sin, heads, kv_heads, dim, q_norm=None, k_norm=No
 
 
 def attention64(q, k_cache, v_cache, table, lens, scale=None, window=0, k_scale=None, v_scale=None):
-    """(out [B, T, heads, dim], lse [B, T, heads]) in 64 bits, one token at a time over exactly the positions it sees.
-    Everything on the CPU; k_cache and v_cache [pages, kv_heads, page_size, dim]."""
+    """In 64 bits on the CPU, one token at a time over exactly the positions it sees: out [B, T, heads, dim], lse [B, T,
+    heads], and for error bounds sum of weight * |v| (like out) and the largest sum of |q_i k_i| * |scale| (like lse).
+    k_cache and v_cache [pages, kv_heads, page_size, dim]."""
     B, T, Hq, D = q.shape
     pages, H, P, _ = k_cache.shape
     scale = D ** -0.5 if scale is None else scale
-    out = torch.zeros(B, T, Hq, D, dtype=torch.float64)
-    lse = torch.full((B, T, Hq), -math.inf, dtype=torch.float64)
+    out, size = torch.zeros(2, B, T, Hq, D, dtype=torch.float64)
+    lse, terms = torch.full((B, T, Hq), -math.inf, dtype=torch.float64), torch.zeros(B, T, Hq, dtype=torch.float64)
+    G = Hq // H
     for b in range(B):
-        n = min(int(lens[b]), table.shape[1] * P)
+        n = max(0, min(int(lens[b]), table.shape[1] * P))
+        at = torch.arange(n)
+        page = table[b].long()[at // P]
         for t in range(T):
             end = n - (T - 1 - t)
-            first = max(0, end - window) if window else 0
-            at = [p for p in range(first, max(first, end)) if 0 <= int(table[b, p // P]) < pages]
-            if not at:
+            see = (at < end) & (page >= 0) & (page < pages)
+            if window:
+                see &= at >= end - window
+            if not see.any():
                 continue
-            at = torch.tensor(at)
-            pg, off = table[b].long()[at // P], at % P
+            pg, off = page[see], at[see] % P
             k = codes(k_cache[pg, :, off]) * (1.0 if k_scale is None else k_scale.double()[None, :, None])
             v = codes(v_cache[pg, :, off]) * (1.0 if v_scale is None else v_scale.double()[None, :, None])
-            for h in range(Hq):
-                a = k[:, h // (Hq // H)] @ q[b, t, h].double() * scale
-                lse[b, t, h] = torch.logsumexp(a, 0)
-                out[b, t, h] = torch.softmax(a, 0) @ v[:, h // (Hq // H)]
-    return out, lse
+            k, v, x = k.transpose(0, 1), v.transpose(0, 1), q[b, t].double().view(H, G, D)
+            a = torch.matmul(x, k.transpose(1, 2)) * scale
+            w = torch.softmax(a, -1)
+            lse[b, t] = torch.logsumexp(a, -1).view(Hq)
+            out[b, t] = torch.matmul(w, v).view(Hq, D)
+            size[b, t] = torch.matmul(w, v.abs()).view(Hq, D)
+            terms[b, t] = (torch.matmul(x.abs(), k.abs().transpose(1, 2)).amax(-1) * abs(scale)).view(Hq)
+    return out, lse, size, terms
 
 
 def lora64(y, x, A, B, ids, scaling, splits):

@@ -70,3 +70,50 @@ def test_rope_table_refuses(bad):
     from paia_gemv import ops
     with pytest.raises(RuntimeError):
         ops.rope_table(**bad)
+
+
+def attention(lib, c, **change):
+    a = dict(q=A, strides=(4096, 4096, 128), table=A, stride=64, width=64, lens=A, window=0, out=A, lse=None, B=2, T=1,
+             heads=32, space=A, bytes=1 << 40)
+    a.update(change)
+    st = (ctypes.c_longlong * 3)(*a["strides"]) if a["strides"] else None
+    return lib._lib.paia_paged_attention(a["q"], st, ctypes.byref(c) if c else None, a["table"], a["stride"], a["width"],
+                                         a["lens"], 0.1, a["window"], a["out"], a["lse"], a["B"], a["T"], a["heads"],
+                                         a["space"], a["bytes"], None)
+
+
+def test_paged_attention_refusals(gemv_lib):
+    for bad in BAD_CACHES:
+        assert attention(gemv_lib, cache(**bad)) == -2, bad
+    assert attention(gemv_lib, None) == -2
+    for bad in (dict(q=None), dict(q=A + 8), dict(strides=None), dict(strides=(4096, 4096, 132)),
+                dict(strides=(-4096, 4096, 128)), dict(table=None), dict(table=A + 2), dict(stride=-1), dict(width=-1),
+                dict(lens=None), dict(lens=A + 1), dict(window=-1), dict(out=None), dict(out=A + 8), dict(lse=A + 2),
+                dict(B=-1), dict(T=0), dict(heads=0), dict(heads=30), dict(space=None), dict(space=A + 8), dict(bytes=100),
+                dict(T=1 << 30), dict(B=1 << 28)):
+        assert attention(gemv_lib, cache(), **bad) == -2, bad
+    assert attention(gemv_lib, cache(), B=0) == 0
+
+
+def test_paged_attention_workspace(gemv_lib):
+    need = lambda w, B=2, T=1, heads=32, **c: gemv_lib._lib.paia_paged_attention_workspace(  # noqa: E731
+        ctypes.byref(cache(**c)), w, B, T, heads)
+    assert need(0) == 0 and need(1) == 0                 # sequences of one piece are not joined
+    assert 0 < need(1000) <= need(8192) and need(8192) == need(100000)   # bounded by the chip, not by the length
+    assert need(100, heads=30) == -2 and need(-1) == -2 and need(100, T=0) == -2 and need(100, page_size=0) == -2
+    assert need(2 ** 31 - 1, page_size=2 ** 31 - 1) > 0
+    assert gemv_lib.paged_attention_workspace(cache(), 1000, 2, 1, 32) == need(1000)
+    with pytest.raises(RuntimeError, match="-2"):
+        gemv_lib.paged_attention_workspace(cache(), 1000, 2, 1, 30)
+
+
+def test_paged_attention_meta_shapes():
+    from paia_gemv import ops
+    ops.load()
+    m = torch.device("meta")
+    kc = torch.empty(4, 2, 16, 64, dtype=torch.bfloat16, device=m)
+    q = torch.empty(3, 4, 8, 64, dtype=torch.bfloat16, device=m)
+    table, lens = torch.empty(3, 5, dtype=torch.int32, device=m), torch.empty(3, dtype=torch.int32, device=m)
+    assert torch.ops.paia_gemv.paged_attention(q, kc, kc, table, lens).shape == q.shape
+    out, lse = torch.ops.paia_gemv.paged_attention_lse(q, kc, kc, table, lens)
+    assert out.shape == q.shape and lse.shape == (3, 4, 8) and lse.dtype == torch.float32
