@@ -199,6 +199,19 @@ PAIA_API int paia_paged_attention(const void* q, const long long* q_strides, con
                                   float scale, int window, void* out, void* lse, int B, int T, int heads, void* workspace,
                                   long long workspace_bytes, void* stream);
 
+/* Low-rank adapters of M rows beside a shared projection: out[m][n] = y[m][n] + scaling[a] * sum_r B[a][n][r] *
+ * h[m][j * rank + r], h[m] = A[a] x[m], a = ids[m]. The N = sum(splits) outputs come in `slices` <= 8 slices (q | k | v, gate |
+ * up; splits: host ints), j the slice of n, each with its own `rank` rows of A. y, out bf16 [M][N] and x bf16 [M][K] with row
+ * strides in elements (out may be y); A bf16 [adapters][slices * rank][K], B bf16 [adapters][N][rank], ids int32 [M] (outside
+ * [0, adapters): the row keeps y), scaling fp32 [adapters] or NULL (1). fp32 sums, one rounding at the end. rank % 8 == 0,
+ * rank <= 256, K % 8 == 0; x, A, B and x's rows 16-byte aligned; M = 0 does nothing. workspace as for paged attention, 16-byte
+ * aligned, of paia_lora_add_workspace() bytes (-2: outside the contract). */
+PAIA_API long long paia_lora_add_workspace(int M, int rank, int slices);
+PAIA_API int paia_lora_add(const void* y, long long y_stride, const void* x, long long x_stride, const void* A,
+                           const void* B, const void* ids, const void* scaling, void* out, long long out_stride, int M,
+                           int K, int rank, const int* splits, int slices, int adapters, void* workspace,
+                           long long workspace_bytes, void* stream);
+
 /* no reference counterpart: a human-readable build tag */
 PAIA_API const char* paia_gemv_build_info(void);
 

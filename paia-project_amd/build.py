@@ -43,7 +43,7 @@ HIP_FLAGS = [
 ]
 HIP_SOURCES = ["gemv_runtime.hip", "gemv_bf16.hip", "gemv_fp8.hip", "gemv_int4.hip", "gemv_dequant.hip",
                "gemv_select.hip", "quantize.hip", "gemv_batch.hip",
-               "gemv_tile.hip", "rope_append.hip", "paged_attention.hip"]
+               "gemv_tile.hip", "rope_append.hip", "paged_attention.hip", "lora.hip"]
 
 TORCH_SOURCES = ["torch_ops.cpp", "torch_decode_ops.cpp"]
 

@@ -232,6 +232,65 @@ int64_t paged_attention_workspace(const at::Tensor& k_cache, int64_t table_width
     return need;
 }
 
+// -------------------------------------------------------------------------------------------------------------
+bool rows_of(const at::Tensor& t) { return t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1); }
+
+void lora_add_out(const at::Tensor& y, const at::Tensor& x, const at::Tensor& A, const at::Tensor& B, const at::Tensor& ids,
+                  const std::optional<at::Tensor>& scaling, at::OptionalIntArrayRef splits,
+                  const std::optional<at::Tensor>& workspace, at::Tensor& out)
+{
+    TORCH_CHECK(A.is_cuda(), "A must be on a GPU, found ", A.device());
+    const auto bf16 = [](const at::Tensor& t) { return t.scalar_type() == at::kBFloat16; };
+    TORCH_CHECK(A.dim() == 3 && bf16(A) && A.is_contiguous(), "A must be contiguous bfloat16 [adapters, slices * rank, K]");
+    TORCH_CHECK(B.dim() == 3 && bf16(B) && B.is_contiguous(), "B must be contiguous bfloat16 [adapters, N, rank]");
+    const int64_t L = A.size(0), K = A.size(2), N = B.size(1), R = B.size(2);
+    TORCH_CHECK(B.size(0) == L && L > 0, "A and B must hold the same adapters, at least one");
+    TORCH_CHECK(bf16(x) && rows_of(x) && x.size(1) == K, "x must be bfloat16 [M, K] with contiguous rows");
+    const int64_t M = x.size(0);
+    TORCH_CHECK(bf16(y) && rows_of(y) && y.size(0) == M && y.size(1) == N, "y must be bfloat16 [M, N] with contiguous rows");
+    TORCH_CHECK(bf16(out) && rows_of(out) && out.sizes() == y.sizes(), "out must be bfloat16 [M, N] with contiguous rows");
+    check_index(ids, at::kInt, M, A, "ids");
+    on_device_of(A, B, "B");
+    on_device_of(A, x, "x");
+    on_device_of(A, y, "y");
+    on_device_of(A, out, "out");
+    int parts[8], slices = 0;
+    int64_t sum = 0;
+    if (splits.has_value()) {
+        TORCH_CHECK(splits->size() >= 1 && splits->size() <= 8, "splits must name 1 to 8 slices");
+        for (const int64_t n : *splits) parts[slices++] = to_int(n, "a slice"), sum += n;
+    } else {
+        parts[slices++] = to_int(N, "N"), sum = N;
+    }
+    TORCH_CHECK(sum == N, "splits must sum to N (", N, "), found ", sum);
+    TORCH_CHECK(A.size(1) == slices * R, "A must hold rank rows (", R, ") for each of ", slices, " slices");
+    c10::DeviceGuard g(A.device());
+    const long long need = paia_lora_add_workspace(to_int(M, "M"), to_int(R, "rank"), slices);
+    check_rc(need < 0 ? (int)need : 0, "paia_lora_add");
+    at::Tensor space;
+    if (workspace.has_value()) {
+        TORCH_CHECK(workspace->is_contiguous() && (int64_t)workspace->nbytes() >= need,
+                    "workspace must be contiguous and hold ", need, " bytes");
+        on_device_of(A, *workspace, "workspace");
+        space = *workspace;
+    } else {
+        space = at::empty({need}, A.options().dtype(at::kByte));
+    }
+    check_rc(paia_lora_add(y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), A.data_ptr(), B.data_ptr(), ids.data_ptr(),
+                           opt_ptr(scaling, at::kFloat, L, A, "scaling"), out.data_ptr(), out.stride(0), (int)M,
+                           to_int(K, "K"), (int)R, parts, slices, to_int(L, "adapters"), space.data_ptr(),
+                           (long long)space.nbytes(), stream_of(A)),
+             "paia_lora_add");
+}
+at::Tensor lora_add(const at::Tensor& y, const at::Tensor& x, const at::Tensor& A, const at::Tensor& B,
+                    const at::Tensor& ids, const std::optional<at::Tensor>& scaling, at::OptionalIntArrayRef splits,
+                    const std::optional<at::Tensor>& workspace)
+{
+    at::Tensor out = at::empty(y.sizes(), y.options());
+    lora_add_out(y, x, A, B, ids, scaling, splits, workspace, out);
+    return out;
+}
+
 // ---- Meta (shape-only) kernels ------------------------------------------------------------------------------
 at::Tensor rope_append_meta(const at::Tensor& qkv, const at::Tensor&, const at::Tensor&, at::Tensor& k_cache, at::Tensor&,
                             const at::Tensor&, int64_t num_heads, const std::optional<at::Tensor>&,
@@ -262,6 +321,15 @@ void paged_attention_out_meta(const at::Tensor&, const at::Tensor&, const at::Te
                               std::optional<double>, int64_t, const std::optional<at::Tensor>&,
                               const std::optional<at::Tensor>&, const std::optional<at::Tensor>&, at::Tensor&) {}
 
+at::Tensor lora_add_meta(const at::Tensor& y, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                         const std::optional<at::Tensor>&, at::OptionalIntArrayRef, const std::optional<at::Tensor>&)
+{
+    return at::empty(y.sizes(), y.options());
+}
+void lora_add_out_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                       const std::optional<at::Tensor>&, at::OptionalIntArrayRef, const std::optional<at::Tensor>&,
+                       at::Tensor&) {}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(paia_gemv, m)
@@ -279,6 +347,10 @@ TORCH_LIBRARY_FRAGMENT(paia_gemv, m)
           "-> (Tensor, Tensor)");
     m.def("paged_attention_out(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor lens, float? scale, "
           "int window, Tensor? k_scale, Tensor? v_scale, Tensor(a!)? workspace, Tensor(b!) out) -> ()");
+    m.def("lora_add(Tensor y, Tensor x, Tensor A, Tensor B, Tensor ids, Tensor? scaling=None, int[]? splits=None, "
+          "Tensor(a!)? workspace=None) -> Tensor");
+    m.def("lora_add_out(Tensor y, Tensor x, Tensor A, Tensor B, Tensor ids, Tensor? scaling, int[]? splits, "
+          "Tensor(a!)? workspace, Tensor(b!) out) -> ()");
     m.def("paged_attention_workspace(Tensor k_cache, int table_width, int B, int T, int num_heads) -> int");
 }
 
@@ -290,6 +362,8 @@ TORCH_LIBRARY_IMPL(paia_gemv, CUDA, m)
     m.impl("paged_attention_lse", &paged_attention_lse);
     m.impl("paged_attention_out", &paged_attention_out);
     m.impl("paged_attention_workspace", &paged_attention_workspace);
+    m.impl("lora_add", &lora_add);
+    m.impl("lora_add_out", &lora_add_out);
 }
 
 TORCH_LIBRARY_IMPL(paia_gemv, Meta, m)
@@ -299,4 +373,6 @@ TORCH_LIBRARY_IMPL(paia_gemv, Meta, m)
     m.impl("paged_attention", &paged_attention_meta);
     m.impl("paged_attention_lse", &paged_attention_lse_meta);
     m.impl("paged_attention_out", &paged_attention_out_meta);
+    m.impl("lora_add", &lora_add_meta);
+    m.impl("lora_add_out", &lora_add_out_meta);
 }

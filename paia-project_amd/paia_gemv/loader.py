@@ -8,7 +8,7 @@ torch's current stream, so calls can be captured into a HIP graph (torch.cuda.CU
 Additions for the gfx950 build: `bf16_bias`, `fp8_bias`, `int4_zp` (asymmetric INT4 with optional bias),
 `dequant_fp8`, `dequant_int4`, `dequant_int4_zp`, `quantize_fp8_rowwise`, `quantize_int4_g128`,
 `quantize_int4_zp_g128`, `pick_variant`, `launch_kind`, `build_info`, and between the projections of a decode step
-`rope_append` and `paged_attention` (on a `KVCache` description of the paged cache).
+`rope_append` and `paged_attention` (on a `KVCache` description of the paged cache), beside them `lora_add`.
 """
 from __future__ import annotations
 
@@ -94,6 +94,7 @@ class GemvLib:
             "paia_rope_append": [_P, _L, _P, _P, _I, _I, _I, _P, _P, _F, _P, ctypes.POINTER(KVCache), _P, _I, _I, _P],
             "paia_paged_attention": [_P, ctypes.POINTER(_L), ctypes.POINTER(KVCache), _P, _L, _I, _P, _F, _I, _P, _P, _I,
                                      _I, _I, _P, _L, _P],
+            "paia_lora_add": [_P, _L, _P, _L, _P, _P, _P, _P, _P, _L, _I, _I, _I, ctypes.POINTER(_I), _I, _I, _P, _L, _P],
         }
         for name, argtypes in sig.items():
             fn = getattr(lib, name)
@@ -101,6 +102,8 @@ class GemvLib:
             fn.argtypes = argtypes
         lib.paia_paged_attention_workspace.restype = _L
         lib.paia_paged_attention_workspace.argtypes = [ctypes.POINTER(KVCache), _I, _I, _I, _I]
+        lib.paia_lora_add_workspace.restype = _L
+        lib.paia_lora_add_workspace.argtypes = [_I, _I, _I]
         lib.paia_gemv_build_info.restype = ctypes.c_char_p
         lib.paia_gemv_build_info.argtypes = []
         self.variants_fp8 = self._qvariants(lib, "fp8")
@@ -285,6 +288,23 @@ class GemvLib:
                                                    table_width if table_stride is None else table_stride, table_width,
                                                    lens_ptr, scale, window, out_ptr, lse_ptr, B, T, heads, workspace_ptr,
                                                    workspace_bytes, self._st(stream)), "paia_paged_attention")
+
+    def lora_add_workspace(self, M, rank, slices):
+        """Bytes of device memory that lora_add takes as its workspace."""
+        need = self._lib.paia_lora_add_workspace(M, rank, slices)
+        self._check(min(need, 0), "paia_lora_add_workspace")
+        return need
+
+    def lora_add(self, y_ptr, x_ptr, A_ptr, B_ptr, ids_ptr, scaling_ptr, out_ptr, M, K, rank, splits, adapters,
+                 workspace_ptr, workspace_bytes, y_stride=None, x_stride=None, out_stride=None, stream=None):
+        """out [M, sum(splits)] = y + the rows' adapters; see ops.lora_add. Strides in elements, rows contiguous by
+        default."""
+        N = sum(splits)
+        self._check(self._lib.paia_lora_add(y_ptr, N if y_stride is None else y_stride, x_ptr,
+                                            K if x_stride is None else x_stride, A_ptr, B_ptr, ids_ptr, scaling_ptr,
+                                            out_ptr, N if out_stride is None else out_stride, M, K, rank,
+                                            (_I * len(splits))(*splits), len(splits), adapters, workspace_ptr,
+                                            workspace_bytes, self._st(stream)), "paia_lora_add")
 
     def build_info(self):
         return self._lib.paia_gemv_build_info().decode()

@@ -166,3 +166,18 @@ def paged_attention_workspace(k_cache, table_width, B, T, num_heads):
     """Bytes that paged_attention's workspace takes for these sizes."""
     load()
     return torch.ops.paia_gemv.paged_attention_workspace(k_cache, table_width, B, T, num_heads)
+
+
+def lora_add(y, x, A, B, ids, scaling=None, splits=None, out=None, workspace=None):
+    """Low-rank adapters of M rows beside a shared projection: y + scaling[a] * (B[a] (A[a] x)), a = ids[m], bf16 [M, N].
+
+    y [M, N] and x [M, K] are bf16 (rows may be strided); A bf16 [adapters, slices * rank, K], B bf16 [adapters, N, rank],
+    ids int32 [M] (-1, or any number outside the adapters: the row keeps y), scaling fp32 [adapters]. A fused projection
+    names its slices in `splits` (q, k, v or gate, up: their sum is N); each slice has its own `rank` rows of A. Rank and K
+    are multiples of 8, rank at most 256. out may be y. Rows that share an adapter read it once for every 16 of them."""
+    load()
+    args = (y, x, A, B, ids, scaling, splits, workspace)
+    if out is None:
+        return torch.ops.paia_gemv.lora_add(*args)
+    torch.ops.paia_gemv.lora_add_out(*args, out)
+    return out

@@ -117,3 +117,36 @@ def test_paged_attention_meta_shapes():
     assert torch.ops.paia_gemv.paged_attention(q, kc, kc, table, lens).shape == q.shape
     out, lse = torch.ops.paia_gemv.paged_attention_lse(q, kc, kc, table, lens)
     assert out.shape == q.shape and lse.shape == (3, 4, 8) and lse.dtype == torch.float32
+
+
+def lora(lib, splits=(64, 32), **change):
+    a = dict(y=A, ys=96, x=A, xs=128, A=A, B=A, ids=A, scaling=None, out=A, os=96, M=4, K=128, rank=16, adapters=3, space=A,
+             bytes=1 << 40, slices=len(splits) if splits else 1)
+    a.update(change)
+    sp = (ctypes.c_int * len(splits))(*splits) if splits else None
+    return lib._lib.paia_lora_add(a["y"], a["ys"], a["x"], a["xs"], a["A"], a["B"], a["ids"], a["scaling"], a["out"],
+                                  a["os"], a["M"], a["K"], a["rank"], sp, a["slices"], a["adapters"], a["space"],
+                                  a["bytes"], None)
+
+
+def test_lora_add_refusals(gemv_lib):
+    for bad in (dict(y=None), dict(y=A + 1), dict(ys=-1), dict(x=A + 8), dict(xs=100), dict(xs=-128), dict(A=None),
+                dict(A=A + 4), dict(B=A + 2), dict(ids=None), dict(ids=A + 2), dict(scaling=A + 2), dict(out=None),
+                dict(out=A + 1), dict(os=95), dict(M=-1), dict(K=0), dict(K=100), dict(rank=0), dict(rank=12),
+                dict(rank=264), dict(adapters=0), dict(slices=0), dict(slices=9, splits=(1,) * 9), dict(splits=None),
+                dict(splits=(64, 0)), dict(splits=(64, -1)), dict(splits=(2 ** 31 - 1, 2 ** 31 - 1)), dict(space=None),
+                dict(space=A + 4), dict(bytes=64)):
+        assert lora(gemv_lib, **bad) == -2, bad
+    assert lora(gemv_lib, M=0) == 0
+    assert gemv_lib._lib.paia_lora_add_workspace(4, 12, 1) == -2
+    assert gemv_lib.lora_add_workspace(1000, 16, 3) == gemv_lib.lora_add_workspace(256, 16, 3)
+    with pytest.raises(RuntimeError, match="-2"):
+        gemv_lib.lora_add_workspace(4, 16, 9)
+
+
+def test_lora_add_meta_shape():
+    from paia_gemv import ops
+    ops.load()
+    e = lambda *s: torch.empty(*s, dtype=torch.bfloat16, device="meta")  # noqa: E731
+    out = torch.ops.paia_gemv.lora_add(e(3, 40), e(3, 64), e(2, 8, 64), e(2, 40, 8), torch.empty(3, device="meta"))
+    assert out.shape == (3, 40) and out.dtype == torch.bfloat16
