@@ -8,18 +8,24 @@
 
 namespace paia {
 
+// n / d for n < 2^31 as one multiplication: with s = ceil(log2 d) and m = ceil(2^(31+s) / d), m d exceeds 2^(31+s) by less
+// than d <= 2^s, so floor(n m / 2^(31+s)) is the quotient; 2 n m >> 32 >> s in 32-bit operations.
+struct Divisor {
+    uint32_t m, s, d;
+    explicit Divisor(uint32_t by = 1) : s(0), d(by)
+    {
+        while ((1ull << s) < by) ++s;
+        m = (uint32_t)(((1ull << (31 + s)) + by - 1) / by);
+    }
+    __device__ __forceinline__ uint32_t of(uint32_t n) const { return __umulhi(2u * n, m) >> s; }
+};
+
 struct CacheView {
     uint8_t *k, *v;
     const float *k_scale, *v_scale;         // fp32 [kv_heads] or null
     int64_t kp, kh, kr, vp, vh, vr;         // strides of page, head and position, in bytes
-    int pages, page_size, page_shift;       // page_shift: log2(page_size), or -1
-    int kv_heads;
-
-    // Pages of a power of two, the usual ones, take a shift where the others take a division (some 30 VALU).
-    __device__ __forceinline__ uint32_t page_of(uint32_t pos) const
-    {
-        return page_shift >= 0 ? pos >> page_shift : pos / (uint32_t)page_size;
-    }
+    int pages, page_size, kv_heads;
+    Divisor by_page;                        // by page_size
 };
 
 // Fills `c` from the caller's description; false where it is outside the contract.
@@ -41,7 +47,7 @@ inline bool cache_view(const paia_kv_cache* d, CacheView* c)
     c->vp = d->v_strides[0] * size, c->vh = d->v_strides[1] * size, c->vr = d->v_strides[2] * size;
     c->pages = d->pages;
     c->page_size = d->page_size;
-    c->page_shift = (d->page_size & (d->page_size - 1)) ? -1 : __builtin_ctz((unsigned)d->page_size);
+    c->by_page = Divisor((uint32_t)d->page_size);
     c->kv_heads = d->kv_heads;
     return true;
 }

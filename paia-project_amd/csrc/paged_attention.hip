@@ -38,7 +38,7 @@ constexpr int kCols = 16;            // columns (token, head) of a unit
 constexpr int kAttnWaves = 4, kAttnBlock = kAttnWaves * kWave;
 // Blocks that a CU holds at the registers a wave takes (one wave of a block on each SIMD).
 constexpr int blocks_per_cu(int dim) { return dim <= 64 ? 3 : dim <= 128 ? 2 : 1; }
-constexpr int kMinTiles = 8;         // a piece is at least this many tiles, where the sequence has them
+constexpr int kMinTiles = 4;         // a piece is at least this many tiles, where the sequence has them
 
 struct AttnParams {
     const uint8_t* q;
@@ -49,89 +49,103 @@ struct AttnParams {
     int64_t table_stride;
     CacheView cache;
     float *part_o, *part_ml;         // [item][kv head][column][D], [item][kv head][column][2]
+    int2* part_of;                   // [sequence]: first item, number of items
     float scale;                     // scale * log2(e)
     int B, T, heads, group, cols, col_groups;
     int window, max_len;             // positions the table can hold
-    int target;                      // pieces aimed at per kv head and column group
+    int goal;                        // pieces per kv head at most, the items of the grid; above B
     int units;                       // items * kv heads
+    Divisor by_kv_heads, by_group, by_col_groups;
 };
 
 // ---- the split of the sequences into pieces -------------------------------------------------------------------------
 struct Span {
-    int len, tile0, tiles;           // positions, first tile seen by any token, number of tiles
+    int len, tile0, tiles;           // positions, first tile seen by any token, number of tiles (below 2^26)
 };
 __device__ __forceinline__ Span span_of(const AttnParams& p, int b)
 {
-    Span s;
-    s.len = min(max(p.lens[b], 0), p.max_len);
-    const int first = p.window > 0 ? max(0, s.len - (p.T - 1) - p.window) : 0;
-    s.tile0 = first / kTile;
-    s.tiles = (int)(((int64_t)s.len + kTile - 1) / kTile) - s.tile0;
+    Span s{0, 0, 0};
+    if (b < p.B) {
+        s.len = min(max(p.lens[b], 0), p.max_len);
+        const int first = p.window > 0 ? max(0, s.len - (p.T - 1) - p.window) : 0;
+        s.tile0 = first / kTile;
+        s.tiles = (s.len + kTile - 1) / kTile - s.tile0;
+    }
     return s;
 }
-__device__ __forceinline__ int64_t wave_sum_i64(int64_t v)
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ uint32_t dpp_add_u32(uint32_t v)
 {
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) v += __shfl_xor(v, d);
-    return v;
+    return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROW_MASK, 0xF, false);
 }
-// Tiles a piece takes at most: the sequences' tiles over the pieces aimed at, less one a sequence for its last, shorter
-// piece. With pieces of this size there are at most max(target, target / 2 + B).
-__device__ __forceinline__ int piece_tiles(const AttnParams& p, const Span& first_chunk)
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v)      // inclusive; lane 63 holds the sum
 {
-    const int lane = lane_id();
-    int64_t total = lane < p.B ? first_chunk.tiles : 0;
-    for (int b = kWave + lane; b < p.B; b += kWave) total += span_of(p, b).tiles;
-    total = wave_sum_i64(total);
-    const int aim = max(p.target - p.B, (p.target + 1) / 2);
-    const int64_t n = (total + aim - 1) / aim;
-    return (int)min((int64_t)(1 << 27), (max(n, (int64_t)kMinTiles) + kAttnWaves - 1) / kAttnWaves * kAttnWaves);
+    v = dpp_add_u32<0x111, 0xF>(v);   // row_shr:1, 2, 4, 8
+    v = dpp_add_u32<0x112, 0xF>(v);
+    v = dpp_add_u32<0x114, 0xF>(v);
+    v = dpp_add_u32<0x118, 0xF>(v);
+    v = dpp_add_u32<0x142, 0xA>(v);   // row_bcast:15 into rows 1, 3
+    return dpp_add_u32<0x143, 0xC>(v);   // row_bcast:31 into rows 2, 3
 }
-// Pieces of a sequence, at least one, and tiles of each but the last.
-__device__ __forceinline__ int pieces_of(int tiles, int most, int* each)
+__device__ __forceinline__ uint32_t last_lane(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, kWave - 1); }
+// Pieces of a sequence at `most` tiles a piece, at least one. The float quotient is within one of the true one (there are
+// at most p.goal pieces, a few thousand) and is corrected.
+__device__ __forceinline__ uint32_t pieces_of(int tiles, int most, float inverse)
 {
-    const int n = max(1, (tiles + most - 1) / most);
-    *each = max(1, (tiles + n - 1) / n);
-    return max(1, (tiles + *each - 1) / *each);
+    int n = (int)((float)tiles * inverse);
+    int left = tiles - n * most;
+    if (left < 0) --n, left += most;
+    if (left >= most) ++n, left -= most;
+    return (uint32_t)max(1, n + (left > 0 ? 1 : 0));
 }
-__device__ __forceinline__ int wave_scan(int v)      // inclusive
+__device__ __forceinline__ int whole_rounds(float tiles)       // the next multiple of the block's waves above `tiles`
 {
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-        const int o = __shfl_up(v, d);
-        if (lane_id() >= d) v += o;
-    }
-    return v;
+    return ((int)tiles / kAttnWaves + 1) * kAttnWaves;
 }
 struct Piece {
-    int b, len, tile0, tile1, count;     // sequence, its length, the piece's tiles, pieces of the sequence
+    int b, len, tile0, tile1;        // sequence, its length, the piece's tiles
+    int index, count;                // number of the piece in its sequence, pieces of the sequence
 };
+// The piece with number `item`. Every wave finds the same tile count per piece, `most`: from the mean over p.goal pieces up,
+// until the sequences' pieces, each sequence's last one shorter, are no more than p.goal.
 __device__ __forceinline__ bool find_piece(const AttnParams& p, int item, Piece* r)
 {
     const int lane = lane_id();
-    Span s{0, 0, 0};
-    if (lane < p.B) s = span_of(p, lane);
-    const int most = piece_tiles(p, s);
-    for (int b0 = 0, before = 0; b0 < p.B; b0 += kWave) {
-        const int b = b0 + lane;
-        if (b0 > 0 && b < p.B) s = span_of(p, b);
-        int each = 1;
-        const int n = b < p.B ? pieces_of(s.tiles, most, &each) : 0;
-        const int end = before + wave_scan(n);
-        const uint64_t here = __ballot(item < end && item >= end - n);
+    Span s = span_of(p, lane);
+    float total = (float)last_lane(wave_scan((uint32_t)s.tiles));
+    for (int b = kWave; b < p.B; b += kWave) total += (float)last_lane(wave_scan((uint32_t)span_of(p, b + lane).tiles));
+    const float per = __builtin_amdgcn_rcpf((float)p.goal);
+    int most = max(kMinTiles, whole_rounds(total * per));
+    float inverse = 0.0f;
+    for (int tries = 0; tries < 5; ++tries) {
+        inverse = __builtin_amdgcn_rcpf((float)most);
+        uint32_t count = last_lane(wave_scan(lane < p.B ? pieces_of(s.tiles, most, inverse) : 0u));
+        for (int b = kWave; b < p.B; b += kWave)
+            count += last_lane(wave_scan(b + lane < p.B ? pieces_of(span_of(p, b + lane).tiles, most, inverse) : 0u));
+        if (count <= (uint32_t)p.goal) break;
+        // the last try holds for any lengths: total / most + B pieces at most (with room for the roundings of `total`)
+        most = tries < 3 ? whole_rounds((float)most * (float)count * per)
+                         : whole_rounds(total * 1.001f * __builtin_amdgcn_rcpf((float)(p.goal - p.B)));
+    }
+    uint32_t before = 0;
+    for (int b0 = 0; b0 < p.B; b0 += kWave) {
+        if (b0 > 0) s = span_of(p, b0 + lane);
+        const uint32_t n = b0 + lane < p.B ? pieces_of(s.tiles, most, inverse) : 0u;
+        const uint32_t end = before + wave_scan(n);
+        const uint64_t here = __ballot((uint32_t)item < end && (uint32_t)item >= end - n);
         if (here != 0) {
             const int src = __builtin_ctzll(here);
-            const int j = item - __builtin_amdgcn_readlane(end - n, src);
             const int tiles = __builtin_amdgcn_readlane(s.tiles, src), t0 = __builtin_amdgcn_readlane(s.tile0, src);
-            each = __builtin_amdgcn_readlane(each, src);
             r->b = b0 + src;
             r->len = __builtin_amdgcn_readlane(s.len, src);
-            r->tile0 = t0 + min(tiles, j * each);
-            r->tile1 = t0 + min(tiles, (j + 1) * each);
-            r->count = __builtin_amdgcn_readlane(n, src);
+            r->count = __builtin_amdgcn_readlane((int)n, src);
+            r->index = item - (__builtin_amdgcn_readlane((int)end, src) - r->count);
+            const int each = tiles / r->count, more = tiles - each * r->count;     // the first `more` pieces get one more
+            r->tile0 = t0 + r->index * each + min(r->index, more);
+            r->tile1 = r->tile0 + each + (r->index < more ? 1 : 0);
             return true;
         }
-        before = __builtin_amdgcn_readlane(end, kWave - 1);
+        before = last_lane(end);
     }
     return false;
 }
@@ -162,6 +176,7 @@ __device__ __forceinline__ f32x4 mfma(const u32x4 a, const u32x4 b, const f32x4 
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 template <int N> struct Words { uint32_t w[N]; };
 template <int N>
 __device__ __forceinline__ Words<N> load_words(const uint8_t* p)
@@ -170,15 +185,15 @@ __device__ __forceinline__ Words<N> load_words(const uint8_t* p)
     if constexpr (N >= 4) {
 #pragma unroll
         for (int i = 0; i < N / 4; ++i) {
-            const u32x4 v = reinterpret_cast<const u32x4*>(p)[i];
+            const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p) + i);
 #pragma unroll
             for (int e = 0; e < 4; ++e) r.w[4 * i + e] = v[e];
         }
     } else if constexpr (N == 2) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        const u32x2 v = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
         r.w[0] = v.x, r.w[1] = v.y;
     } else {
-        r.w[0] = *reinterpret_cast<const uint32_t*>(p);
+        r.w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
     }
     return r;
 }
@@ -211,19 +226,24 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
     __shared__ __attribute__((aligned(16))) uint8_t smem[kAttnWaves * L::kWaveLds];
     __shared__ float stats[kAttnWaves][2][kCols];
     // the column groups of a unit on one XCD, next to each other: they read the same cache rows
-    const int cg = (int)(blockIdx.x / 8) % p.col_groups;
-    const int unit = (int)(blockIdx.x / 8 / p.col_groups) * 8 + (int)(blockIdx.x % 8);
+    int cg = 0, unit = (int)blockIdx.x;
+    if (p.col_groups > 1) {
+        const uint32_t eight = blockIdx.x / 8, of = p.by_col_groups.of(eight);
+        cg = (int)(eight - of * (uint32_t)p.col_groups);
+        unit = (int)(of * 8 + blockIdx.x % 8);
+    }
     if (unit >= p.units) return;
-    const int hkv = p.cache.kv_heads, item = unit / hkv, h = unit % hkv;
+    const int item = (int)p.by_kv_heads.of((uint32_t)unit), h = unit - item * p.cache.kv_heads;
     Piece pc;
     if (!find_piece(p, item, &pc)) return;
+    if (p.part_of != nullptr && pc.index == 0 && h == 0 && cg == 0 && threadIdx.x == 0) p.part_of[pc.b] = int2{item, pc.count};
 
     const int lane = lane_id(), wave = wave_id(), n = lane & 15, g = lane >> 4;
-    const int c0 = cg * kCols, col = c0 + n;
-    const bool live = col < p.cols;
-    const int tok = live ? col / p.group : 0, head = h * p.group + (live ? col % p.group : 0);
+    // columns past the last (of a head group that is no multiple of 16) repeat it, and are not written
+    const int c0 = cg * kCols, col = min(c0 + n, p.cols - 1);
+    const int tok = (int)p.by_group.of((uint32_t)col), head = h * p.group + col - tok * p.group;
     const int hi = pc.len - (p.T - 1 - tok), lo = p.window > 0 ? hi - p.window : 0;   // positions this column sees
-    const int t_first = c0 / p.group, t_last = min(c0 + kCols, p.cols) - 1 >= 0 ? (min(c0 + kCols, p.cols) - 1) / p.group : 0;
+    const int t_first = __builtin_amdgcn_readlane(tok, 0), t_last = __builtin_amdgcn_readlane(tok, kCols - 1);
     // positions that every token of the block sees
     const int all_hi = pc.len - (p.T - 1 - t_first), all_lo = p.window > 0 ? pc.len - (p.T - 1 - t_last) - p.window : 0;
 
@@ -231,7 +251,7 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
     {
         const uint8_t* src = p.q + pc.b * p.qb + tok * p.qt + head * p.qh + 16 * g;
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) q[j] = live ? *reinterpret_cast<const u32x4*>(src + 64 * j) : u32x4{0, 0, 0, 0};
+        for (int j = 0; j < D / 32; ++j) q[j] = *reinterpret_cast<const u32x4*>(src + 64 * j);
     }
     const float score_scale = p.scale * (p.cache.k_scale != nullptr ? p.cache.k_scale[h] : 1.0f);
     const int32_t* table = p.table + pc.b * p.table_stride;
@@ -248,10 +268,10 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
         const uint32_t p0 = (uint32_t)tile * kTile;
 #pragma unroll
         for (int i = 0; i < L::kKPages; ++i)
-            kpage[i] = table[p.cache.page_of(position(p0 + krow + i * L::kKStep, L::kKStep))];
+            kpage[i] = table[p.cache.by_page.of(position(p0 + krow + i * L::kKStep, L::kKStep))];
 #pragma unroll
         for (int i = 0; i < L::kVPages; ++i)
-            vpage[i] = table[p.cache.page_of(position(p0 + 8 * g + i * L::kVStep, L::kVStep))];
+            vpage[i] = table[p.cache.by_page.of(position(p0 + 8 * g + i * L::kVStep, L::kVStep))];
     };
     auto in_cache = [&](int page) { return (uint32_t)page < (uint32_t)p.cache.pages; };
     Words<4> k[L::kKLoads];
@@ -260,7 +280,7 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
 #pragma unroll
         for (int i = 0; i < L::kKPages; ++i) {
             const uint32_t pos = position((uint32_t)tile * kTile + krow + i * L::kKStep, L::kKStep);
-            const uint32_t at = pos - p.cache.page_of(pos) * (uint32_t)p.cache.page_size;
+            const uint32_t at = pos - p.cache.by_page.of(pos) * (uint32_t)p.cache.page_size;
             const uint8_t* row = kbase + (in_cache(kpage[i]) ? kpage[i] : 0) * p.cache.kp + at * p.cache.kr;
 #pragma unroll
             for (int e = 0; e < L::kKStep; ++e) k[i * L::kKStep + e] = load_words<4>(row + e * p.cache.kr);
@@ -273,7 +293,7 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
 #pragma unroll
         for (int i = 0; i < L::kVPages; ++i) {
             const uint32_t pos = position((uint32_t)tile * kTile + 8 * g + i * L::kVStep, L::kVStep);
-            const uint32_t at = pos - p.cache.page_of(pos) * (uint32_t)p.cache.page_size;
+            const uint32_t at = pos - p.cache.by_page.of(pos) * (uint32_t)p.cache.page_size;
             const bool in = in_cache(vpage[i]);
             vrow[i] = vbase + (in ? vpage[i] : 0) * p.cache.vp + at * p.cache.vr;
             if (in) ok |= (P8 ? 0xFFu : 1u) << i;
@@ -448,7 +468,8 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
             if (d == 0) p.part_ml[2 * at] = all, p.part_ml[2 * at + 1] = sum;
             continue;
         }
-        const int64_t row = ((int64_t)pc.b * p.T + c / p.group) * p.heads + h * p.group + c % p.group;
+        const int t = (int)p.by_group.of((uint32_t)c);
+        const int64_t row = ((int64_t)pc.b * p.T + t) * p.heads + h * p.group + c - t * p.group;
         const float f = sum == 0.0f ? 0.0f : v_scale / sum;
         const uint2 y = {pack_bf16x2(acc[0] * f, acc[1] * f), pack_bf16x2(acc[2] * f, acc[3] * f)};
         *reinterpret_cast<uint2*>(p.out + row * D + d) = y;
@@ -457,39 +478,43 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
 }
 
 // Joins the pieces of the sequences that have several: a block per sequence, kv head and column; D/4 lanes hold the output,
-// the block's groups of them take the pieces in turn.
+// the block's groups of them take the pieces in turn, kJoinAhead loads of each in flight.
+constexpr int kJoinAhead = 4;
 template <int D>
 __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
 {
     constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
     __shared__ f32x4 acc_of[kGroups][kLanes];
     __shared__ float m_of[kGroups], l_of[kGroups];
-    const int hkv = p.cache.kv_heads;
-    const int c = (int)(blockIdx.x % (uint32_t)p.cols), h = (int)(blockIdx.x / (uint32_t)p.cols) % hkv;
-    const int b = (int)(blockIdx.x / ((uint32_t)p.cols * (uint32_t)hkv));
-    const int lane = lane_id();
-    Span s{0, 0, 0};
-    if (lane < p.B) s = span_of(p, lane);
-    const int most = piece_tiles(p, s);
-    // pieces of this sequence and of all before it
-    int count, each, before = 0;
-    count = pieces_of(span_of(p, b).tiles, most, &each);
-    if (count == 1) return;
-    for (int i = lane; i < b; i += kWave) before += pieces_of(span_of(p, i).tiles, most, &each);
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) before += __shfl_xor(before, d);
-
+    const int b = (int)blockIdx.x, h = (int)blockIdx.y, c = (int)blockIdx.z, hkv = p.cache.kv_heads;
+    const int2 items = p.part_of[b];
+    if (items.y == 1) return;
     const int grp = (int)threadIdx.x / kLanes, i4 = (int)threadIdx.x % kLanes;
     float m = -INFINITY, l = 0.0f;
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int j = grp; j < count; j += kGroups) {
-        const int64_t at = ((int64_t)(before + j) * hkv + h) * p.cols + c;
-        const f32x4 x = *reinterpret_cast<const f32x4*>(p.part_o + at * D + 4 * i4);
-        const float pm = p.part_ml[2 * at], pl = p.part_ml[2 * at + 1];
-        const float top = fmaxf(m, pm), base = top == -INFINITY ? 0.0f : top;
-        const float fa = __builtin_amdgcn_exp2f(m - base), fb = __builtin_amdgcn_exp2f(pm - base);
-        acc = acc * fa + x * fb;
-        l = l * fa + pl * fb;
+    for (int j = grp; j < items.y; j += kGroups * kJoinAhead) {
+        f32x4 x[kJoinAhead];
+        float pm[kJoinAhead], pl[kJoinAhead];
+#pragma unroll
+        for (int i = 0; i < kJoinAhead; ++i) {
+            const bool in = j + i * kGroups < items.y;
+            const int64_t at = ((int64_t)(items.x + (in ? j + i * kGroups : j)) * hkv + h) * p.cols + c;
+            x[i] = *reinterpret_cast<const f32x4*>(p.part_o + at * D + 4 * i4);
+            pm[i] = p.part_ml[2 * at], pl[i] = p.part_ml[2 * at + 1];
+            if (!in) pm[i] = -INFINITY, pl[i] = 0.0f, x[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < kJoinAhead; ++i) top = fmaxf(top, pm[i]);
+        const float base = top == -INFINITY ? 0.0f : top, fade = __builtin_amdgcn_exp2f(m - base);
+        acc *= fade;
+        l *= fade;
+#pragma unroll
+        for (int i = 0; i < kJoinAhead; ++i) {
+            const float f = __builtin_amdgcn_exp2f(pm[i] - base);
+            acc += x[i] * f;
+            l += pl[i] * f;
+        }
         m = top;
     }
     acc_of[grp][i4] = acc;
@@ -507,7 +532,8 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
         sum += f * l_of[w];
         acc += f * acc_of[w][i4];
     }
-    const int64_t row = ((int64_t)b * p.T + c / p.group) * p.heads + h * p.group + c % p.group;
+    const int t = (int)p.by_group.of((uint32_t)c);
+    const int64_t row = ((int64_t)b * p.T + t) * p.heads + h * p.group + c - t * p.group;
     const float f = sum == 0.0f ? 0.0f : (p.cache.v_scale != nullptr ? p.cache.v_scale[h] : 1.0f) / sum;
     const uint2 y = {pack_bf16x2(acc[0] * f, acc[1] * f), pack_bf16x2(acc[2] * f, acc[3] * f)};
     *reinterpret_cast<uint2*>(p.out + row * D + 4 * i4) = y;
@@ -524,22 +550,27 @@ static bool attention_plan(const paia_kv_cache* c, int table_width, int B, int T
     const int64_t cols = (int64_t)T * p->group, max_len = (int64_t)table_width * c->page_size;
     // tile numbers times 32, with a tile to spare, stay within 31 bits
     p->max_len = (int)(max_len < INT_MAX - 4096 ? max_len : INT_MAX - 4096);
-    if (cols > INT_MAX / 2) return false;
+    if (cols > 65535 || c->kv_heads > 65535) return false;      // dimensions of the joining grid
     p->cols = (int)cols;
     p->col_groups = (p->cols + kCols - 1) / kCols;
     const int64_t wide = (int64_t)c->kv_heads * p->col_groups, slots = (int64_t)device_facts().cus * blocks_per_cu(c->head_dim);
     int64_t target = slots / wide;
-    target = target < 1 ? 1 : target;
-    // pieces per sequence that the table's width allows, and the bound of piece_tiles
+    target = target < 2 ? 2 : target;
+    // One round of blocks where the sequences are few; many sequences have a piece of their own each, and as many more as
+    // half a round.
+    const int64_t goal = B <= target / 2 ? target : target / 2 + B;
+    // pieces per sequence that the table's width allows
     const int64_t per_seq = ((int64_t)p->max_len / kTile + 1 + kMinTiles - 1) / kMinTiles;
-    int64_t items = target > (target + 1) / 2 + B ? target : (target + 1) / 2 + B;
-    if (items > per_seq * B) items = per_seq * B;
-    p->target = (int)target;
+    const int64_t items = goal < per_seq * B ? goal : per_seq * B;
     const int64_t units = items * c->kv_heads, blocks = (units + 7) / 8 * 8 * p->col_groups;
-    if (blocks > INT_MAX || (int64_t)B * c->kv_heads * p->cols > INT_MAX) return false;
+    if (blocks > INT_MAX || goal > INT_MAX) return false;
+    p->goal = (int)goal;
     p->units = (int)units;
+    p->by_kv_heads = Divisor((uint32_t)c->kv_heads);
+    p->by_group = Divisor((uint32_t)p->group);
+    p->by_col_groups = Divisor((uint32_t)p->col_groups);
     // one piece a sequence at most: nothing is joined
-    *bytes = per_seq <= 1 ? 0 : units * p->cols * (c->head_dim + 2) * (int64_t)sizeof(float);
+    *bytes = per_seq <= 1 ? 0 : units * p->cols * (c->head_dim + 2) * (int64_t)sizeof(float) + B * (int64_t)sizeof(int2);
     return true;
 }
 
@@ -553,7 +584,7 @@ static int launch_attention(const AttnParams& p, bool fp8, bool join, hipStream_
     else p8 ? go(paged_attention_kernel<D, false, true>) : go(paged_attention_kernel<D, false, false>);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return (int)e;
     if (join) {
-        hipLaunchKernelGGL((attention_join_kernel<D>), dim3((uint32_t)(p.B * p.cache.kv_heads * p.cols)), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((attention_join_kernel<D>), dim3((uint32_t)p.B, (uint32_t)p.cache.kv_heads, (uint32_t)p.cols), dim3(256), 0, st, p);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return (int)e;
     }
     return 0;
@@ -596,6 +627,7 @@ int paia_paged_attention(const void* q, const long long* q_strides, const paia_k
     p.window = window >= (int64_t)p.max_len + T ? 0 : window;    // it hides nothing
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = p.part_o + (int64_t)p.units * p.cols * cache->head_dim;
+    p.part_of = bytes > 0 ? reinterpret_cast<int2*>(p.part_ml + (int64_t)p.units * p.cols * 2) : nullptr;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     switch (cache->head_dim) {
     case 64: return launch_attention<64>(p, cache->fp8, bytes > 0, st);

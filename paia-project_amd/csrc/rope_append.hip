@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kRopeBlock) rope_append_kernel(const RopeParam
     }
     const int64_t slot = p.slots[m];
     if (slot < 0 || slot >= (int64_t)p.cache.pages * p.cache.page_size) return;
-    const int64_t page = p.cache.page_shift >= 0 ? slot >> p.cache.page_shift : slot / p.cache.page_size;
+    const int64_t page = slot >> 31 == 0 ? (int64_t)p.cache.by_page.of((uint32_t)slot) : slot / p.cache.page_size;
     const int64_t at = slot - page * p.cache.page_size;
     const int h = head - p.heads - (is_v ? hkv : 0);
     const float* scale = is_v ? p.cache.v_scale : p.cache.k_scale;
