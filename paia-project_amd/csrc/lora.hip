@@ -16,6 +16,7 @@
 #include <stdint.h>
 
 #include "gemv_kernel.h"
+#include "kv_cache.h"
 #include "paia_gemv.h"
 
 namespace paia {
@@ -24,9 +25,9 @@ constexpr int kLoraBlock = 256, kLoraWaves = kLoraBlock / kWave;
 constexpr int kLoraRows = 256;           // rows of a launch
 constexpr int kChunk = 16;               // rows that share a pass over an adapter
 constexpr int kMaxSlices = 8, kMaxPieces = 8;
-constexpr int kShrinkUnits = 512;        // blocks aimed at by the first product's split of K
-constexpr int kShrinkAhead = 4;          // steps of K whose loads a wave has in flight
-constexpr int kTilesPerWave = 4;         // tiles of 16 outputs a wave takes of a unit
+constexpr int kShrinunits = 512;        // blocks aimed at by the first product's split of K
+constexpr int kShrinkCols = 64;          // columns of K a wave takes at a time
+constexpr int kShrinkAhead = 3;          // such steps whose loads a wave has in flight
 
 struct LoraParams {
     const uint16_t *x, *A, *B, *y;
@@ -38,6 +39,7 @@ struct LoraParams {
     int M, K, N, R, adapters, slices, h_rows, h_stride;     // h_rows: slices * R; h_stride: that rounded up to 16
     int first[kMaxSlices + 1];           // first output of each slice, N at the end
     int unit_first[kMaxSlices + 1];      // first expand unit of each slice within a chunk
+    Divisor by_row;                      // by R / 8, the 16-byte pieces of a row of B
     bool wide;                           // out and y take 8-byte accesses
 };
 
@@ -90,7 +92,7 @@ __device__ __forceinline__ int k_pieces(const LoraParams& p, int chunks)
 {
     const int units = chunks * (p.h_stride / 16);
     const int most = min(kMaxPieces, (p.K + 255) / 256);
-    return max(1, min(most, kShrinkUnits / units));
+    return max(1, min(most, kShrinunits / units));
 }
 
 __device__ __forceinline__ f32x4 lora_mfma(const u32x4 a, const u32x4 b, const f32x4 c)
@@ -108,39 +110,72 @@ __device__ __forceinline__ float rest(float v, uint32_t rounded)
     return fabsf(__uint_as_float(rounded)) < 3.4e38f ? v - __uint_as_float(rounded) : 0.0f;
 }
 
-// h: a unit is (chunk, 16 rows of A, piece of K); the block's waves take its steps of 32 columns in turn.
+__device__ __forceinline__ void lora_lds_order()     // a wave's LDS operations stay in order; the compiler has to keep them so
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// h: a unit is (chunk, 16 rows of A, piece of K); the block's waves take its steps of 64 columns in turn. Eight lanes load
+// 128 bytes of a row, of A and of x alike; a wave-private piece of LDS brings both into the matrix layout (row n at piece
+// c ^ n / 2: the 16 rows of a read cover all banks).
 __global__ void __launch_bounds__(kLoraBlock) lora_shrink_kernel(const LoraParams p)
 {
     __shared__ RowChunks rows;
+    __shared__ u32x4 stage[kLoraWaves][2][kChunk * 8];
     __shared__ f32x4 sums[kLoraWaves][kWave];
     row_chunks(p, &rows);
-    const int tiles = p.h_stride / 16, pieces = k_pieces(p, rows.count), steps = (p.K + 31) / 32;
+    const int tiles = p.h_stride / 16, pieces = k_pieces(p, rows.count), steps = (p.K + kShrinkCols - 1) / kShrinkCols;
     const int lane = lane_id(), wave = wave_id(), n = lane & 15, g = lane >> 4;
+    const int lr = lane >> 3, lc = lane & 7;      // row (and that plus 8) and piece of a row that the lane loads
     for (int unit = (int)blockIdx.x; unit < rows.count * tiles * pieces; unit += (int)gridDim.x) {
         const int piece = unit % pieces, tile = unit / pieces % tiles, chunk = unit / pieces / tiles;
         const int start = rows.start[chunk], held = rows.start[chunk + 1] - start;
-        const int m = rows.order[start + min(n, held - 1)], id = rows.key[rows.order[start]];
+        const int id = rows.key[rows.order[start]];
         if (id == INT_MAX) break;        // the last chunks: rows without an adapter
-        const int r = tile * 16 + n;
-        const uint16_t* a = p.A + ((int64_t)id * p.h_rows + min(r, p.h_rows - 1)) * p.K + 8 * g;
-        const uint16_t* x = p.x + m * p.x_stride + 8 * g;
         const int s0 = (int)((int64_t)steps * piece / pieces), s1 = (int)((int64_t)steps * (piece + 1) / pieces);
+        const uint16_t *a[2], *x[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            a[i] = p.A + ((int64_t)id * p.h_rows + min(tile * 16 + 8 * i + lr, p.h_rows - 1)) * p.K + 8 * lc;
+            x[i] = p.x + rows.order[start + min(8 * i + lr, held - 1)] * p.x_stride + 8 * lc;
+        }
+        u32x4 u[kShrinkAhead][2], v[kShrinkAhead][2];
+        auto load = [&](int s, int at) {          // a step past the piece's end loads nothing and adds nothing
+            const bool in = s < s1 && kShrinkCols * s + 8 * lc < p.K;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                u[at][i] = load16_if(a[i] + kShrinkCols * (int64_t)s, in);
+                v[at][i] = load16_if(x[i] + kShrinkCols * (int64_t)s, in && 8 * i < held);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < kShrinkAhead; ++i) load(s0 + wave + i * kLoraWaves, i);
         f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int s = s0 + wave; s < s1; s += kShrinkAhead * kLoraWaves) {
-            u32x4 u[kShrinkAhead], v[kShrinkAhead];
 #pragma unroll
             for (int i = 0; i < kShrinkAhead; ++i) {
-                const int at = s + i * kLoraWaves;
-                const bool in = at < s1 && 32 * at + 8 * g < p.K;
-                u[i] = load16_if(a + 32 * at, in && r < p.h_rows);
-                v[i] = load16_if(x + 32 * at, in && n < held);
-            }
 #pragma unroll
-            for (int i = 0; i < kShrinkAhead; ++i) acc = lora_mfma(u[i], v[i], acc);
+                for (int e = 0; e < 2; ++e) {
+                    const int r = 8 * e + lr, at = r * 8 + (lc ^ (r >> 1));
+                    stage[wave][0][at] = u[i][e];
+                    stage[wave][1][at] = v[i][e];
+                }
+                lora_lds_order();
+                load(s + (kShrinkAhead + i) * kLoraWaves, i);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int at = n * 8 + ((4 * j + g) ^ (n >> 1));
+                    acc = lora_mfma(stage[wave][0][at], stage[wave][1][at], acc);
+                }
+                lora_lds_order();
+            }
         }
         sums[wave][lane] = acc;
         __syncthreads();
         if (wave == 0 && n < held) {
+            const int m = rows.order[start + n];
 #pragma unroll
             for (int w = 1; w < kLoraWaves; ++w) acc += sums[w][lane];
             *reinterpret_cast<f32x4*>(p.part + ((int64_t)piece * p.M + m) * p.h_stride + tile * 16 + 4 * g) = acc;
@@ -149,14 +184,22 @@ __global__ void __launch_bounds__(kLoraBlock) lora_shrink_kernel(const LoraParam
     }
 }
 
-// out: a unit is (chunk, slice, kLoraWaves * kTilesPerWave tiles of 16 outputs of the slice). STEPS: 32-value steps of R.
+// out: a unit is (chunk, slice, kLoraWaves * ROWS outputs of the slice). STEPS: 32-value steps of R. A wave's ROWS rows of B
+// are contiguous memory, ROWS R / 8 pieces of 16 bytes, loaded as such and brought into the matrix layout through its own
+// piece of LDS (rows an odd number of pieces apart: no bank conflicts). The block sums the pieces of h for its chunk once.
+constexpr int expand_rows(int steps) { return steps <= 2 ? 64 : steps <= 4 ? 32 : 16; }
 template <int STEPS, bool WIDE>
 __global__ void __launch_bounds__(kLoraBlock) lora_expand_kernel(const LoraParams p)
 {
+    constexpr int ROWS = expand_rows(STEPS), kTiles = ROWS / 16, kLoads = ROWS * STEPS * 4 / kWave;
+    constexpr int kHPitch = STEPS * 4 + 1, kBPitch = STEPS * 4 + 1;      // 16-byte pieces
     __shared__ RowChunks rows;
+    __shared__ u32x4 h_of[2][kChunk * kHPitch];
+    __shared__ u32x4 b_of[kLoraWaves][ROWS * kBPitch];
     row_chunks(p, &rows);
     const int pieces = k_pieces(p, rows.count), per_chunk = p.unit_first[p.slices];
     const int lane = lane_id(), wave = wave_id(), n = lane & 15, g = lane >> 4;
+    const int row_pieces = p.R / 8, pitch = row_pieces | 1;
     for (int unit = (int)blockIdx.x; unit < rows.count * per_chunk; unit += (int)gridDim.x) {
         const int chunk = unit / per_chunk, u = unit % per_chunk;
         int slice = 0;
@@ -166,64 +209,95 @@ __global__ void __launch_bounds__(kLoraBlock) lora_expand_kernel(const LoraParam
         const bool live = n < held, bare = id == INT_MAX;
         if (bare && p.out == p.y && p.out_stride == p.y_stride) continue;
         const int end = p.first[slice + 1];
-        const int n0 = p.first[slice] + ((u - p.unit_first[slice]) * kLoraWaves + wave) * kTilesPerWave * 16;
-        if (n0 >= end) continue;
+        const int n0 = p.first[slice] + ((u - p.unit_first[slice]) * kLoraWaves + wave) * ROWS;
+        const int count = min(ROWS, end - n0);         // outputs of this wave, none where it is not positive
 
-        u32x4 b[kTilesPerWave][STEPS];
-        const uint16_t* B = p.B + ((int64_t)(bare ? 0 : id) * p.N) * p.R;
+        u32x4 b[kLoads];
+        const u32x4* B = reinterpret_cast<const u32x4*>(p.B + ((int64_t)(bare ? 0 : id) * p.N + n0) * p.R);
 #pragma unroll
-        for (int t = 0; t < kTilesPerWave; ++t)
-#pragma unroll
-            for (int s = 0; s < STEPS; ++s) {
-                const int row = n0 + 16 * t + n, r = 32 * s + 8 * g;
-                b[t][s] = load16_if(B + (int64_t)min(row, end - 1) * p.R + r, !bare && row < end && r < p.R);
-            }
-        // the lane's values of h: the pieces' sums in order, times the adapter's factor, as value and remainder
-        u32x4 hi[STEPS], lo[STEPS];
-        const float factor = bare || p.scaling == nullptr ? 1.0f : p.scaling[id];
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            const int r = 32 * s + 8 * g;
-            float h[8] = {};
-            if (live && !bare && r < p.R) {
-                const float* src = p.part + (int64_t)m * p.h_stride + slice * p.R + r;
-                for (int i = 0; i < pieces; ++i, src += (int64_t)p.M * p.h_stride) {
-                    const f32x4 u0 = reinterpret_cast<const f32x4*>(src)[0], u1 = reinterpret_cast<const f32x4*>(src)[1];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) h[e] += u0[e], h[4 + e] += u1[e];
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float v = h[2 * e] * factor, w = h[2 * e + 1] * factor;
-                hi[s][e] = pack_bf16x2(v, w);
-                lo[s][e] = pack_bf16x2(rest(v, hi[s][e] << 16), rest(w, hi[s][e] & 0xFFFF0000u));
-            }
+        for (int i = 0; i < kLoads; ++i) {
+            const int at = i * kWave + lane;
+            b[i] = !bare && at < count * row_pieces ? B[at] : u32x4{0, 0, 0, 0};
         }
         const uint16_t* y = p.y + m * p.y_stride;
         uint16_t* out = p.out + m * p.out_stride;
+        uint2 was[kTiles];
 #pragma unroll
-        for (int t = 0; t < kTilesPerWave; ++t) {
+        for (int t = 0; t < kTiles; ++t) {
+            const int at = 16 * t + 4 * g;
+            was[t] = uint2{0, 0};
+            if (!live || at >= count) continue;
+            if (WIDE && at + 4 <= count) {
+                was[t] = *reinterpret_cast<const uint2*>(y + n0 + at);
+            } else {
+                const uint16_t* from = y + n0 + at;
+                was[t].x = from[0] | (at + 1 < count ? (uint32_t)from[1] << 16 : 0u);
+                was[t].y = at + 2 < count ? from[2] | (at + 3 < count ? (uint32_t)from[3] << 16 : 0u) : 0u;
+            }
+        }
+        if (!bare) {
+            // the chunk's values of this slice of h: the pieces' sums in order, times the adapter's factor, as bf16 value
+            // and remainder
+            const float factor = p.scaling == nullptr ? 1.0f : p.scaling[id];
+            for (int e = (int)threadIdx.x; e < held * (p.R / 4); e += kLoraBlock) {
+                const int c4 = e / held, r = e - c4 * held;
+                const float* src = p.part + (int64_t)rows.order[start + r] * p.h_stride + slice * p.R + 4 * c4;
+                f32x4 term[kMaxPieces], h = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < kMaxPieces; ++i)
+                    term[i] = i < pieces ? *reinterpret_cast<const f32x4*>(src + (int64_t)i * p.M * p.h_stride)
+                                         : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < kMaxPieces; ++i) h += term[i];
+                h *= factor;
+                const uint2 hi = {pack_bf16x2(h[0], h[1]), pack_bf16x2(h[2], h[3])};
+                const uint2 lo = {pack_bf16x2(rest(h[0], hi.x << 16), rest(h[1], hi.x & 0xFFFF0000u)),
+                                  pack_bf16x2(rest(h[2], hi.y << 16), rest(h[3], hi.y & 0xFFFF0000u))};
+                reinterpret_cast<uint2*>(h_of[0])[r * (2 * kHPitch) + c4] = hi;
+                reinterpret_cast<uint2*>(h_of[1])[r * (2 * kHPitch) + c4] = lo;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const uint32_t at = (uint32_t)(i * kWave + lane), r = p.by_row.of(at);
+            if (r < (uint32_t)ROWS) b_of[wave][r * pitch + at - r * row_pieces] = b[i];
+        }
+        lora_lds_order();
+        u32x4 hi[STEPS], lo[STEPS];
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const bool in = !bare && 4 * s + g < row_pieces;
+            hi[s] = in ? h_of[0][min(n, held - 1) * kHPitch + 4 * s + g] : u32x4{0, 0, 0, 0};
+            lo[s] = in ? h_of[1][min(n, held - 1) * kHPitch + 4 * s + g] : u32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
             f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) {
-                acc = lora_mfma(b[t][s], lo[s], acc);
-                acc = lora_mfma(b[t][s], hi[s], acc);
+                const u32x4 w = 4 * s + g < row_pieces ? b_of[wave][(16 * t + n) * pitch + 4 * s + g] : u32x4{0, 0, 0, 0};
+                acc = lora_mfma(w, lo[s], acc);
+                acc = lora_mfma(w, hi[s], acc);
             }
-            const int at = n0 + 16 * t + 4 * g;
-            if (!live || at >= end) continue;
-            if (WIDE && at + 4 <= end) {
-                uint2 v = *reinterpret_cast<const uint2*>(y + at);
-                v.x = bare ? v.x : pack_bf16x2(bf16_to_f32(v.x & 0xFFFFu) + acc[0], __uint_as_float(v.x & 0xFFFF0000u) + acc[1]);
-                v.y = bare ? v.y : pack_bf16x2(bf16_to_f32(v.y & 0xFFFFu) + acc[2], __uint_as_float(v.y & 0xFFFF0000u) + acc[3]);
-                *reinterpret_cast<uint2*>(out + at) = v;
+            const int at = 16 * t + 4 * g;
+            if (!live || at >= count) continue;
+            uint2 v = was[t];
+            if (!bare) {
+                v.x = pack_bf16x2(bf16_to_f32(v.x & 0xFFFFu) + acc[0], __uint_as_float(v.x & 0xFFFF0000u) + acc[1]);
+                v.y = pack_bf16x2(bf16_to_f32(v.y & 0xFFFFu) + acc[2], __uint_as_float(v.y & 0xFFFF0000u) + acc[3]);
+            }
+            uint16_t* to = out + n0 + at;
+            if (WIDE && at + 4 <= count) {
+                *reinterpret_cast<uint2*>(to) = v;
             } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (at + e < end)
-                        out[at + e] = bare ? y[at + e] : (uint16_t)f32_to_bf16_out(bf16_to_f32(y[at + e]) + acc[e]);
+                to[0] = (uint16_t)v.x;
+                if (at + 1 < count) to[1] = (uint16_t)(v.x >> 16);
+                if (at + 2 < count) to[2] = (uint16_t)v.y;
+                if (at + 3 < count) to[3] = (uint16_t)(v.y >> 16);
             }
         }
+        __syncthreads();
     }
 }
 
@@ -270,15 +344,15 @@ int paia_lora_add(const void* y, long long y_stride, const void* x, long long x_
     if (!lora_sizes(M, rank, slices) || K <= 0 || K % 8 || adapters <= 0 || splits == nullptr) return -2;
     LoraParams p;
     int64_t N = 0, units = 0;
-    constexpr int kUnit = kLoraWaves * kTilesPerWave * 16;
+    const int unit = kLoraWaves * expand_rows((rank + 31) / 32);
     p.wide = true;
     for (int j = 0; j < slices; ++j) {
         if (splits[j] <= 0) return -2;
         p.first[j] = (int)N, p.unit_first[j] = (int)units;
-        N += splits[j], units += ((int64_t)splits[j] + kUnit - 1) / kUnit;
+        N += splits[j], units += ((int64_t)splits[j] + unit - 1) / unit;
         p.wide = p.wide && p.first[j] % 4 == 0;
         // outputs and units of a launch are counted in 31 bits
-        if (N > INT_MAX - kUnit || units * kLoraRows > INT_MAX) return -2;
+        if (N > INT_MAX - unit || units * kLoraRows > INT_MAX) return -2;
     }
     p.first[slices] = (int)N, p.unit_first[slices] = (int)units;
     if (M == 0) return 0;
@@ -294,6 +368,7 @@ int paia_lora_add(const void* y, long long y_stride, const void* x, long long x_
     p.part = static_cast<float*>(workspace);
     p.x_stride = x_stride, p.y_stride = y_stride, p.out_stride = out_stride;
     p.K = K, p.N = (int)N, p.R = rank, p.adapters = adapters, p.slices = slices;
+    p.by_row = Divisor((uint32_t)(rank / 8));
     p.h_rows = slices * rank, p.h_stride = (p.h_rows + 15) / 16 * 16;
     for (int m = 0; m < M; m += kLoraRows) {
         p.M = M - m < kLoraRows ? M - m : kLoraRows;
