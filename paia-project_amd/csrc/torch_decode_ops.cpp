@@ -265,7 +265,7 @@ void lora_add_out(const at::Tensor& y, const at::Tensor& x, const at::Tensor& A,
     TORCH_CHECK(sum == N, "splits must sum to N (", N, "), found ", sum);
     TORCH_CHECK(A.size(1) == slices * R, "A must hold rank rows (", R, ") for each of ", slices, " slices");
     c10::DeviceGuard g(A.device());
-    const long long need = paia_lora_add_workspace(to_int(M, "M"), to_int(R, "rank"), slices);
+    const long long need = paia_lora_add_workspace(to_int(M, "M"), to_int(K, "K"), to_int(R, "rank"), parts, slices);
     check_rc(need < 0 ? (int)need : 0, "paia_lora_add");
     at::Tensor space;
     if (workspace.has_value()) {
@@ -273,13 +273,14 @@ void lora_add_out(const at::Tensor& y, const at::Tensor& x, const at::Tensor& A,
                     "workspace must be contiguous and hold ", need, " bytes");
         on_device_of(A, *workspace, "workspace");
         space = *workspace;
-    } else {
+    } else if (need > 0) {
         space = at::empty({need}, A.options().dtype(at::kByte));
     }
     check_rc(paia_lora_add(y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), A.data_ptr(), B.data_ptr(), ids.data_ptr(),
                            opt_ptr(scaling, at::kFloat, L, A, "scaling"), out.data_ptr(), out.stride(0), (int)M,
-                           to_int(K, "K"), (int)R, parts, slices, to_int(L, "adapters"), space.data_ptr(),
-                           (long long)space.nbytes(), stream_of(A)),
+                           (int)K, (int)R, parts, slices, to_int(L, "adapters"),
+                           space.defined() ? space.data_ptr() : nullptr,
+                           space.defined() ? (long long)space.nbytes() : 0, stream_of(A)),
              "paia_lora_add");
 }
 at::Tensor lora_add(const at::Tensor& y, const at::Tensor& x, const at::Tensor& A, const at::Tensor& B,

@@ -103,7 +103,7 @@ class GemvLib:
         lib.paia_paged_attention_workspace.restype = _L
         lib.paia_paged_attention_workspace.argtypes = [ctypes.POINTER(KVCache), _I, _I, _I, _I]
         lib.paia_lora_add_workspace.restype = _L
-        lib.paia_lora_add_workspace.argtypes = [_I, _I, _I]
+        lib.paia_lora_add_workspace.argtypes = [_I, _I, _I, ctypes.POINTER(_I), _I]
         lib.paia_gemv_build_info.restype = ctypes.c_char_p
         lib.paia_gemv_build_info.argtypes = []
         self.variants_fp8 = self._qvariants(lib, "fp8")
@@ -289,9 +289,9 @@ class GemvLib:
                                                    lens_ptr, scale, window, out_ptr, lse_ptr, B, T, heads, workspace_ptr,
                                                    workspace_bytes, self._st(stream)), "paia_paged_attention")
 
-    def lora_add_workspace(self, M, rank, slices):
-        """Bytes of device memory that lora_add takes as its workspace."""
-        need = self._lib.paia_lora_add_workspace(M, rank, slices)
+    def lora_add_workspace(self, M, K, rank, splits):
+        """Bytes of device memory that lora_add takes as its workspace (0 for few rows of a low rank)."""
+        need = self._lib.paia_lora_add_workspace(M, K, rank, (_I * len(splits))(*splits), len(splits))
         self._check(min(need, 0), "paia_lora_add_workspace")
         return need
 

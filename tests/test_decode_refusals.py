@@ -120,7 +120,7 @@ def test_paged_attention_meta_shapes():
 
 
 def lora(lib, splits=(64, 32), **change):
-    a = dict(y=A, ys=96, x=A, xs=128, A=A, B=A, ids=A, scaling=None, out=A, os=96, M=4, K=128, rank=16, adapters=3, space=A,
+    a = dict(y=A, ys=96, x=A, xs=128, A=A, B=A, ids=A, scaling=None, out=A, os=96, M=4, K=128, rank=40, adapters=3, space=A,
              bytes=1 << 40, slices=len(splits) if splits else 1)
     a.update(change)
     sp = (ctypes.c_int * len(splits))(*splits) if splits else None
@@ -138,10 +138,12 @@ def test_lora_add_refusals(gemv_lib):
                 dict(space=A + 4), dict(bytes=64)):
         assert lora(gemv_lib, **bad) == -2, bad
     assert lora(gemv_lib, M=0) == 0
-    assert gemv_lib._lib.paia_lora_add_workspace(4, 12, 1) == -2
-    assert gemv_lib.lora_add_workspace(1000, 16, 3) == gemv_lib.lora_add_workspace(256, 16, 3)
-    with pytest.raises(RuntimeError, match="-2"):
-        gemv_lib.lora_add_workspace(4, 16, 9)
+    need = gemv_lib.lora_add_workspace
+    assert need(1000, 512, 40, [64, 32]) == need(256, 512, 40, [64, 32]) > need(4, 512, 40, [64, 32]) > 0
+    assert need(1, 4096, 16, [4096, 1024, 1024]) == 0            # one launch, nothing kept
+    for bad in ((4, 512, 12, [64]), (4, 512, 16, [64] * 9), (-1, 512, 16, [64]), (4, 100, 16, [64]), (4, 512, 16, [64, 0])):
+        with pytest.raises(RuntimeError, match="-2"):
+            need(*bad)
 
 
 def test_lora_add_meta_shape():

@@ -55,9 +55,10 @@ def test_ranks_and_slices(cuda, rank, splits):
 def test_row_counts(cuda, M):
     """Chunks of sixteen rows, launches of 256; every row its own adapter, all the same, two, and none."""
     for ids in (list(range(M)), [3] * M, [m % 2 for m in range(M)], [-1] * M, [m if m % 3 else -1 for m in range(M)]):
-        note(f"lora M={M} ids={ids[:3]}..")
-        o = operands(M, 264, [100], 16, max(M, 4), seed=M, ids=ids)
-        check(o, call(o, cuda, None), [100])
+        for rank in (16, 40):
+            note(f"lora M={M} rank={rank} ids={ids[:3]}..")
+            o = operands(M, 264, [100], rank, max(M, 4), seed=M, ids=ids)
+            check(o, call(o, cuda, None), [100])
 
 
 def test_long_rows(cuda):
@@ -68,15 +69,17 @@ def test_long_rows(cuda):
 
 
 def test_ids_outside_and_no_scaling(cuda):
-    o = operands(6, 128, [96], 8, 3, ids=[-1, 3, 2 ** 31 - 1, -2 ** 31, 2, 0])
-    o["scaling"] = None
-    check(o, call(o, cuda, None), [96])
+    for rank in (8, 40):
+        o = operands(6, 128, [96], rank, 3, ids=[-1, 3, 2 ** 31 - 1, -2 ** 31, 2, 0])
+        o["scaling"] = None
+        check(o, call(o, cuda, None), [96])
 
 
-def test_in_place_strided_and_workspace(cuda):
+@pytest.mark.parametrize("rank", [24, 40])     # the form for few rows of low ranks, and the other
+def test_in_place_strided_and_workspace(cuda, rank):
     """out = y in place, y, x and out as parts of wider tensors (even and odd offsets), a caller's workspace of NaN."""
     splits = [70, 58]
-    o = operands(9, 256, splits, 24, 3)
+    o = operands(9, 256, splits, rank, 3)
     want = call(o, cuda, splits)
     d = {k: v.to(cuda) for k, v in o.items()}
     args = (d["x"], d["A"], d["B"], d["ids"])
@@ -89,15 +92,16 @@ def test_in_place_strided_and_workspace(cuda):
         part.copy_(d["y"])
         xw = torch.full((9, 512), float("nan"), dtype=torch.bfloat16, device=cuda)
         xw[:, 16:272] = d["x"]
-        space = torch.full((load_lib().lora_add_workspace(9, 24, 2) // 4,), float("nan"), device=cuda)
+        space = torch.full((load_lib().lora_add_workspace(9, 256, rank, splits) // 4,), float("nan"), device=cuda)
         ops.lora_add(part, xw[:, 16:272], *args[1:], scaling=d["scaling"], splits=splits, out=part, workspace=space)
         torch.cuda.synchronize()
         assert torch.equal(bits(part), bits(want)) and wide[:, :left].isnan().all() and wide[:, left + 128:].isnan().all()
 
 
-def test_not_finite_values_stay_in_their_rows(cuda):
+@pytest.mark.parametrize("rank", [16, 40])
+def test_not_finite_values_stay_in_their_rows(cuda, rank):
     """NaN and infinities in one row's x, in one adapter and in an adapter that nobody uses."""
-    o = operands(20, 96, [80], 16, 4, ids=[0] * 10 + [1] * 10)
+    o = operands(20, 96, [80], rank, 4, ids=[0] * 10 + [1] * 10)
     want = call(o, cuda, None).cpu()
     o["A"][2], o["B"][3] = float("nan"), float("inf")
     o["x"][4, 7], o["x"][15, 0] = float("nan"), float("inf")
@@ -107,16 +111,21 @@ def test_not_finite_values_stay_in_their_rows(cuda):
     assert torch.equal(bits(got[rows]), bits(want[rows]))
 
 
-def test_an_infinite_product_is_infinite(cuda):
+@pytest.mark.parametrize("rank", [8, 40])
+def test_an_infinite_product_is_infinite(cuda, rank):
     """h beyond fp32's range: the remainder term must not turn the infinity into NaN."""
-    o = operands(1, 8, [16], 8, 1, ids=[0])
+    o = operands(1, 8, [16], rank, 1, ids=[0])
     o["A"][:], o["x"][:], o["B"][:] = 1e30, 1e30, 0.5
     assert (call(o, cuda, None).cpu().float() == float("inf")).all()
 
 
 def test_offsets_beyond_32_bits(cuda):
-    """The last of adapters that fill 5 GiB of A and 5 of B."""
-    K, N, R = 4096, 4096, 64
+    """The last of adapters that fill 5 GiB of A and 5 of B, in both forms."""
+    for R in (64, 16):
+        far_adapters(cuda, 4096, 4096, R)
+
+
+def far_adapters(cuda, K, N, R):
     L = 5 * 2 ** 30 // (R * K * 2)
     o = operands(3, K, [N], R, 2, ids=[1, 0, 1])
     want = call(o, cuda, None)
@@ -130,10 +139,11 @@ def test_offsets_beyond_32_bits(cuda):
     assert torch.equal(bits(got), bits(want))
 
 
-def test_graph_follows_the_ids(cuda):
+@pytest.mark.parametrize("rank", [16, 40])
+def test_graph_follows_the_ids(cuda, rank):
     """One captured call replayed with other requests in its rows, eager work between the replays."""
     splits = [200, 56]
-    o = operands(8, 512, splits, 16, 5)
+    o = operands(8, 512, splits, rank, 5)
     d = {k: v.to(cuda) for k, v in o.items()}
     call_it = lambda: ops.lora_add(d["y"], d["x"], d["A"], d["B"], d["ids"], scaling=d["scaling"], splits=splits)  # noqa: E731
     call_it()
@@ -155,18 +165,18 @@ def test_graph_follows_the_ids(cuda):
 
 def test_c_abi_and_another_stream(cuda):
     splits = [96, 32]
-    o = operands(7, 320, splits, 16, 3)
+    o = operands(7, 320, splits, 40, 3)
     want = call(o, cuda, splits)
     d = {k: v.to(cuda) for k, v in o.items()}
     lib, out = load_lib(), torch.empty(7, 128, dtype=torch.bfloat16, device=cuda)
-    need = lib.lora_add_workspace(7, 16, 2)
+    need = lib.lora_add_workspace(7, 320, 40, splits)
     st = torch.cuda.Stream()
     st.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(st):
         space = torch.empty(need, dtype=torch.uint8, device=cuda)
         x = (d["x"].float() * 2.0).to(torch.bfloat16).div_(2.0)
         lib.lora_add(d["y"].data_ptr(), x.data_ptr(), d["A"].data_ptr(), d["B"].data_ptr(), d["ids"].data_ptr(),
-                     d["scaling"].data_ptr(), out.data_ptr(), 7, 320, 16, splits, 3, space.data_ptr(), need)
+                     d["scaling"].data_ptr(), out.data_ptr(), 7, 320, 40, splits, 3, space.data_ptr(), need)
     st.synchronize()
     assert torch.equal(bits(out), bits(want))
 
@@ -201,7 +211,8 @@ def test_refusals(cuda):
     refused("sum to N", splits=[16, 17])
     refused("rank rows", splits=[16, 16])
     refused("1 to 8", splits=[])
-    refused("workspace", workspace=torch.empty(8, device=cuda))
+    w = {k: v.to(cuda) for k, v in operands(4, 64, [32], 40, 3).items()}
+    refused("workspace", **w, workspace=torch.empty(8, device=cuda))
     refused("-2", A=d["A"][..., :60].contiguous(), x=d["x"][:, :60].contiguous())
     refused("-2", A=d["A"][:, :4].contiguous(), B=d["B"][..., :4].contiguous())
     refused("-2", splits=[32, 0], A=d["A"].repeat(1, 2, 1))
