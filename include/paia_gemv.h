@@ -204,7 +204,7 @@ PAIA_API int paia_paged_attention(const void* q, const long long* q_strides, con
  * up; splits: host ints), j the slice of n, each with its own `rank` rows of A. y, out bf16 [M][N] and x bf16 [M][K] with row
  * strides in elements (out may be y); A bf16 [adapters][slices * rank][K], B bf16 [adapters][N][rank], ids int32 [M] (outside
  * [0, adapters): the row keeps y), scaling fp32 [adapters] or NULL (1). fp32 sums, one rounding at the end. rank % 8 == 0,
- * rank <= 256, K % 8 == 0; x, A, B and x's rows 16-byte aligned; M = 0 does nothing. workspace as for paged attention, 16-byte
+ * rank <= 256, K % 8 == 0, at most 2^24 - 1 adapters; x, A, B and x's rows 16-byte aligned; M = 0 does nothing. workspace as for paged attention, 16-byte
  * aligned, of paia_lora_add_workspace() bytes (0: few rows of a low rank, NULL will do; -2: outside the contract). */
 PAIA_API long long paia_lora_add_workspace(int M, int K, int rank, const int* splits, int slices);
 PAIA_API int paia_lora_add(const void* y, long long y_stride, const void* x, long long x_stride, const void* A,

@@ -26,8 +26,9 @@ namespace paia {
 constexpr int kLoraBlock = 256, kLoraWaves = kLoraBlock / kWave;
 constexpr int kLoraRows = 256;           // rows of a launch
 constexpr int kChunk = 16;               // rows that share a pass over an adapter
+constexpr uint32_t kNoAdapter = 0xFFFFFFu;
 constexpr int kMaxSlices = 8, kMaxPieces = 8;
-constexpr int kShrinunits = 512;        // blocks aimed at by the first product's split of K
+constexpr int kShrinkUnits = 512;        // blocks aimed at by the first product's split of K
 constexpr int kShrinkCols = 64;          // columns of K a wave takes at a time
 constexpr int kSmallBlock = 512, kSmallWaves = kSmallBlock / kWave;
 constexpr int kSmallRank = 32;           // rank up to which the small form takes a row's h in registers
@@ -51,58 +52,68 @@ struct LoraParams {
     int M, K, N, R, adapters, slices, h_rows, h_stride;     // h_rows: slices * R; h_stride: that rounded up to 16
     int first[kMaxSlices + 1];           // first output of each slice, N at the end
     int unit_first[kMaxSlices + 1];      // first expand unit of each slice within a chunk
-    Divisor by_row;                      // by R / 8, the 16-byte pieces of a row of B
+    Divisor by_row, by_chunk;            // by R / 8, the 16-byte pieces of a row of B; by a chunk's expand units
     bool wide;                           // out and y take 8-byte accesses
 };
 
 // The rows in the order of their adapters, cut into chunks of at most kChunk rows of one adapter; rows without one last.
 struct RowChunks {
-    int4 keys[kLoraRows / 4];            // adapter of each row, INT_MAX without and past the last row
-    int order[kLoraRows];                // rows by (key, row)
-    int start[kLoraRows + 1];            // first place in `order` of each chunk
-    int marks[kLoraWaves];
+    uint4 keys[kLoraRows / 4];           // adapter << 8 | row, kNoAdapter without one; past the last row the largest key
+    uint32_t sorted[kLoraRows];          // the keys in order
+    int start[kLoraRows + 1];            // first place in `sorted` of each chunk
+    uint64_t begins[kLoraWaves];         // places where another adapter begins
+    int marks[kLoraWaves];               // chunks that begin in each wave's places
     int count;
-    __device__ __forceinline__ int& key(int row) { return reinterpret_cast<int*>(keys)[row]; }
+    __device__ __forceinline__ int row(int place) const { return (int)(sorted[place] & 255u); }
+    __device__ __forceinline__ int adapter(int place) const      // -1: rows without one
+    {
+        const uint32_t id = sorted[place] >> 8;
+        return id == kNoAdapter ? -1 : (int)id;
+    }
 };
 __device__ __forceinline__ void row_chunks(const LoraParams& p, RowChunks* s)
 {
-    const int t = (int)threadIdx.x;
-    int key = INT_MAX;
+    static_assert(kLoraRows == kLoraBlock, "a thread has a row");
+    const int t = (int)threadIdx.x, lane = lane_id(), wave = wave_id();
+    uint32_t key = ~0u;
     if (t < p.M) {
         const int id = p.ids[t];
-        if (id >= 0 && id < p.adapters) key = id;
+        key = (id >= 0 && id < p.adapters ? (uint32_t)id : kNoAdapter) << 8 | (uint32_t)t;
     }
-    s->key(t) = key;
+    reinterpret_cast<uint32_t*>(s->keys)[t] = key;
     __syncthreads();
-    int place = 0, same = 0;
-    for (int j = 0; j < p.M; j += 16) {
-        int4 k[4];
+    if (wave * kWave < p.M) {            // a row's place: the keys below its own
+        int place = 0;
+        for (int j = 0; j < p.M; j += 16) {
+            uint4 k[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) k[i] = s->keys[j / 4 + i];
+            for (int i = 0; i < 4; ++i) k[i] = s->keys[j / 4 + i];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = j + 4 * i;
-            same += (k[i].x == key && at < t) + (k[i].y == key && at + 1 < t) + (k[i].z == key && at + 2 < t) +
-                    (k[i].w == key && at + 3 < t);
-            place += (k[i].x < key) + (k[i].y < key) + (k[i].z < key) + (k[i].w < key);
+            for (int i = 0; i < 4; ++i) place += (k[i].x < key) + (k[i].y < key) + (k[i].z < key) + (k[i].w < key);
         }
+        if (t < p.M) s->sorted[place] = key;
     }
-    place += same;
-    if (t < p.M) s->order[place] = t | (same % kChunk == 0 ? 1 << 16 : 0);
     __syncthreads();
-    const int row = t < p.M ? s->order[t] : 0;
-    const bool begins = row >> 16;
-    const uint64_t mark = __ballot(begins);
-    if (lane_id() == 0) s->marks[wave_id()] = __popcll(mark);
+    const bool begins = t < p.M && (t == 0 || s->sorted[t] >> 8 != s->sorted[t - 1] >> 8);
+    const uint64_t mask = __ballot(begins);
+    if (lane == 0) s->begins[wave] = mask;
+    __syncthreads();
+    // the place where this place's adapter begins: the last mark at or before it
+    uint64_t marks = mask & (~0ull >> (63 - lane));
+    int w = wave;
+    while (marks == 0 && w > 0) marks = s->begins[--w];
+    const int from = w * kWave + 63 - (marks != 0 ? __builtin_clzll(marks) : 63);
+    const bool cut = t < p.M && (t - from) % kChunk == 0;
+    const uint64_t cuts = __ballot(cut);
+    if (lane == 0) s->marks[wave] = __popcll(cuts);
     __syncthreads();
     int before = 0, count = 0;
 #pragma unroll
-    for (int w = 0; w < kLoraWaves; ++w) {
-        before += w < wave_id() ? s->marks[w] : 0;
-        count += s->marks[w];
+    for (int i = 0; i < kLoraWaves; ++i) {
+        before += i < wave ? s->marks[i] : 0;
+        count += s->marks[i];
     }
-    if (begins) s->start[before + __popcll(mark & ((1ull << lane_id()) - 1))] = t;
-    if (t < p.M) s->order[t] = row & 0xFFFF;
+    if (cut) s->start[before + __popcll(cuts & ((1ull << lane) - 1))] = t;
     if (t == 0) s->start[count] = p.M, s->count = count;
     __syncthreads();
 }
@@ -112,7 +123,7 @@ __device__ __forceinline__ int k_pieces(const LoraParams& p, int chunks)
 {
     const int units = chunks * (p.h_stride / 16);
     const int most = min(kMaxPieces, (p.K + 255) / 256);
-    return max(1, min(most, kShrinunits / units));
+    return max(1, min(most, kShrinkUnits / units));
 }
 
 __device__ __forceinline__ f32x4 lora_mfma(const u32x4 a, const u32x4 b, const f32x4 c)
@@ -153,22 +164,21 @@ __global__ void __launch_bounds__(kLoraBlock) lora_shrink_kernel(const LoraParam
         if (threadIdx.x == 0) p.list->count = rows.count, p.list->pieces = pieces;
         for (int e = (int)threadIdx.x; e < rows.count * kChunk; e += kLoraBlock) {
             const int c = e / kChunk, i = e % kChunk, start = rows.start[c], held = rows.start[c + 1] - start;
-            const int row = rows.order[start + min(i, held - 1)], id = rows.key(row);
-            p.list->chunk[c].rows[i] = row;
-            if (i == 0) p.list->chunk[c].adapter = id == INT_MAX ? -1 : id, p.list->chunk[c].held = held;
+            p.list->chunk[c].rows[i] = rows.row(start + min(i, held - 1));
+            if (i == 0) p.list->chunk[c].adapter = rows.adapter(start), p.list->chunk[c].held = held;
         }
     }
     for (int unit = (int)blockIdx.x; unit < rows.count * tiles * pieces; unit += (int)gridDim.x) {
         const int piece = unit % pieces, tile = unit / pieces % tiles, chunk = unit / pieces / tiles;
         const int start = rows.start[chunk], held = rows.start[chunk + 1] - start;
-        const int id = rows.key(rows.order[start]);
-        if (id == INT_MAX) break;        // the last chunks: rows without an adapter
+        const int id = rows.adapter(start);
+        if (id < 0) break;               // the last chunks: rows without an adapter
         const int s0 = (int)((int64_t)steps * piece / pieces), s1 = (int)((int64_t)steps * (piece + 1) / pieces);
         const uint16_t *a[2], *x[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             a[i] = p.A + ((int64_t)id * p.h_rows + min(tile * 16 + 8 * i + lr, p.h_rows - 1)) * p.K + 8 * lc;
-            x[i] = p.x + rows.order[start + min(8 * i + lr, held - 1)] * p.x_stride + 8 * lc;
+            x[i] = p.x + rows.row(start + min(8 * i + lr, held - 1)) * p.x_stride + 8 * lc;
         }
         u32x4 u[kShrinkAhead][2], v[kShrinkAhead][2];
         auto load = [&](int s, int at) {          // a step past the piece's end loads nothing and adds nothing
@@ -204,7 +214,7 @@ __global__ void __launch_bounds__(kLoraBlock) lora_shrink_kernel(const LoraParam
         sums[wave][lane] = acc;
         __syncthreads();
         if (wave == 0 && n < held) {
-            const int m = rows.order[start + n];
+            const int m = rows.row(start + n);
 #pragma unroll
             for (int w = 1; w < kLoraWaves; ++w) acc += sums[w][lane];
             *reinterpret_cast<f32x4*>(p.part + ((int64_t)piece * p.M + m) * p.h_stride + tile * 16 + 4 * g) = acc;
@@ -213,10 +223,12 @@ __global__ void __launch_bounds__(kLoraBlock) lora_shrink_kernel(const LoraParam
     }
 }
 
-// out: a unit is (chunk, slice, kLoraWaves * ROWS outputs of the slice). STEPS: 32-value steps of R. A wave's ROWS rows of B
-// are contiguous memory, ROWS R / 8 pieces of 16 bytes, loaded as such and brought into the matrix layout through its own
-// piece of LDS (rows an odd number of pieces apart: no bank conflicts). The block sums the pieces of h for its chunk once.
-constexpr int expand_rows(int steps) { return steps <= 1 ? 64 : steps <= 2 ? 32 : 16; }
+// out: a unit is (chunk, slice, kLoraWaves * ROWS outputs of the slice), ROWS of them a wave's. STEPS: 32-value steps of R.
+// A wave's ROWS rows of B are contiguous memory, ROWS R / 8 pieces of 16 bytes, loaded as such and brought into the matrix
+// layout through its own piece of LDS (rows an odd number of pieces apart: no bank conflicts). A block takes consecutive
+// units, with kExpandAhead units' loads in flight, and sums the pieces of h anew only where the chunk or slice changes.
+constexpr int expand_rows(int steps) { return steps <= 2 ? 32 : 16; }
+constexpr int kExpandAhead = 2;
 template <int STEPS, bool WIDE>
 __global__ void __launch_bounds__(kLoraBlock) lora_expand_kernel(const LoraParams p)
 {
@@ -225,105 +237,145 @@ __global__ void __launch_bounds__(kLoraBlock) lora_expand_kernel(const LoraParam
     __shared__ u32x4 h_of[2][kChunk * kHPitch];
     __shared__ u32x4 b_of[kLoraWaves][ROWS * kBPitch];
     const int lane = lane_id(), wave = wave_id(), n = lane & 15, g = lane >> 4;
-    const int row_pieces = p.R / 8, pitch = row_pieces | 1, u = (int)blockIdx.x;
-    int slice = 0;
-    while (u >= p.unit_first[slice + 1]) ++slice;
+    const int row_pieces = p.R / 8, pitch = row_pieces | 1, per_chunk = p.unit_first[p.slices];
     const int count = p.list->count, pieces = p.list->pieces;
-    for (int chunk = (int)blockIdx.y; chunk < count; chunk += (int)gridDim.y) {
-        const auto& c = p.list->chunk[chunk];
-        const int id = c.adapter, held = c.held, m = c.rows[n];
-        const bool live = n < held, bare = id < 0;
-        if (bare && p.out == p.y && p.out_stride == p.y_stride) continue;
-        const int end = p.first[slice + 1];
-        const int n0 = p.first[slice] + ((u - p.unit_first[slice]) * kLoraWaves + wave) * ROWS;
-        const int width = min(ROWS, end - n0);         // outputs of this wave, none where it is not positive
+    const int64_t units = (int64_t)count * per_chunk;
+    const int first = (int)(units * blockIdx.x / gridDim.x), last = (int)(units * (blockIdx.x + 1) / gridDim.x);
+    if (first >= last) return;
 
-        u32x4 b[kLoads];
-        const u32x4* B = reinterpret_cast<const u32x4*>(p.B + ((int64_t)(bare ? 0 : id) * p.N + n0) * p.R);
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int at = i * kWave + lane;
-            b[i] = !bare && at < width * row_pieces ? B[at] : u32x4{0, 0, 0, 0};
+    // where a unit lies
+    struct Place {
+        int chunk, slice, n0, width;     // width: outputs of this wave, none where it is not positive
+    };
+    const auto place_of = [&](int unit) {
+        Place r;
+        r.chunk = (int)p.by_chunk.of((uint32_t)unit);
+        const int u = unit - r.chunk * per_chunk;
+        r.slice = 0;
+        while (u >= p.unit_first[r.slice + 1]) ++r.slice;
+        r.n0 = p.first[r.slice] + ((u - p.unit_first[r.slice]) * kLoraWaves + wave) * ROWS;
+        r.width = min(ROWS, p.first[r.slice + 1] - r.n0);
+        return r;
+    };
+    Place at[kExpandAhead];
+    u32x4 b[kExpandAhead][kLoads];
+    uint2 was[kExpandAhead][kTiles];
+    int ahead_chunk = -1, ahead_row = 0, ahead_id = 0, ahead_held = 0;     // of the last unit that was loaded
+    const auto load = [&](int unit, int i) {
+        if (unit >= last) return;
+        const Place r = place_of(unit);
+        at[i] = r;
+        if (r.chunk != ahead_chunk) {
+            ahead_chunk = r.chunk;
+            ahead_id = p.list->chunk[r.chunk].adapter;
+            ahead_held = p.list->chunk[r.chunk].held;
+            ahead_row = p.list->chunk[r.chunk].rows[n];
         }
-        const uint16_t* y = p.y + m * p.y_stride;
-        uint16_t* out = p.out + m * p.out_stride;
-        uint2 was[kTiles];
+        const u32x4* B = reinterpret_cast<const u32x4*>(p.B + ((int64_t)max(ahead_id, 0) * p.N + r.n0) * p.R);
+#pragma unroll
+        for (int e = 0; e < kLoads; ++e) {
+            const int c = e * kWave + lane;
+            b[i][e] = ahead_id >= 0 && c < r.width * row_pieces ? B[c] : u32x4{0, 0, 0, 0};
+        }
+        const uint16_t* y = p.y + ahead_row * p.y_stride + r.n0;
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
-            const int at = 16 * t + 4 * g;
-            was[t] = uint2{0, 0};
-            if (!live || at >= width) continue;
-            if (WIDE && at + 4 <= width) {
-                was[t] = *reinterpret_cast<const uint2*>(y + n0 + at);
-            } else {
-                const uint16_t* from = y + n0 + at;
-                was[t].x = from[0] | (at + 1 < width ? (uint32_t)from[1] << 16 : 0u);
-                was[t].y = at + 2 < width ? from[2] | (at + 3 < width ? (uint32_t)from[3] << 16 : 0u) : 0u;
+            const int o = 16 * t + 4 * g;
+            uint2 v = {0, 0};
+            if (n < ahead_held && o < r.width) {
+                if (WIDE && o + 4 <= r.width) {
+                    v = *reinterpret_cast<const uint2*>(y + o);
+                } else {
+                    v.x = y[o] | (o + 1 < r.width ? (uint32_t)y[o + 1] << 16 : 0u);
+                    v.y = o + 2 < r.width ? y[o + 2] | (o + 3 < r.width ? (uint32_t)y[o + 3] << 16 : 0u) : 0u;
+                }
             }
+            was[i][t] = v;
         }
-        if (!bare) {
-            // the chunk's values of this slice of h: the pieces' sums in order, times the adapter's factor, as bf16 value
-            // and remainder
-            const float factor = p.scaling == nullptr ? 1.0f : p.scaling[id];
-            for (int e = (int)threadIdx.x; e < held * (p.R / 4); e += kLoraBlock) {
-                const int c4 = e / held, r = e - c4 * held;
-                const float* src = p.part + (int64_t)c.rows[r] * p.h_stride + slice * p.R + 4 * c4;
-                f32x4 term[kMaxPieces], h = {0.0f, 0.0f, 0.0f, 0.0f};
+    };
 #pragma unroll
-                for (int i = 0; i < kMaxPieces; ++i)
-                    term[i] = i < pieces ? *reinterpret_cast<const f32x4*>(src + (int64_t)i * p.M * p.h_stride)
-                                         : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < kExpandAhead; ++i) load(first + i, i);
+
+    int chunk = -1, slice = -1, m = 0, id = -1, held = 0;
+    u32x4 hi[STEPS], lo[STEPS];
+    for (int unit0 = first; unit0 < last; unit0 += kExpandAhead) {
 #pragma unroll
-                for (int i = 0; i < kMaxPieces; ++i) h += term[i];
-                h *= factor;
-                const uint2 hi = {pack_bf16x2(h[0], h[1]), pack_bf16x2(h[2], h[3])};
-                const uint2 lo = {pack_bf16x2(rest(h[0], hi.x << 16), rest(h[1], hi.x & 0xFFFF0000u)),
-                                  pack_bf16x2(rest(h[2], hi.y << 16), rest(h[3], hi.y & 0xFFFF0000u))};
-                reinterpret_cast<uint2*>(h_of[0])[r * (2 * kHPitch) + c4] = hi;
-                reinterpret_cast<uint2*>(h_of[1])[r * (2 * kHPitch) + c4] = lo;
+        for (int i = 0; i < kExpandAhead; ++i) {
+            const int unit = unit0 + i;
+            if (unit >= last) break;
+            const Place r = at[i];
+            if (r.chunk != chunk || r.slice != slice) {
+                chunk = r.chunk, slice = r.slice;
+                const auto& c = p.list->chunk[chunk];
+                id = c.adapter, held = c.held, m = c.rows[n];
+                // the chunk's values of this slice of h: the pieces' sums in order, times the adapter's factor, as bf16 value
+                // and remainder
+                __syncthreads();
+                const float factor = id < 0 || p.scaling == nullptr ? 1.0f : p.scaling[id];
+                for (int e = (int)threadIdx.x; e < (id < 0 ? 0 : held * (p.R / 4)); e += kLoraBlock) {
+                    const int c4 = e / held, row = e - c4 * held;
+                    const float* src = p.part + (int64_t)c.rows[row] * p.h_stride + slice * p.R + 4 * c4;
+                    f32x4 term[kMaxPieces], h = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int k = 0; k < kMaxPieces; ++k)
+                        term[k] = k < pieces ? *reinterpret_cast<const f32x4*>(src + (int64_t)k * p.M * p.h_stride)
+                                             : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int k = 0; k < kMaxPieces; ++k) h += term[k];
+                    h *= factor;
+                    const uint2 top = {pack_bf16x2(h[0], h[1]), pack_bf16x2(h[2], h[3])};
+                    const uint2 low = {pack_bf16x2(rest(h[0], top.x << 16), rest(h[1], top.x & 0xFFFF0000u)),
+                                       pack_bf16x2(rest(h[2], top.y << 16), rest(h[3], top.y & 0xFFFF0000u))};
+                    reinterpret_cast<uint2*>(h_of[0])[row * (2 * kHPitch) + c4] = top;
+                    reinterpret_cast<uint2*>(h_of[1])[row * (2 * kHPitch) + c4] = low;
+                }
+                __syncthreads();
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) {
+                    const bool in = id >= 0 && 4 * s + g < row_pieces;
+                    hi[s] = in ? h_of[0][min(n, held - 1) * kHPitch + 4 * s + g] : u32x4{0, 0, 0, 0};
+                    lo[s] = in ? h_of[1][min(n, held - 1) * kHPitch + 4 * s + g] : u32x4{0, 0, 0, 0};
+                }
             }
-        }
-        __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const uint32_t at = (uint32_t)(i * kWave + lane), r = p.by_row.of(at);
-            if (r < (uint32_t)ROWS) b_of[wave][r * pitch + at - r * row_pieces] = b[i];
-        }
-        lora_lds_order();
-        u32x4 hi[STEPS], lo[STEPS];
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            const bool in = !bare && 4 * s + g < row_pieces;
-            hi[s] = in ? h_of[0][min(n, held - 1) * kHPitch + 4 * s + g] : u32x4{0, 0, 0, 0};
-            lo[s] = in ? h_of[1][min(n, held - 1) * kHPitch + 4 * s + g] : u32x4{0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-            f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int s = 0; s < STEPS; ++s) {
-                const u32x4 w = 4 * s + g < row_pieces ? b_of[wave][(16 * t + n) * pitch + 4 * s + g] : u32x4{0, 0, 0, 0};
-                acc = lora_mfma(w, lo[s], acc);
-                acc = lora_mfma(w, hi[s], acc);
+            for (int e = 0; e < kLoads; ++e) {
+                const uint32_t c = (uint32_t)(e * kWave + lane), row = p.by_row.of(c);
+                if (row < (uint32_t)ROWS) b_of[wave][row * pitch + c - row * row_pieces] = b[i][e];
             }
-            const int at = 16 * t + 4 * g;
-            if (!live || at >= width) continue;
-            uint2 v = was[t];
-            if (!bare) {
-                v.x = pack_bf16x2(bf16_to_f32(v.x & 0xFFFFu) + acc[0], __uint_as_float(v.x & 0xFFFF0000u) + acc[1]);
-                v.y = pack_bf16x2(bf16_to_f32(v.y & 0xFFFFu) + acc[2], __uint_as_float(v.y & 0xFFFF0000u) + acc[3]);
+            uint2 y[kTiles];
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) y[t] = was[i][t];
+            lora_lds_order();
+            load(unit + kExpandAhead, i);
+            uint16_t* out = p.out + m * p.out_stride + r.n0;
+            const bool same = id < 0 && p.out == p.y && p.out_stride == p.y_stride;     // the row keeps y where it is
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) {
+                f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) {
+                    const u32x4 w = 4 * s + g < row_pieces ? b_of[wave][(16 * t + n) * pitch + 4 * s + g] : u32x4{0, 0, 0, 0};
+                    acc = lora_mfma(w, lo[s], acc);
+                    acc = lora_mfma(w, hi[s], acc);
+                }
+                const int o = 16 * t + 4 * g;
+                if (n >= held || o >= r.width || same) continue;
+                uint2 v = y[t];
+                if (id >= 0) {
+                    v.x = pack_bf16x2(bf16_to_f32(v.x & 0xFFFFu) + acc[0], __uint_as_float(v.x & 0xFFFF0000u) + acc[1]);
+                    v.y = pack_bf16x2(bf16_to_f32(v.y & 0xFFFFu) + acc[2], __uint_as_float(v.y & 0xFFFF0000u) + acc[3]);
+                }
+                if (WIDE && o + 4 <= r.width) {
+                    *reinterpret_cast<uint2*>(out + o) = v;
+                } else {
+                    out[o] = (uint16_t)v.x;
+                    if (o + 1 < r.width) out[o + 1] = (uint16_t)(v.x >> 16);
+                    if (o + 2 < r.width) out[o + 2] = (uint16_t)v.y;
+                    if (o + 3 < r.width) out[o + 3] = (uint16_t)(v.y >> 16);
+                }
             }
-            uint16_t* to = out + n0 + at;
-            if (WIDE && at + 4 <= width) {
-                *reinterpret_cast<uint2*>(to) = v;
-            } else {
-                to[0] = (uint16_t)v.x;
-                if (at + 1 < width) to[1] = (uint16_t)(v.x >> 16);
-                if (at + 2 < width) to[2] = (uint16_t)v.y;
-                if (at + 3 < width) to[3] = (uint16_t)(v.y >> 16);
-            }
+            lora_lds_order();
         }
-        __syncthreads();
     }
 }
 
@@ -395,9 +447,8 @@ static int launch_lora(const LoraParams& p, hipStream_t st)
     const int64_t shrink = (int64_t)p.M * (p.h_stride / 16) * kMaxPieces;
     hipLaunchKernelGGL(lora_shrink_kernel, dim3((uint32_t)(shrink < cap ? shrink : cap)), dim3(kLoraBlock), 0, st, p);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return (int)e;
-    // a row of blocks for each chunk that there may be, up to 8192 blocks, beyond which a block takes several chunks
-    const int per_chunk = p.unit_first[p.slices], rows = 8192 / per_chunk;
-    const dim3 grid((uint32_t)per_chunk, (uint32_t)(rows < 1 ? 1 : rows < p.M ? rows : p.M));
+    const int64_t expand = (int64_t)p.M * p.unit_first[p.slices];
+    const dim3 grid((uint32_t)(expand < cap ? expand : cap));
     auto go = [&](auto wide, auto narrow) { hipLaunchKernelGGL(p.wide ? wide : narrow, grid, dim3(kLoraBlock), 0, st, p); };
     const int steps = (p.R + 31) / 32;
     if (steps <= 1) go(lora_expand_kernel<1, true>, lora_expand_kernel<1, false>);
@@ -455,7 +506,7 @@ int paia_lora_add(const void* y, long long y_stride, const void* x, long long x_
                   const int* splits, int slices, int adapters, void* workspace, long long workspace_bytes, void* stream)
 {
     using namespace paia;
-    if (!lora_sizes(M, K, rank, splits, slices) || adapters <= 0) return -2;
+    if (!lora_sizes(M, K, rank, splits, slices) || adapters <= 0 || adapters > (int)kNoAdapter) return -2;
     LoraParams p;
     int64_t N = 0, units = 0;
     const bool small = use_small(M, K, rank, splits, slices);
@@ -469,6 +520,7 @@ int paia_lora_add(const void* y, long long y_stride, const void* x, long long x_
         if (N > INT_MAX - unit || units * kLoraRows > INT_MAX) return -2;
     }
     p.first[slices] = (int)N, p.unit_first[slices] = (int)units;
+    p.by_chunk = Divisor((uint32_t)units);
     if (M == 0) return 0;
     if (y == nullptr || x == nullptr || A == nullptr || B == nullptr || ids == nullptr || out == nullptr) return -2;
     if (!aligned(x, 16) || !aligned(A, 16) || !aligned(B, 16) || !aligned(y, 2) || !aligned(out, 2) || !aligned(ids, 4) ||
