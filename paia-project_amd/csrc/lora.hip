@@ -24,7 +24,9 @@
 namespace paia {
 
 constexpr int kLoraBlock = 256, kLoraWaves = kLoraBlock / kWave;
-constexpr int kLoraRows = 256;           // rows of a launch
+constexpr int kLoraRows = 256;           // rows of a launch, a thread each
+constexpr int kRowWaves = kLoraRows / kWave;
+constexpr int kShrinkBlock = 512, kShrinkWaves = kShrinkBlock / kWave;
 constexpr int kChunk = 16;               // rows that share a pass over an adapter
 constexpr uint32_t kNoAdapter = 0xFFFFFFu;
 constexpr int kMaxSlices = 8, kMaxPieces = 8;
@@ -61,8 +63,8 @@ struct RowChunks {
     uint4 keys[kLoraRows / 4];           // adapter << 8 | row, kNoAdapter without one; past the last row the largest key
     uint32_t sorted[kLoraRows];          // the keys in order
     int start[kLoraRows + 1];            // first place in `sorted` of each chunk
-    uint64_t begins[kLoraWaves];         // places where another adapter begins
-    int marks[kLoraWaves];               // chunks that begin in each wave's places
+    uint64_t begins[kRowWaves];          // places where another adapter begins
+    int marks[kRowWaves];                // chunks that begin in each wave's places
     int count;
     __device__ __forceinline__ int row(int place) const { return (int)(sorted[place] & 255u); }
     __device__ __forceinline__ int adapter(int place) const      // -1: rows without one
@@ -73,14 +75,13 @@ struct RowChunks {
 };
 __device__ __forceinline__ void row_chunks(const LoraParams& p, RowChunks* s)
 {
-    static_assert(kLoraRows == kLoraBlock, "a thread has a row");
     const int t = (int)threadIdx.x, lane = lane_id(), wave = wave_id();
     uint32_t key = ~0u;
     if (t < p.M) {
         const int id = p.ids[t];
         key = (id >= 0 && id < p.adapters ? (uint32_t)id : kNoAdapter) << 8 | (uint32_t)t;
     }
-    reinterpret_cast<uint32_t*>(s->keys)[t] = key;
+    if (t < kLoraRows) reinterpret_cast<uint32_t*>(s->keys)[t] = key;
     __syncthreads();
     if (wave * kWave < p.M) {            // a row's place: the keys below its own
         int place = 0;
@@ -96,20 +97,20 @@ __device__ __forceinline__ void row_chunks(const LoraParams& p, RowChunks* s)
     __syncthreads();
     const bool begins = t < p.M && (t == 0 || s->sorted[t] >> 8 != s->sorted[t - 1] >> 8);
     const uint64_t mask = __ballot(begins);
-    if (lane == 0) s->begins[wave] = mask;
+    if (lane == 0 && wave < kRowWaves) s->begins[wave] = mask;
     __syncthreads();
     // the place where this place's adapter begins: the last mark at or before it
     uint64_t marks = mask & (~0ull >> (63 - lane));
-    int w = wave;
+    int w = min(wave, kRowWaves);
     while (marks == 0 && w > 0) marks = s->begins[--w];
     const int from = w * kWave + 63 - (marks != 0 ? __builtin_clzll(marks) : 63);
     const bool cut = t < p.M && (t - from) % kChunk == 0;
     const uint64_t cuts = __ballot(cut);
-    if (lane == 0) s->marks[wave] = __popcll(cuts);
+    if (lane == 0 && wave < kRowWaves) s->marks[wave] = __popcll(cuts);
     __syncthreads();
     int before = 0, count = 0;
 #pragma unroll
-    for (int i = 0; i < kLoraWaves; ++i) {
+    for (int i = 0; i < kRowWaves; ++i) {
         before += i < wave ? s->marks[i] : 0;
         count += s->marks[i];
     }
@@ -151,18 +152,18 @@ __device__ __forceinline__ void lora_lds_order()     // a wave's LDS operations 
 // h: a unit is (chunk, 16 rows of A, piece of K); the block's waves take its steps of 64 columns in turn. Eight lanes load
 // 128 bytes of a row, of A and of x alike; a wave-private piece of LDS brings both into the matrix layout (row n at piece
 // c ^ n / 2: the 16 rows of a read cover all banks).
-__global__ void __launch_bounds__(kLoraBlock) lora_shrink_kernel(const LoraParams p)
+__global__ void __launch_bounds__(kShrinkBlock) lora_shrink_kernel(const LoraParams p)
 {
     __shared__ RowChunks rows;
-    __shared__ u32x4 stage[kLoraWaves][2][kChunk * 8];
-    __shared__ f32x4 sums[kLoraWaves][kWave];
+    __shared__ u32x4 stage[kShrinkWaves][2][kChunk * 8];
+    __shared__ f32x4 sums[kShrinkWaves][kWave];
     row_chunks(p, &rows);
     const int tiles = p.h_stride / 16, pieces = k_pieces(p, rows.count), steps = (p.K + kShrinkCols - 1) / kShrinkCols;
     const int lane = lane_id(), wave = wave_id(), n = lane & 15, g = lane >> 4;
     const int lr = lane >> 3, lc = lane & 7;      // row (and that plus 8) and piece of a row that the lane loads
     if (blockIdx.x == 0) {
         if (threadIdx.x == 0) p.list->count = rows.count, p.list->pieces = pieces;
-        for (int e = (int)threadIdx.x; e < rows.count * kChunk; e += kLoraBlock) {
+        for (int e = (int)threadIdx.x; e < rows.count * kChunk; e += kShrinkBlock) {
             const int c = e / kChunk, i = e % kChunk, start = rows.start[c], held = rows.start[c + 1] - start;
             p.list->chunk[c].rows[i] = rows.row(start + min(i, held - 1));
             if (i == 0) p.list->chunk[c].adapter = rows.adapter(start), p.list->chunk[c].held = held;
@@ -190,9 +191,9 @@ __global__ void __launch_bounds__(kLoraBlock) lora_shrink_kernel(const LoraParam
             }
         };
 #pragma unroll
-        for (int i = 0; i < kShrinkAhead; ++i) load(s0 + wave + i * kLoraWaves, i);
+        for (int i = 0; i < kShrinkAhead; ++i) load(s0 + wave + i * kShrinkWaves, i);
         f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s = s0 + wave; s < s1; s += kShrinkAhead * kLoraWaves) {
+        for (int s = s0 + wave; s < s1; s += kShrinkAhead * kShrinkWaves) {
 #pragma unroll
             for (int i = 0; i < kShrinkAhead; ++i) {
 #pragma unroll
@@ -202,7 +203,7 @@ __global__ void __launch_bounds__(kLoraBlock) lora_shrink_kernel(const LoraParam
                     stage[wave][1][at] = v[i][e];
                 }
                 lora_lds_order();
-                load(s + (kShrinkAhead + i) * kLoraWaves, i);
+                load(s + (kShrinkAhead + i) * kShrinkWaves, i);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const int at = n * 8 + ((4 * j + g) ^ (n >> 1));
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(kLoraBlock) lora_shrink_kernel(const LoraParam
         if (wave == 0 && n < held) {
             const int m = rows.row(start + n);
 #pragma unroll
-            for (int w = 1; w < kLoraWaves; ++w) acc += sums[w][lane];
+            for (int w = 1; w < kShrinkWaves; ++w) acc += sums[w][lane];
             *reinterpret_cast<f32x4*>(p.part + ((int64_t)piece * p.M + m) * p.h_stride + tile * 16 + 4 * g) = acc;
         }
         __syncthreads();
@@ -443,12 +444,15 @@ __global__ void __launch_bounds__(kSmallBlock) lora_small_kernel(const LoraParam
 
 static int launch_lora(const LoraParams& p, hipStream_t st)
 {
-    const int cap = device_facts().cus * 4;
+    // Blocks that are resident together (registers: two of eight waves, three of four here), fewer where there are fewer
+    // units: the rest would only find the rows again (128 rows of 12 adapters 15.4 us at four a CU, 13.8 so; sixteen of rank
+    // 64 even).
+    const int cap = device_facts().cus * 2, cap_expand = device_facts().cus * 3;
     const int64_t shrink = (int64_t)p.M * (p.h_stride / 16) * kMaxPieces;
-    hipLaunchKernelGGL(lora_shrink_kernel, dim3((uint32_t)(shrink < cap ? shrink : cap)), dim3(kLoraBlock), 0, st, p);
+    hipLaunchKernelGGL(lora_shrink_kernel, dim3((uint32_t)(shrink < cap ? shrink : cap)), dim3(kShrinkBlock), 0, st, p);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return (int)e;
     const int64_t expand = (int64_t)p.M * p.unit_first[p.slices];
-    const dim3 grid((uint32_t)(expand < cap ? expand : cap));
+    const dim3 grid((uint32_t)(expand < cap_expand ? expand : cap_expand));
     auto go = [&](auto wide, auto narrow) { hipLaunchKernelGGL(p.wide ? wide : narrow, grid, dim3(kLoraBlock), 0, st, p); };
     const int steps = (p.R + 31) / 32;
     if (steps <= 1) go(lora_expand_kernel<1, true>, lora_expand_kernel<1, false>);
