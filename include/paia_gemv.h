@@ -189,7 +189,7 @@ PAIA_API int paia_rope_append(const void* qkv, long long qkv_stride, const void*
  * on a page number outside [0, pages) (lengths beyond the table's width end there). With s_p = scale * k_scale[head] *
  * <q, k_p>: out bf16 [B][T][heads][head_dim] (16-byte aligned) = v_scale[head] * sum softmax(s)_p v_p, lse fp32
  * [B][T][heads] or NULL = log(sum exp(s_p)); a token that sees nothing has out 0, lse -inf. Scores, statistics and sums in
- * fp32; the weights are rounded to bf16 for their product with v. Nothing a token does not see reaches its output, NaN and
+ * fp32; the weights enter their product with v as two bf16 terms. Nothing a token does not see reaches its output, NaN and
  * infinities included. The lengths are read on the device: a captured call serves sequences as they grow.
  * workspace: device memory, 16-byte aligned, of at least paia_paged_attention_workspace() bytes (for the same cache, width,
  * B, T and heads; 0 = NULL will do, -2 = outside the contract). Calls that overlap need a workspace each. */

@@ -18,8 +18,8 @@
 //     V rows are loaded contiguously too, D/16 dims of eight positions per lane: 16 lanes are the 16 rows of the V^T
 //     operand, whose eight contraction values are the eight positions; one v_perm_b32 per register pairs them up.
 //   * e4m3 codes become bf16 exactly (v_cvt_scalef32_pk_bf16_fp8); the heads' factors go to the scores and the output.
-// Scores, statistics and sums are fp32. P is rounded to bf16 for the second product (2^-9 of each weight, independent of
-// each other, against the output's own rounding of the same size); the sum l is that of the unrounded weights.
+// Scores, statistics and sums are fp32. P enters the second product as two bf16 terms (value and remainder, 16 bits): one more
+// MFMA a product, 0.3 to 1% of the time; with the value alone the output's error was 1.3 times that of its rounding.
 // What no token sees (positions past the end, before the window, on a page outside the cache) contributes nothing, whatever
 // its bytes are: scores are replaced, V rows zeroed, and where tokens differ in what they see, each takes its own product.
 #include <hip/hip_runtime.h>
@@ -111,6 +111,15 @@ struct Piece {
 __device__ __forceinline__ bool find_piece(const AttnParams& p, int item, Piece* r)
 {
     const int lane = lane_id();
+    if (p.B == 1) {                      // the same without sums over sequences
+        const Span s = span_of(p, 0);
+        const int most = max(kMinTiles, whole_rounds((float)s.tiles * __builtin_amdgcn_rcpf((float)p.goal)));
+        const int count = max(1, (s.tiles + most - 1) / most);
+        const int each = s.tiles / count, more = s.tiles - each * count;
+        *r = {0, s.len, s.tile0 + item * each + min(item, more), 0, item, count};
+        r->tile1 = r->tile0 + each + (item < more ? 1 : 0);
+        return item < count;
+    }
     Span s = span_of(p, lane);
     float total = (float)last_lane(wave_scan((uint32_t)s.tiles));
     for (int b = kWave; b < p.B; b += kWave) total += (float)last_lane(wave_scan((uint32_t)span_of(p, b + lane).tiles));
@@ -178,22 +187,29 @@ __device__ __forceinline__ f32x4 mfma(const u32x4 a, const u32x4 b, const f32x4 
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 template <int N> struct Words { uint32_t w[N]; };
-template <int N>
+template <bool STREAM, typename T>
+__device__ __forceinline__ T load_as(const uint8_t* p)
+{
+    const T* at = reinterpret_cast<const T*>(p);
+    if constexpr (STREAM) return __builtin_nontemporal_load(at);
+    return *at;
+}
+template <int N, bool STREAM>
 __device__ __forceinline__ Words<N> load_words(const uint8_t* p)
 {
     Words<N> r;
     if constexpr (N >= 4) {
 #pragma unroll
         for (int i = 0; i < N / 4; ++i) {
-            const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p) + i);
+            const u32x4 v = load_as<STREAM, u32x4>(p + 16 * i);
 #pragma unroll
             for (int e = 0; e < 4; ++e) r.w[4 * i + e] = v[e];
         }
     } else if constexpr (N == 2) {
-        const u32x2 v = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
+        const u32x2 v = load_as<STREAM, u32x2>(p);
         r.w[0] = v.x, r.w[1] = v.y;
     } else {
-        r.w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+        r.w[0] = load_as<STREAM, uint32_t>(p);
     }
     return r;
 }
@@ -219,7 +235,8 @@ struct Layout {
     }
 };
 
-template <int D, bool FP8, bool P8>
+// STREAM: a cache row is read by one block alone, and need not stay in the caches
+template <int D, bool FP8, bool P8, bool STREAM>
 __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_kernel(const AttnParams p)
 {
     using L = Layout<D, FP8, P8>;
@@ -283,7 +300,7 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
             const uint32_t at = pos - p.cache.by_page.of(pos) * (uint32_t)p.cache.page_size;
             const uint8_t* row = kbase + (in_cache(kpage[i]) ? kpage[i] : 0) * p.cache.kp + at * p.cache.kr;
 #pragma unroll
-            for (int e = 0; e < L::kKStep; ++e) k[i * L::kKStep + e] = load_words<4>(row + e * p.cache.kr);
+            for (int e = 0; e < L::kKStep; ++e) k[i * L::kKStep + e] = load_words<4, STREAM>(row + e * p.cache.kr);
         }
     };
     const uint8_t* vrow[L::kVPages];
@@ -305,7 +322,7 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
         for (int i = 0; i < L::kVPages; ++i)
 #pragma unroll
             for (int e = 0; e < L::kVStep; ++e)
-                v[i * L::kVStep + e] = load_words<L::kVWords>(vrow[i] + e * p.cache.vr);
+                v[i * L::kVStep + e] = load_words<L::kVWords, STREAM>(vrow[i] + e * p.cache.vr);
     };
 
     float m = -INFINITY, l = 0.0f;
@@ -387,7 +404,13 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
             w[i] = __builtin_amdgcn_exp2f(s[i / 4][i % 4] - base);
             l += w[i];
         }
-        const u32x4 pw = {pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3]), pack_bf16x2(w[4], w[5]), pack_bf16x2(w[6], w[7])};
+        u32x4 top8, rest8;               // the lane's eight weights as bf16 values and remainders
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            top8[i] = pack_bf16x2(w[2 * i], w[2 * i + 1]);
+            rest8[i] = pack_bf16x2(w[2 * i] - __uint_as_float(top8[i] << 16),
+                                   w[2 * i + 1] - __uint_as_float(top8[i] & 0xFFFF0000u));
+        }
         // O^T += V^T P^T: rows 8 g + i, i = 0..7, of the tile against the lane's own eight weights. `see`: bit i keeps row
         // i; `take`: the product is this lane's (of its token), or nobody's business.
         auto add_pv = [&](uint32_t see, bool all, bool take) {
@@ -406,7 +429,8 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
                                     __builtin_amdgcn_perm(x[5], x[4], 0x05040100u), __builtin_amdgcn_perm(x[7], x[6], 0x05040100u)};
                 const u32x4 odd = {__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u),
                                    __builtin_amdgcn_perm(x[5], x[4], 0x07060302u), __builtin_amdgcn_perm(x[7], x[6], 0x07060302u)};
-                const f32x4 a = mfma(even, pw, o[2 * d]), b = mfma(odd, pw, o[2 * d + 1]);
+                const f32x4 a = mfma(even, top8, mfma(even, rest8, o[2 * d]));
+                const f32x4 b = mfma(odd, top8, mfma(odd, rest8, o[2 * d + 1]));
                 if (all) {
                     o[2 * d] = a, o[2 * d + 1] = b;
                 } else {
@@ -556,9 +580,9 @@ static bool attention_plan(const paia_kv_cache* c, int table_width, int B, int T
     const int64_t wide = (int64_t)c->kv_heads * p->col_groups, slots = (int64_t)device_facts().cus * blocks_per_cu(c->head_dim);
     int64_t target = slots / wide;
     target = target < 2 ? 2 : target;
-    // One round of blocks where the sequences are few; many sequences have a piece of their own each, and as many more as
-    // half a round.
-    const int64_t goal = B <= target / 2 ? target : target / 2 + B;
+    // One round of blocks where the sequences are few; many sequences have a piece of their own each, and as many more as a
+    // round (200 sequences of 30 to 3000: 114 us; half a round more 125, two rounds 111, but 64 of 1000 48, 51 and 53).
+    const int64_t goal = B <= target / 2 ? target : target + B;
     // pieces per sequence that the table's width allows
     const int64_t per_seq = ((int64_t)p->max_len / kTile + 1 + kMinTiles - 1) / kMinTiles;
     const int64_t items = goal < per_seq * B ? goal : per_seq * B;
@@ -574,14 +598,22 @@ static bool attention_plan(const paia_kv_cache* c, int table_width, int B, int T
     return true;
 }
 
+// Several column groups read the same rows, next to each other on one XCD: with streaming loads its L2 served them worse (five
+// tokens of 8 heads a group, 12000 positions each: 141 us against 117; heads of 256: 532 against 281). Two tiles of columns in
+// one block instead need twice the outputs and queries in registers, one wave a SIMD: 166.
+template <int D, bool FP8>
+static auto attention_kernel(bool p8, bool stream)
+{
+    return stream ? (p8 ? paged_attention_kernel<D, FP8, true, true> : paged_attention_kernel<D, FP8, false, true>)
+                  : (p8 ? paged_attention_kernel<D, FP8, true, false> : paged_attention_kernel<D, FP8, false, false>);
+}
 template <int D>
 static int launch_attention(const AttnParams& p, bool fp8, bool join, hipStream_t st)
 {
     const dim3 grid((uint32_t)((p.units + 7) / 8 * 8 * p.col_groups));
     const bool p8 = p.cache.page_size % 8 == 0;
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kAttnBlock), 0, st, p); };
-    if (fp8) p8 ? go(paged_attention_kernel<D, true, true>) : go(paged_attention_kernel<D, true, false>);
-    else p8 ? go(paged_attention_kernel<D, false, true>) : go(paged_attention_kernel<D, false, false>);
+    const auto kernel = fp8 ? attention_kernel<D, true>(p8, p.col_groups == 1) : attention_kernel<D, false>(p8, p.col_groups == 1);
+    hipLaunchKernelGGL(kernel, grid, dim3(kAttnBlock), 0, st, p);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return (int)e;
     if (join) {
         hipLaunchKernelGGL((attention_join_kernel<D>), dim3((uint32_t)p.B, (uint32_t)p.cache.kv_heads, (uint32_t)p.cols), dim3(256), 0, st, p);

@@ -53,7 +53,7 @@ def piece_tiles(tiles, goal, jitter):
 
 
 def plan(B, target, max_len):
-    goal = target if B <= target // 2 else target // 2 + B
+    goal = target if B <= target // 2 else target + B
     per_seq = (max_len // TILE + 1 + MIN_TILES - 1) // MIN_TILES
     return goal, min(goal, per_seq * B), per_seq
 
