@@ -32,6 +32,10 @@ LAYER = {
     "llama31_8b": [("qkv", 6144, 4096), ("o", 4096, 4096), ("gate_up", 28672, 4096), ("down", 4096, 14336)],
     "qwen25_7b": [("qkv", 4608, 3584), ("o", 3584, 3584), ("gate_up", 37888, 3584), ("down", 3584, 18944)],
 }
+# Query heads, key-value heads and head dim behind the projections above (q_proj = heads * dim, k_proj = kv_heads * dim), and
+# the base of the rotation's frequencies.
+HEADS = {"llama31_8b": (32, 8, 128), "qwen25_7b": (28, 4, 128)}
+ROPE_BASE = {"llama31_8b": 500000.0, "qwen25_7b": 1000000.0}
 LM_HEAD = {"llama31_8b": (128256, 4096), "qwen25_7b": (152064, 3584)}
 
 
