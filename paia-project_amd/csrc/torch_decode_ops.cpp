@@ -7,6 +7,7 @@
 // [pages, page_size, kv_heads, head_dim] is passed as its transpose(1, 2).
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
@@ -58,6 +59,28 @@ void check_index(const at::Tensor& t, at::ScalarType type, int64_t n, const at::
                 " must be a contiguous ", at::toString(type), " tensor [", n, "]");
     on_device_of(on, t, name);
 }
+
+// A call's workspace: the caller's tensor, or memory of torch's allocator for as long as the call is made (its next user on
+// this stream comes behind the call's kernels, as with a tensor that goes out of scope).
+struct Workspace {
+    c10::DataPtr held;
+    void* data = nullptr;
+    long long bytes = 0;
+    Workspace(const std::optional<at::Tensor>& given, long long need, const at::Tensor& on)
+    {
+        if (given.has_value()) {
+            TORCH_CHECK(given->is_contiguous() && (int64_t)given->nbytes() >= need,
+                        "workspace must be contiguous and hold ", need, " bytes");
+            on_device_of(on, *given, "workspace");
+            data = given->data_ptr();
+            bytes = (long long)given->nbytes();
+        } else if (need > 0) {
+            held = c10::hip::HIPCachingAllocator::get()->allocate((size_t)need);
+            data = held.get();
+            bytes = need;
+        }
+    }
+};
 
 paia_kv_cache cache_of(const at::Tensor& k, const at::Tensor& v, const std::optional<at::Tensor>& k_scale,
                        const std::optional<at::Tensor>& v_scale, const at::Tensor& on)
@@ -175,21 +198,12 @@ void paged_attention_run(const at::Tensor& q, const at::Tensor& k_cache, const a
     c10::DeviceGuard g(q.device());
     const long long need = paia_paged_attention_workspace(&c, width, B, T, heads);
     check_rc(need < 0 ? (int)need : 0, "paia_paged_attention");
-    at::Tensor space;
-    if (workspace.has_value()) {
-        TORCH_CHECK(workspace->is_contiguous() && (int64_t)workspace->nbytes() >= need,
-                    "workspace must be contiguous and hold ", need, " bytes");
-        on_device_of(q, *workspace, "workspace");
-        space = *workspace;
-    } else if (need > 0) {
-        space = at::empty({need}, q.options().dtype(at::kByte));
-    }
+    const Workspace space(workspace, need, q);
     const double s = scale.has_value() ? *scale : 1.0 / std::sqrt((double)c.head_dim);
     check_rc(paia_paged_attention(q.data_ptr(), y.strides, &c, block_table.data_ptr(), block_table.stride(0), width,
                                   lens.data_ptr(), (float)s, to_int(window, "window"), out.data_ptr(),
-                                  lse.defined() ? lse.data_ptr() : nullptr, B, T, heads,
-                                  space.defined() ? space.data_ptr() : nullptr,
-                                  space.defined() ? (long long)space.nbytes() : 0, stream_of(q)),
+                                  lse.defined() ? lse.data_ptr() : nullptr, B, T, heads, space.data, space.bytes,
+                                  stream_of(q)),
              "paia_paged_attention");
 }
 at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
@@ -267,20 +281,10 @@ void lora_add_out(const at::Tensor& y, const at::Tensor& x, const at::Tensor& A,
     c10::DeviceGuard g(A.device());
     const long long need = paia_lora_add_workspace(to_int(M, "M"), to_int(K, "K"), to_int(R, "rank"), parts, slices);
     check_rc(need < 0 ? (int)need : 0, "paia_lora_add");
-    at::Tensor space;
-    if (workspace.has_value()) {
-        TORCH_CHECK(workspace->is_contiguous() && (int64_t)workspace->nbytes() >= need,
-                    "workspace must be contiguous and hold ", need, " bytes");
-        on_device_of(A, *workspace, "workspace");
-        space = *workspace;
-    } else if (need > 0) {
-        space = at::empty({need}, A.options().dtype(at::kByte));
-    }
+    const Workspace space(workspace, need, A);
     check_rc(paia_lora_add(y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), A.data_ptr(), B.data_ptr(), ids.data_ptr(),
                            opt_ptr(scaling, at::kFloat, L, A, "scaling"), out.data_ptr(), out.stride(0), (int)M,
-                           (int)K, (int)R, parts, slices, to_int(L, "adapters"),
-                           space.defined() ? space.data_ptr() : nullptr,
-                           space.defined() ? (long long)space.nbytes() : 0, stream_of(A)),
+                           (int)K, (int)R, parts, slices, to_int(L, "adapters"), space.data, space.bytes, stream_of(A)),
              "paia_lora_add");
 }
 at::Tensor lora_add(const at::Tensor& y, const at::Tensor& x, const at::Tensor& A, const at::Tensor& B,
