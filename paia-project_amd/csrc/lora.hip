@@ -33,8 +33,7 @@ constexpr int kMaxSlices = 8, kMaxPieces = 8;
 constexpr int kShrinkUnits = 512;        // blocks aimed at by the first product's split of K
 constexpr int kShrinkCols = 64;          // columns of K a wave takes at a time
 constexpr int kSmallBlock = 512, kSmallWaves = kSmallBlock / kWave;
-constexpr int kSmallRank = 32;           // rank up to which the small form takes a row's h in registers
-constexpr int64_t kSmallA = 1 << 20, kSmallReads = 64 << 20;     // bytes of A that a block, all blocks may read there
+constexpr int kSmallRank = 32;           // rank up to which the small form holds a row's h in registers
 constexpr int kShrinkAhead = 3;          // such steps whose loads a wave has in flight
 
 // What the first product tells the second: the pieces of K, and chunks of rows that share an adapter (-1: rows without one).
@@ -472,13 +471,23 @@ static int launch_small(const LoraParams& p, hipStream_t st)
     return (int)hipGetLastError();
 }
 
-// The small form reads a slice's rows of A once for every kSmallBlock outputs and row.
+// The small form reads a slice's rows of A once for every kSmallBlock outputs and row, and takes K at 4096 columns a step; its
+// ranks above 16 take each step's loads in two parts. So it is the faster one up to some bytes of A a block, and in all (us in
+// a graph, small / two launches; every row its own adapter, or in brackets all the same):
+//   rank 16: one row 4096 -> 6144 5.0 / 9.2, 14336 -> 4096 7.3 / 9.6; 16 rows of 4096 -> 6144 (25 MB) 8.2 / 11.4 (5.1 / 10.2);
+//            64 of 3584 -> 3584 (51 MB) 12.1 / 14.5; 16 of 4096 -> 28672 (117 MB) 13.4 / 15.5 (10.9 / 9.5); 16 of 14336 ->
+//            4096 (59 MB) 12.8 / 10.8 (7.4 / 10.1)
+//   rank 8:  64 rows of 4096 -> 6144 (50 MB) 11.8 / 16.3 (5.7 / 11.0); of 14336 -> 4096 (117 MB) 21.3 / 15.8 (8.9 / 10.4)
+//   rank 32: one row 4096 -> 6144 8.6 / 9.2, 14336 -> 4096 13.8 / 9.6; 4 of 3584 -> 3584 (6 MB) 8.5 / 9.3; 8 of them (13 MB)
+//            11.1 / 9.2 (8.5 / 8.9)
 static bool use_small(int M, int K, int R, const int* splits, int slices)
 {
-    if (R > kSmallRank || (int64_t)R * K * 2 > kSmallA) return false;
+    if (R > kSmallRank) return false;
+    const int64_t block = (int64_t)R * K * 2, most = R <= 16 ? 640 << 10 : 256 << 10, reads = R <= 16 ? 64 << 20 : 8 << 20;
+    if (block > most) return false;
     int64_t blocks = 0;
     for (int j = 0; j < slices; ++j) blocks += ((int64_t)splits[j] + kSmallBlock - 1) / kSmallBlock;
-    return blocks * M <= kSmallReads / ((int64_t)R * K * 2);
+    return blocks * M <= reads / block;
 }
 
 static bool lora_sizes(int M, int K, int R, const int* splits, int slices)
