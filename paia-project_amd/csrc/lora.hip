@@ -75,6 +75,15 @@ struct RowChunks {
 __device__ __forceinline__ void row_chunks(const LoraParams& p, RowChunks* s)
 {
     const int t = (int)threadIdx.x, lane = lane_id(), wave = wave_id();
+    if (p.M == 1) {                      // nothing to sort (rank 64 beside 4096 -> 6144: 9.6 -> 8.8 us a call)
+        if (t == 0) {
+            const int id = p.ids[0];
+            s->sorted[0] = (id >= 0 && id < p.adapters ? (uint32_t)id : kNoAdapter) << 8;
+            s->start[0] = 0, s->start[1] = 1, s->count = 1;
+        }
+        __syncthreads();
+        return;
+    }
     uint32_t key = ~0u;
     if (t < p.M) {
         const int id = p.ids[t];
