@@ -175,7 +175,7 @@ typedef struct {
  * (fp32 [context][rotary]: rotary/2 cosines, then the sines): dims i and i + rotary/2, or 2i and 2i+1 (interleaved).
  * Everything in fp32, rounded once to bf16 (nearest even) or, divided by the head's scale and clamped to +-448, to e4m3.
  * A slot outside [0, pages * page_size) is not written; a position outside [0, context) gives NaN in its rotated dims. Two
- * tokens of a call must not share a slot. rotary % 16 == 0, 0 < rotary <= head_dim; qkv, cos_sin, q_out, norm weights
+ * tokens of a call must not share a slot; q_out overlaps neither qkv nor the cache. rotary % 16 == 0, 0 < rotary <= head_dim; qkv, cos_sin, q_out, norm weights
  * 16-byte aligned, qkv_stride % 8 == 0; positions and slots are int64. M = 0 does nothing. */
 PAIA_API int paia_rope_append(const void* qkv, long long qkv_stride, const void* positions, const void* cos_sin,
                               int context, int rotary, int interleaved, const void* q_norm, const void* k_norm, float eps,
@@ -192,7 +192,8 @@ PAIA_API int paia_rope_append(const void* qkv, long long qkv_stride, const void*
  * fp32; the weights enter their product with v as two bf16 terms. Nothing a token does not see reaches its output, NaN and
  * infinities included. The lengths are read on the device: a captured call serves sequences as they grow.
  * workspace: device memory, 16-byte aligned, of at least paia_paged_attention_workspace() bytes (for the same cache, width,
- * B, T and heads; 0 = NULL will do, -2 = outside the contract). Calls that overlap need a workspace each. */
+ * B, T and heads; 0 = NULL will do, -2 = outside the contract). Calls that overlap need a workspace each. out overlaps no
+ * other operand. At most 65535 kv heads and T * heads / kv_heads. */
 PAIA_API long long paia_paged_attention_workspace(const paia_kv_cache* cache, int table_width, int B, int T, int heads);
 PAIA_API int paia_paged_attention(const void* q, const long long* q_strides, const paia_kv_cache* cache,
                                   const void* block_table, long long table_stride, int table_width, const void* lens,
@@ -202,7 +203,7 @@ PAIA_API int paia_paged_attention(const void* q, const long long* q_strides, con
 /* Low-rank adapters of M rows beside a shared projection: out[m][n] = y[m][n] + scaling[a] * sum_r B[a][n][r] *
  * h[m][j * rank + r], h[m] = A[a] x[m], a = ids[m]. The N = sum(splits) outputs come in `slices` <= 8 slices (q | k | v, gate |
  * up; splits: host ints), j the slice of n, each with its own `rank` rows of A. y, out bf16 [M][N] and x bf16 [M][K] with row
- * strides in elements (out may be y); A bf16 [adapters][slices * rank][K], B bf16 [adapters][N][rank], ids int32 [M] (outside
+ * strides in elements (out may be y, and overlaps nothing else); A bf16 [adapters][slices * rank][K], B bf16 [adapters][N][rank], ids int32 [M] (outside
  * [0, adapters): the row keeps y), scaling fp32 [adapters] or NULL (1). fp32 sums, one rounding at the end. rank % 8 == 0,
  * rank <= 256, K % 8 == 0, at most 2^24 - 1 adapters; x, A, B and x's rows 16-byte aligned; M = 0 does nothing. workspace as for paged attention, 16-byte
  * aligned, of paia_lora_add_workspace() bytes (0: few rows of a low rank, NULL will do; -2: outside the contract). */

@@ -88,12 +88,14 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v)      // inclusive; lan
     return dpp_add_u32<0x143, 0xC>(v);   // row_bcast:31 into rows 2, 3
 }
 __device__ __forceinline__ uint32_t last_lane(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, kWave - 1); }
-// Pieces of a sequence at `most` tiles a piece, at least one. The float quotient is within one of the true one (there are
-// at most p.goal pieces, a few thousand) and is corrected.
+// Pieces of a sequence at `most` tiles a piece, at least one: ceil(tiles / most) by a float quotient, which below 2^26 tiles is a
+// few off at most, its remainder's own quotient, which is within one, and a correction.
 __device__ __forceinline__ uint32_t pieces_of(int tiles, int most, float inverse)
 {
     int n = (int)((float)tiles * inverse);
     int left = tiles - n * most;
+    const int more = (int)((float)left * inverse);
+    n += more, left -= more * most;
     if (left < 0) --n, left += most;
     if (left >= most) ++n, left -= most;
     return (uint32_t)max(1, n + (left > 0 ? 1 : 0));
@@ -106,57 +108,67 @@ struct Piece {
     int b, len, tile0, tile1;        // sequence, its length, the piece's tiles
     int index, count;                // number of the piece in its sequence, pieces of the sequence
 };
-// The piece with number `item`. Every wave finds the same tile count per piece, `most`: from the mean over p.goal pieces up,
-// until the sequences' pieces, each sequence's last one shorter, are no more than p.goal.
+__device__ __forceinline__ void take_piece(int b, const Span& s, int count, int index, Piece* r)
+{
+    const int each = s.tiles / count, more = s.tiles - each * count;     // the first `more` pieces get one more
+    r->b = b, r->len = s.len, r->index = index, r->count = count;
+    r->tile0 = s.tile0 + index * each + min(index, more);
+    r->tile1 = r->tile0 + each + (index < more ? 1 : 0);
+}
+__device__ __forceinline__ Span lane_span(const Span& s, int lane)
+{
+    return {__builtin_amdgcn_readlane(s.len, lane), __builtin_amdgcn_readlane(s.tile0, lane),
+            __builtin_amdgcn_readlane(s.tiles, lane)};
+}
+// The piece with number `item`. Every wave finds the same tile count per piece, `most`: from the least up, by the factor that
+// the sequences' pieces are too many, until they are no more than p.goal.
 __device__ __forceinline__ bool find_piece(const AttnParams& p, int item, Piece* r)
 {
     const int lane = lane_id();
-    if (p.B == 1) {                      // the same without sums over sequences
+    if (p.B == 1) {
         const Span s = span_of(p, 0);
-        const int most = max(kMinTiles, whole_rounds((float)s.tiles * __builtin_amdgcn_rcpf((float)p.goal)));
+        const int mean = (s.tiles + p.goal - 1) / p.goal;
+        const int most = max(kMinTiles, (mean + kAttnWaves - 1) / kAttnWaves * kAttnWaves);
         const int count = max(1, (s.tiles + most - 1) / most);
-        const int each = s.tiles / count, more = s.tiles - each * count;
-        *r = {0, s.len, s.tile0 + item * each + min(item, more), 0, item, count};
-        r->tile1 = r->tile0 + each + (item < more ? 1 : 0);
+        take_piece(0, s, count, item, r);
         return item < count;
     }
     Span s = span_of(p, lane);
-    float total = (float)last_lane(wave_scan((uint32_t)s.tiles));
-    for (int b = kWave; b < p.B; b += kWave) total += (float)last_lane(wave_scan((uint32_t)span_of(p, b + lane).tiles));
     const float per = __builtin_amdgcn_rcpf((float)p.goal);
-    int most = max(kMinTiles, whole_rounds(total * per));
-    float inverse = 0.0f;
-    for (int tries = 0; tries < 5; ++tries) {
+    int most = kMinTiles;
+    float inverse = 0.0f, tiles = 0.0f;
+    uint32_t n = 0, end = 0;
+#pragma nounroll
+    for (int tries = 0; tries < 6; ++tries) {
         inverse = __builtin_amdgcn_rcpf((float)most);
-        uint32_t count = last_lane(wave_scan(lane < p.B ? pieces_of(s.tiles, most, inverse) : 0u));
+        n = lane < p.B ? pieces_of(s.tiles, most, inverse) : 0u;
+        end = wave_scan(n);
+        uint64_t count = last_lane(end);
+#pragma nounroll
         for (int b = kWave; b < p.B; b += kWave)
             count += last_lane(wave_scan(b + lane < p.B ? pieces_of(span_of(p, b + lane).tiles, most, inverse) : 0u));
-        if (count <= (uint32_t)p.goal) break;
-        // the last try holds for any lengths: total / most + B pieces at most (with room for the roundings of `total`)
-        most = tries < 3 ? whole_rounds((float)most * (float)count * per)
-                         : whole_rounds(total * 1.001f * __builtin_amdgcn_rcpf((float)(p.goal - p.B)));
+        if (count <= (uint64_t)p.goal) break;
+        const float held = (float)most * (float)count;       // no less than the tiles there are
+        if (tries == 0) tiles = held;
+        // the fourth step holds for any lengths: tiles / most + B pieces at most (with room for the roundings)
+        most = tries < 3 ? whole_rounds(held * per) : whole_rounds(tiles * 1.001f * __builtin_amdgcn_rcpf((float)(p.goal - p.B)));
     }
     uint32_t before = 0;
-    for (int b0 = 0; b0 < p.B; b0 += kWave) {
-        if (b0 > 0) s = span_of(p, b0 + lane);
-        const uint32_t n = b0 + lane < p.B ? pieces_of(s.tiles, most, inverse) : 0u;
-        const uint32_t end = before + wave_scan(n);
+#pragma nounroll
+    for (int b0 = 0;;) {
         const uint64_t here = __ballot((uint32_t)item < end && (uint32_t)item >= end - n);
         if (here != 0) {
-            const int src = __builtin_ctzll(here);
-            const int tiles = __builtin_amdgcn_readlane(s.tiles, src), t0 = __builtin_amdgcn_readlane(s.tile0, src);
-            r->b = b0 + src;
-            r->len = __builtin_amdgcn_readlane(s.len, src);
-            r->count = __builtin_amdgcn_readlane((int)n, src);
-            r->index = item - (__builtin_amdgcn_readlane((int)end, src) - r->count);
-            const int each = tiles / r->count, more = tiles - each * r->count;     // the first `more` pieces get one more
-            r->tile0 = t0 + r->index * each + min(r->index, more);
-            r->tile1 = r->tile0 + each + (r->index < more ? 1 : 0);
+            const int src = __builtin_ctzll(here), count = __builtin_amdgcn_readlane((int)n, src);
+            take_piece(b0 + src, lane_span(s, src), count, item - (__builtin_amdgcn_readlane((int)end, src) - count), r);
             return true;
         }
         before = last_lane(end);
+        b0 += kWave;
+        if (b0 >= p.B) return false;
+        s = span_of(p, b0 + lane);
+        n = b0 + lane < p.B ? pieces_of(s.tiles, most, inverse) : 0u;
+        end = before + wave_scan(n);
     }
-    return false;
 }
 
 // ---- lanes l, l^16, l^32, l^48 ---------------------------------------------------------------------------------------
@@ -644,7 +656,7 @@ int paia_paged_attention(const void* q, const long long* q_strides, const paia_k
     if (B == 0) return 0;
     if (q == nullptr || q_strides == nullptr || lens == nullptr || out == nullptr || (block_table == nullptr && table_width > 0))
         return -2;
-    if (!aligned(q, 16) || !aligned(block_table, 4) || !aligned(lens, 4) || !aligned(out, 16) || !aligned(lse, 4)) return -2;
+    if (out == q || !aligned(q, 16) || !aligned(block_table, 4) || !aligned(lens, 4) || !aligned(out, 16) || !aligned(lse, 4)) return -2;
     for (int i = 0; i < 3; ++i)
         if (q_strides[i] < 0 || q_strides[i] % 8) return -2;
     if (bytes > 0 && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < bytes)) return -2;

@@ -209,7 +209,7 @@ int paia_rope_append(const void* qkv, long long qkv_stride, const void* position
     if (context <= 0 || rotary <= 0 || rotary % 16 || rotary > cache->head_dim) return -2;
     if (M == 0) return 0;
     if (qkv == nullptr || positions == nullptr || cos_sin == nullptr || slots == nullptr || q_out == nullptr) return -2;
-    if (!aligned(qkv, 16) || !aligned(cos_sin, 16) || !aligned(q_out, 16) || !aligned(q_norm, 16) || !aligned(k_norm, 16) ||
+    if (q_out == qkv || !aligned(qkv, 16) || !aligned(cos_sin, 16) || !aligned(q_out, 16) || !aligned(q_norm, 16) || !aligned(k_norm, 16) ||
         !aligned(positions, 8) || !aligned(slots, 8) || qkv_stride % 8)
         return -2;
     p.qkv = static_cast<const uint8_t*>(qkv);

@@ -22,6 +22,8 @@ def f32(v):
 def pieces_of(tiles, most, inverse):
     n = int(f32(f32(tiles) * inverse))
     left = tiles - n * most
+    more = int(f32(f32(left) * inverse))
+    n, left = n + more, left - more * most
     if left < 0:
         n, left = n - 1, left + most
     if left >= most:
@@ -37,18 +39,20 @@ def whole_rounds(tiles):
 def piece_tiles(tiles, goal, jitter):
     """`jitter`: relative error of the hardware's reciprocal, at most 1 ulp."""
     rcp = lambda v: f32(f32(1.0 / v) * (1.0 + jitter))  # noqa: E731
-    total = 0.0
-    for b in range(0, len(tiles), 64):
-        total = f32(total + f32(sum(tiles[b:b + 64])))
-    per = rcp(goal)
-    most = max(MIN_TILES, whole_rounds(f32(total * per)))
-    for tries in range(5):
+    if len(tiles) == 1:
+        mean = -(-tiles[0] // goal)
+        most = max(MIN_TILES, -(-mean // WAVES) * WAVES)
+        return most, rcp(most), 0
+    per, most = rcp(goal), MIN_TILES
+    for tries in range(6):
         inverse = rcp(most)
         count = sum(pieces_of(t, most, inverse) for t in tiles)
         if count <= goal:
             break
-        most = whole_rounds(f32(f32(most * f32(count)) * per) if tries < 3
-                            else f32(f32(total * f32(1.001)) * rcp(goal - len(tiles))))
+        held = f32(most * f32(count))
+        if tries == 0:
+            total = held
+        most = whole_rounds(f32(held * per) if tries < 3 else f32(f32(total * f32(1.001)) * rcp(goal - len(tiles))))
     return most, inverse, tries
 
 
@@ -72,7 +76,8 @@ def test_pieces_cover_every_tile_once_and_fit(seed):
         assert tries <= 4
         used = 0
         for tile0, tiles in spans:
-            n = pieces_of(tiles, most, inverse)
+            n = max(1, -(-tiles // most))
+            assert B == 1 or n == pieces_of(tiles, most, inverse)
             used += n
             each, more = divmod(tiles, n)
             ends = [(j * each + min(j, more), (j + 1) * each + min(j + 1, more)) for j in range(n)]

@@ -27,7 +27,7 @@ BAD_CACHES = [dict(k=None), dict(v=A + 8), dict(pages=0), dict(page_size=0), dic
 
 def rope(lib, c, **change):
     a = dict(qkv=A, stride=48 * 128, positions=A, cos_sin=A, context=100, rotary=128, q_norm=None, k_norm=None, slots=A,
-             q=A, M=4, heads=32)
+             q=A + 4096, M=4, heads=32)
     a.update(change)
     return lib._lib.paia_rope_append(a["qkv"], a["stride"], a["positions"], a["cos_sin"], a["context"], a["rotary"], 0,
                                      a["q_norm"], a["k_norm"], 1e-6, a["slots"], ctypes.byref(c) if c else None, a["q"],
@@ -40,7 +40,7 @@ def test_rope_append_refusals(gemv_lib):
     assert rope(gemv_lib, None) == -2
     for bad in (dict(qkv=A + 8), dict(qkv=None), dict(stride=6148), dict(positions=A + 4), dict(cos_sin=A + 4),
                 dict(context=0), dict(rotary=0), dict(rotary=136), dict(rotary=144), dict(rotary=24), dict(q_norm=A + 8),
-                dict(k_norm=A + 2), dict(slots=None), dict(q=A + 4), dict(M=-1), dict(heads=0)):
+                dict(k_norm=A + 2), dict(slots=None), dict(q=A + 4), dict(q=A), dict(M=-1), dict(heads=0)):
         assert rope(gemv_lib, cache(), **bad) == -2, bad
     assert rope(gemv_lib, cache(), M=0) == 0
 
@@ -73,7 +73,7 @@ def test_rope_table_refuses(bad):
 
 
 def attention(lib, c, **change):
-    a = dict(q=A, strides=(4096, 4096, 128), table=A, stride=64, width=64, lens=A, window=0, out=A, lse=None, B=2, T=1,
+    a = dict(q=A, strides=(4096, 4096, 128), table=A, stride=64, width=64, lens=A, window=0, out=A + 4096, lse=None, B=2, T=1,
              heads=32, space=A, bytes=1 << 40)
     a.update(change)
     st = (ctypes.c_longlong * 3)(*a["strides"]) if a["strides"] else None
@@ -88,7 +88,7 @@ def test_paged_attention_refusals(gemv_lib):
     assert attention(gemv_lib, None) == -2
     for bad in (dict(q=None), dict(q=A + 8), dict(strides=None), dict(strides=(4096, 4096, 132)),
                 dict(strides=(-4096, 4096, 128)), dict(table=None), dict(table=A + 2), dict(stride=-1), dict(width=-1),
-                dict(lens=None), dict(lens=A + 1), dict(window=-1), dict(out=None), dict(out=A + 8), dict(lse=A + 2),
+                dict(lens=None), dict(lens=A + 1), dict(window=-1), dict(out=None), dict(out=A + 8), dict(out=A), dict(lse=A + 2),
                 dict(B=-1), dict(T=0), dict(heads=0), dict(heads=30), dict(space=None), dict(space=A + 8), dict(bytes=100),
                 dict(T=1 << 30), dict(B=1 << 28)):
         assert attention(gemv_lib, cache(), **bad) == -2, bad
