@@ -157,11 +157,11 @@ PAIA_API int paia_gemv_batch_int4_zp(const void* Wq, const void* scales, const v
  *      an entry point takes a workspace, the caller owns it, its contents need no preparation and nothing is kept in it
  *      from one call to the next. -------------------------------------------------------------------------------- */
 
-/* A paged key-value cache: pages of page_size positions for each of kv_heads heads of head_dim values. Element (page,
- * head, position, i) of k lies at k + page * k_strides[0] + head * k_strides[1] + position * k_strides[2] + i (in
- * elements), so heads and positions may come in either order. fp8 = 0: bf16; 1: e4m3fn codes, which stand for code *
- * k_scale[head] (fp32 [kv_heads], NULL = 1). head_dim 64, 128 or 256; k and v 16-byte aligned, strides >= 0 and multiples
- * of 16 bytes; page_size >= 1 of any size. Slot s is position s % page_size of page s / page_size. */
+/* A paged key-value cache: pages of page_size positions for each of kv_heads heads of head_dim values. Element
+ * (page, head, position, i) of k lies at k + page * k_strides[0] + head * k_strides[1] + position * k_strides[2] +
+ * i (in elements), so heads and positions may come in either order. fp8 = 0: bf16; 1: e4m3fn codes, which stand for
+ * code * k_scale[head] (fp32 [kv_heads], NULL = 1). head_dim 64, 128 or 256; k and v 16-byte aligned, strides >= 0
+ * and multiples of 16 bytes; page_size >= 1 of any size. Slot s is position s % page_size of page s / page_size. */
 typedef struct {
     void *k, *v;
     const float *k_scale, *v_scale;
@@ -169,31 +169,33 @@ typedef struct {
     int pages, page_size, kv_heads, head_dim, fp8;
 } paia_kv_cache;
 
-/* One token's fused projection q|k|v (qkv bf16, row m at qkv + m * qkv_stride, (heads + 2 kv_heads) * head_dim values) ->
- * q_out bf16 [M][heads][head_dim] and, at slot slots[m], k and v in the cache. q and k heads: x *= rsqrt(mean(x^2) + eps)
- * * norm weight where a weight (bf16 [head_dim]) is given, then the first `rotary` dims turn by row positions[m] of cos_sin
- * (fp32 [context][rotary]: rotary/2 cosines, then the sines): dims i and i + rotary/2, or 2i and 2i+1 (interleaved).
- * Everything in fp32, rounded once to bf16 (nearest even) or, divided by the head's scale and clamped to +-448, to e4m3.
- * A slot outside [0, pages * page_size) is not written; a position outside [0, context) gives NaN in its rotated dims. Two
- * tokens of a call must not share a slot; q_out overlaps neither qkv nor the cache. rotary % 16 == 0, 0 < rotary <= head_dim; qkv, cos_sin, q_out, norm weights
- * 16-byte aligned, qkv_stride % 8 == 0; positions and slots are int64. M = 0 does nothing. */
+/* One token's fused projection q|k|v (qkv bf16, row m at qkv + m * qkv_stride, (heads + 2 kv_heads) * head_dim
+ * values) -> q_out bf16 [M][heads][head_dim] and, at slot slots[m], k and v in the cache. q and k heads: x *=
+ * rsqrt(mean(x^2) + eps) * norm weight where a weight (bf16 [head_dim]) is given, then the first `rotary` dims turn
+ * by row positions[m] of cos_sin (fp32 [context][rotary]: rotary/2 cosines, then the sines): dims i and i +
+ * rotary/2, or 2i and 2i+1 (interleaved). Everything in fp32, rounded once to bf16 (nearest even) or, divided by
+ * the head's scale and clamped to +-448, to e4m3. A slot outside [0, pages * page_size) is not written; a position
+ * outside [0, context) gives NaN in its rotated dims. Two tokens of a call must not share a slot; q_out overlaps
+ * neither qkv nor the cache. rotary % 16 == 0, 0 < rotary <= head_dim; qkv, cos_sin, q_out, norm weights 16-byte
+ * aligned, qkv_stride % 8 == 0; positions and slots are int64. M = 0 does nothing. */
 PAIA_API int paia_rope_append(const void* qkv, long long qkv_stride, const void* positions, const void* cos_sin,
                               int context, int rotary, int interleaved, const void* q_norm, const void* k_norm, float eps,
                               const void* slots, const paia_kv_cache* cache, void* q_out, int M, int heads, void* stream);
 
-/* Attention of each sequence's T newest tokens over the cache. q bf16, element (b, t, head, i) at q + b * q_strides[0] +
- * t * q_strides[1] + head * q_strides[2] + i (elements, multiples of 8; q 16-byte aligned); heads % kv_heads == 0, query
- * head j reads kv head j / (heads / kv_heads). lens int32 [B]: positions of sequence b in the cache, the T tokens' own
- * included; block_table int32, row b at block_table + b * table_stride: table_width page numbers, position p on page
- * number p / page_size. Token t sees positions p < lens[b] - (T-1-t), of these the last `window` where window > 0, and none
- * on a page number outside [0, pages) (lengths beyond the table's width end there). With s_p = scale * k_scale[head] *
- * <q, k_p>: out bf16 [B][T][heads][head_dim] (16-byte aligned) = v_scale[head] * sum softmax(s)_p v_p, lse fp32
- * [B][T][heads] or NULL = log(sum exp(s_p)); a token that sees nothing has out 0, lse -inf. Scores, statistics and sums in
- * fp32; the weights enter their product with v as two bf16 terms. Nothing a token does not see reaches its output, NaN and
- * infinities included. The lengths are read on the device: a captured call serves sequences as they grow.
- * workspace: device memory, 16-byte aligned, of at least paia_paged_attention_workspace() bytes (for the same cache, width,
- * B, T and heads; 0 = NULL will do, -2 = outside the contract). Calls that overlap need a workspace each. out overlaps no
- * other operand. At most 65535 kv heads and T * heads / kv_heads. */
+/* Attention of each sequence's T newest tokens over the cache. q bf16, element (b, t, head, i) at q + b *
+ * q_strides[0] + t * q_strides[1] + head * q_strides[2] + i (elements, multiples of 8; q 16-byte aligned); heads %
+ * kv_heads == 0, query head j reads kv head j / (heads / kv_heads). lens int32 [B]: positions of sequence b in the
+ * cache, the T tokens' own included; block_table int32, row b at block_table + b * table_stride: table_width page
+ * numbers, position p on page number p / page_size. Token t sees positions p < lens[b] - (T-1-t), of these the last
+ * `window` where window > 0, and none on a page number outside [0, pages) (lengths beyond the table's width end
+ * there). With s_p = scale * k_scale[head] * <q, k_p>: out bf16 [B][T][heads][head_dim] (16-byte aligned) =
+ * v_scale[head] * sum softmax(s)_p v_p, lse fp32 [B][T][heads] or NULL = log(sum exp(s_p)); a token that sees
+ * nothing has out 0, lse -inf. Scores, statistics and sums in fp32; the weights enter their product with v as two
+ * bf16 terms. Nothing a token does not see reaches its output, NaN and infinities included. The lengths are read on
+ * the device: a captured call serves sequences as they grow. workspace: device memory, 16-byte aligned, of at least
+ * paia_paged_attention_workspace() bytes (for the same cache, width, B, T and heads; 0 = NULL will do, -2 = outside
+ * the contract). Calls that overlap need a workspace each. out overlaps no other operand. At most 65535 kv heads
+ * and T * heads / kv_heads. */
 PAIA_API long long paia_paged_attention_workspace(const paia_kv_cache* cache, int table_width, int B, int T, int heads);
 PAIA_API int paia_paged_attention(const void* q, const long long* q_strides, const paia_kv_cache* cache,
                                   const void* block_table, long long table_stride, int table_width, const void* lens,
@@ -201,11 +203,12 @@ PAIA_API int paia_paged_attention(const void* q, const long long* q_strides, con
                                   long long workspace_bytes, void* stream);
 
 /* Low-rank adapters of M rows beside a shared projection: out[m][n] = y[m][n] + scaling[a] * sum_r B[a][n][r] *
- * h[m][j * rank + r], h[m] = A[a] x[m], a = ids[m]. The N = sum(splits) outputs come in `slices` <= 8 slices (q | k | v, gate |
- * up; splits: host ints), j the slice of n, each with its own `rank` rows of A. y, out bf16 [M][N] and x bf16 [M][K] with row
- * strides in elements (out may be y, and overlaps nothing else); A bf16 [adapters][slices * rank][K], B bf16 [adapters][N][rank], ids int32 [M] (outside
- * [0, adapters): the row keeps y), scaling fp32 [adapters] or NULL (1). fp32 sums, one rounding at the end. rank % 8 == 0,
- * rank <= 256, K % 8 == 0, at most 2^24 - 1 adapters; x, A, B and x's rows 16-byte aligned; M = 0 does nothing. workspace as for paged attention, 16-byte
+ * h[m][j * rank + r], h[m] = A[a] x[m], a = ids[m]. The N = sum(splits) outputs come in `slices` <= 8 slices (q | k
+ * | v, gate | up; splits: host ints), j the slice of n, each with its own `rank` rows of A. y, out bf16 [M][N] and
+ * x bf16 [M][K] with row strides in elements (out may be y, and overlaps nothing else); A bf16 [adapters][slices *
+ * rank][K], B bf16 [adapters][N][rank], ids int32 [M] (outside [0, adapters): the row keeps y), scaling fp32
+ * [adapters] or NULL (1). fp32 sums, one rounding at the end. rank % 8 == 0, rank <= 256, K % 8 == 0, at most 2^24
+ * - 1 adapters; x, A, B and x's rows 16-byte aligned; M = 0 does nothing. workspace as for paged attention, 16-byte
  * aligned, of paia_lora_add_workspace() bytes (0: few rows of a low rank, NULL will do; -2: outside the contract). */
 PAIA_API long long paia_lora_add_workspace(int M, int K, int rank, const int* splits, int slices);
 PAIA_API int paia_lora_add(const void* y, long long y_stride, const void* x, long long x_stride, const void* A,

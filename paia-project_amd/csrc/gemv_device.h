@@ -340,6 +340,22 @@ __device__ __forceinline__ float quad_sum(float v)
     return v;
 }
 
+// LDS order between a lane's writes and other lanes' reads of one wave: the hardware keeps a wave's LDS operations in
+// order, the compiler has to (no instruction comes of it).
+__device__ __forceinline__ void wave_lds_order()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// D = A B + C on the matrix cores: lane l holds row (A) or column (B) l % 16 and contraction values 8 (l / 16) .. + 7, of C and
+// D column l % 16 and rows 4 (l / 16) .. + 3.
+__device__ __forceinline__ f32x4 mfma_16x16x32(const u32x4 a, const u32x4 b, const f32x4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
 __device__ __forceinline__ int lane_id() { return (int)(threadIdx.x & 63); }
 

@@ -81,15 +81,6 @@ __host__ __device__ constexpr uint32_t tile_wave_bytes()
     return x + w > (uint32_t)P * 1024u ? x + w : (uint32_t)P * 1024u;
 }
 
-// LDS order between a lane's writes and other lanes' reads of one wave: the hardware keeps a wave's LDS operations in
-// order, the compiler has to (no instruction comes of it).
-__device__ __forceinline__ void wave_lds_order()
-{
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // INT4: the 128 terms of a group, up to 15 |x| each, could leave fp32's range where |x| reaches 2^116 although the output
 // (scales are small) does not. So nibbles and sums of x carry a factor 2^-11: no finite x overflows, and at the other end
 // nothing is lost (a bf16 x is a multiple of 2^-133, its products of 2^-144, and the matrix cores keep subnormals down to

@@ -17,8 +17,8 @@
 #include <limits.h>
 #include <stdint.h>
 
+#include "divisor.h"
 #include "gemv_kernel.h"
-#include "kv_cache.h"
 #include "paia_gemv.h"
 
 namespace paia {
@@ -135,10 +135,6 @@ __device__ __forceinline__ int k_pieces(const LoraParams& p, int chunks)
     return max(1, min(most, kShrinkUnits / units));
 }
 
-__device__ __forceinline__ f32x4 lora_mfma(const u32x4 a, const u32x4 b, const f32x4 c)
-{
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
 __device__ __forceinline__ u32x4 load16_if(const uint16_t* p, bool take)
 {
     return take ? *reinterpret_cast<const u32x4*>(p) : u32x4{0, 0, 0, 0};
@@ -148,13 +144,6 @@ __device__ __forceinline__ u32x4 load16_if(const uint16_t* p, bool take)
 __device__ __forceinline__ float rest(float v, uint32_t rounded)
 {
     return fabsf(__uint_as_float(rounded)) < 3.4e38f ? v - __uint_as_float(rounded) : 0.0f;
-}
-
-__device__ __forceinline__ void lora_lds_order()     // a wave's LDS operations stay in order; the compiler has to keep them so
-{
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 // h: a unit is (chunk, 16 rows of A, piece of K); the block's waves take its steps of 64 columns in turn. Eight lanes load
@@ -210,14 +199,14 @@ __global__ void __launch_bounds__(kShrinkBlock) lora_shrink_kernel(const LoraPar
                     stage[wave][0][at] = u[i][e];
                     stage[wave][1][at] = v[i][e];
                 }
-                lora_lds_order();
+                wave_lds_order();
                 load(s + (kShrinkAhead + i) * kShrinkWaves, i);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const int at = n * 8 + ((4 * j + g) ^ (n >> 1));
-                    acc = lora_mfma(stage[wave][0][at], stage[wave][1][at], acc);
+                    acc = mfma_16x16x32(stage[wave][0][at], stage[wave][1][at], acc);
                 }
-                lora_lds_order();
+                wave_lds_order();
             }
         }
         sums[wave][lane] = acc;
@@ -354,7 +343,7 @@ __global__ void __launch_bounds__(kLoraBlock) lora_expand_kernel(const LoraParam
             uint2 y[kTiles];
 #pragma unroll
             for (int t = 0; t < kTiles; ++t) y[t] = was[i][t];
-            lora_lds_order();
+            wave_lds_order();
             load(unit + kExpandAhead, i);
             uint16_t* out = p.out + m * p.out_stride + r.n0;
             const bool same = id < 0 && p.out == p.y && p.out_stride == p.y_stride;     // the row keeps y where it is
@@ -364,8 +353,8 @@ __global__ void __launch_bounds__(kLoraBlock) lora_expand_kernel(const LoraParam
 #pragma unroll
                 for (int s = 0; s < STEPS; ++s) {
                     const u32x4 w = 4 * s + g < row_pieces ? b_of[wave][(16 * t + n) * pitch + 4 * s + g] : u32x4{0, 0, 0, 0};
-                    acc = lora_mfma(w, lo[s], acc);
-                    acc = lora_mfma(w, hi[s], acc);
+                    acc = mfma_16x16x32(w, lo[s], acc);
+                    acc = mfma_16x16x32(w, hi[s], acc);
                 }
                 const int o = 16 * t + 4 * g;
                 if (n >= held || o >= r.width || same) continue;
@@ -383,7 +372,7 @@ __global__ void __launch_bounds__(kLoraBlock) lora_expand_kernel(const LoraParam
                     if (o + 3 < r.width) out[o + 3] = (uint16_t)(v.y >> 16);
                 }
             }
-            lora_lds_order();
+            wave_lds_order();
         }
     }
 }

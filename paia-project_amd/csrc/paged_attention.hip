@@ -186,17 +186,6 @@ __device__ __forceinline__ float col_sum(float v)
     r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-__device__ __forceinline__ void lds_order()      // a wave's LDS operations stay in order; the compiler has to keep them so
-{
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-__device__ __forceinline__ f32x4 mfma(const u32x4 a, const u32x4 b, const f32x4 c)
-{
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 template <int N> struct Words { uint32_t w[N]; };
 template <bool STREAM, typename T>
@@ -359,7 +348,7 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
             *reinterpret_cast<u32x4*>(mine + r * L::kRow + 16 * (kpiece ^ L::swizzle(r))) =
                 u32x4{k[i].w[0], k[i].w[1], k[i].w[2], k[i].w[3]};
         }
-        lds_order();
+        wave_lds_order();
         uint32_t vok_next = 0;
         if (more) {
             load_k(next);
@@ -384,10 +373,10 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
                 } else {
                     a = *reinterpret_cast<const u32x4*>(row + 16 * ((4 * j + g) ^ L::swizzle(r)));
                 }
-                s[half] = mfma(a, q[j], s[half]);
+                s[half] = mfma_16x16x32(a, q[j], s[half]);
             }
         }
-        lds_order();
+        wave_lds_order();
         const int p0 = tile * kTile;
         const bool masked = p0 + kTile > all_hi || p0 < all_lo || __ballot(vok != 0xFFu) != 0;
         float top = -INFINITY;
@@ -441,8 +430,8 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
                                     __builtin_amdgcn_perm(x[5], x[4], 0x05040100u), __builtin_amdgcn_perm(x[7], x[6], 0x05040100u)};
                 const u32x4 odd = {__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u),
                                    __builtin_amdgcn_perm(x[5], x[4], 0x07060302u), __builtin_amdgcn_perm(x[7], x[6], 0x07060302u)};
-                const f32x4 a = mfma(even, top8, mfma(even, rest8, o[2 * d]));
-                const f32x4 b = mfma(odd, top8, mfma(odd, rest8, o[2 * d + 1]));
+                const f32x4 a = mfma_16x16x32(even, top8, mfma_16x16x32(even, rest8, o[2 * d]));
+                const f32x4 b = mfma_16x16x32(odd, top8, mfma_16x16x32(odd, rest8, o[2 * d + 1]));
                 if (all) {
                     o[2 * d] = a, o[2 * d + 1] = b;
                 } else {

@@ -101,7 +101,7 @@ def test_uniform_lengths_use_what_is_aimed_at():
 
 
 def test_division_by_multiplication():
-    """csrc/kv_cache.h, Divisor: exact for every dividend below 2^31."""
+    """csrc/divisor.h: exact for every dividend below 2^31."""
     r = random.Random(1)
     for d in list(range(1, 300)) + [2 ** k + e for k in range(8, 31) for e in (-1, 0, 1)] + [2 ** 31 - 1]:
         s = 0
