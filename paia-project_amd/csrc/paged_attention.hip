@@ -5,7 +5,8 @@
 //
 // Each cache byte is used for T G products a value (G query heads share a kv head), a few operations per byte: bound by
 // reading the cache once. The pieces of the design:
-//   * Work: a unit is one piece of one sequence for one kv head and up to 16 columns (token, query head of the group). The
+//   * Work: a unit is one piece of one sequence for one kv head and 16 columns (token, query head of the group), or
+//     up to 48 where the cache is large (most_tiles). The
 //     lengths are on the device and the grid is fixed by the host, so each block derives the split from the lengths
 //     itself (find_piece): about as many equal pieces as blocks fit the chip, whatever the lengths are. A captured call
 //     stays balanced as the sequences grow. Pieces of one sequence leave (m, l, o) in the workspace, joined by a second
@@ -14,7 +15,8 @@
 //     barrier until the end), and one tile of K and V loads in flight ahead of the one in work.
 //   * S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_bf16. Both leave a column (token, head) on the same lane, so
 //     P goes from the first product's result to the second's operand in registers, and the rescaling is per lane.
-//   * K rows are loaded contiguously and brought to the matrix layout through a wave-private piece of LDS (XOR swizzle).
+//   * K rows are loaded contiguously and brought to the matrix layout through a wave-private piece of LDS (XOR swizzle), by way
+//     of registers or, where those are short (loads_direct), straight there.
 //     V rows are loaded contiguously too, D/16 dims of eight positions per lane: 16 lanes are the 16 rows of the V^T
 //     operand, whose eight contraction values are the eight positions; one v_perm_b32 per register pairs them up.
 //   * e4m3 codes become bf16 exactly (v_cvt_scalef32_pk_bf16_fp8); the heads' factors go to the scores and the output.
@@ -34,10 +36,19 @@
 namespace paia {
 
 constexpr int kTile = 32;            // positions a wave takes at a time
-constexpr int kCols = 16;            // columns (token, head) of a unit
+constexpr int kCols = 16;            // columns (token, head) of a matrix tile; a block takes up to most_tiles() such tiles
+// Tiles of columns that a block takes together, so that each row is read and taken apart once for all: as many as a lane's
+// registers hold the outputs of (e4m3 heads of 128 spill with two: 84 us for 61). A block of several tiles stages its queries
+// and does more after its last row, so it takes caches that fill the chip for longer: kTogether bytes, as the block table's
+// size bounds them. Five tokens of 4 and of 8 heads a group, 8 sequences, us with one tile a block / together:
+//   bf16 heads of 128, 2500 positions 20.6 / 22.9 and 23.7 / 27.0; 6000 (164 MB) 46.0 / 44.2 and 51.8 / 52.6; 16000 91 / 86
+//   and 114 / 100; heads of 64, 6000 (82 MB) 22.5 / 23.5 and 28.8 / 29.3; 16000 (200 MB) 54 / 47 and 66 / 52; e4m3, 16000
+//   (100 MB) 40.7 / 38.7 and 53.9 / 49.2.
+constexpr int most_tiles(int dim, bool fp8, bool p8) { return dim <= 64 ? 3 : dim <= 128 && p8 && !fp8 ? 2 : 1; }
+constexpr int64_t kTogether = 120 << 20;
 constexpr int kAttnWaves = 4, kAttnBlock = kAttnWaves * kWave;
 // Blocks that a CU holds at the registers a wave takes (one wave of a block on each SIMD).
-constexpr int blocks_per_cu(int dim) { return dim <= 64 ? 3 : dim <= 128 ? 2 : 1; }
+constexpr int blocks_per_cu(int dim, int tiles) { return dim <= 64 ? (tiles == 1 ? 3 : 2) : dim <= 128 ? 2 : 1; }
 constexpr int kMinTiles = 4;         // a piece is at least this many tiles, where the sequence has them
 
 struct AttnParams {
@@ -51,7 +62,7 @@ struct AttnParams {
     float *part_o, *part_ml;         // [item][kv head][column][D], [item][kv head][column][2]
     int2* part_of;                   // [sequence]: first item, number of items
     float scale;                     // scale * log2(e)
-    int B, T, heads, group, cols, col_groups;
+    int B, T, heads, group, cols, col_groups, tiles;     // tiles of columns a block takes
     int window, max_len;             // positions the table can hold
     int goal;                        // pieces per kv head at most, the items of the grid; above B
     int units;                       // items * kv heads
@@ -188,6 +199,13 @@ __device__ __forceinline__ float col_sum(float v)
 }
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 template <int N> struct Words { uint32_t w[N]; };
+// 16 bytes from each lane's address to LDS, at the wave's base + 16 * lane.
+template <bool STREAM>
+__device__ __forceinline__ void lds_load16(uint8_t* base, const uint8_t* p)
+{
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
+                                     (__attribute__((address_space(3))) void*)base, 16, 0, STREAM ? 2 : 0);
+}
 template <bool STREAM, typename T>
 __device__ __forceinline__ T load_as(const uint8_t* p)
 {
@@ -215,6 +233,11 @@ __device__ __forceinline__ Words<N> load_words(const uint8_t* p)
     return r;
 }
 
+// K goes straight to LDS where its registers would spill or halve the waves of a CU: bf16 heads of 256 (12000 positions of 8
+// sequences 161 -> 146 us) and of 128 with two tiles of columns. Elsewhere a tile in registers is the better prefetch: its
+// LDS place is free as soon as it is written, not when the scores are done (e4m3 139 us against 143 so, bf16 248 and 245).
+constexpr bool loads_direct(int dim, bool fp8, int tiles) { return !fp8 && (dim == 256 || (dim == 128 && tiles > 1)); }
+
 // P8: pages are multiples of eight positions, so eight aligned positions lie on one page
 template <int D, bool FP8, bool P8>
 struct Layout {
@@ -225,8 +248,15 @@ struct Layout {
     static constexpr int kKStep = P8 ? (kKLoads < 8 ? kKLoads : 8) : 1;    // positions per page lookup
     static constexpr int kVStep = P8 ? 8 : 1;
     static constexpr int kKPages = kKLoads / kKStep, kVPages = 8 / kVStep;
+    static constexpr int kQueryPitch = D / 8 + 1;            // 16-byte pieces between the queries in LDS
     static constexpr int kOutStride = D + 4;                 // floats between the columns of a wave's output in LDS
     static constexpr int kWaveLds = kCols * kOutStride * 4 > kTile * kRow ? kCols * kOutStride * 4 : kTile * kRow;
+    // Where row r of a tile lies in the wave's LDS; loaded directly, by load (r % kKLoads) and lane group (r / kKLoads).
+    template <bool DIRECT>
+    static __device__ __forceinline__ int place(int r)
+    {
+        return DIRECT ? r % kKLoads * 1024 + r / kKLoads * kRow : r * kRow;
+    }
     // Row r of a tile, 16-byte piece c, lies at piece c ^ swizzle(r): the 16 rows that one read takes (four of every
     // eight) then cover all banks.
     static __device__ __forceinline__ int swizzle(int r)
@@ -237,12 +267,14 @@ struct Layout {
 };
 
 // STREAM: a cache row is read by one block alone, and need not stay in the caches
-template <int D, bool FP8, bool P8, bool STREAM>
-__global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_kernel(const AttnParams p)
+// NT: tiles of columns. One tile's queries stay in registers; those of more, which would not fit beside NT outputs, in LDS.
+template <int D, bool FP8, bool P8, bool STREAM, int NT>
+__global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D, NT)) paged_attention_kernel(const AttnParams p)
 {
     using L = Layout<D, FP8, P8>;
     __shared__ __attribute__((aligned(16))) uint8_t smem[kAttnWaves * L::kWaveLds];
     __shared__ float stats[kAttnWaves][2][kCols];
+    __shared__ u32x4 queries[NT == 1 ? 1 : NT * kCols * L::kQueryPitch];
     // the column groups of a unit on one XCD, next to each other: they read the same cache rows
     int cg = 0, unit = (int)blockIdx.x;
     if (p.col_groups > 1) {
@@ -258,23 +290,44 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
 
     const int lane = lane_id(), wave = wave_id(), n = lane & 15, g = lane >> 4;
     // columns past the last (of a head group that is no multiple of 16) repeat it, and are not written
-    const int c0 = cg * kCols, col = min(c0 + n, p.cols - 1);
-    const int tok = (int)p.by_group.of((uint32_t)col), head = h * p.group + col - tok * p.group;
-    const int hi = pc.len - (p.T - 1 - tok), lo = p.window > 0 ? hi - p.window : 0;   // positions this column sees
-    const int t_first = __builtin_amdgcn_readlane(tok, 0), t_last = __builtin_amdgcn_readlane(tok, kCols - 1);
+    const int c0 = cg * kCols * NT;
+    const auto query_of = [&](int col, int* tok) {       // a column's query, and its token
+        col = min(col, p.cols - 1);
+        *tok = (int)p.by_group.of((uint32_t)col);
+        return p.q + pc.b * p.qb + *tok * p.qt + (h * p.group + col - *tok * p.group) * p.qh;
+    };
+    int tok[NT], hi[NT], lo[NT];         // the token of the lane's columns, and the positions that it sees
+    u32x4 q[NT == 1 ? D / 32 : 1];
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+        const uint8_t* src = query_of(c0 + c * kCols + n, &tok[c]) + 16 * g;
+        hi[c] = pc.len - (p.T - 1 - tok[c]), lo[c] = p.window > 0 ? hi[c] - p.window : 0;
+        if constexpr (NT == 1) {
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) q[j] = *reinterpret_cast<const u32x4*>(src + 64 * j);
+        }
+    }
+    if constexpr (NT > 1) {
+        // column n's 16-byte piece i at n * kQueryPitch + i: an odd number of pieces apart, so a read covers all banks
+        for (int e = (int)threadIdx.x; e < NT * kCols * (D / 8); e += kAttnBlock) {
+            int t;
+            const uint8_t* src = query_of(c0 + e / (D / 8), &t);
+            queries[e / (D / 8) * L::kQueryPitch + e % (D / 8)] = *reinterpret_cast<const u32x4*>(src + e % (D / 8) * 16);
+        }
+        __syncthreads();
+    }
+    const auto query = [&](int c, int j) {
+        if constexpr (NT == 1) return q[j];
+        else return queries[(c * kCols + n) * L::kQueryPitch + 4 * j + g];
+    };
+    const int t_first = __builtin_amdgcn_readlane(tok[0], 0), t_last = __builtin_amdgcn_readlane(tok[NT - 1], kCols - 1);
     // positions that every token of the block sees
     const int all_hi = pc.len - (p.T - 1 - t_first), all_lo = p.window > 0 ? pc.len - (p.T - 1 - t_last) - p.window : 0;
 
-    u32x4 q[D / 32];
-    {
-        const uint8_t* src = p.q + pc.b * p.qb + tok * p.qt + head * p.qh + 16 * g;
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) q[j] = *reinterpret_cast<const u32x4*>(src + 64 * j);
-    }
     const float score_scale = p.scale * (p.cache.k_scale != nullptr ? p.cache.k_scale[h] : 1.0f);
     const int32_t* table = p.table + pc.b * p.table_stride;
     const int kpiece = lane % L::kRowLanes, krow = lane / L::kRowLanes * L::kKLoads;
-    const uint8_t* kbase = p.cache.k + h * p.cache.kh + 16 * kpiece;
+    const uint8_t* kbase = p.cache.k + h * p.cache.kh;
     const uint8_t* vbase = p.cache.v + h * p.cache.vh + 4 * L::kVWords * n;
     const uint32_t last = (uint32_t)pc.len - 1;
     uint8_t* mine = smem + wave * L::kWaveLds;
@@ -292,7 +345,8 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
             vpage[i] = table[p.cache.by_page.of(position(p0 + 8 * g + i * L::kVStep, L::kVStep))];
     };
     auto in_cache = [&](int page) { return (uint32_t)page < (uint32_t)p.cache.pages; };
-    Words<4> k[L::kKLoads];
+    constexpr bool kDirect = loads_direct(D, FP8, NT);
+    Words<4> k[kDirect ? 1 : L::kKLoads];
     Words<L::kVWords> v[8];
     auto load_k = [&](int tile) {
 #pragma unroll
@@ -301,7 +355,13 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
             const uint32_t at = pos - p.cache.by_page.of(pos) * (uint32_t)p.cache.page_size;
             const uint8_t* row = kbase + (in_cache(kpage[i]) ? kpage[i] : 0) * p.cache.kp + at * p.cache.kr;
 #pragma unroll
-            for (int e = 0; e < L::kKStep; ++e) k[i * L::kKStep + e] = load_words<4, STREAM>(row + e * p.cache.kr);
+            for (int e = 0; e < L::kKStep; ++e) {
+                const int j = i * L::kKStep + e;       // row krow + j; directly, the lane asks for the piece its place holds
+                if constexpr (kDirect)
+                    lds_load16<STREAM>(mine + 1024 * j, row + e * p.cache.kr + 16 * (kpiece ^ L::swizzle(krow + j)));
+                else
+                    k[j] = load_words<4, STREAM>(row + e * p.cache.kr + 16 * kpiece);
+            }
         }
     };
     const uint8_t* vrow[L::kVPages];
@@ -326,10 +386,14 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
                 v[i * L::kVStep + e] = load_words<L::kVWords, STREAM>(vrow[i] + e * p.cache.vr);
     };
 
-    float m = -INFINITY, l = 0.0f;
-    f32x4 o[D / 16];
+    float m[NT], l[NT];
+    f32x4 o[NT][D / 16];
 #pragma unroll
-    for (int j = 0; j < D / 16; ++j) o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c = 0; c < NT; ++c) {
+        m[c] = -INFINITY, l[c] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) o[c][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
 
     int tile = pc.tile0 + wave;
     if (tile < pc.tile1) {
@@ -342,79 +406,112 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
     for (; tile < pc.tile1; tile += kAttnWaves) {
         const int next = tile + kAttnWaves;
         const bool more = next < pc.tile1;
-#pragma unroll
-        for (int i = 0; i < L::kKLoads; ++i) {
-            const int r = krow + i;
-            *reinterpret_cast<u32x4*>(mine + r * L::kRow + 16 * (kpiece ^ L::swizzle(r))) =
-                u32x4{k[i].w[0], k[i].w[1], k[i].w[2], k[i].w[3]};
-        }
-        wave_lds_order();
         uint32_t vok_next = 0;
-        if (more) {
+        const auto load_next = [&]() {
+            if (!more) return;
             load_k(next);
             vok_next = address_v(next);
             if (next + kAttnWaves < pc.tile1) lookup(next + kAttnWaves);
+        };
+        if constexpr (kDirect) {
+            __builtin_amdgcn_s_waitcnt(0x0F70);      // vmcnt(0): the tile's rows are there
+            wave_lds_order();
+        } else {
+#pragma unroll
+            for (int i = 0; i < L::kKLoads; ++i) {
+                const int r = krow + i;
+                *reinterpret_cast<u32x4*>(mine + L::template place<false>(r) + 16 * (kpiece ^ L::swizzle(r))) =
+                    u32x4{k[i].w[0], k[i].w[1], k[i].w[2], k[i].w[3]};
+            }
+            wave_lds_order();
+            load_next();
         }
-        // S^T: row m of half `half` is position 8 (m / 4) + 4 half + m % 4 of the tile, so a lane ends with positions
-        // 8 g + 4 half + i, i = 0..3, of its column
-        f32x4 s[2];
+        const int p0 = tile * kTile;
+        const bool masked = p0 + kTile > all_hi || p0 < all_lo || __ballot(vok != 0xFFu) != 0;
+        u32x4 top8[NT], rest8[NT];       // the lane's eight weights of each column as bf16 values and remainders
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int r = (n >> 2) * 8 + half * 4 + (n & 3);
-            const uint8_t* row = mine + r * L::kRow;
-            s[half] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int c = 0; c < NT; ++c) {
+            // S^T: row m of half `half` is position 8 (m / 4) + 4 half + m % 4 of the tile, so a lane ends with positions
+            // 8 g + 4 half + i, i = 0..3, of its column
+            f32x4 s[2];
 #pragma unroll
-            for (int j = 0; j < D / 32; ++j) {
-                u32x4 a;
-                if constexpr (FP8) {
-                    const uint2 w = *reinterpret_cast<const uint2*>(row + 16 * ((2 * j + (g >> 1)) ^ L::swizzle(r)) + 8 * (g & 1));
-                    a = u32x4{fp8x2_to_bf16x2<false>(w.x), fp8x2_to_bf16x2<true>(w.x), fp8x2_to_bf16x2<false>(w.y),
-                              fp8x2_to_bf16x2<true>(w.y)};
-                } else {
-                    a = *reinterpret_cast<const u32x4*>(row + 16 * ((4 * j + g) ^ L::swizzle(r)));
+            for (int half = 0; half < 2; ++half) {
+                const int r = (n >> 2) * 8 + half * 4 + (n & 3);
+                const uint8_t* row = mine + L::template place<kDirect>(r);
+                s[half] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < D / 32; ++j) {
+                    u32x4 a;
+                    if constexpr (FP8) {
+                        const uint2 w = *reinterpret_cast<const uint2*>(row + 16 * ((2 * j + (g >> 1)) ^ L::swizzle(r)) + 8 * (g & 1));
+                        a = u32x4{fp8x2_to_bf16x2<false>(w.x), fp8x2_to_bf16x2<true>(w.x), fp8x2_to_bf16x2<false>(w.y),
+                                  fp8x2_to_bf16x2<true>(w.y)};
+                    } else {
+                        a = *reinterpret_cast<const u32x4*>(row + 16 * ((4 * j + g) ^ L::swizzle(r)));
+                    }
+                    s[half] = mfma_16x16x32(a, query(c, j), s[half]);
                 }
-                s[half] = mfma_16x16x32(a, q[j], s[half]);
+            }
+            float top = -INFINITY, x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = s[i / 4][i % 4] * score_scale;
+                if (masked) {
+                    const int pos = p0 + 8 * g + i;
+                    x[i] = pos < hi[c] && pos >= lo[c] && (vok >> i & 1u) ? x[i] : -INFINITY;
+                }
+                top = fmaxf(top, x[i]);
+            }
+            top = fmaxf(m[c], col_max(top));
+            const float base = top == -INFINITY ? 0.0f : top;
+            if (__ballot(top > m[c]) != 0) {
+                const float fade = __builtin_amdgcn_exp2f(m[c] - base);
+                l[c] *= fade;
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j) o[c][j] *= fade;
+                m[c] = top;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = __builtin_amdgcn_exp2f(x[i] - base);
+                l[c] += x[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t t = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+                top8[c][i] = t;
+                rest8[c][i] = pack_bf16x2(x[2 * i] - __uint_as_float(t << 16), x[2 * i + 1] - __uint_as_float(t & 0xFFFF0000u));
             }
         }
         wave_lds_order();
-        const int p0 = tile * kTile;
-        const bool masked = p0 + kTile > all_hi || p0 < all_lo || __ballot(vok != 0xFFu) != 0;
-        float top = -INFINITY;
+        if constexpr (kDirect) {
+            __builtin_amdgcn_s_waitcnt(0xC07F);      // lgkmcnt(0): the tile's rows are read, the next one's may take their place
+            wave_lds_order();
+            load_next();
+        }
+        // What no token sees of the tile goes out of V here. Where the tokens differ in what they see, weights of 0 keep the rest
+        // of it out, unless a value there is not finite: then each token takes a product of its own.
+        bool together = true;
+        if (masked) {
+            const int last_hi = pc.len - (p.T - 1 - t_last), first_lo = p.window > 0 ? pc.len - (p.T - 1 - t_first) - p.window : 0;
+            uint32_t odd = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float x = s[i / 4][i % 4] * score_scale;
-            if (masked) {
+            for (int i = 0; i < 8; ++i) {
                 const int pos = p0 + 8 * g + i;
-                x = pos < hi && pos >= lo && (vok >> i & 1u) ? x : -INFINITY;
+                const bool some = pos < last_hi && pos >= first_lo && (vok >> i & 1u);
+#pragma unroll
+                for (int e = 0; e < L::kVWords; ++e) {
+                    const uint32_t w = some ? v[i].w[e] : 0u;
+                    v[i].w[e] = w;
+                    // the top bit of each value whose exponent (e4m3: everything but the sign) is all ones
+                    odd |= FP8 ? ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u : ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
+                }
             }
-            s[i / 4][i % 4] = x;
-            top = fmaxf(top, x);
-        }
-        top = fmaxf(m, col_max(top));
-        const float base = top == -INFINITY ? 0.0f : top;
-        if (__ballot(top > m) != 0) {
-            const float fade = __builtin_amdgcn_exp2f(m - base);
-            l *= fade;
-#pragma unroll
-            for (int j = 0; j < D / 16; ++j) o[j] *= fade;
-            m = top;
-        }
-        float w[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            w[i] = __builtin_amdgcn_exp2f(s[i / 4][i % 4] - base);
-            l += w[i];
-        }
-        u32x4 top8, rest8;               // the lane's eight weights as bf16 values and remainders
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            top8[i] = pack_bf16x2(w[2 * i], w[2 * i + 1]);
-            rest8[i] = pack_bf16x2(w[2 * i] - __uint_as_float(top8[i] << 16),
-                                   w[2 * i + 1] - __uint_as_float(top8[i] & 0xFFFF0000u));
+            together = t_first == t_last || __ballot(odd != 0) == 0;
         }
         // O^T += V^T P^T: rows 8 g + i, i = 0..7, of the tile against the lane's own eight weights. `see`: bit i keeps row
-        // i; `take`: the product is this lane's (of its token), or nobody's business.
-        auto add_pv = [&](uint32_t see, bool all, bool take) {
+        // i; with `all` every row and column takes the product, else those of token t.
+        auto add_pv = [&](uint32_t see, bool all, int t) {
 #pragma unroll
             for (int d = 0; d < D / 32; ++d) {
                 uint32_t x[8];
@@ -430,21 +527,24 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
                                     __builtin_amdgcn_perm(x[5], x[4], 0x05040100u), __builtin_amdgcn_perm(x[7], x[6], 0x05040100u)};
                 const u32x4 odd = {__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u),
                                    __builtin_amdgcn_perm(x[5], x[4], 0x07060302u), __builtin_amdgcn_perm(x[7], x[6], 0x07060302u)};
-                const f32x4 a = mfma_16x16x32(even, top8, mfma_16x16x32(even, rest8, o[2 * d]));
-                const f32x4 b = mfma_16x16x32(odd, top8, mfma_16x16x32(odd, rest8, o[2 * d + 1]));
-                if (all) {
-                    o[2 * d] = a, o[2 * d + 1] = b;
-                } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        o[2 * d][e] = take ? a[e] : o[2 * d][e];
-                        o[2 * d + 1][e] = take ? b[e] : o[2 * d + 1][e];
+                for (int c = 0; c < NT; ++c) {
+                    const f32x4 a = mfma_16x16x32(even, top8[c], mfma_16x16x32(even, rest8[c], o[c][2 * d]));
+                    const f32x4 b = mfma_16x16x32(odd, top8[c], mfma_16x16x32(odd, rest8[c], o[c][2 * d + 1]));
+                    if (all) {
+                        o[c][2 * d] = a, o[c][2 * d + 1] = b;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            o[c][2 * d][e] = tok[c] == t ? a[e] : o[c][2 * d][e];
+                            o[c][2 * d + 1][e] = tok[c] == t ? b[e] : o[c][2 * d + 1][e];
+                        }
                     }
                 }
             }
         };
-        if (!masked) {
-            add_pv(0xFFu, true, true);
+        if (together) {
+            add_pv(0xFFu, true, 0);
         } else {
             for (int t = t_first; t <= t_last; ++t) {
                 const int thi = pc.len - (p.T - 1 - t), tlo = p.window > 0 ? thi - p.window : 0;
@@ -454,51 +554,55 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D)) paged_attention_
                     const int pos = p0 + 8 * g + i;
                     if (pos < thi && pos >= tlo) see |= 1u << i;
                 }
-                add_pv(see & vok, false, tok == t);
+                add_pv(see, false, t);
             }
         }
         vok = vok_next;
         if (more) load_v();
     }
-    l = col_sum(l);
 
-    // join the block's waves: column n of a wave's O^T lies at [n][dim], dims (4 g + i) D/16 + j
+    // join the block's waves, a tile of columns at a time: column n of a wave's O^T lies at [n][dim], dims (4 g + i) D/16 + j
+    const float v_scale = p.cache.v_scale != nullptr ? p.cache.v_scale[h] : 1.0f;
     float* part = reinterpret_cast<float*>(mine);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int ct = 0; ct < NT; ++ct) {
+        if (ct > 0) __syncthreads();
 #pragma unroll
-        for (int j = 0; j < D / 16; j += 4)
-            *reinterpret_cast<f32x4*>(part + n * L::kOutStride + (4 * g + i) * (D / 16) + j) =
-                f32x4{o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]};
-    if (g == 0) stats[wave][0][n] = m, stats[wave][1][n] = l;
-    __syncthreads();
-    const float v_scale = p.cache.v_scale != nullptr ? p.cache.v_scale[h] : 1.0f;
-    for (int e = (int)threadIdx.x; e < kCols * (D / 4); e += kAttnBlock) {
-        const int cn = e / (D / 4), d = e % (D / 4) * 4, c = c0 + cn;
-        if (c >= p.cols) break;
-        float all = -INFINITY, sum = 0.0f;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int w = 0; w < kAttnWaves; ++w) all = fmaxf(all, stats[w][0][cn]);
-        const float base = all == -INFINITY ? 0.0f : all;
-        f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int j = 0; j < D / 16; j += 4)
+                *reinterpret_cast<f32x4*>(part + n * L::kOutStride + (4 * g + i) * (D / 16) + j) =
+                    f32x4{o[ct][j][i], o[ct][j + 1][i], o[ct][j + 2][i], o[ct][j + 3][i]};
+        const float weight = col_sum(l[ct]);
+        if (g == 0) stats[wave][0][n] = m[ct], stats[wave][1][n] = weight;
+        __syncthreads();
+        for (int e = (int)threadIdx.x; e < kCols * (D / 4); e += kAttnBlock) {
+            const int cn = e / (D / 4), d = e % (D / 4) * 4, c = c0 + ct * kCols + cn;
+            if (c >= p.cols) break;
+            float all = -INFINITY, sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kAttnWaves; ++w) {
-            const float f = __builtin_amdgcn_exp2f(stats[w][0][cn] - base);
-            sum += f * stats[w][1][cn];
-            acc += f * *reinterpret_cast<const f32x4*>(smem + w * L::kWaveLds + 4 * (cn * L::kOutStride + d));
+            for (int w = 0; w < kAttnWaves; ++w) all = fmaxf(all, stats[w][0][cn]);
+            const float base = all == -INFINITY ? 0.0f : all;
+            f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < kAttnWaves; ++w) {
+                const float f = __builtin_amdgcn_exp2f(stats[w][0][cn] - base);
+                sum += f * stats[w][1][cn];
+                acc += f * *reinterpret_cast<const f32x4*>(smem + w * L::kWaveLds + 4 * (cn * L::kOutStride + d));
+            }
+            if (pc.count > 1) {
+                const int64_t at = (int64_t)unit * p.cols + c;
+                *reinterpret_cast<f32x4*>(p.part_o + at * D + d) = acc;
+                if (d == 0) p.part_ml[2 * at] = all, p.part_ml[2 * at + 1] = sum;
+                continue;
+            }
+            const int t = (int)p.by_group.of((uint32_t)c);
+            const int64_t row = ((int64_t)pc.b * p.T + t) * p.heads + h * p.group + c - t * p.group;
+            const float f = sum == 0.0f ? 0.0f : v_scale / sum;
+            const uint2 y = {pack_bf16x2(acc[0] * f, acc[1] * f), pack_bf16x2(acc[2] * f, acc[3] * f)};
+            *reinterpret_cast<uint2*>(p.out + row * D + d) = y;
+            if (d == 0 && p.lse != nullptr) p.lse[row] = (all + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
         }
-        if (pc.count > 1) {
-            const int64_t at = (int64_t)unit * p.cols + c;
-            *reinterpret_cast<f32x4*>(p.part_o + at * D + d) = acc;
-            if (d == 0) p.part_ml[2 * at] = all, p.part_ml[2 * at + 1] = sum;
-            continue;
-        }
-        const int t = (int)p.by_group.of((uint32_t)c);
-        const int64_t row = ((int64_t)pc.b * p.T + t) * p.heads + h * p.group + c - t * p.group;
-        const float f = sum == 0.0f ? 0.0f : v_scale / sum;
-        const uint2 y = {pack_bf16x2(acc[0] * f, acc[1] * f), pack_bf16x2(acc[2] * f, acc[3] * f)};
-        *reinterpret_cast<uint2*>(p.out + row * D + d) = y;
-        if (d == 0 && p.lse != nullptr) p.lse[row] = (all + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
     }
 }
 
@@ -577,8 +681,13 @@ static bool attention_plan(const paia_kv_cache* c, int table_width, int B, int T
     p->max_len = (int)(max_len < INT_MAX - 4096 ? max_len : INT_MAX - 4096);
     if (cols > 65535 || c->kv_heads > 65535) return false;      // dimensions of the joining grid
     p->cols = (int)cols;
-    p->col_groups = (p->cols + kCols - 1) / kCols;
-    const int64_t wide = (int64_t)c->kv_heads * p->col_groups, slots = (int64_t)device_facts().cus * blocks_per_cu(c->head_dim);
+    // The columns' tiles over the fewest blocks, evenly, as far as a lane's registers hold its outputs.
+    const double row = 2.0 * c->kv_heads * c->head_dim * (c->fp8 ? 1 : 2);
+    const bool large = row * B * p->max_len >= (double)kTogether;
+    const int tiles = (p->cols + kCols - 1) / kCols, most = large ? most_tiles(c->head_dim, c->fp8, c->page_size % 8 == 0) : 1;
+    p->tiles = (tiles + (tiles + most - 1) / most - 1) / ((tiles + most - 1) / most);
+    p->col_groups = (tiles + p->tiles - 1) / p->tiles;
+    const int64_t wide = (int64_t)c->kv_heads * p->col_groups, slots = (int64_t)device_facts().cus * blocks_per_cu(c->head_dim, p->tiles);
     int64_t target = slots / wide;
     target = target < 2 ? 2 : target;
     // One round of blocks where the sequences are few; many sequences have a piece of their own each, and as many more as a
@@ -599,21 +708,25 @@ static bool attention_plan(const paia_kv_cache* c, int table_width, int B, int T
     return true;
 }
 
-// Several column groups read the same rows, next to each other on one XCD: with streaming loads its L2 served them worse (five
-// tokens of 8 heads a group, 12000 positions each: 141 us against 117; heads of 256: 532 against 281). Two tiles of columns in
-// one block instead need twice the outputs and queries in registers, one wave a SIMD: 166.
-template <int D, bool FP8>
-static auto attention_kernel(bool p8, bool stream)
+// Several column groups read the same rows, next to each other on one XCD: with streaming loads its L2 served them worse (heads
+// of 256, five tokens of 8 heads a group, 12000 positions: 532 us against 281).
+template <int D, bool FP8, bool P8>
+static auto attention_kernel(int tiles, bool stream)
 {
-    return stream ? (p8 ? paged_attention_kernel<D, FP8, true, true> : paged_attention_kernel<D, FP8, false, true>)
-                  : (p8 ? paged_attention_kernel<D, FP8, true, false> : paged_attention_kernel<D, FP8, false, false>);
+    if constexpr (most_tiles(D, FP8, P8) >= 2)
+        if (tiles == 2) return paged_attention_kernel<D, FP8, P8, false, 2>;
+    if constexpr (most_tiles(D, FP8, P8) >= 3)
+        if (tiles == 3) return paged_attention_kernel<D, FP8, P8, false, 3>;
+    return stream ? paged_attention_kernel<D, FP8, P8, true, 1> : paged_attention_kernel<D, FP8, P8, false, 1>;
 }
 template <int D>
 static int launch_attention(const AttnParams& p, bool fp8, bool join, hipStream_t st)
 {
     const dim3 grid((uint32_t)((p.units + 7) / 8 * 8 * p.col_groups));
     const bool p8 = p.cache.page_size % 8 == 0;
-    const auto kernel = fp8 ? attention_kernel<D, true>(p8, p.col_groups == 1) : attention_kernel<D, false>(p8, p.col_groups == 1);
+    const bool alone = p.col_groups == 1;
+    const auto kernel = fp8 ? (p8 ? attention_kernel<D, true, true>(p.tiles, alone) : attention_kernel<D, true, false>(p.tiles, alone))
+                            : (p8 ? attention_kernel<D, false, true>(p.tiles, alone) : attention_kernel<D, false, false>(p.tiles, alone));
     hipLaunchKernelGGL(kernel, grid, dim3(kAttnBlock), 0, st, p);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return (int)e;
     if (join) {

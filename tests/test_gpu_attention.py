@@ -308,3 +308,28 @@ def test_refusals(cuda):
             workspace=torch.empty(64, device=cuda))
     odd = torch.empty(2, 8 * 128 + 4, dtype=torch.bfloat16, device=cuda)
     refused("-2", q=odd[:, :1024].unflatten(1, (8, 128)))
+
+
+@pytest.mark.parametrize("dim,fp8,page", [(64, False, 16), (64, True, 7), (128, False, 16), (128, False, 9), (128, True, 16)])
+def test_column_tiles_together(cuda, dim, fp8, page):
+    """Tables wide enough for the forms whose blocks take two or three tiles of columns (and those that never do): the same
+    sequences in a narrow and a wide table, with drafts, a window, holes and values nobody sees."""
+    wide = -(-(300 << 20) // (2 * 2 * 2 * dim * (1 if fp8 else 2) * page))
+    for T, heads, window in ((5, 8, 0), (5, 16, 0), (3, 40, 100), (1, 70, 0)):
+        note(f"attention column tiles dim={dim} fp8={fp8} page={page} T={T} heads={heads} window={window}")
+        o = operands([700, 37], T, heads, 2, dim, fp8, "phd", page, seed=T + heads)
+        o["table"][0, 2] = -1
+        narrow = call(o, cuda, window=window)
+        check(o, *narrow, window=window)
+        table = torch.full((2, wide), -1, dtype=torch.int32)
+        table[:, :o["table"].shape[1]] = o["table"]
+        got = call({**o, "table": table}, cuda, window=window)
+        check(o, *got, window=window)
+        if T > 1:      # the last row of a sequence, which only its last token sees
+            p = 699
+            for c in ("k_cache", "v_cache"):
+                o[c] = o[c].clone()
+                o[c][int(o["table"][0, p // page]), :, p % page] = float("nan")
+            bad = call({**o, "table": table}, cuda, window=window)
+            assert torch.equal(bits(bad[0][:, :T - 1]), bits(got[0][:, :T - 1])) and torch.equal(bad[1][:, :T - 1], got[1][:, :T - 1])
+            assert bad[0][0, T - 1].isnan().all() and torch.equal(bits(bad[0][1]), bits(got[0][1]))
