@@ -454,14 +454,17 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D, NT)) paged_attent
             }
             float top = -INFINITY, x[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] = s[i / 4][i % 4] * score_scale;
-                if (masked) {
+            for (int i = 0; i < 8; ++i) x[i] = s[i / 4][i % 4] * score_scale;
+            if (masked) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
                     const int pos = p0 + 8 * g + i;
-                    x[i] = pos < hi[c] && pos >= lo[c] && (vok >> i & 1u) ? x[i] : -INFINITY;
+                    const bool seen = (pos < hi[c]) & (pos >= lo[c]) & ((vok >> i & 1u) != 0u);
+                    x[i] = seen ? x[i] : -INFINITY;
                 }
-                top = fmaxf(top, x[i]);
             }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i]);
             top = fmaxf(m[c], col_max(top));
             const float base = top == -INFINITY ? 0.0f : top;
             if (__ballot(top > m[c]) != 0) {
@@ -498,7 +501,7 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D, NT)) paged_attent
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int pos = p0 + 8 * g + i;
-                const bool some = pos < last_hi && pos >= first_lo && (vok >> i & 1u);
+                const bool some = (pos < last_hi) & (pos >= first_lo) & ((vok >> i & 1u) != 0u);
 #pragma unroll
                 for (int e = 0; e < L::kVWords; ++e) {
                     const uint32_t w = some ? v[i].w[e] : 0u;
