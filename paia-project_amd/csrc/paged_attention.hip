@@ -38,7 +38,7 @@ namespace paia {
 constexpr int kTile = 32;            // positions a wave takes at a time
 constexpr int kCols = 16;            // columns (token, head) of a matrix tile; a block takes up to most_tiles() such tiles
 // Tiles of columns that a block takes together, so that each row is read and taken apart once for all: as many as a lane's
-// registers hold the outputs of (e4m3 heads of 128 spill with two: 84 us for 61). A block of several tiles stages its queries
+// registers hold the outputs of (e4m3 heads of 128 spill with two: 84 us for 71). A block of several tiles stages its queries
 // and does more after its last row, so it takes caches that fill the chip for longer: kTogether bytes, as the block table's
 // size bounds them. Five tokens of 4 and of 8 heads a group, 8 sequences, us with one tile a block / together:
 //   bf16 heads of 128, 2500 positions 20.6 / 22.9 and 23.7 / 27.0; 6000 (164 MB) 46.0 / 44.2 and 51.8 / 52.6; 16000 91 / 86
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D, NT)) paged_attent
         // What no token sees of the tile goes out of V here. Where the tokens differ in what they see, weights of 0 keep the rest
         // of it out, unless a value there is not finite: then each token takes a product of its own.
         bool together = true;
-        if (masked) {
+        if (__builtin_expect(masked, 0)) {
             const int last_hi = pc.len - (p.T - 1 - t_last), first_lo = p.window > 0 ? pc.len - (p.T - 1 - t_first) - p.window : 0;
             uint32_t odd = 0;
 #pragma unroll
@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D, NT)) paged_attent
                 }
             }
         };
-        if (together) {
+        if (__builtin_expect(together, 1)) {
             add_pv(0xFFu, true, 0);
         } else {
             for (int t = t_first; t <= t_last; ++t) {
