@@ -6,11 +6,10 @@
 // Each cache byte is used for T G products a value (G query heads share a kv head), a few operations per byte: bound by
 // reading the cache once. The pieces of the design:
 //   * Work: a unit is one piece of one sequence for one kv head and 16 columns (token, query head of the group), or
-//     up to 48 where the cache is large (most_tiles). The
-//     lengths are on the device and the grid is fixed by the host, so each block derives the split from the lengths
-//     itself (find_piece): about as many equal pieces as blocks fit the chip, whatever the lengths are. A captured call
-//     stays balanced as the sequences grow. Pieces of one sequence leave (m, l, o) in the workspace, joined by a second
-//     kernel; a sequence of one piece is written by its block.
+//     up to 48 where the cache is large (most_tiles). The lengths are on the device and the grid is fixed by the host, so
+//     each block derives the split from the lengths itself (find_piece): about as many equal pieces as blocks fit the
+//     chip, whatever the lengths are. A captured call stays balanced as the sequences grow. Pieces of one sequence leave
+//     (m, l, o) in the workspace, joined by a second kernel; a sequence of one piece is written by its block.
 //   * A block's four waves take its 32-position tiles in turn, each with its own running maximum, sum and output (no
 //     barrier until the end), and one tile of K and V loads in flight ahead of the one in work.
 //   * S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_bf16. Both leave a column (token, head) on the same lane, so
@@ -23,7 +22,8 @@
 // Scores, statistics and sums are fp32. P enters the second product as two bf16 terms (value and remainder, 16 bits): one more
 // MFMA a product, 0.3 to 1% of the time; with the value alone the output's error was 1.3 times that of its rounding.
 // What no token sees (positions past the end, before the window, on a page outside the cache) contributes nothing, whatever
-// its bytes are: scores are replaced, V rows zeroed, and where tokens differ in what they see, each takes its own product.
+// its bytes are: scores are replaced, V rows zeroed, and where tokens differ in what they see and a value there is not finite,
+// each takes its own product.
 #include <hip/hip_runtime.h>
 #include <limits.h>
 #include <math.h>
@@ -38,13 +38,13 @@ namespace paia {
 constexpr int kTile = 32;            // positions a wave takes at a time
 constexpr int kCols = 16;            // columns (token, head) of a matrix tile; a block takes up to most_tiles() such tiles
 // Tiles of columns that a block takes together, so that each row is read and taken apart once for all: as many as a lane's
-// registers hold the outputs of (e4m3 heads of 128 spill with two: 84 us for 71). A block of several tiles stages its queries
-// and does more after its last row, so it takes caches that fill the chip for longer: kTogether bytes, as the block table's
-// size bounds them. Five tokens of 4 and of 8 heads a group, 8 sequences, us with one tile a block / together:
-//   bf16 heads of 128, 2500 positions 20.6 / 22.9 and 23.7 / 27.0; 6000 (164 MB) 46.0 / 44.2 and 51.8 / 52.6; 16000 91 / 86
-//   and 114 / 100; heads of 64, 6000 (82 MB) 22.5 / 23.5 and 28.8 / 29.3; 16000 (200 MB) 54 / 47 and 66 / 52; e4m3, 16000
-//   (100 MB) 40.7 / 38.7 and 53.9 / 49.2.
-constexpr int most_tiles(int dim, bool fp8, bool p8) { return dim <= 64 ? 3 : dim <= 128 && p8 && !fp8 ? 2 : 1; }
+// registers hold the outputs of (e4m3 heads of 128 spill 132 bytes with two, and gain all the same). A block of several tiles
+// stages its queries and does more after its last row, so it takes caches that fill the chip for longer: kTogether bytes, as
+// the block table's size bounds them. Five tokens of 4 and of 8 heads a group, 8 sequences, us with one tile a block / together:
+//   bf16 heads of 128, 2500 positions 20.7 / 22.2 and 23.9 / 25.9; 6000 (164 MB) 43.7 / 41.0 and 53.1 / 49.0; 16000 86.5 / 81.3
+//   and 115.8 / 94.0; heads of 64, 6000 (82 MB) 22.0 / 24.5 and 28.9 / 29.3; 16000 (200 MB) 51.6 / 46.8 and 64.4 / 50.8; e4m3
+//   heads of 128, 16000 (200 MB) 66.7 / 54.2 and 98.7 / 86.0; of 64 (100 MB) 43.3 / 40.6 and 57.3 / 47.2.
+constexpr int most_tiles(int dim, bool p8) { return dim <= 64 ? 3 : dim <= 128 && p8 ? 2 : 1; }
 constexpr int64_t kTogether = 120 << 20;
 constexpr int kAttnWaves = 4, kAttnBlock = kAttnWaves * kWave;
 // Blocks that a CU holds at the registers a wave takes (one wave of a block on each SIMD).
@@ -687,7 +687,7 @@ static bool attention_plan(const paia_kv_cache* c, int table_width, int B, int T
     // The columns' tiles over the fewest blocks, evenly, as far as a lane's registers hold its outputs.
     const double row = 2.0 * c->kv_heads * c->head_dim * (c->fp8 ? 1 : 2);
     const bool large = row * B * p->max_len >= (double)kTogether;
-    const int tiles = (p->cols + kCols - 1) / kCols, most = large ? most_tiles(c->head_dim, c->fp8, c->page_size % 8 == 0) : 1;
+    const int tiles = (p->cols + kCols - 1) / kCols, most = large ? most_tiles(c->head_dim, c->page_size % 8 == 0) : 1;
     p->tiles = (tiles + (tiles + most - 1) / most - 1) / ((tiles + most - 1) / most);
     p->col_groups = (tiles + p->tiles - 1) / p->tiles;
     const int64_t wide = (int64_t)c->kv_heads * p->col_groups, slots = (int64_t)device_facts().cus * blocks_per_cu(c->head_dim, p->tiles);
@@ -716,9 +716,9 @@ static bool attention_plan(const paia_kv_cache* c, int table_width, int B, int T
 template <int D, bool FP8, bool P8>
 static auto attention_kernel(int tiles, bool stream)
 {
-    if constexpr (most_tiles(D, FP8, P8) >= 2)
+    if constexpr (most_tiles(D, P8) >= 2)
         if (tiles == 2) return paged_attention_kernel<D, FP8, P8, false, 2>;
-    if constexpr (most_tiles(D, FP8, P8) >= 3)
+    if constexpr (most_tiles(D, P8) >= 3)
         if (tiles == 3) return paged_attention_kernel<D, FP8, P8, false, 3>;
     return stream ? paged_attention_kernel<D, FP8, P8, true, 1> : paged_attention_kernel<D, FP8, P8, false, 1>;
 }
