@@ -19,7 +19,7 @@
 //     V rows are loaded contiguously too, D/16 dims of eight positions per lane: 16 lanes are the 16 rows of the V^T
 //     operand, whose eight contraction values are the eight positions; one v_perm_b32 per register pairs them up.
 //   * e4m3 codes become bf16 exactly (v_cvt_scalef32_pk_bf16_fp8); the heads' factors go to the scores and the output.
-// Scores, statistics and sums are fp32. P enters the second product as two bf16 terms (value and remainder, 16 bits): one more
+// Scores, statistics and sums are fp32. P enters the second product as two bf16 terms (split_weights, 16 bits or more): one more
 // MFMA a product, 0.3 to 1% of the time; with the value alone the output's error was 1.3 times that of its rounding.
 // What no token sees (positions past the end, before the window, on a page outside the cache) contributes nothing, whatever
 // its bytes are: scores are replaced, V rows zeroed, and where tokens differ in what they see and a value there is not finite,
@@ -231,6 +231,23 @@ __device__ __forceinline__ Words<N> load_words(const uint8_t* p)
         r.w[0] = load_as<STREAM, uint32_t>(p);
     }
     return r;
+}
+
+// Two weights as bf16 values and what they keep beyond them, as bf16 too. FINITE: V holds no infinities (e4m3 has none), and the
+// values are the nearest (17 bits together). Else they are cut toward zero (16 bits) and no remainder of a weight above 0 is 0: both
+// terms then have the weight's sign, and an infinity in V meets neither a 0 nor a negative term, which would make NaN of it.
+template <bool FINITE>
+__device__ __forceinline__ u32x2 split_weights(float a, float b)
+{
+    if constexpr (FINITE) {
+        const uint32_t top = pack_bf16x2(a, b);
+        return {top, pack_bf16x2(a - __uint_as_float(top << 16), b - __uint_as_float(top & 0xFFFF0000u))};
+    } else {
+        const auto over = [](float v) {       // v is 0, at least the smallest normal value, or NaN, which its own value keeps
+            return __builtin_amdgcn_fmed3f(v - __uint_as_float(__float_as_uint(v) & 0xFFFF0000u), 0x1p-126f, v);
+        };
+        return {__builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u), pack_bf16x2(over(a), over(b))};
+    }
 }
 
 // K goes straight to LDS where its registers would spill or halve the waves of a CU: bf16 heads of 256 (12000 positions of 8
@@ -481,9 +498,8 @@ __global__ void __launch_bounds__(kAttnBlock, blocks_per_cu(D, NT)) paged_attent
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t t = pack_bf16x2(x[2 * i], x[2 * i + 1]);
-                top8[c][i] = t;
-                rest8[c][i] = pack_bf16x2(x[2 * i] - __uint_as_float(t << 16), x[2 * i + 1] - __uint_as_float(t & 0xFFFF0000u));
+                const u32x2 w = split_weights<FP8>(x[2 * i], x[2 * i + 1]);
+                top8[c][i] = w.x, rest8[c][i] = w.y;
             }
         }
         wave_lds_order();
