@@ -12,7 +12,7 @@
 //     the other. The first leaves partial sums of h over pieces of K in the workspace (added in order by the second: no
 //     atomics), so that few adapters still fill the chip, and the list of chunks of rows: each of its blocks finds the rows
 //     that share an adapter from ids itself (row_chunks), nothing has to be sorted or counted before the call. h goes to the
-//     second product as two bf16 terms (value and remainder, 16 bits together), so that out has the one rounding that matters.
+//     second product as two bf16 terms (rest_bf16, 16 bits together), so that out has the one rounding that matters.
 #include <hip/hip_runtime.h>
 #include <limits.h>
 #include <stdint.h>
@@ -140,10 +140,14 @@ __device__ __forceinline__ u32x4 load16_if(const uint16_t* p, bool take)
     return take ? *reinterpret_cast<const u32x4*>(p) : u32x4{0, 0, 0, 0};
 }
 
-// What a value keeps beyond its bf16 rounding; nothing where that is not finite.
-__device__ __forceinline__ float rest(float v, uint32_t rounded)
+// A value cut to bf16 toward zero is its upper half; this is what it keeps beyond that, as bf16. Both terms have the value's sign, or
+// an infinity in B would meet terms of both signs, or a 0: so what rounds to 0 is the smallest value instead, unless the value is 0,
+// and the rest of what is not finite is the same again.
+__device__ __forceinline__ uint32_t rest_bf16(float v)
 {
-    return fabsf(__uint_as_float(rounded)) < 3.4e38f ? v - __uint_as_float(rounded) : 0.0f;
+    const uint32_t w = __float_as_uint(v);
+    const uint32_t r = f32_to_bf16_out(fabsf(v) < __builtin_inff() ? v - __uint_as_float(w & 0xFFFF0000u) : v);
+    return (r & 0x7FFFu) == 0 && v != 0.0f ? (w >> 16 & 0x8000u) | 1u : r;
 }
 
 // h: a unit is (chunk, 16 rows of A, piece of K); the block's waves take its steps of 64 columns in turn. Eight lanes load
@@ -306,8 +310,8 @@ __global__ void __launch_bounds__(kLoraBlock) lora_expand_kernel(const LoraParam
                 chunk = r.chunk, slice = r.slice;
                 const auto& c = p.list->chunk[chunk];
                 id = c.adapter, held = c.held, m = c.rows[n];
-                // the chunk's values of this slice of h: the pieces' sums in order, times the adapter's factor, as bf16 value
-                // and remainder
+                // the chunk's values of this slice of h: the pieces' sums in order, times the adapter's factor, in two
+                // bf16 terms
                 __syncthreads();
                 const float factor = id < 0 || p.scaling == nullptr ? 1.0f : p.scaling[id];
                 for (int e = (int)threadIdx.x; e < (id < 0 ? 0 : held * (p.R / 4)); e += kLoraBlock) {
@@ -321,9 +325,11 @@ __global__ void __launch_bounds__(kLoraBlock) lora_expand_kernel(const LoraParam
 #pragma unroll
                     for (int k = 0; k < kMaxPieces; ++k) h += term[k];
                     h *= factor;
-                    const uint2 top = {pack_bf16x2(h[0], h[1]), pack_bf16x2(h[2], h[3])};
-                    const uint2 low = {pack_bf16x2(rest(h[0], top.x << 16), rest(h[1], top.x & 0xFFFF0000u)),
-                                       pack_bf16x2(rest(h[2], top.y << 16), rest(h[3], top.y & 0xFFFF0000u))};
+                    uint32_t u[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) u[k] = __float_as_uint(h[k]);
+                    const uint2 top = {u[0] >> 16 | (u[1] & 0xFFFF0000u), u[2] >> 16 | (u[3] & 0xFFFF0000u)};
+                    const uint2 low = {rest_bf16(h[0]) | rest_bf16(h[1]) << 16, rest_bf16(h[2]) | rest_bf16(h[3]) << 16};
                     reinterpret_cast<uint2*>(h_of[0])[row * (2 * kHPitch) + c4] = top;
                     reinterpret_cast<uint2*>(h_of[1])[row * (2 * kHPitch) + c4] = low;
                 }
