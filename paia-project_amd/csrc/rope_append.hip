@@ -76,6 +76,8 @@ __device__ __forceinline__ void store8(uint8_t* p, const float v[8], float s)
 }
 
 constexpr int kRopeBlock = 256;
+// A launch has less than 2^32 threads: tokens beyond kRopeMaxBlocks blocks go into a further one.
+constexpr int64_t kRopeMaxBlocks = 1 << 23;
 
 // PAIRS: pairs (2i, 2i+1) instead of halves; NORM: at least one norm weight is given
 template <int D, bool FP8, bool PAIRS, bool NORM>
@@ -178,8 +180,7 @@ int launch_rope(RopeParams p, bool pairs, int64_t M, hipStream_t st)
     const uint32_t units = ((uint32_t)p.heads + 2u * (uint32_t)p.cache.kv_heads + kHeads - 1) / kHeads;    // waves a token
     p.by_units = Divisor(units);
     const bool norm = p.q_norm != nullptr || p.k_norm != nullptr;
-    // wave numbers stay below 2^31: launches of at most 2^30 waves
-    const int64_t step = (1ll << 30) / units;
+    const int64_t step = kRopeMaxBlocks * kWaves / units;
     for (int64_t m = 0; m < M; m += step) {
         RopeParams s = p;
         s.tokens = (uint32_t)(M - m < step ? M - m : step);
