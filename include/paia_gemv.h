@@ -195,7 +195,7 @@ PAIA_API int paia_rope_append(const void* qkv, long long qkv_stride, const void*
  * the device: a captured call serves sequences as they grow. workspace: device memory, 16-byte aligned, of at least
  * paia_paged_attention_workspace() bytes (for the same cache, width, B, T and heads; 0 = NULL will do, -2 = outside
  * the contract). Calls that overlap need a workspace each. out overlaps no other operand. At most 65535 kv heads
- * and T * heads / kv_heads. */
+ * and T * heads / kv_heads = n, and about 2^24 of B * kv_heads * ceil(n / 16), the blocks of a launch. */
 PAIA_API long long paia_paged_attention_workspace(const paia_kv_cache* cache, int table_width, int B, int T, int heads);
 PAIA_API int paia_paged_attention(const void* q, const long long* q_strides, const paia_kv_cache* cache,
                                   const void* block_table, long long table_stride, int table_width, const void* lens,

@@ -689,6 +689,9 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
+// A launch has less than 2^32 threads; a block of the first grid for every sequence at least, so the joining one is bounded too.
+constexpr int64_t kMostBlocks = ((1ll << 32) - 1) / 256;
+static_assert(kAttnBlock == 256);
 // The launch's plan; false where its sizes leave the contract.
 static bool attention_plan(const paia_kv_cache* c, int table_width, int B, int T, int heads, AttnParams* p, int64_t* bytes)
 {
@@ -716,7 +719,7 @@ static bool attention_plan(const paia_kv_cache* c, int table_width, int B, int T
     const int64_t per_seq = ((int64_t)p->max_len / kTile + 1 + kMinTiles - 1) / kMinTiles;
     const int64_t items = goal < per_seq * B ? goal : per_seq * B;
     const int64_t units = items * c->kv_heads, blocks = (units + 7) / 8 * 8 * p->col_groups;
-    if (blocks > INT_MAX || goal > INT_MAX) return false;
+    if (blocks > kMostBlocks) return false;
     p->goal = (int)goal;
     p->units = (int)units;
     p->by_kv_heads = Divisor((uint32_t)c->kv_heads);
