@@ -36,6 +36,9 @@ void on_device_of(const at::Tensor& on, const at::Tensor& t, const char* name)
     TORCH_CHECK(t.device() == on.device(), name, " must be on ", on.device(), ", found ", t.device());
 }
 
+// The stride of a dimension as the C ABI takes it: 0 where there is only one element, whose stride may be anything.
+int64_t stride_of(const at::Tensor& t, int64_t dim) { return t.size(dim) <= 1 ? 0 : t.stride(dim); }
+
 // The data of an optional operand of the given type and length, null where there is none.
 const void* opt_ptr(const std::optional<at::Tensor>& t, at::ScalarType type, int64_t n, const at::Tensor& on,
                     const char* name)
@@ -108,8 +111,8 @@ paia_kv_cache cache_of(const at::Tensor& k, const at::Tensor& v, const std::opti
     c.k_scale = static_cast<const float*>(opt_ptr(k_scale, at::kFloat, c.kv_heads, on, "k_scale"));
     c.v_scale = static_cast<const float*>(opt_ptr(v_scale, at::kFloat, c.kv_heads, on, "v_scale"));
     for (int i = 0; i < 3; ++i) {
-        c.k_strides[i] = k.stride(i);
-        c.v_strides[i] = v.stride(i);
+        c.k_strides[i] = stride_of(k, i);
+        c.v_strides[i] = stride_of(v, i);
     }
     return c;
 }
@@ -137,7 +140,7 @@ void rope_append_out(const at::Tensor& qkv, const at::Tensor& positions, const a
                 "out must be a contiguous bfloat16 tensor [M, num_heads, head_dim]");
     on_device_of(qkv, out, "out");
     c10::DeviceGuard g(qkv.device());
-    check_rc(paia_rope_append(qkv.data_ptr(), qkv.stride(0), positions.data_ptr(), cos_sin.data_ptr(),
+    check_rc(paia_rope_append(qkv.data_ptr(), stride_of(qkv, 0), positions.data_ptr(), cos_sin.data_ptr(),
                               to_int(cos_sin.size(0), "context"), to_int(cos_sin.size(1), "rotary dims"), interleaved,
                               opt_ptr(q_norm, at::kBFloat16, D, qkv, "q_norm"),
                               opt_ptr(k_norm, at::kBFloat16, D, qkv, "k_norm"), (float)eps, slots.data_ptr(), &c,
@@ -169,7 +172,8 @@ Query query_of(const at::Tensor& q)
                 "q must be bfloat16 [B, heads, head_dim] or [B, T, heads, head_dim]");
     TORCH_CHECK(q.numel() == 0 || q.stride(-1) == 1, "q's last dimension must be contiguous");
     const int64_t d = q.dim();
-    return {q.size(0), d == 4 ? q.size(1) : 1, q.size(d - 2), {q.stride(0), d == 4 ? q.stride(1) : 0, q.stride(d - 2)}};
+    return {q.size(0), d == 4 ? q.size(1) : 1, q.size(d - 2),
+            {stride_of(q, 0), d == 4 ? stride_of(q, 1) : 0, stride_of(q, d - 2)}};
 }
 
 // lse may be an undefined tensor: not wanted.
@@ -186,7 +190,7 @@ void paged_attention_run(const at::Tensor& q, const at::Tensor& k_cache, const a
                 ") must be a multiple of the cache's (", c.kv_heads, "), its tokens at least one");
     check_index(lens, at::kInt, y.B, q, "lens");
     TORCH_CHECK(block_table.dim() == 2 && block_table.scalar_type() == at::kInt && block_table.size(0) == y.B &&
-                    (block_table.numel() == 0 || block_table.stride(1) == 1),
+                    (block_table.size(1) <= 1 || block_table.numel() == 0 || block_table.stride(1) == 1),
                 "block_table must be int32 [B, pages of a sequence] with contiguous rows");
     on_device_of(q, block_table, "block_table");
     TORCH_CHECK(out.scalar_type() == at::kBFloat16 && out.is_contiguous() && out.numel() == y.B * y.T * y.heads * c.head_dim,
@@ -200,7 +204,7 @@ void paged_attention_run(const at::Tensor& q, const at::Tensor& k_cache, const a
     check_rc(need < 0 ? (int)need : 0, "paia_paged_attention");
     const Workspace space(workspace, need, q);
     const double s = scale.has_value() ? *scale : 1.0 / std::sqrt((double)c.head_dim);
-    check_rc(paia_paged_attention(q.data_ptr(), y.strides, &c, block_table.data_ptr(), block_table.stride(0), width,
+    check_rc(paia_paged_attention(q.data_ptr(), y.strides, &c, block_table.data_ptr(), stride_of(block_table, 0), width,
                                   lens.data_ptr(), (float)s, to_int(window, "window"), out.data_ptr(),
                                   lse.defined() ? lse.data_ptr() : nullptr, B, T, heads, space.data, space.bytes,
                                   stream_of(q)),
@@ -282,9 +286,10 @@ void lora_add_out(const at::Tensor& y, const at::Tensor& x, const at::Tensor& A,
     const long long need = paia_lora_add_workspace(to_int(M, "M"), to_int(K, "K"), to_int(R, "rank"), parts, slices);
     check_rc(need < 0 ? (int)need : 0, "paia_lora_add");
     const Workspace space(workspace, need, A);
-    check_rc(paia_lora_add(y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), A.data_ptr(), B.data_ptr(), ids.data_ptr(),
-                           opt_ptr(scaling, at::kFloat, L, A, "scaling"), out.data_ptr(), out.stride(0), (int)M,
-                           (int)K, (int)R, parts, slices, to_int(L, "adapters"), space.data, space.bytes, stream_of(A)),
+    check_rc(paia_lora_add(y.data_ptr(), stride_of(y, 0), x.data_ptr(), stride_of(x, 0), A.data_ptr(), B.data_ptr(),
+                           ids.data_ptr(), opt_ptr(scaling, at::kFloat, L, A, "scaling"), out.data_ptr(), stride_of(out, 0),
+                           (int)M, (int)K, (int)R, parts, slices, to_int(L, "adapters"), space.data, space.bytes,
+                           stream_of(A)),
              "paia_lora_add");
 }
 at::Tensor lora_add(const at::Tensor& y, const at::Tensor& x, const at::Tensor& A, const at::Tensor& B,
