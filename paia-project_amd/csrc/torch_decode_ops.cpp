@@ -85,8 +85,8 @@ struct Workspace {
     }
 };
 
-paia_kv_cache cache_of(const at::Tensor& k, const at::Tensor& v, const std::optional<at::Tensor>& k_scale,
-                       const std::optional<at::Tensor>& v_scale, const at::Tensor& on)
+// A cache's sizes, type and strides, which tracing has too; no addresses.
+paia_kv_cache shape_of(const at::Tensor& k, const at::Tensor& v)
 {
     const auto is_code = [](const at::Tensor& t) {
         return t.scalar_type() == at::kFloat8_e4m3fn || t.scalar_type() == at::kByte;
@@ -97,23 +97,29 @@ paia_kv_cache cache_of(const at::Tensor& k, const at::Tensor& v, const std::opti
                 "k_cache and v_cache must both be bfloat16 or both e4m3 (float8_e4m3fn or uint8)");
     TORCH_CHECK(k.numel() > 0, "the cache must not be empty");
     TORCH_CHECK(k.stride(3) == 1 && v.stride(3) == 1, "the cache's last dimension must be contiguous");
-    on_device_of(on, k, "k_cache");
-    on_device_of(on, v, "v_cache");
-    TORCH_CHECK(is_code(k) || (!k_scale.has_value() && !v_scale.has_value()), "k_scale and v_scale go with an e4m3 cache");
-    paia_kv_cache c;
-    c.k = k.data_ptr();
-    c.v = v.data_ptr();
+    paia_kv_cache c{};
     c.pages = to_int(k.size(0), "pages");
     c.kv_heads = to_int(k.size(1), "kv_heads");
     c.page_size = to_int(k.size(2), "page_size");
     c.head_dim = to_int(k.size(3), "head_dim");
     c.fp8 = is_code(k);
-    c.k_scale = static_cast<const float*>(opt_ptr(k_scale, at::kFloat, c.kv_heads, on, "k_scale"));
-    c.v_scale = static_cast<const float*>(opt_ptr(v_scale, at::kFloat, c.kv_heads, on, "v_scale"));
     for (int i = 0; i < 3; ++i) {
         c.k_strides[i] = stride_of(k, i);
         c.v_strides[i] = stride_of(v, i);
     }
+    return c;
+}
+paia_kv_cache cache_of(const at::Tensor& k, const at::Tensor& v, const std::optional<at::Tensor>& k_scale,
+                       const std::optional<at::Tensor>& v_scale, const at::Tensor& on)
+{
+    paia_kv_cache c = shape_of(k, v);
+    on_device_of(on, k, "k_cache");
+    on_device_of(on, v, "v_cache");
+    TORCH_CHECK(c.fp8 || (!k_scale.has_value() && !v_scale.has_value()), "k_scale and v_scale go with an e4m3 cache");
+    c.k = k.data_ptr();
+    c.v = v.data_ptr();
+    c.k_scale = static_cast<const float*>(opt_ptr(k_scale, at::kFloat, c.kv_heads, on, "k_scale"));
+    c.v_scale = static_cast<const float*>(opt_ptr(v_scale, at::kFloat, c.kv_heads, on, "v_scale"));
     return c;
 }
 
@@ -241,9 +247,13 @@ void paged_attention_out(const at::Tensor& q, const at::Tensor& k_cache, const a
 {
     paged_attention_run(q, k_cache, v_cache, block_table, lens, scale, window, k_scale, v_scale, out, {}, workspace);
 }
+// On tensors without memory too (tracing): the sizes alone count, so the addresses only have to be ones that the C ABI takes.
 int64_t paged_attention_workspace(const at::Tensor& k_cache, int64_t table_width, int64_t B, int64_t T, int64_t num_heads)
 {
-    const paia_kv_cache c = cache_of(k_cache, k_cache, {}, {}, k_cache);
+    paia_kv_cache c = shape_of(k_cache, k_cache);
+    c.k = c.v = reinterpret_cast<void*>(16);
+    c10::OptionalDeviceGuard g;
+    if (k_cache.is_cuda()) g.reset_device(k_cache.device());
     const long long need = paia_paged_attention_workspace(&c, to_int(table_width, "table_width"), to_int(B, "B"),
                                                           to_int(T, "T"), to_int(num_heads, "num_heads"));
     check_rc(need < 0 ? (int)need : 0, "paia_paged_attention_workspace");
@@ -383,6 +393,7 @@ TORCH_LIBRARY_IMPL(paia_gemv, Meta, m)
     m.impl("paged_attention", &paged_attention_meta);
     m.impl("paged_attention_lse", &paged_attention_lse_meta);
     m.impl("paged_attention_out", &paged_attention_out_meta);
+    m.impl("paged_attention_workspace", &paged_attention_workspace);
     m.impl("lora_add", &lora_add_meta);
     m.impl("lora_add_out", &lora_add_out_meta);
 }
