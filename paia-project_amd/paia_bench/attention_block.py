@@ -86,7 +86,8 @@ class AttentionBlock:
         need = [-(-(n + room) // page_size) for n in lengths]
         self.page_size, width = page_size, max(need)
         order = torch.randperm(sum(need), generator=gen, device=device).int()
-        self.table = torch.full((B, width), -1, dtype=torch.int32, device=device)
+        # a column more than any sequence has pages, for positions past the room: page -1, nothing is written or attended there
+        self.table = torch.full((B, width + 1), -1, dtype=torch.int32, device=device)
         at = 0
         for b, n in enumerate(need):
             self.table[b, :n] = order[at:at + n]
@@ -104,14 +105,19 @@ class AttentionBlock:
         self.positions = torch.tensor(lengths, dtype=torch.int64, device=device)    # of the next token
         self.cos_sin = ops.rope_table(width * page_size, dim, ROPE_BASE[model], device=device)
         self.ids = (torch.arange(B, device=device) % (adapters + 1) - 1).int()      # row 0 without an adapter
-        self.workspace = torch.empty(max(16, ops.paged_attention_workspace(self.k_cache, width, B, 1, heads)),
+        self.workspace = torch.empty(max(16, ops.paged_attention_workspace(self.k_cache, width + 1, B, 1, heads)),
                                      dtype=torch.uint8, device=device)
 
+    def slots(self):
+        """Where the next token of every sequence goes, negative past its room."""
+        column = (self.positions // self.page_size).clamp(max=self.table.shape[1] - 1)
+        return self.table.gather(1, column[:, None])[:, 0].long() * self.page_size + self.positions % self.page_size
+
     def step(self, x):
-        """x bf16 [batch, hidden] -> y bf16 [batch, hidden]: the next token of every sequence."""
+        """x bf16 [batch, hidden] -> y bf16 [batch, hidden]: the next token of every sequence. Past its room a sequence's cache stays
+        as it is."""
         heads, _, dim = self.heads
-        page = self.table.gather(1, (self.positions // self.page_size)[:, None])[:, 0].long()
-        slots = page * self.page_size + self.positions % self.page_size
+        slots = self.slots()
         lens = (self.positions + 1).int()
         qkv = self.qkv(x, self.ids)
         q = ops.rope_append(qkv, self.positions, self.cos_sin, self.k_cache, self.v_cache, slots, heads,
