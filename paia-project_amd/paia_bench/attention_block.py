@@ -8,6 +8,9 @@ sequence; it advances the positions on the device, so a captured step is replaye
 and adapters are random (seeded); Qwen2.5's qkv projection has its bias.
 
     python -m paia_bench.attention_block --model llama31_8b --fmt fp8 --cache fp8 --batch 8 --context 4096 --adapters 4
+
+times a step. One layer's weights and cache can lie in the 256 MiB last-level cache whole, so the command steps as many blocks in
+turn (`copies`) as keep any of them from being found there when it is next used.
 """
 from __future__ import annotations
 
@@ -20,7 +23,7 @@ import torch
 from paia_gemv import ops, quant
 from paia_gemv.shapes import HEADS, LAYER, ROPE_BASE, gemv_bytes
 
-from .timing import capture, replay_ms, stats
+from .timing import capture, plan_rotation, replay_ms, stats
 
 
 class Projection:
@@ -128,12 +131,13 @@ class AttentionBlock:
         self.positions += 1
         return y
 
-    def bytes(self):
-        """Bytes a step cannot do without: weights, activations and the cache as it stands (adapters left out)."""
+    def bytes(self, later=0):
+        """Bytes that the step after `later` more cannot do without: weights, activations and the cache as it stands then (adapters
+        left out)."""
         _, kv_heads, dim = self.heads
         M = len(self.positions)
         return (self.qkv.bytes(M) + self.o.bytes(M)
-                + int(self.positions.sum() + M) * 2 * kv_heads * dim * self.k_cache.element_size())
+                + int(self.positions.sum() + M * (later + 1)) * 2 * kv_heads * dim * self.k_cache.element_size())
 
 
 def main(argv=None):
@@ -150,13 +154,19 @@ def main(argv=None):
     if not 1 <= a.batch <= 16:
         ap.error("--batch: the projections take 1 to 16 rows")
     lengths = [max(1, a.context * (a.batch - b) // a.batch) for b in range(a.batch)]
-    block = AttentionBlock(a.model, a.fmt, lengths, room=a.steps + 16, cache=a.cache, adapters=a.adapters, rank=a.rank)
-    x = torch.randn(a.batch, block.qkv.K, device="cuda").to(torch.bfloat16)
-    nbytes = block.bytes()
-    graph = capture(lambda: block.step(x))
-    us = stats(replay_ms(graph, a.steps))["median"] * 1e3
+    make = lambda seed: AttentionBlock(a.model, a.fmt, lengths, room=a.steps + 16, cache=a.cache, adapters=a.adapters,  # noqa: E731
+                                       rank=a.rank, seed=seed)
+    blocks = [make(0)]
+    warm = 2
+    nbytes = blocks[0].bytes(warm + a.steps // 2)       # of the middle one of the timed steps
+    plan = plan_rotation(nbytes)
+    blocks += [make(seed) for seed in range(1, plan["n_copies"])]
+    x = torch.randn(a.batch, blocks[0].qkv.K, device="cuda").to(torch.bfloat16)
+    graph = capture(lambda: [block.step(x) for block in blocks], warm=warm)
+    us = stats(replay_ms(graph, a.steps))["median"] * 1e3 / len(blocks)
     print(json.dumps({"model": a.model, "fmt": a.fmt, "cache": a.cache, "batch": a.batch, "context": a.context,
-                      "adapters": a.adapters, "us_per_step": round(us, 2), "gbps": round(nbytes / us / 1e3, 1)}))
+                      "adapters": a.adapters, "copies": len(blocks), "llc_safe": plan["llc_safe"], "us_per_step": round(us, 2),
+                      "gbps": round(nbytes / us / 1e3, 1)}))
     return 0
 
 
