@@ -699,9 +699,10 @@ static bool attention_plan(const paia_kv_cache* c, int table_width, int B, int T
     p->B = B, p->T = T, p->heads = heads;
     p->group = heads / c->kv_heads;
     const int64_t cols = (int64_t)T * p->group, max_len = (int64_t)table_width * c->page_size;
-    // tile numbers times 32, with a tile to spare, stay within 31 bits
-    p->max_len = (int)(max_len < INT_MAX - 4096 ? max_len : INT_MAX - 4096);
     if (cols > 65535 || c->kv_heads > 65535) return false;      // dimensions of the joining grid
+    // tile numbers times 32, with a tile to spare, and a length less T and a window (below max_len) stay within 32 bits
+    constexpr int kLongest = INT_MAX - (1 << 17);
+    p->max_len = (int)(max_len < kLongest ? max_len : kLongest);
     p->cols = (int)cols;
     // The columns' tiles over the fewest blocks, evenly, as far as a lane's registers hold its outputs.
     const double row = 2.0 * c->kv_heads * c->head_dim * (c->fp8 ? 1 : 2);
@@ -792,7 +793,7 @@ int paia_paged_attention(const void* q, const long long* q_strides, const paia_k
     p.lens = static_cast<const int32_t*>(lens);
     p.table_stride = table_stride;
     p.scale = scale * 1.4426950408889634f;
-    p.window = window >= (int64_t)p.max_len + T ? 0 : window;    // it hides nothing
+    p.window = window >= p.max_len ? 0 : window;     // it hides nothing
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = p.part_o + (int64_t)p.units * p.cols * cache->head_dim;
     p.part_of = bytes > 0 ? reinterpret_cast<int2*>(p.part_ml + (int64_t)p.units * p.cols * 2) : nullptr;
