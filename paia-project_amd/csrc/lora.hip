@@ -230,9 +230,13 @@ __global__ void __launch_bounds__(kShrinkBlock) lora_shrink_kernel(const LoraPar
 // layout through its own piece of LDS (rows an odd number of pieces apart: no bank conflicts). A block takes consecutive
 // units, with kExpandAhead units' loads in flight, and sums the pieces of h anew only where the chunk or slice changes.
 constexpr int expand_rows(int steps) { return steps <= 2 ? 32 : 16; }
+// Blocks of the expand kernel that are launched for each CU, one wave of each on a SIMD: no more than its registers let be resident.
+// Beyond rank 128 that is two: a third ran behind them (us at three / two: sixteen rows and adapters of rank 256 beside 4096 -> 6144
+// 41.4 / 38.6 and -> 28672 72.4 / 64.7, of rank 192 beside 3584 -> 3584 21.1 / 18.1).
+constexpr int expand_blocks(int steps) { return steps <= 4 ? 3 : 2; }
 constexpr int kExpandAhead = 2;
 template <int STEPS, bool WIDE>
-__global__ void __launch_bounds__(kLoraBlock) lora_expand_kernel(const LoraParams p)
+__global__ void __launch_bounds__(kLoraBlock, expand_blocks(STEPS)) lora_expand_kernel(const LoraParams p)
 {
     constexpr int ROWS = expand_rows(STEPS), kTiles = ROWS / 16, kLoads = ROWS * STEPS * 4 / kWave;
     constexpr int kHPitch = STEPS * 4 + 1, kBPitch = STEPS * 4 + 1;      // 16-byte pieces
@@ -447,17 +451,16 @@ __global__ void __launch_bounds__(kSmallBlock) lora_small_kernel(const LoraParam
 
 static int launch_lora(const LoraParams& p, hipStream_t st)
 {
-    // Blocks that are resident together (registers: two of eight waves, three of four here), fewer where there are fewer
-    // units: the rest would only find the rows again (128 rows of 12 adapters 15.4 us at four a CU, 13.8 so; sixteen of rank
-    // 64 even).
-    const int cap = device_facts().cus * 2, cap_expand = device_facts().cus * 3;
+    // Blocks that are resident together, fewer where there are fewer units: the rest would only find the rows again (128 rows of 12
+    // adapters 15.4 us at four a CU, 13.8 so; sixteen of rank 64 even).
+    const int steps = (p.R + 31) / 32;
+    const int cap = device_facts().cus * 2, cap_expand = device_facts().cus * expand_blocks(steps);
     const int64_t shrink = (int64_t)p.M * (p.h_stride / 16) * kMaxPieces;
     hipLaunchKernelGGL(lora_shrink_kernel, dim3((uint32_t)(shrink < cap ? shrink : cap)), dim3(kShrinkBlock), 0, st, p);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return (int)e;
     const int64_t expand = (int64_t)p.M * p.unit_first[p.slices];
     const dim3 grid((uint32_t)(expand < cap_expand ? expand : cap_expand));
     auto go = [&](auto wide, auto narrow) { hipLaunchKernelGGL(p.wide ? wide : narrow, grid, dim3(kLoraBlock), 0, st, p); };
-    const int steps = (p.R + 31) / 32;
     if (steps <= 1) go(lora_expand_kernel<1, true>, lora_expand_kernel<1, false>);
     else if (steps <= 2) go(lora_expand_kernel<2, true>, lora_expand_kernel<2, false>);
     else if (steps <= 4) go(lora_expand_kernel<4, true>, lora_expand_kernel<4, false>);
