@@ -6,7 +6,7 @@
 // Each cache byte is used for T G products a value (G query heads share a kv head), a few operations per byte: bound by
 // reading the cache once. The pieces of the design:
 //   * Work: a unit is one piece of one sequence for one kv head and 16 columns (token, query head of the group), or
-//     up to 48 where the cache is large (most_tiles). The lengths are on the device and the grid is fixed by the host, so
+//     up to 48 where the tables are large (attention_tiles.h). The lengths are on the device and the grid is fixed by the host, so
 //     each block derives the split from the lengths itself (find_piece): about as many equal pieces as blocks fit the
 //     chip, whatever the lengths are. A captured call stays balanced as the sequences grow. Pieces of one sequence leave
 //     (m, l, o) in the workspace, joined by a second kernel; a sequence of one piece is written by its block.
@@ -29,6 +29,7 @@
 #include <math.h>
 #include <stdint.h>
 
+#include "attention_tiles.h"
 #include "gemv_kernel.h"
 #include "kv_cache.h"
 #include "paia_gemv.h"
@@ -36,16 +37,6 @@
 namespace paia {
 
 constexpr int kTile = 32;            // positions a wave takes at a time
-constexpr int kCols = 16;            // columns (token, head) of a matrix tile; a block takes up to most_tiles() such tiles
-// Tiles of columns that a block takes together, so that each row is read and taken apart once for all: as many as a lane's
-// registers hold the outputs of (e4m3 heads of 128 spill 132 bytes with two, and gain all the same). A block of several tiles
-// stages its queries and does more after its last row, so it takes caches that fill the chip for longer: kTogether bytes, as
-// the block table's size bounds them. Five tokens of 4 and of 8 heads a group, 8 sequences, us with one tile a block / together:
-//   bf16 heads of 128, 2500 positions 20.7 / 22.2 and 23.9 / 25.9; 6000 (164 MB) 43.7 / 41.0 and 53.1 / 49.0; 16000 86.5 / 81.3
-//   and 115.8 / 94.0; heads of 64, 6000 (82 MB) 22.0 / 24.5 and 28.9 / 29.3; 16000 (200 MB) 51.6 / 46.8 and 64.4 / 50.8; e4m3
-//   heads of 128, 16000 (200 MB) 66.7 / 54.2 and 98.7 / 86.0; of 64 (100 MB) 43.3 / 40.6 and 57.3 / 47.2.
-constexpr int most_tiles(int dim, bool p8) { return dim <= 64 ? 3 : dim <= 128 && p8 ? 2 : 1; }
-constexpr int64_t kTogether = 120 << 20;
 constexpr int kAttnWaves = 4, kAttnBlock = kAttnWaves * kWave;
 // Blocks that a CU holds at the registers a wave takes (one wave of a block on each SIMD).
 constexpr int blocks_per_cu(int dim, int tiles) { return dim <= 64 ? (tiles == 1 ? 3 : 2) : dim <= 128 ? 2 : 1; }
@@ -692,22 +683,12 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
 // A launch has less than 2^32 threads; a block of the first grid for every sequence at least, so the joining one is bounded too.
 constexpr int64_t kMostBlocks = ((1ll << 32) - 1) / 256;
 static_assert(kAttnBlock == 256);
-// The launch's plan; false where its sizes leave the contract.
-static bool attention_plan(const paia_kv_cache* c, int table_width, int B, int T, int heads, AttnParams* p, int64_t* bytes)
+// The launch's plan with up to `most` tiles of columns a block, and its workspace; false where it is more than a launch takes.
+static bool plan_blocks(const paia_kv_cache* c, int most, AttnParams* p, int64_t* bytes)
 {
-    if (!cache_view(c, &p->cache) || table_width < 0 || B < 0 || T <= 0 || heads <= 0 || heads % c->kv_heads) return false;
-    p->B = B, p->T = T, p->heads = heads;
-    p->group = heads / c->kv_heads;
-    const int64_t cols = (int64_t)T * p->group, max_len = (int64_t)table_width * c->page_size;
-    if (cols > 65535 || c->kv_heads > 65535) return false;      // dimensions of the joining grid
-    // tile numbers times 32, with a tile to spare, and a length less T and a window (below max_len) stay within 32 bits
-    constexpr int kLongest = INT_MAX - (1 << 17);
-    p->max_len = (int)(max_len < kLongest ? max_len : kLongest);
-    p->cols = (int)cols;
-    // The columns' tiles over the fewest blocks, evenly, as far as a lane's registers hold its outputs.
-    const double row = 2.0 * c->kv_heads * c->head_dim * (c->fp8 ? 1 : 2);
-    const bool large = row * B * p->max_len >= (double)kTogether;
-    const int tiles = (p->cols + kCols - 1) / kCols, most = large ? most_tiles(c->head_dim, c->page_size % 8 == 0) : 1;
+    const int B = p->B;
+    // The columns' tiles over the fewest blocks, evenly.
+    const int tiles = (p->cols + kCols - 1) / kCols;
     p->tiles = (tiles + (tiles + most - 1) / most - 1) / ((tiles + most - 1) / most);
     p->col_groups = (tiles + p->tiles - 1) / p->tiles;
     const int64_t wide = (int64_t)c->kv_heads * p->col_groups, slots = (int64_t)device_facts().cus * blocks_per_cu(c->head_dim, p->tiles);
@@ -728,6 +709,30 @@ static bool attention_plan(const paia_kv_cache* c, int table_width, int B, int T
     p->by_col_groups = Divisor((uint32_t)p->col_groups);
     // one piece a sequence at most: nothing is joined
     *bytes = per_seq <= 1 ? 0 : units * p->cols * (c->head_dim + 2) * (int64_t)sizeof(float) + B * (int64_t)sizeof(int2);
+    return true;
+}
+// The same for a call; false where its sizes leave the contract. The workspace serves any window: where the tiles that a block takes go
+// by the window, it is the larger one of both forms.
+static bool attention_plan(const paia_kv_cache* c, int table_width, int B, int T, int heads, int window, AttnParams* p, int64_t* bytes)
+{
+    if (!cache_view(c, &p->cache) || table_width < 0 || B < 0 || T <= 0 || heads <= 0 || heads % c->kv_heads || window < 0) return false;
+    p->B = B, p->T = T, p->heads = heads;
+    p->group = heads / c->kv_heads;
+    const int64_t cols = (int64_t)T * p->group, max_len = (int64_t)table_width * c->page_size;
+    if (cols > 65535 || c->kv_heads > 65535) return false;      // dimensions of the joining grid
+    // tile numbers times 32, with a tile to spare, and a length less T and a window (below max_len) stay within 32 bits
+    constexpr int kLongest = INT_MAX - (1 << 17);
+    p->max_len = (int)(max_len < kLongest ? max_len : kLongest);
+    p->cols = (int)cols;
+    p->window = window >= p->max_len ? 0 : window;     // it hides nothing
+    const double row = 2.0 * c->kv_heads * c->head_dim * (c->fp8 ? 1 : 2);
+    const int most = most_tiles(c->head_dim, c->page_size % 8 == 0);
+    if (!table_is_large(row, B, p->max_len)) return plan_blocks(c, 1, p, bytes);
+    const bool together = window_is_large(row, B, T, p->window);
+    int64_t other = 0;
+    if (!plan_blocks(c, together ? 1 : most, p, &other)) other = 0;
+    if (!plan_blocks(c, together ? most : 1, p, bytes)) return false;
+    *bytes = *bytes > other ? *bytes : other;
     return true;
 }
 
@@ -767,7 +772,7 @@ long long paia_paged_attention_workspace(const paia_kv_cache* cache, int table_w
 {
     paia::AttnParams p;
     int64_t bytes = 0;
-    return paia::attention_plan(cache, table_width, B, T, heads, &p, &bytes) ? bytes : -2;
+    return paia::attention_plan(cache, table_width, B, T, heads, 0, &p, &bytes) ? bytes : -2;
 }
 
 int paia_paged_attention(const void* q, const long long* q_strides, const paia_kv_cache* cache, const void* block_table,
@@ -777,7 +782,7 @@ int paia_paged_attention(const void* q, const long long* q_strides, const paia_k
     using namespace paia;
     AttnParams p;
     int64_t bytes = 0;
-    if (!attention_plan(cache, table_width, B, T, heads, &p, &bytes) || window < 0 || table_stride < 0) return -2;
+    if (!attention_plan(cache, table_width, B, T, heads, window, &p, &bytes) || table_stride < 0) return -2;
     if (B == 0) return 0;
     if (q == nullptr || q_strides == nullptr || lens == nullptr || out == nullptr || (block_table == nullptr && table_width > 0))
         return -2;
@@ -793,7 +798,6 @@ int paia_paged_attention(const void* q, const long long* q_strides, const paia_k
     p.lens = static_cast<const int32_t*>(lens);
     p.table_stride = table_stride;
     p.scale = scale * 1.4426950408889634f;
-    p.window = window >= p.max_len ? 0 : window;     // it hides nothing
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = p.part_o + (int64_t)p.units * p.cols * cache->head_dim;
     p.part_of = bytes > 0 ? reinterpret_cast<int2*>(p.part_ml + (int64_t)p.units * p.cols * 2) : nullptr;
