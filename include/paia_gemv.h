@@ -191,11 +191,12 @@ PAIA_API int paia_rope_append(const void* qkv, long long qkv_stride, const void*
  * there). With s_p = scale * k_scale[head] * <q, k_p>: out bf16 [B][T][heads][head_dim] (16-byte aligned) =
  * v_scale[head] * sum softmax(s)_p v_p, lse fp32 [B][T][heads] or NULL = log(sum exp(s_p)); a token that sees
  * nothing has out 0, lse -inf. Scores, statistics and sums in fp32; the weights enter their product with v as two
- * bf16 terms. Nothing a token does not see reaches its output, NaN and infinities included. The lengths are read on
- * the device: a captured call serves sequences as they grow. workspace: device memory, 16-byte aligned, of at least
- * paia_paged_attention_workspace() bytes (for the same cache, width, B, T and heads; 0 = NULL will do, -2 = outside
- * the contract). Calls that overlap need a workspace each. out overlaps no other operand. At most 65535 kv heads
- * and T * heads / kv_heads = n, and about 2^24 of B * kv_heads * ceil(n / 16), the blocks of a launch. */
+ * bf16 terms (16 bits). Nothing a token does not see reaches its output, NaN and infinities included; an infinity in
+ * v that it sees gives that infinity, both signs NaN. The lengths are read on the device: a captured call serves
+ * sequences as they grow. workspace: device memory, 16-byte aligned, of at least paia_paged_attention_workspace()
+ * bytes (for the same cache, width, B, T and heads, any window; 0 = NULL will do, -2 = outside the contract). Calls
+ * that overlap need a workspace each. out overlaps no other operand. At most 65535 kv heads and T * heads / kv_heads
+ * = n, and about 2^24 of B * kv_heads * ceil(n / 16), the blocks of a launch. */
 PAIA_API long long paia_paged_attention_workspace(const paia_kv_cache* cache, int table_width, int B, int T, int heads);
 PAIA_API int paia_paged_attention(const void* q, const long long* q_strides, const paia_kv_cache* cache,
                                   const void* block_table, long long table_stride, int table_width, const void* lens,
