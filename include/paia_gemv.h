@@ -217,6 +217,66 @@ PAIA_API int paia_lora_add(const void* y, long long y_stride, const void* x, lon
                            int K, int rank, const int* splits, int slices, int adapters, void* workspace,
                            long long workspace_bytes, void* stream);
 
+/* ---- the feed-forward half of a layer with experts (no reference counterpart): residual and norms, each token's experts,
+ *      the experts' products. Same conventions. ------------------------------------------------------------------- */
+
+/* Between the halves of a layer: with y = x[m], or sum_j weights[m][j] x[m][j] where pairs > 0 (a pair of weight 0 adds
+ * nothing, whatever its row holds), and rms(v, w) = v / sqrt(mean(v^2) + eps) * w (* (1 + w) where plus_one):
+ *   y = rms(y, post_norm) where post_norm is given; r = residual[m] + scale * gate * y; out[m] = rms(r, norm).
+ * x bf16 [M][D] or [M][pairs][D] (row m at x + m * x_stride, its pair j pair_stride further each), weights fp32
+ * [M][pairs] (with pairs), residual [M][D], bf16 or fp32, or NULL (0), post_norm (or NULL) and norm bf16 [D], gate bf16,
+ * row m at gate + m * gate_stride (0: one row for all; NULL: 1). out bf16 [M][D], and residual_out (or NULL: not
+ * wanted), of the residual's type, has r. Everything in fp32 (out is made of the r that is not rounded yet), each output
+ * rounded once. All pointers but weights 16-byte aligned, strides in elements and multiples of 8; D % 8 == 0, D <= 32768.
+ * residual_out may be residual, out may be x (without pairs); else the outputs overlap nothing. M = 0 does nothing. */
+PAIA_API int paia_add_norm(const void* x, long long x_stride, const void* weights, long long pair_stride, int pairs,
+                           const void* residual, long long residual_stride, int residual_fp32, const void* post_norm,
+                           const void* gate, long long gate_stride, float scale, const void* norm, int plus_one, float eps,
+                           void* out, long long out_stride, void* residual_out, long long residual_out_stride, int M, int D,
+                           void* stream);
+
+/* Each token's k of `experts` experts, from logits bf16 or fp32 [M][experts] (row stride in elements): those of the
+ * largest key, the logit itself or (sigmoid = 1) sigmoid(logit) + bias (fp32 [experts] or NULL), the lower index first
+ * among equal ones. ids int32 [M][k] in that order; weights fp32 [M][k] = scale * score, the score being the softmax of
+ * the row's logits at the expert, or sigmoid(logit) (the bias decides the choice alone), and with renormalize divided
+ * by the sum of the token's k scores. Experts whose logit or bias is -inf or NaN are closed; where fewer than k are
+ * open, ids end with -1, weights with 0. Then the pairs m * k + j in the experts' order: order int32 [M * k], sorted by
+ * expert, in their own order within one, those without an expert at the end; offsets int32 [experts + 1], expert e's at
+ * order[offsets[e]] .. order[offsets[e + 1] - 1]. Keys of the sigmoid and all weights in fp64, rounded once. experts <=
+ * 1024, k <= 64, M * k < 2^26; M = 0 writes the offsets (zeros) alone. paia_expert_order: the order alone, from ids that
+ * the caller has (outside [0, experts): no expert; given twice by one token: two pairs). workspace: device memory, 16-byte
+ * aligned, of paia_route_experts_workspace() bytes for either (0 for few tokens, NULL will do; -2 = outside the contract);
+ * nothing is kept in it from one call to the next, calls that overlap need one each. The outputs overlap nothing. */
+PAIA_API long long paia_route_experts_workspace(int M, int experts, int k);
+PAIA_API int paia_route_experts(const void* logits, int logits_fp32, long long logits_stride, const void* bias, int sigmoid,
+                                int renormalize, float scale, void* ids, void* weights, void* order, void* offsets, int M,
+                                int experts, int k, void* workspace, long long workspace_bytes, void* stream);
+PAIA_API int paia_expert_order(const void* ids, void* order, void* offsets, int M, int experts, int k, void* workspace,
+                               long long workspace_bytes, void* stream);
+
+/* The experts' products: for each pair p = order[i], offsets[e] <= i < offsets[e + 1] (as paia_route_experts leaves them),
+ *   out[p][n] = sum_k deq(W[e][n][k]) * x[p / (pairs / x_rows)][k] (+ bias[e][n]),
+ * x bf16 [x_rows][K], x_rows a divisor of pairs: with x_rows = M the k pairs of a token share its row, with x_rows =
+ * pairs each has its own. gated = 1: rows n and N/2 + n of an expert are a gate and what it opens, out[p][n] =
+ * silu(first) * second, [pairs][N/2] (silu(g) = g / (1 + exp(-g))). Outputs of pairs without an expert (order from
+ * offsets[experts] on) are 0. fp32 sums, one rounding at the end; W, scale(s), zeros and bias as [experts] times the
+ * operands of the M = 1 entry point of the format, same alignment and rules for K. x and its rows 16-byte aligned, out
+ * bf16, its rows anywhere; strides in elements. out overlaps nothing. order and offsets are read on the device (a captured
+ * call follows them); entries outside their ranges are not followed. experts <= 1024, pairs < 2^26, N and K <= 2^26, and at most
+ * 2^22 blocks of a launch (about pairs / 256 times N / 256 of them); pairs = 0 does nothing. */
+PAIA_API int paia_experts_bf16(const void* W, const void* x, long long x_stride, int x_rows, const void* order,
+                               const void* offsets, const void* bias, void* out, long long out_stride, int experts, int N,
+                               int K, int pairs, int gated, void* stream);
+PAIA_API int paia_experts_fp8(const void* Wq, const void* scale, const void* x, long long x_stride, int x_rows,
+                              const void* order, const void* offsets, const void* bias, void* out, long long out_stride,
+                              int experts, int N, int K, int pairs, int gated, void* stream);
+PAIA_API int paia_experts_int4(const void* Wq, const void* scales, const void* x, long long x_stride, int x_rows,
+                               const void* order, const void* offsets, void* out, long long out_stride, int experts, int N,
+                               int K, int pairs, int gated, void* stream);
+PAIA_API int paia_experts_int4_zp(const void* Wq, const void* scales, const void* zeros, const void* x, long long x_stride,
+                                  int x_rows, const void* order, const void* offsets, const void* bias, void* out,
+                                  long long out_stride, int experts, int N, int K, int pairs, int gated, void* stream);
+
 /* no reference counterpart: a human-readable build tag */
 PAIA_API const char* paia_gemv_build_info(void);
 

@@ -43,9 +43,11 @@ HIP_FLAGS = [
 ]
 HIP_SOURCES = ["gemv_runtime.hip", "gemv_bf16.hip", "gemv_fp8.hip", "gemv_int4.hip", "gemv_dequant.hip",
                "gemv_select.hip", "quantize.hip", "gemv_batch.hip",
-               "gemv_tile.hip", "rope_append.hip", "paged_attention.hip", "lora.hip"]
+               "gemv_tile.hip", "rope_append.hip", "paged_attention.hip", "lora.hip", "add_norm.hip",
+               "route_experts.hip", "experts.hip", "experts_bf16.hip", "experts_fp8.hip", "experts_int4.hip",
+               "experts_int4_zp.hip"]
 
-TORCH_SOURCES = ["torch_ops.cpp", "torch_decode_ops.cpp"]
+TORCH_SOURCES = ["torch_ops.cpp", "torch_decode_ops.cpp", "torch_expert_ops.cpp"]
 
 
 def _run(cmd, quiet_warn=True):

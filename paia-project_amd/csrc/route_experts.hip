@@ -1,0 +1,457 @@
+// Each token's experts, and the pairs of token and expert in the experts' order.
+//
+//   key[m, e] = logits[m, e]                     softmax, whose order is that of the logits
+//             = sigmoid(logits[m, e]) + bias[e]  sigmoid; the bias decides the choice, not the weight
+//   ids[m, :] = the k experts of the largest keys, the lower index first among equal ones
+//   weights[m, j] = scale * s(m, ids[m, j]) (/ their sum),  s = softmax over the row's experts, or sigmoid
+//
+// Experts whose logit (or bias) is -inf or NaN are closed to the token; where fewer than k are open the rest of ids is -1, of
+// weight 0. A wave has a token, a lane every 64th expert of it: the largest key comes of one DPP maximum, its lowest index of
+// the lanes' ballots, k times. Keys that are computed (sigmoid), and all weights, are so in 64 bits: neighbouring keys decide
+// which experts run, and there are few of them.
+//
+// order: the pairs m * k + j sorted by expert, in their own order within one, those without an expert at the end. A block counts
+// its pairs by wave and expert in LDS and gives each its place: the lanes with the same expert find each other by one ballot
+// a bit of the id. Few tokens are one launch of one block. Otherwise each block leaves its counts in the workspace and the second
+// launch's blocks add up those before their own (integers: the order of sums does not matter, nothing is atomic across blocks).
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "gemv_kernel.h"
+#include "paia_gemv.h"
+
+namespace paia {
+
+constexpr int kRouteBlock = 1024, kRouteWaves = kRouteBlock / kWave;
+constexpr int kRouteExperts = 1024;      // experts at most: a thread each in the scan
+constexpr int kRouteBlocks = 256;        // blocks at most that share the tokens
+constexpr int kRouteTokens = 32;         // tokens up to which one block does all of it
+
+struct RouteParams {
+    const void* logits;                  // bf16 or fp32 [M][E]
+    const float* bias;                   // [E] or null
+    int32_t *ids, *order, *offsets;
+    float* weights;
+    int32_t* counts;                     // workspace: [block][E + 1]
+    int64_t stride;                      // elements
+    int M, E, k, tokens;                 // tokens: of a block
+    int id_bits;
+    bool fp32, renormalize;
+    float scale;
+};
+
+// Bits whose order is that of the values, 0 below all of them; -0 counts as 0.
+__device__ __forceinline__ uint32_t sortable(float v)
+{
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return b >> 31 ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t sortable(double v)
+{
+    const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
+    return b >> 63 ? ~b : b | 1ull << 63;
+}
+
+__device__ __forceinline__ double wave_add(double v)
+{
+#pragma unroll
+    for (int i = 1; i < kWave; i *= 2) v += __shfl_xor(v, i, kWave);
+    return v;
+}
+
+// The largest key of the wave and its lowest index (lane + 64 i); false where all are 0. The key found is set to 0.
+template <int NE>
+__device__ __forceinline__ bool take_largest(uint32_t (&key)[NE], int* index)
+{
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) most = max(most, key[i]);
+    most = wave_max_u32(most);
+    if (most == 0) return false;
+    int at = -1;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+        const uint64_t here = __ballot(key[i] == most);
+        if (at < 0 && here != 0) at = 64 * i + __builtin_ctzll(here);
+    }
+    *index = at;
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
+        if (at == 64 * i + lane_id()) key[i] = 0;
+    return true;
+}
+template <int NE>
+__device__ __forceinline__ bool take_largest(uint64_t (&key)[NE], int* index)
+{
+    uint32_t high = 0, low = 0;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) high = max(high, (uint32_t)(key[i] >> 32));
+    high = wave_max_u32(high);
+    if (high == 0) return false;         // open keys are finite sums above -2^1024: their upper halves are not 0
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
+        if ((uint32_t)(key[i] >> 32) == high) low = max(low, (uint32_t)key[i]);
+    low = wave_max_u32(low);
+    const uint64_t most = (uint64_t)high << 32 | low;
+    int at = -1;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+        const uint64_t here = __ballot(key[i] == most);
+        if (at < 0 && here != 0) at = 64 * i + __builtin_ctzll(here);
+    }
+    *index = at;
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
+        if (at == 64 * i + lane_id()) key[i] = 0;
+    return true;
+}
+
+// The choice of one token by one wave; the lanes j < k hold (id, weight) j afterwards.
+template <int NE, bool SIGMOID>
+__device__ __forceinline__ void choose(const RouteParams& p, int m, int* id, float* weight)
+{
+    const int lane = lane_id();
+    float v[NE];
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+        const int e = lane + 64 * i;
+        v[i] = -__builtin_inff();
+        if (e < p.E) {
+            const int64_t at = m * p.stride + e;
+            v[i] = p.fp32 ? static_cast<const float*>(p.logits)[at] : bf16_to_f32(static_cast<const uint16_t*>(p.logits)[at]);
+        }
+    }
+    using Key = typename std::conditional<SIGMOID, uint64_t, uint32_t>::type;
+    Key key[NE];
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+        const bool open = v[i] > -__builtin_inff();
+        if constexpr (SIGMOID) {
+            const double b = p.bias != nullptr && lane + 64 * i < p.E ? (double)p.bias[lane + 64 * i] : 0.0;
+            const bool both = open && b > -__builtin_inf();
+            key[i] = both ? sortable(1.0 / (1.0 + exp(-(double)v[i])) + b) : 0;
+        } else {
+            key[i] = open ? sortable(v[i]) : 0;
+        }
+    }
+    double all = 0.0;
+    float top = 0.0f;
+    bool first = true;
+    *id = -1;
+    float mine = 0.0f;                   // the logit of the lane's expert
+    for (int j = 0; j < p.k; ++j) {
+        int e;
+        if (!take_largest<NE>(key, &e)) break;
+        float logit = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NE; ++i)
+            if (e >> 6 == i) logit = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v[i]), e & 63));
+        if (first) top = logit, first = false;
+        if (lane == j) *id = e, mine = logit;
+    }
+    double w = 0.0;
+    if constexpr (SIGMOID) {
+        if (*id >= 0) w = 1.0 / (1.0 + exp(-(double)mine));
+        all = p.renormalize ? wave_add(w) : 1.0;
+    } else {
+        if (*id >= 0) w = exp((double)mine - (double)top);
+        if (p.renormalize) {
+            all = wave_add(w);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NE; ++i)
+                if (v[i] > -__builtin_inff()) all += exp((double)v[i] - (double)top);
+            all = wave_add(all);
+        }
+    }
+    *weight = (float)(all > 0.0 || all != all ? w / all * (double)p.scale : 0.0);
+}
+
+__device__ __forceinline__ int inclusive(int v)
+{
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+
+// Counts or places of a wave's pairs by expert, 64 at a time in their order. at[e]: the count so far, or the next place.
+struct SortSpace {
+    int32_t at[kRouteWaves][kRouteExperts + 1];
+    int32_t sums[kRouteWaves];
+};
+template <bool PLACE>
+__device__ __forceinline__ void walk(const RouteParams& p, int32_t* at, int first, int last)
+{
+    const int lane = lane_id();
+    for (int q0 = first; q0 < last; q0 += kWave) {
+        const int q = q0 + lane;
+        const bool in = q < last;
+        int id = in ? p.ids[q] : -1;
+        if ((uint32_t)id >= (uint32_t)p.E) id = p.E;
+        uint64_t same = __ballot(in);
+        for (int b = 0; b < p.id_bits; ++b) {
+            const uint64_t set = __ballot(id >> b & 1);
+            same &= id >> b & 1 ? set : ~set;
+        }
+        if (in) {
+            const int before = __popcll(same & ((1ull << lane) - 1)), base = at[id];
+            if (PLACE) p.order[base + before] = q;
+            wave_lds_order();
+            if (before == 0) at[id] = base + __popcll(same);
+        }
+        wave_lds_order();
+    }
+}
+
+// An exclusive scan over the block's threads; total in every thread.
+__device__ __forceinline__ int block_scan(int v, int32_t* sums, int* total)
+{
+    const int upto = inclusive(v);
+    if (lane_id() == 63) sums[wave_id()] = upto;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kRouteWaves; ++w) {
+        before += w < wave_id() ? sums[w] : 0;
+        all += sums[w];
+    }
+    *total = all;
+    return before + upto - v;
+}
+
+// A block's pairs [first, last) by wave: each wave takes a range of whole 64s.
+__device__ __forceinline__ void wave_range(int first, int last, int* from, int* to)
+{
+    const int steps = (last - first + kWave - 1) / kWave, wave = wave_id();
+    *from = first + steps * wave / kRouteWaves * kWave;
+    *to = min(last, first + steps * (wave + 1) / kRouteWaves * kWave);
+}
+
+// ONE: the only block, which does the order too. SELECT: choose the experts first (else ids are given).
+template <int NE, bool SIGMOID, bool SELECT, bool ONE>
+__global__ void __launch_bounds__(kRouteBlock) route_kernel(const RouteParams p)
+{
+    __shared__ SortSpace s;
+    const int wave = wave_id(), t = (int)threadIdx.x;
+    const int m0 = (int)blockIdx.x * p.tokens, m1 = min(p.M, m0 + p.tokens);
+    if constexpr (SELECT) {
+        for (int m = m0 + wave; m < m1; m += kRouteWaves) {
+            int id;
+            float weight;
+            choose<NE, SIGMOID>(p, m, &id, &weight);
+            if (lane_id() < p.k) {
+                p.ids[m * p.k + lane_id()] = id;
+                p.weights[m * p.k + lane_id()] = weight;
+            }
+        }
+    }
+    for (int e = t; e <= p.E; e += kRouteBlock)
+#pragma unroll
+        for (int w = 0; w < kRouteWaves; ++w) s.at[w][e] = 0;
+    __threadfence_block();
+    __syncthreads();
+    int from, to;
+    wave_range(m0 * p.k, m1 * p.k, &from, &to);
+    walk<false>(p, s.at[wave], from, to);
+    __syncthreads();
+    if constexpr (!ONE) {
+        for (int e = t; e <= p.E; e += kRouteBlock) {
+            int sum = 0;
+#pragma unroll
+            for (int w = 0; w < kRouteWaves; ++w) sum += s.at[w][e];
+            p.counts[(int64_t)blockIdx.x * (p.E + 1) + e] = sum;
+        }
+    } else {
+        int own = 0, total;
+        if (t < p.E)
+#pragma unroll
+            for (int w = 0; w < kRouteWaves; ++w) own += s.at[w][t];
+        int at = block_scan(own, s.sums, &total);
+        const auto places = [&](int e, int place) {
+#pragma unroll
+            for (int w = 0; w < kRouteWaves; ++w) {
+                const int n = s.at[w][e];
+                s.at[w][e] = place;
+                place += n;
+            }
+        };
+        if (t < p.E) p.offsets[t] = at, places(t, at);
+        if (t == 0) p.offsets[p.E] = total, places(p.E, total);
+        __syncthreads();
+        walk<true>(p, s.at[wave], from, to);
+    }
+}
+
+// The second launch: block b's places follow from all blocks' counts.
+__global__ void __launch_bounds__(kRouteBlock) route_order_kernel(const RouteParams p)
+{
+    __shared__ SortSpace s;
+    const int wave = wave_id(), t = (int)threadIdx.x, bins = p.E + 1;
+    const int m0 = (int)blockIdx.x * p.tokens, m1 = min(p.M, m0 + p.tokens);
+    for (int b = t; b < bins; b += kRouteBlock)
+#pragma unroll
+        for (int w = 0; w < kRouteWaves; ++w) s.at[w][b] = 0;
+    // counts of expert t before this block, and in all; with few experts several threads share one
+    int width = kWave;
+    while (width < bins) width *= 2;
+    const int groups = max(1, kRouteBlock / width), e = t % width, g = t / width;
+    int before = 0, all = 0, none_before = 0;
+    if (e < bins && g < groups) {
+        for (int b = g; b < (int)gridDim.x; b += groups) {
+            const int n = p.counts[(int64_t)b * bins + e];
+            all += n;
+            before += b < (int)blockIdx.x ? n : 0;
+        }
+    }
+    if (width > kRouteBlock) {           // 1024 experts: the last bin has no thread of its own
+        if (t == 0)
+            for (int b = 0; b < (int)blockIdx.x; ++b) none_before += p.counts[(int64_t)b * bins + p.E];
+    }
+    __shared__ int32_t sum[2][kRouteBlock];
+    sum[0][t] = before, sum[1][t] = all;
+    __syncthreads();
+    int from, to;
+    wave_range(m0 * p.k, m1 * p.k, &from, &to);
+    walk<false>(p, s.at[wave], from, to);
+    before = all = 0;
+    if (t < min(width, kRouteBlock))
+        for (int i = 0; i < groups; ++i) before += sum[0][i * width + t], all += sum[1][i * width + t];
+    if (width <= kRouteBlock && t == 0)
+        for (int i = 0; i < groups; ++i) none_before += sum[0][i * width + p.E];
+    int total;
+    const int at = block_scan(t < p.E ? all : 0, s.sums, &total);
+    __syncthreads();
+    const auto places = [&](int bin, int place) {
+#pragma unroll
+        for (int w = 0; w < kRouteWaves; ++w) {
+            const int n = s.at[w][bin];
+            s.at[w][bin] = place;
+            place += n;
+        }
+    };
+    if (t < p.E) {
+        if (blockIdx.x == 0) p.offsets[t] = at;
+        places(t, at + before);
+    }
+    if (t == 0) {
+        if (blockIdx.x == 0) p.offsets[p.E] = total;
+        places(p.E, total + none_before);
+    }
+    __syncthreads();
+    walk<true>(p, s.at[wave], from, to);
+}
+
+// Tokens that a block takes, and the blocks.
+static int route_blocks(int M, int* tokens)
+{
+    *tokens = M <= kRouteTokens ? M : (M + kRouteBlocks - 1) / kRouteBlocks;
+    if (M > kRouteTokens && *tokens < kRouteWaves) *tokens = kRouteWaves;
+    return (M + *tokens - 1) / *tokens;
+}
+static bool route_sizes(int M, int E, int k)
+{
+    return M >= 0 && E > 0 && E <= kRouteExperts && k > 0 && k <= kWave && (int64_t)M * k < 1 << 26;
+}
+static int64_t route_workspace(int M, int E)
+{
+    int tokens;
+    return M <= kRouteTokens ? 0 : (int64_t)route_blocks(M, &tokens) * (E + 1) * (int64_t)sizeof(int32_t);
+}
+
+template <bool SIGMOID, bool SELECT, bool ONE>
+static void launch_route(const RouteParams& p, int blocks, hipStream_t st)
+{
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(kRouteBlock), 0, st, p); };
+    if (!SELECT || p.E <= 64) go(route_kernel<1, SIGMOID, SELECT, ONE>);
+    else if (p.E <= 128) go(route_kernel<2, SIGMOID, SELECT, ONE>);
+    else if (p.E <= 256) go(route_kernel<4, SIGMOID, SELECT, ONE>);
+    else if (p.E <= 512) go(route_kernel<8, SIGMOID, SELECT, ONE>);
+    else go(route_kernel<16, SIGMOID, SELECT, ONE>);
+}
+
+static int run_route(RouteParams& p, bool select, bool sigmoid, void* workspace, long long bytes, hipStream_t st)
+{
+    const int64_t need = route_workspace(p.M, p.E);
+    if (need > 0 && (workspace == nullptr || !aligned(workspace, 16) || bytes < need)) return -2;
+    p.counts = static_cast<int32_t*>(workspace);
+    p.id_bits = 0;
+    while (p.E >> p.id_bits) ++p.id_bits;        // ids 0 .. E
+    const int blocks = route_blocks(p.M, &p.tokens);
+    const bool one = need == 0;
+    if (!select) one ? launch_route<false, false, true>(p, 1, st) : launch_route<false, false, false>(p, blocks, st);
+    else if (sigmoid) one ? launch_route<true, true, true>(p, 1, st) : launch_route<true, true, false>(p, blocks, st);
+    else one ? launch_route<false, true, true>(p, 1, st) : launch_route<false, true, false>(p, blocks, st);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess || one) return (int)e;
+    hipLaunchKernelGGL(route_order_kernel, dim3((uint32_t)blocks), dim3(kRouteBlock), 0, st, p);
+    return (int)hipGetLastError();
+}
+
+// No tokens: every expert has none.
+__global__ void __launch_bounds__(kRouteBlock) route_nothing_kernel(int32_t* offsets, int E)
+{
+    for (int e = (int)threadIdx.x; e <= E; e += kRouteBlock) offsets[e] = 0;
+}
+static int route_nothing(void* offsets, int E, hipStream_t st)
+{
+    hipLaunchKernelGGL(route_nothing_kernel, dim3(1), dim3(kRouteBlock), 0, st, static_cast<int32_t*>(offsets), E);
+    return (int)hipGetLastError();
+}
+
+}  // namespace paia
+
+extern "C" {
+
+long long paia_route_experts_workspace(int M, int experts, int k)
+{
+    return paia::route_sizes(M, experts, k) ? paia::route_workspace(M, experts) : -2;
+}
+
+int paia_route_experts(const void* logits, int logits_fp32, long long logits_stride, const void* bias, int sigmoid,
+                       int renormalize, float scale, void* ids, void* weights, void* order, void* offsets, int M, int experts,
+                       int k, void* workspace, long long workspace_bytes, void* stream)
+{
+    using namespace paia;
+    if (!route_sizes(M, experts, k) || k > experts || (logits_fp32 != 0 && logits_fp32 != 1) ||
+        (sigmoid != 0 && sigmoid != 1) || (renormalize != 0 && renormalize != 1) || (bias != nullptr && !sigmoid))
+        return -2;
+    if (offsets == nullptr || !aligned(offsets, 4)) return -2;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (M == 0) return route_nothing(offsets, experts, st);
+    if (logits == nullptr || ids == nullptr || weights == nullptr || order == nullptr ||
+        !aligned(logits, logits_fp32 ? 4 : 2) || !aligned(bias, 4) || !aligned(ids, 4) || !aligned(weights, 4) ||
+        !aligned(order, 4) || logits_stride < 0)
+        return -2;
+    RouteParams p{};
+    p.logits = logits;
+    p.bias = static_cast<const float*>(bias);
+    p.ids = static_cast<int32_t*>(ids);
+    p.weights = static_cast<float*>(weights);
+    p.order = static_cast<int32_t*>(order);
+    p.offsets = static_cast<int32_t*>(offsets);
+    p.stride = logits_stride;
+    p.M = M, p.E = experts, p.k = k;
+    p.fp32 = logits_fp32, p.renormalize = renormalize, p.scale = scale;
+    return run_route(p, true, sigmoid, workspace, workspace_bytes, st);
+}
+
+int paia_expert_order(const void* ids, void* order, void* offsets, int M, int experts, int k, void* workspace,
+                      long long workspace_bytes, void* stream)
+{
+    using namespace paia;
+    if (!route_sizes(M, experts, k) || offsets == nullptr || !aligned(offsets, 4)) return -2;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (M == 0) return route_nothing(offsets, experts, st);
+    if (ids == nullptr || order == nullptr || !aligned(ids, 4) || !aligned(order, 4)) return -2;
+    RouteParams p{};
+    p.ids = static_cast<int32_t*>(const_cast<void*>(ids));
+    p.order = static_cast<int32_t*>(order);
+    p.offsets = static_cast<int32_t*>(offsets);
+    p.M = M, p.E = experts, p.k = k;
+    return run_route(p, false, false, workspace, workspace_bytes, st);
+}
+
+}  // extern "C"

@@ -8,7 +8,8 @@ torch's current stream, so calls can be captured into a HIP graph (torch.cuda.CU
 Additions for the gfx950 build: `bf16_bias`, `fp8_bias`, `int4_zp` (asymmetric INT4 with optional bias),
 `dequant_fp8`, `dequant_int4`, `dequant_int4_zp`, `quantize_fp8_rowwise`, `quantize_int4_g128`,
 `quantize_int4_zp_g128`, `pick_variant`, `launch_kind`, `build_info`, and between the projections of a decode step
-`rope_append` and `paged_attention` (on a `KVCache` description of the paged cache), beside them `lora_add`.
+`rope_append` and `paged_attention` (on a `KVCache` description of the paged cache), beside them `lora_add`; for a layer's
+feed-forward half with experts `add_norm`, `route_experts`, `expert_order` and `experts_bf16/fp8/int4/int4_zp`.
 """
 from __future__ import annotations
 
@@ -95,6 +96,13 @@ class GemvLib:
             "paia_paged_attention": [_P, ctypes.POINTER(_L), ctypes.POINTER(KVCache), _P, _L, _I, _P, _F, _I, _P, _P, _I,
                                      _I, _I, _P, _L, _P],
             "paia_lora_add": [_P, _L, _P, _L, _P, _P, _P, _P, _P, _L, _I, _I, _I, ctypes.POINTER(_I), _I, _I, _P, _L, _P],
+            "paia_add_norm": [_P, _L, _P, _L, _I, _P, _L, _I, _P, _P, _L, _F, _P, _I, _F, _P, _L, _P, _L, _I, _I, _P],
+            "paia_route_experts": [_P, _I, _L, _P, _I, _I, _F, _P, _P, _P, _P, _I, _I, _I, _P, _L, _P],
+            "paia_expert_order": [_P, _P, _P, _I, _I, _I, _P, _L, _P],
+            "paia_experts_bf16": [_P, _P, _L, _I, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _P],
+            "paia_experts_fp8": [_P, _P, _P, _L, _I, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _P],
+            "paia_experts_int4": [_P, _P, _P, _L, _I, _P, _P, _P, _L, _I, _I, _I, _I, _I, _P],
+            "paia_experts_int4_zp": [_P, _P, _P, _P, _L, _I, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _P],
         }
         for name, argtypes in sig.items():
             fn = getattr(lib, name)
@@ -104,6 +112,8 @@ class GemvLib:
         lib.paia_paged_attention_workspace.argtypes = [ctypes.POINTER(KVCache), _I, _I, _I, _I]
         lib.paia_lora_add_workspace.restype = _L
         lib.paia_lora_add_workspace.argtypes = [_I, _I, _I, ctypes.POINTER(_I), _I]
+        lib.paia_route_experts_workspace.restype = _L
+        lib.paia_route_experts_workspace.argtypes = [_I, _I, _I]
         lib.paia_gemv_build_info.restype = ctypes.c_char_p
         lib.paia_gemv_build_info.argtypes = []
         self.variants_fp8 = self._qvariants(lib, "fp8")
@@ -305,6 +315,67 @@ class GemvLib:
                                             out_ptr, N if out_stride is None else out_stride, M, K, rank,
                                             (_I * len(splits))(*splits), len(splits), adapters, workspace_ptr,
                                             workspace_bytes, self._st(stream)), "paia_lora_add")
+
+    def add_norm(self, x_ptr, residual_ptr, norm_ptr, out_ptr, residual_out_ptr, M, D, weights_ptr=None, pairs=0,
+                 post_norm_ptr=None, gate_ptr=None, gate_stride=0, scale=1.0, eps=1e-6, plus_one=False, residual_fp32=False,
+                 x_stride=None, pair_stride=None, residual_stride=None, out_stride=None, residual_out_stride=None,
+                 stream=None):
+        """out, residual_out [M, D] of x [M, D] or [M, pairs, D]; see ops.add_norm. Strides in elements, all contiguous by
+        default; gate_stride 0: one row of gates for all."""
+        d = lambda stride, plain: plain if stride is None else stride  # noqa: E731
+        self._check(self._lib.paia_add_norm(x_ptr, d(x_stride, max(1, pairs) * D), weights_ptr, d(pair_stride, D), pairs,
+                                            residual_ptr, d(residual_stride, D), int(residual_fp32), post_norm_ptr, gate_ptr,
+                                            gate_stride, scale, norm_ptr, int(plus_one), eps, out_ptr, d(out_stride, D),
+                                            residual_out_ptr, d(residual_out_stride, D), M, D, self._st(stream)),
+                    "paia_add_norm")
+
+    def route_experts_workspace(self, M, experts, k):
+        """Bytes of device memory that route_experts and expert_order take as their workspace (0 for few tokens)."""
+        need = self._lib.paia_route_experts_workspace(M, experts, k)
+        self._check(min(need, 0), "paia_route_experts_workspace")
+        return need
+
+    def route_experts(self, logits_ptr, ids_ptr, weights_ptr, order_ptr, offsets_ptr, M, experts, k, workspace_ptr=None,
+                      workspace_bytes=0, bias_ptr=None, sigmoid=False, renormalize=True, scale=1.0, fp32=False,
+                      logits_stride=None, stream=None):
+        """Each token's experts and their order; see ops.route_experts."""
+        self._check(self._lib.paia_route_experts(logits_ptr, int(fp32), experts if logits_stride is None else logits_stride,
+                                                 bias_ptr, int(sigmoid), int(renormalize), scale, ids_ptr, weights_ptr,
+                                                 order_ptr, offsets_ptr, M, experts, k, workspace_ptr, workspace_bytes,
+                                                 self._st(stream)), "paia_route_experts")
+
+    def expert_order(self, ids_ptr, order_ptr, offsets_ptr, M, experts, k, workspace_ptr=None, workspace_bytes=0,
+                     stream=None):
+        self._check(self._lib.paia_expert_order(ids_ptr, order_ptr, offsets_ptr, M, experts, k, workspace_ptr,
+                                                workspace_bytes, self._st(stream)), "paia_expert_order")
+
+    def _experts(self, name, weights, x_ptr, x_rows, order_ptr, offsets_ptr, bias, out_ptr, experts, N, K, pairs, gated,
+                 x_stride, out_stride, stream):
+        cols = N // 2 if gated else N
+        self._check(getattr(self._lib, name)(*weights, x_ptr, K if x_stride is None else x_stride, x_rows, order_ptr,
+                                             offsets_ptr, *bias, out_ptr, cols if out_stride is None else out_stride, experts,
+                                             N, K, pairs, int(gated), self._st(stream)), name)
+
+    def experts_bf16(self, W_ptr, x_ptr, x_rows, order_ptr, offsets_ptr, out_ptr, experts, N, K, pairs, bias_ptr=None,
+                     gated=False, x_stride=None, out_stride=None, stream=None):
+        """out [pairs, N] (gated: N // 2) of the experts' matrices and the rows of x; see ops.experts_bf16."""
+        self._experts("paia_experts_bf16", (W_ptr,), x_ptr, x_rows, order_ptr, offsets_ptr, (bias_ptr,), out_ptr, experts, N,
+                      K, pairs, gated, x_stride, out_stride, stream)
+
+    def experts_fp8(self, Wq_ptr, scale_ptr, x_ptr, x_rows, order_ptr, offsets_ptr, out_ptr, experts, N, K, pairs,
+                    bias_ptr=None, gated=False, x_stride=None, out_stride=None, stream=None):
+        self._experts("paia_experts_fp8", (Wq_ptr, scale_ptr), x_ptr, x_rows, order_ptr, offsets_ptr, (bias_ptr,), out_ptr,
+                      experts, N, K, pairs, gated, x_stride, out_stride, stream)
+
+    def experts_int4(self, Wq_ptr, scales_ptr, x_ptr, x_rows, order_ptr, offsets_ptr, out_ptr, experts, N, K, pairs,
+                     gated=False, x_stride=None, out_stride=None, stream=None):
+        self._experts("paia_experts_int4", (Wq_ptr, scales_ptr), x_ptr, x_rows, order_ptr, offsets_ptr, (), out_ptr, experts,
+                      N, K, pairs, gated, x_stride, out_stride, stream)
+
+    def experts_int4_zp(self, Wq_ptr, scales_ptr, zeros_ptr, x_ptr, x_rows, order_ptr, offsets_ptr, out_ptr, experts, N, K,
+                        pairs, bias_ptr=None, gated=False, x_stride=None, out_stride=None, stream=None):
+        self._experts("paia_experts_int4_zp", (Wq_ptr, scales_ptr, zeros_ptr), x_ptr, x_rows, order_ptr, offsets_ptr,
+                      (bias_ptr,), out_ptr, experts, N, K, pairs, gated, x_stride, out_stride, stream)
 
     def build_info(self):
         return self._lib.paia_gemv_build_info().decode()

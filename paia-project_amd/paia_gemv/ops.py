@@ -181,3 +181,97 @@ def lora_add(y, x, A, B, ids, scaling=None, splits=None, out=None, workspace=Non
         return torch.ops.paia_gemv.lora_add(*args)
     torch.ops.paia_gemv.lora_add_out(*args, out)
     return out
+
+
+def add_norm(x, residual, norm, post_norm=None, gate=None, weights=None, scale=1.0, eps=1e-6, plus_one=False, out=None,
+             residual_out=None):
+    """What joins the halves of a layer, in one pass over its rows: (out, residual_out), both [M, D], with
+
+        y = x, or the sum of a token's experts, weights[m, j] x[m, j] over j (x [M, pairs, D], weights fp32 [M, pairs];
+            a pair of weight 0 adds nothing, whatever its row holds)
+        y = rms(y) * post_norm                      (a norm behind the block, where given)
+        residual_out = residual + scale * gate * y  (gate bf16 [D], or [M, D]; residual bf16 or fp32, or None: 0)
+        out = rms(residual_out) * norm              (of the sum as it is before its rounding)
+
+    rms(v) = v / sqrt(mean(v^2) + eps). x bf16, norm weights bf16 [D], with plus_one kept less 1. out is bf16, residual_out
+    of the residual's type and possibly the residual itself. Rows may be strided; D is a multiple of 8 up to 32768."""
+    load()
+    args = (x, residual, norm, post_norm, gate, weights, scale, eps, plus_one)
+    if out is None and residual_out is None:
+        return torch.ops.paia_gemv.add_norm(*args)
+    if out is None:
+        out = torch.empty(x.shape[0], x.shape[-1], dtype=torch.bfloat16, device=x.device)
+    if residual_out is None:
+        residual_out = torch.empty(x.shape[0], x.shape[-1], device=x.device,
+                                   dtype=torch.bfloat16 if residual is None else residual.dtype)
+    torch.ops.paia_gemv.add_norm_out(*args, out, residual_out)
+    return out, residual_out
+
+
+def route_experts(logits, k, bias=None, scoring="softmax", renormalize=True, scale=1.0, workspace=None):
+    """Each token's k experts and the order that the experts' products take them in: (ids int32 [M, k], weights fp32 [M, k],
+    order int32 [M * k], offsets int32 [experts + 1]).
+
+    logits bf16 or fp32 [M, experts] (rows may be strided). The experts of the largest logits, or with scoring "sigmoid" of
+    the largest sigmoid(logit) + bias (fp32 [experts]); equal ones by the lower index. weights are scale times the softmax
+    over the row, or the sigmoid (without the bias), with renormalize divided by their sum over the token's k. An expert whose
+    logit or bias is -inf or NaN is closed; where fewer than k are open the ids end with -1, of weight 0 (a row of -inf is a
+    token that is not there). order lists the pairs m * k + j by expert, offsets[e] is where expert e's begin, and what comes
+    from offsets[-1] on has no expert. experts up to 1024, k up to 64."""
+    load()
+    return torch.ops.paia_gemv.route_experts(logits, k, bias, scoring, renormalize, scale, workspace)
+
+
+def expert_order(ids, experts, workspace=None):
+    """route_experts' (order, offsets) for ids int32 [M, k] chosen otherwise (outside [0, experts): no expert)."""
+    load()
+    return torch.ops.paia_gemv.expert_order(ids, experts, workspace)
+
+
+def route_experts_workspace(M, experts, k):
+    """Bytes that the workspace of route_experts and expert_order takes for these sizes (0 for few tokens)."""
+    load()
+    return torch.ops.paia_gemv.route_experts_workspace(M, experts, k)
+
+
+def experts_bf16(W, x, order, offsets, bias=None, gated=False, out=None):
+    """Products with the experts' matrices, W bf16 [experts, N, K]: out[p] = W[e] x[p // (pairs // rows)] (+ bias[e]) for every
+    pair p of token and expert, bf16 [pairs, N].
+
+    order and offsets as route_experts makes them. x bf16 [rows, K] (rows may be strided) has a row for each token, whose
+    pairs share it, or for each pair (the down projection). gated: an expert's rows are N/2 gates and N/2 values,
+    out = silu(gate) * value, [pairs, N/2]. bias bf16 [experts, N]. Pairs without an expert give 0. Any number of tokens:
+    a few are bound by reading the chosen experts once, many run on the matrix cores."""
+    load()
+    if out is None:
+        return torch.ops.paia_gemv.experts_bf16(W, x, order, offsets, bias, gated)
+    torch.ops.paia_gemv.experts_bf16_out(W, x, order, offsets, bias, gated, out)
+    return out
+
+
+def experts_fp8(Wq, scale, x, order, offsets, bias=None, gated=False, out=None):
+    """experts_bf16 with e4m3 weights [experts, N, K] and fp32 scales [experts, N]."""
+    load()
+    if out is None:
+        return torch.ops.paia_gemv.experts_fp8(Wq, scale, x, order, offsets, bias, gated)
+    torch.ops.paia_gemv.experts_fp8_out(Wq, scale, x, order, offsets, bias, gated, out)
+    return out
+
+
+def experts_int4(Wq, scales, x, order, offsets, gated=False, out=None):
+    """experts_bf16 with the reference's INT4 format: Wq uint8 [experts, N, K/2] (or int32 [.., K/8]), fp16 scales
+    [experts, N, K/128], zero point 8."""
+    load()
+    if out is None:
+        return torch.ops.paia_gemv.experts_int4(Wq, scales, x, order, offsets, gated)
+    torch.ops.paia_gemv.experts_int4_out(Wq, scales, x, order, offsets, gated, out)
+    return out
+
+
+def experts_int4_zp(Wq, scales, zeros, x, order, offsets, bias=None, gated=False, out=None):
+    """experts_bf16 with asymmetric INT4: bf16 scales [experts, N, G], zeros uint8 [experts, N, ceil(G/2)]."""
+    load()
+    if out is None:
+        return torch.ops.paia_gemv.experts_int4_zp(Wq, scales, zeros, x, order, offsets, bias, gated)
+    torch.ops.paia_gemv.experts_int4_zp_out(Wq, scales, zeros, x, order, offsets, bias, gated, out)
+    return out

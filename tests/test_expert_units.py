@@ -1,0 +1,94 @@
+"""How blocks find their work among the experts (unit_of in csrc/experts_kernel.h), replayed on the CPU: for offsets in order every
+pair and tile is some block's exactly once and the launch has blocks enough; whatever the offsets hold, what a block takes lies
+within the pairs."""
+import random
+
+import pytest
+
+
+def blocks_of(R, E, BM, tiles):
+    most = (R + min(R, E + 1) * (BM - 1)) // BM
+    return most, most * tiles
+
+
+def units(offsets, R, E, BM, tiles):
+    """[(expert, first, held, tile)] of all blocks, None for one without work."""
+    per = -(-E // 64)
+    most, blocks = blocks_of(R, E, BM, tiles)
+    place = lambda e: min(max(offsets[min(e, E)], 0), R)  # noqa: E731
+    own = []
+    for lane in range(64):
+        n, at = 0, place(lane * per)
+        for i in range(1, per + 1):
+            to = place(lane * per + i)
+            n += (max(to - at, 0) + BM - 1) // BM
+            at = to
+        own.append(min(n, most))
+    upto = [sum(own[:i + 1]) for i in range(64)]
+    chunks = min(upto[63], most)
+    rest = place(E)
+    total = min(chunks + (R - rest + BM - 1) // BM, most) * tiles
+    out = []
+    for b in range(blocks):
+        if b >= total:
+            out.append(None)
+            continue
+        xcd = b % 8
+        u = xcd * (total // 8) + min(xcd, total % 8) + b // 8
+        c = u // tiles
+        if c >= chunks:
+            first = rest + (c - chunks) * BM
+            out.append((E, first, min(BM, R - first), u - c * tiles))
+            continue
+        lane = next(i for i in range(64) if upto[i] > c)
+        found, at, start = (0, 0, 0, 0, 1), upto[lane] - own[lane], place(lane * per)
+        for i in range(1, per + 1):
+            to = place(lane * per + i)
+            k = (max(to - start, 0) + BM - 1) // BM
+            if at <= c < at + k:
+                found = (lane * per + i - 1, at, start, to, k)
+            at, start = at + k, to
+        e, begin, lo, hi, n = found
+        local = u - begin * tiles
+        tile = local // n
+        first = lo + (local - tile * n) * BM
+        out.append((e, first, min(BM, hi - first), tile))
+    return out
+
+
+def counts_of(rng, E, R):
+    cuts = sorted(rng.randint(0, R) for _ in range(E))
+    if rng.random() < 0.5:
+        cuts = sorted(rng.choice(cuts) for _ in range(E))
+    return [0] + cuts
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_every_pair_and_tile_once(seed):
+    rng = random.Random(seed)
+    E, R = rng.choice([1, 2, 8, 63, 64, 65, 200]), rng.choice([1, 2, 7, 64, 300, 1000])
+    BM, tiles = rng.choice([4, 8, 16, 32, 256]), rng.choice([1, 3, 8, 20])
+    offsets = counts_of(rng, E, R)
+    seen = {}
+    for u in units(offsets, R, E, BM, tiles):
+        if u is None:
+            continue
+        e, first, held, tile = u
+        assert 0 < held <= BM and 0 <= tile < tiles
+        assert e == E and first >= offsets[E] or e < E and offsets[e] <= first and first + held <= offsets[e + 1]
+        for i in range(first, first + held):
+            seen[i, tile] = seen.get((i, tile), 0) + 1
+    assert len(seen) == R * tiles and set(seen.values()) == {1}
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_any_offsets_stay_within_the_pairs(seed):
+    rng = random.Random(seed)
+    E, R = rng.choice([1, 3, 64, 65, 130]), rng.choice([1, 5, 64, 333])
+    BM, tiles = rng.choice([4, 16, 64]), rng.choice([1, 5])
+    offsets = [rng.choice([rng.randint(-2 ** 31, 2 ** 31 - 1), rng.randint(-5, R + 5), 0, R]) for _ in range(E + 1)]
+    for u in units(offsets, R, E, BM, tiles):
+        if u is not None:
+            e, first, held, tile = u
+            assert 0 <= e <= E and 0 <= tile < tiles, (offsets, u)
+            assert 0 < held <= BM and 0 <= first and first + held <= R, (offsets, u)
