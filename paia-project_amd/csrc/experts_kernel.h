@@ -444,36 +444,35 @@ __global__ void __launch_bounds__(512) experts_tile_kernel(const ExpertsParams p
     const int64_t row0 = (int64_t)u.expert * p.N;
     const uint8_t* We = p.W + row0 * p.row_bytes;
 
+    // A load of weights lies within a 16-row tile: its base is the wave's, an offset the lane's. x has an address a row.
     const auto w_piece = [](int r) { return RB == 128 ? r & 7 : r >> 1 & 3; };
     const uint8_t* wp[WL];
-    uint32_t wpiece[WL];
+    uint32_t wo[WL];
+    const int wr = lane / WP, xr = lane / XP;
+    const uint32_t wpiece = (uint32_t)((lane % WP) ^ w_piece(wr)) * 16u;         // a load's first row is a multiple of 8
 #pragma unroll
     for (int i = 0; i < WL; ++i) {
-        const int r = (wave * WL + i) * WR + lane / WP, t = r / kTileRows;
+        const int r0 = (wave * WL + i) * WR, t = r0 / kTileRows;
         const int rows = max(1, tile_rows<GATED, T::kTiles>(p, u.tile, t));
-        const int row = min(tile_row<GATED, T::kTiles>(p, u.tile, t), p.N - 1) + min(r % kTileRows, rows - 1);
-        wp[i] = We + (int64_t)row * p.row_bytes;
-        wpiece[i] = (uint32_t)((lane % WP) ^ w_piece(r)) * 16u;
+        wp[i] = We + (int64_t)min(tile_row<GATED, T::kTiles>(p, u.tile, t), p.N - 1) * p.row_bytes;
+        wo[i] = (uint32_t)min(r0 % kTileRows + wr, rows - 1) * p.row_bytes;
     }
     const uint8_t* xp[XL];
-    uint32_t xpiece[XL];
 #pragma unroll
-    for (int i = 0; i < XL; ++i) {
-        const int r = (wave * XL + i) * XR + lane / XP;
-        xp[i] = x_row(p, pair_at(p, u, r));
-        xpiece[i] = (uint32_t)((lane % XP) ^ (r & 7)) * 16u;
-    }
+    for (int i = 0; i < XL; ++i) xp[i] = x_row(p, pair_at(p, u, (wave * XL + i) * XR + xr));
     const int stages = (p.K + C - 1) / C;
     const auto issue = [&](uint8_t* slot, int s) {
         if (s >= stages) return;
+        const uint32_t wc = min((uint32_t)s * RB + wpiece, p.row_bytes - 16u);
 #pragma unroll
-        for (int i = 0; i < WL; ++i)
-            lds_copy16(slot + (wave * WL + i) * 1024, wp[i] + min((uint32_t)s * RB + wpiece[i], p.row_bytes - 16u));
+        for (int i = 0; i < WL; ++i) lds_copy16(slot + (wave * WL + i) * 1024, wp[i] + (wo[i] + wc));
         if (XW == 8 || wave < XW) {
 #pragma unroll
-            for (int i = 0; i < XL; ++i)
-                lds_copy16(slot + T::kWBytes + (wave * XL + i) * 1024,
-                           xp[i] + min((uint32_t)s * XB + xpiece[i], (uint32_t)p.K * 2u - 16u));
+            for (int i = 0; i < XL; ++i) {
+                const int r = (wave * XL + i) * XR + xr;
+                const uint32_t c = (uint32_t)s * XB + (uint32_t)((lane % XP) ^ (r & 7)) * 16u;
+                lds_copy16(slot + T::kWBytes + (wave * XL + i) * 1024, xp[i] + min(c, (uint32_t)p.K * 2u - 16u));
+            }
         }
     };
     // INT4: the words of the stage's group for the wave's columns, a stage ahead
@@ -505,9 +504,7 @@ __global__ void __launch_bounds__(512) experts_tile_kernel(const ExpertsParams p
         const int r = (wn * TN + t) * 16 + ln;
         return *reinterpret_cast<const u32x4*>(slot + r * RB + (((4 * i + lh) ^ w_piece(r)) << 4));
     };
-    const auto use = [&](const uint8_t* slot, int s, auto tail) {
-        constexpr bool TAIL = decltype(tail)::value;
-        const int left = p.K - s * C;
+    const auto use = [&](const uint8_t* slot) {
         if constexpr (I4) {
             u32x4 a[TM][X], w[TN];
             f32x4 xs[TM];
@@ -547,10 +544,7 @@ __global__ void __launch_bounds__(512) experts_tile_kernel(const ExpertsParams p
             for (int j0 = 0; j0 < X; j0 += kWSteps) {
                 u32x4 w[TN];
 #pragma unroll
-                for (int t = 0; t < TN; ++t) {
-                    w[t] = get_w(slot, t, j0 / kWSteps);
-                    if (TAIL && step_col<F>(j0, lh) >= left) w[t] = u32x4{0, 0, 0, 0};
-                }
+                for (int t = 0; t < TN; ++t) w[t] = get_w(slot, t, j0 / kWSteps);
 #pragma unroll
                 for (int k = 0; k < kWSteps; ++k) {
                     u32x4 b[TN];
@@ -559,14 +553,27 @@ __global__ void __launch_bounds__(512) experts_tile_kernel(const ExpertsParams p
                         b[t] = F == kBF16 ? w[t] : (k ? fp8_frag(w[t].z, w[t].w) : fp8_frag(w[t].x, w[t].y));
 #pragma unroll
                     for (int i = 0; i < TM; ++i) {
-                        u32x4 a = get_x(slot, i, j0 + k);
-                        if (TAIL && step_col<F>(j0 + k, lh) >= left) a = u32x4{0, 0, 0, 0};
+                        const u32x4 a = get_x(slot, i, j0 + k);
 #pragma unroll
                         for (int t = 0; t < TN; ++t) acc[i][t] = mfma_16x16x32(a, b[t], acc[i][t]);
                     }
                 }
             }
         }
+    };
+    // The last stage of a K that is no multiple of its columns: what lies past the rows' ends is 0 in both operands.
+    const auto clear_past = [&](uint8_t* slot, int left) {
+        constexpr int kWCols = F == kFP8 ? 16 : 8;
+        const u32x4 none = {0, 0, 0, 0};
+        for (int e = (int)threadIdx.x; e < T::kTiles * kTileRows * WP; e += 512) {
+            const int r = e / WP, at = e % WP;
+            if ((at ^ w_piece(r)) * kWCols >= left) *reinterpret_cast<u32x4*>(slot + r * RB + at * 16) = none;
+        }
+        for (int e = (int)threadIdx.x; e < BM * XP; e += 512) {
+            const int r = e / XP, at = e % XP;
+            if ((at ^ (r & 7)) * 8 >= left) *reinterpret_cast<u32x4*>(slot + T::kWBytes + r * XB + at * 16) = none;
+        }
+        __syncthreads();
     };
     const auto stage = [&](uint8_t* mine, uint8_t* next, int s) {
         wait_loads<0>();
@@ -577,10 +584,8 @@ __global__ void __launch_bounds__(512) experts_tile_kernel(const ExpertsParams p
 #pragma unroll
             for (int t = 0; t < TN; ++t) ahead[t] = i4_meta<F>(p, mrow[t], min(s + 1, p.G - 1));
         }
-        if (busy) {
-            if (I4 || p.K - s * C >= C) use(mine, s, std::false_type{});
-            else use(mine, s, std::true_type{});
-        }
+        if (!I4 && p.K - s * C < C) clear_past(mine, p.K - s * C);
+        if (busy) use(mine);
         if constexpr (I4) {
 #pragma unroll
             for (int t = 0; t < TN; ++t) word[t] = ahead[t];
@@ -593,29 +598,32 @@ __global__ void __launch_bounds__(512) experts_tile_kernel(const ExpertsParams p
     }
     if (!busy) return;
 
+    float scale[TN], bias[TN];
 #pragma unroll
-    for (int t = 0; t < TN; t += GATED ? 2 : 1) {
-        const int i0 = wn * TN + t;
-        const int col = c0 + (GATED ? i0 / 2 : i0) * kTileRows + ln;
-        if (col >= p.cols) continue;
-        float scale[2] = {1.0f, 1.0f}, bias[2] = {0.0f, 0.0f};
+    for (int t = 0; t < TN; ++t) {
+        const int i = wn * TN + t, rows = max(1, tile_rows<GATED, T::kTiles>(p, u.tile, i));
+        const int64_t row = row0 + min(tile_row<GATED, T::kTiles>(p, u.tile, i), p.N - 1) + min(ln, rows - 1);
+        scale[t] = F == kFP8 ? reinterpret_cast<const float*>(p.meta)[row] : 1.0f;
+        bias[t] = p.bias != nullptr ? bf16_to_f32(p.bias[row]) : 0.0f;
+    }
 #pragma unroll
-        for (int h = 0; h < (GATED ? 2 : 1); ++h) {
-            const int64_t row = row0 + (GATED ? h * p.cols : 0) + col;
-            if constexpr (F == kFP8) scale[h] = reinterpret_cast<const float*>(p.meta)[row];
-            if (p.bias != nullptr) bias[h] = bf16_to_f32(p.bias[row]);
-        }
+    for (int i = 0; i < TM; ++i) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+        for (int c = 0; c < 4; ++c) {
+            const int m = (wm * TM + i) * 16 + 4 * lh + c;
+            const int pair = m < u.held ? p.order[u.first + m] : -1;
+            if ((uint32_t)pair >= (uint32_t)p.R) continue;
+            uint16_t* out = p.out + (int64_t)pair * p.out_stride;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int m = (wm * TM + i) * 16 + 4 * lh + c;
-                const int pair = m < u.held ? p.order[u.first + m] : -1;
-                if ((uint32_t)pair >= (uint32_t)p.R) continue;
-                float o = finish<F>(acc[i][t][c], scale[0], bias[0]);
-                if constexpr (GATED) o = silu(o) * finish<F>(acc[i][t + (GATED ? 1 : 0)][c], scale[1], bias[1]);
-                p.out[(int64_t)pair * p.out_stride + col] = (uint16_t)f32_to_bf16_out(o);
+            for (int t = 0; t < TN; t += GATED ? 2 : 1) {
+                const int i0 = wn * TN + t, col = c0 + (GATED ? i0 / 2 : i0) * kTileRows + ln;
+                float o = finish<F>(acc[i][t][c], scale[t], bias[t]);
+                if constexpr (GATED) o = silu(o) * finish<F>(acc[i][t + (GATED ? 1 : 0)][c], scale[t + (GATED ? 1 : 0)],
+                                                             bias[t + (GATED ? 1 : 0)]);
+                if (col < p.cols) out[col] = (uint16_t)f32_to_bf16_out(o);
             }
+        }
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
