@@ -4,7 +4,7 @@
 
 namespace paia {
 
-constexpr int kMostExperts = 1024, kMostPairs = 1 << 26, kMostColumns = 1 << 26;     // K; N too
+constexpr int kMostExperts = 1024, kMostPairs = 1 << 26, kMostColumns = 1 << 25;     // K; N too
 
 struct ExpertOperands {
     const void *W, *meta, *zeros, *x, *order, *offsets, *bias;
@@ -32,7 +32,7 @@ static int run_experts(int fmt, const ExpertOperands& o, hipStream_t st, Launch 
         (o.x_rows > 1 && o.x_stride < o.K) || o.out_stride < 0 || (o.pairs > 1 && o.out_stride < cols))
         return -2;
     ExpertsParams p;
-    p.tiles = p.most = 0;
+    p.tiles = p.most = p.span = 0;
     p.W = static_cast<const uint8_t*>(o.W);
     p.meta = static_cast<const uint8_t*>(o.meta);
     p.zeros = static_cast<const uint8_t*>(o.zeros);
@@ -47,6 +47,8 @@ static int run_experts(int fmt, const ExpertOperands& o, hipStream_t st, Launch 
     p.row_bytes = (uint32_t)(fmt == kBF16 ? 2 * o.K : (fmt == kFP8 ? o.K : o.K / 2));
     p.G = i4 ? o.K / kBlockCols : 0;
     p.zbytes = (uint32_t)(p.G + 1) / 2;
+    const int64_t x_bytes = ((int64_t)(o.x_rows - 1) * o.x_stride + o.K) * 2;
+    p.x_bytes = x_bytes < (1ll << 31) ? (uint32_t)x_bytes : 0;
     p.by_pairs = Divisor((uint32_t)(o.pairs / o.x_rows));
     return launch(p, o.gated != 0, st);
 }

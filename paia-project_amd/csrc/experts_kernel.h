@@ -28,6 +28,8 @@ struct ExpertsParams {
     int E, N, K, R;          // R: pairs
     int cols;                // outputs of a pair: N, or N / 2 where gated
     int tiles;               // units of columns
+    int span;                // groups of columns that a streaming unit takes one after the other
+    uint32_t x_bytes;        // of x, first row's start to last row's end (streaming: below 2^31)
     int lane_experts;        // experts a lane counts: ceil(E / 64)
     int most;                // chunks that the launch has blocks for
     uint32_t row_bytes, zbytes;
@@ -127,14 +129,12 @@ __device__ __forceinline__ void wait_loads()
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
-// Until the wave's reads of LDS are done: what they read can be overwritten.
-__device__ __forceinline__ void wait_reads()
+// A barrier for the block's LDS alone: loads from memory stay on their way.
+__device__ __forceinline__ void block_lds_order()
 {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(0xC07F);
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 // Rows of outputs without an expert are 0.
@@ -172,13 +172,6 @@ __device__ __forceinline__ uint32_t i4_word_of(uint32_t scale, uint32_t zero)
     if constexpr (F == kI4) return __float_as_uint(up);
     return fabsf(up) > kF32Max ? i4zp_word_big(s, zero) : i4zp_word(up, zero);
 }
-template <int F>
-__device__ __forceinline__ uint32_t i4_meta(const ExpertsParams& p, int64_t row, int g)
-{
-    const uint32_t s = reinterpret_cast<const uint16_t*>(p.meta)[row * p.G + g];
-    const uint32_t z = F == kI4ZP ? (uint32_t)p.zeros[row * p.zbytes + (g >> 1)] >> (4 * (g & 1)) & 15u : 8u;
-    return i4_word_of<F>(s, z);
-}
 template <int F> __device__ __forceinline__ float i4_factor(uint32_t m) { return __uint_as_float(F == kI4 ? kI4Exp << 23 : (m & 0xFF00u) << 15); }
 template <int F> __device__ __forceinline__ float i4_scale(uint32_t m) { return __uint_as_float(F == kI4 ? m : m & 0xFFFF0000u); }
 template <int F> __device__ __forceinline__ float i4_zero(uint32_t m) { return F == kI4 ? 8.0f : (float)(m & 0xFFu); }
@@ -206,6 +199,12 @@ __device__ __forceinline__ int tile_rows(const ExpertsParams& p, int unit_tile, 
     return min(kTileRows, p.cols - (unit_tile * (GATED ? TILES / 2 : TILES) + (GATED ? i / 2 : i)) * kTileRows);
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// Few rows an expert: bound by reading the weights. A unit is up to MT pairs and `span` groups of P tiles of 16 weight rows; the
+// WAVES waves of its block share K, a range each, and add their partial sums in LDS, in order, at the end of a group. A wave's
+// stages of all its groups are one stream with D stages of loads in flight in registers (they hold several times what LDS
+// could), which pass through wave-private LDS into the matrix layout: every load is row-contiguous, no barrier within a group.
+// ---------------------------------------------------------------------------------------------------------------
 template <int F>
 struct StreamFmt {
     static constexpr bool kI4F = F == kI4 || F == kI4ZP;
@@ -215,129 +214,127 @@ struct StreamFmt {
     static constexpr int kXRowBytes = 2 * kCols;
 };
 
-// ---------------------------------------------------------------------------------------------------------------
-// Few rows an expert: bound by reading the weights. A unit is up to MT pairs and P tiles of 16 weight rows; the WAVES waves of
-// its block take the stages of K in turn, each through two wave-private places in LDS that are filled straight from memory
-// (no registers, no block barrier), and add their partial sums in LDS at the end, in order.
-// ---------------------------------------------------------------------------------------------------------------
-constexpr int kStreamGroups = 160;       // INT4: groups of a row whose metadata the block keeps (K <= 20480)
-template <int F, int P, int WAVES, int MT, bool GATED>
-struct StreamShape {
-    using T = StreamFmt<F>;
-    static constexpr int kXRows = MT > kChunkBytes / T::kXRowBytes ? MT : kChunkBytes / T::kXRowBytes;
-    static constexpr int kWBytes = P * kTileRows * T::kRowBytes, kXBytes = kXRows * T::kXRowBytes;
-    static constexpr int kSlot = kWBytes + kXBytes > P * 1024 ? kWBytes + kXBytes : P * 1024;
-};
-
-template <int F, int P, int WAVES, int MT, bool GATED>
-__global__ void __launch_bounds__(WAVES * kWave) experts_stream_kernel(const ExpertsParams p)
+template <int F, int P, int WAVES, int MT, int D, bool GATED>
+__global__ void __launch_bounds__(WAVES * kWave, 4) experts_stream_kernel(const ExpertsParams p)
 {
     using T = StreamFmt<F>;
-    using S = StreamShape<F, P, WAVES, MT, GATED>;
     constexpr bool I4 = T::kI4F;
     constexpr int C = T::kCols, RB = T::kRowBytes, X = T::kSteps, L = RB * kTileRows / kChunkBytes;
-    constexpr int WP = RB / 16, WR = kWave / WP, XP = T::kXRowBytes / 16, XR = kWave / XP, XL = S::kXRows / XR;
-    __shared__ __attribute__((aligned(16))) uint8_t slot0[WAVES][S::kSlot];
-    __shared__ __attribute__((aligned(16))) uint8_t slot1[WAVES][S::kSlot];
-    constexpr int kMdStride = P * kTileRows + 1;
-    __shared__ uint32_t md[I4 ? kStreamGroups * kMdStride : 1];      // INT4: metadata words [group][row]
+    constexpr int WP = RB / 16, WR = kWave / WP, XP = T::kXRowBytes / 16, XR = kWave / XP;
+    constexpr int kXRows = MT > XR ? MT : XR, XL = kXRows / XR;
+    constexpr int kWBytes = P * kTileRows * RB, kWaveBytes = kWBytes + kXRows * T::kXRowBytes;
+    constexpr int kOuts = GATED ? P / 2 : P, kOutCols = kOuts * kTileRows;
+    __shared__ __attribute__((aligned(16))) uint8_t place[WAVES][kWaveBytes];
+    __shared__ f32x4 part[WAVES][P][kWave];
 
     const ExpertUnit u = unit_of<MT>(p);
     if (u.expert < 0) return;
     const int lane = lane_id(), wave = wave_id(), ln = lane & 15, lh = lane >> 4;
-    constexpr int kOutCols = (GATED ? P / 2 : P) * kTileRows;
-    const int c0 = u.tile * kOutCols;
+    const int all_groups = (p.cols + kOutCols - 1) / kOutCols;
+    const int group0 = u.tile * p.span, groups = min(p.span, all_groups - group0);
     if (u.expert == p.E) {
-        zero_rows(p, u, c0, min(c0 + kOutCols, p.cols));
+        zero_rows(p, u, group0 * kOutCols, min((group0 + groups) * kOutCols, p.cols));
         return;
     }
     const int64_t row0 = (int64_t)u.expert * p.N;
+    const int stages = (p.K + C - 1) / C;
+    const int k0 = stages * wave / WAVES, n = stages * (wave + 1) / WAVES - k0;      // this wave's stages
 
-    // addresses: one base a tile and load for the weights, one a load for x
-    const uint8_t* wt[P];
-    uint32_t wo[P][L], wpiece;
-    const uint8_t* xp[XL];
-    uint32_t xpiece[XL];
-    {
-        const int r = lane / WP, at = lane % WP;
-        wpiece = (uint32_t)(RB == 128 ? at ^ (r & 7) : at ^ (r >> 1 & 3)) * 16u;
+    // the stream's next stage: stage `it` of group `ig`, the descriptors of whose tiles end with their rows
+    int ig = 0, it = 0;
+    __amdgpu_buffer_rsrc_t rw[P];
+    const auto aim = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < P; ++t) {
-            const int n0 = tile_row<GATED, P>(p, u.tile, t), rows = max(1, tile_rows<GATED, P>(p, u.tile, t));
-            wt[t] = p.W + (row0 + min(n0, p.N - 1)) * p.row_bytes;
-#pragma unroll
-            for (int i = 0; i < L; ++i) wo[t][i] = (uint32_t)min(i * WR + r, rows - 1) * p.row_bytes;
+            const int rows = ig < groups ? max(0, tile_rows<GATED, P>(p, group0 + ig, t)) : 0;
+            const int64_t row = row0 + (rows ? tile_row<GATED, P>(p, group0 + ig, t) : 0);
+            rw[t] = make_rsrc(p.W + row * p.row_bytes, (uint32_t)__builtin_amdgcn_readfirstlane(rows) * p.row_bytes);
         }
+    };
+    const uint32_t lw = (uint32_t)(lane / WP) * p.row_bytes + (uint32_t)(lane % WP) * 16u, wstep = (uint32_t)WR * p.row_bytes;
+    const int cw = (lane % WP) * (C / WP), cx = (lane % XP) * 8;     // first column of the lane's 16 bytes
+    struct Stage {
+        u32x4 w[P][L], x[XL];
+        uint32_t m[I4 ? P : 1], z[F == kI4ZP ? P : 1];
+    };
+    // Unconditional loads (under a branch the compiler would wait for all that are on their way), out of range past the end.
+    const auto issue_w = [&](Stage& B) __attribute__((always_inline)) {
+        const int kb = k0 + it, left = ig < groups ? p.K - kb * C : 0;
+        const uint32_t wo = cw < left ? lw + (uint32_t)kb * (uint32_t)RB : kOOB;
+#pragma unroll
+        for (int t = 0; t < P; ++t)
+#pragma unroll
+            for (int i = 0; i < L; ++i) B.w[t][i] = ld16<2>(rw[t], wo + wstep * (uint32_t)i, 0u);
+        if constexpr (I4) {
+            const int last = p.N - 1;
+#pragma unroll
+            for (int t = 0; t < P; ++t) {
+                const int64_t row = row0 + min(tile_row<GATED, P>(p, group0 + min(ig, groups - 1), t) + ln, last);
+                B.m[t] = reinterpret_cast<const uint16_t*>(p.meta)[row * p.G + min(kb, p.G - 1)];
+                if constexpr (F == kI4ZP) B.z[t] = p.zeros[row * p.zbytes + (min(kb, p.G - 1) >> 1)];
+            }
+        }
+    };
+    uint32_t xo[XL];
+    const __amdgpu_buffer_rsrc_t xrs = make_rsrc(p.x, p.x_bytes);
+    const auto issue_x = [&](Stage& B, int g, int t) __attribute__((always_inline)) {
+        const int kb = k0 + t, left = g < groups ? p.K - kb * C : 0;
+#pragma unroll
+        for (int i = 0; i < XL; ++i) B.x[i] = ld16<0>(xrs, cx < left ? xo[i] + (uint32_t)kb * (2u * C) : kOOB, 0u);
+    };
+    const auto next = [&]() __attribute__((always_inline)) {
+        if (++it == n) it = 0, ++ig, aim();
+    };
+
+    // the weights' first loads go ahead of the chain order -> rows of x
+    Stage buf[D];
+    int pg[D], pt[D];
+    aim();
+    if (n == 0) ig = groups;
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+        pg[d] = ig, pt[d] = it;
+        issue_w(buf[d]);
+        if (n > 0) next();
     }
 #pragma unroll
     for (int i = 0; i < XL; ++i) {
-        const int r = i * XR + lane / XP;
-        xp[i] = x_row(p, pair_at(p, u, r));
-        xpiece[i] = (uint32_t)((lane % XP) ^ (r & 7)) * 16u;
+        const int r = i * XR + lane / XP, pair = pair_at(p, u, r);
+        const bool held = r < u.held && (uint32_t)pair < (uint32_t)p.R;
+        xo[i] = held ? p.by_pairs.of((uint32_t)pair) * (uint32_t)(p.x_stride * 2) + (uint32_t)(lane % XP) * 16u : kOOB;
     }
-    const int stages = (p.K + C - 1) / C, n = (stages - wave + WAVES - 1) / WAVES;
-    const auto issue = [&](uint8_t* slot, int t) {
-        if (t >= n) return;
-        const uint32_t s = (uint32_t)(wave + t * WAVES);
-        // bytes past the row's end are read from its last piece, and dropped in the last stage
-        const uint32_t wc = min(s * RB + wpiece, p.row_bytes - 16u);
+    int pairs[4];
 #pragma unroll
-        for (int t2 = 0; t2 < P; ++t2)
+    for (int c = 0; c < 4; ++c) pairs[c] = 4 * lh + c < u.held ? p.order[u.first + 4 * lh + c] : -1;
 #pragma unroll
-            for (int i = 0; i < L; ++i) lds_copy16(slot + (t2 * L + i) * 1024, wt[t2] + (wo[t2][i] + wc));
-#pragma unroll
-        for (int i = 0; i < XL; ++i)
-            lds_copy16(slot + S::kWBytes + i * 1024, xp[i] + min(s * (2 * C) + xpiece[i], (uint32_t)p.K * 2u - 16u));
-    };
-    issue(slot0[wave], 0);
-    issue(slot1[wave], 1);
+    for (int d = 0; d < D; ++d) issue_x(buf[d], pg[d], pt[d]);
 
-    if constexpr (I4) {
-        for (int i = (int)threadIdx.x; i < P * kTileRows * p.G; i += WAVES * kWave) {
-            const int r = i / p.G, g = i - r * p.G, t = r / kTileRows;
-            const int rows = max(1, tile_rows<GATED, P>(p, u.tile, t));
-            const int row = min(tile_row<GATED, P>(p, u.tile, t), p.N - 1) + min(r % kTileRows, rows - 1);
-            md[g * kMdStride + r] = i4_meta<F>(p, row0 + row, g);
-        }
-        __syncthreads();
-    }
+    uint8_t* mine = place[wave];
+    const auto w_at = [](int row, int piece) {
+        return RB == 128 ? row * 128 + ((piece ^ (row & 7)) << 4) : row * 64 + ((piece ^ (row >> 1 & 3)) << 4);
+    };
+    const auto x_at = [](int row, int piece) { return kWBytes + row * T::kXRowBytes + ((piece ^ (row & 7)) << 4); };
     const uint32_t one2 = (uint32_t)__builtin_amdgcn_readfirstlane((int)kI4Ones);
     const u32x4 ones = {one2, one2, one2, one2};
     f32x4 acc[P];
 #pragma unroll
     for (int t = 0; t < P; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    const auto use = [&](uint8_t* slot, int t) {
-        const int s = wave + t * WAVES, left = p.K - s * C;
-        if (t + 1 < n) wait_loads<P * L + XL>();     // the next stage's may be on their way
-        else wait_loads<0>();
-        u32x4 a[X], w[P][L];
+    const auto consume = [&](const Stage& B, int kb) __attribute__((always_inline)) {
+        wave_lds_order();
+#pragma unroll
+        for (int i = 0; i < XL; ++i) *reinterpret_cast<u32x4*>(mine + x_at(i * XR + lane / XP, lane % XP)) = B.x[i];
+#pragma unroll
+        for (int t = 0; t < P; ++t)
+#pragma unroll
+            for (int i = 0; i < L; ++i)
+                *reinterpret_cast<u32x4*>(mine + t * kTileRows * RB + w_at(i * WR + lane / WP, lane % WP)) = B.w[t][i];
+        wave_lds_order();
+        u32x4 a[X];
 #pragma unroll
         for (int j = 0; j < X; ++j) {
             const int piece = F == kBF16 ? 4 * j + lh : (F == kFP8 ? 8 * (j >> 1) + 2 * lh + (j & 1) : 4 * lh + j);
-            const int r = ln & (S::kXRows - 1);
-            a[j] = *reinterpret_cast<const u32x4*>(slot + S::kWBytes + r * T::kXRowBytes + ((piece ^ (r & 7)) << 4));
-        }
-#pragma unroll
-        for (int t2 = 0; t2 < P; ++t2)
-#pragma unroll
-            for (int i = 0; i < L; ++i) {
-                const int piece = 4 * i + lh;
-                const int at = RB == 128 ? ln * 128 + ((piece ^ (ln & 7)) << 4) : ln * 64 + ((piece ^ (ln >> 1 & 3)) << 4);
-                w[t2][i] = *reinterpret_cast<const u32x4*>(slot + t2 * kTileRows * RB + at);
-            }
-        wait_reads();
-        issue(slot, t + 2);
-        __builtin_amdgcn_sched_barrier(0);
-        if (!I4 && left < C) {                       // the row's end: both operands are 0 past it
-#pragma unroll
-            for (int j = 0; j < X; ++j)
-                if (step_col<F>(j, lh) >= left) a[j] = u32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int t2 = 0; t2 < P; ++t2)
-#pragma unroll
-                for (int i = 0; i < L; ++i)
-                    if (step_col<F>(F == kFP8 ? 2 * i : i, lh) >= left) w[t2][i] = u32x4{0, 0, 0, 0};
+            a[j] = *reinterpret_cast<const u32x4*>(mine + x_at(ln & (kXRows - 1), piece));
         }
         f32x4 xs = {0.0f, 0.0f, 0.0f, 0.0f};
         if constexpr (I4) {
@@ -345,68 +342,114 @@ __global__ void __launch_bounds__(WAVES * kWave) experts_stream_kernel(const Exp
             for (int j = 0; j < X; ++j) xs = mfma_16x16x32(a[j], ones, xs);
         }
 #pragma unroll
-        for (int t2 = 0; t2 < P; ++t2) {
+        for (int t = 0; t < P; ++t) {
+            u32x4 w[L];
+#pragma unroll
+            for (int i = 0; i < L; ++i) w[i] = *reinterpret_cast<const u32x4*>(mine + t * kTileRows * RB + w_at(ln, 4 * i + lh));
             if constexpr (F == kBF16) {
 #pragma unroll
-                for (int j = 0; j < X; ++j) acc[t2] = mfma_16x16x32(a[j], w[t2][j], acc[t2]);
+                for (int j = 0; j < X; ++j) acc[t] = mfma_16x16x32(a[j], w[j], acc[t]);
             } else if constexpr (F == kFP8) {
 #pragma unroll
                 for (int j = 0; j < X; ++j) {
-                    const u32x4 v = w[t2][j >> 1];
-                    acc[t2] = mfma_16x16x32(a[j], j & 1 ? fp8_frag(v.z, v.w) : fp8_frag(v.x, v.y), acc[t2]);
+                    const u32x4 v = w[j >> 1];
+                    acc[t] = mfma_16x16x32(a[j], j & 1 ? fp8_frag(v.z, v.w) : fp8_frag(v.x, v.y), acc[t]);
                 }
             } else {
-                const uint32_t m = md[s * kMdStride + t2 * kTileRows + ln];
+                const uint32_t m = i4_word_of<F>(B.m[t], F == kI4ZP ? B.z[F == kI4ZP ? t : 0] >> (4 * (kb & 1)) & 15u : 8u);
                 const float f = i4_factor<F>(m), sc = i4_scale<F>(m), z = i4_zero<F>(m);
                 f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int j = 0; j < X; ++j) g = mfma_16x16x32(a[j], i4_frag(w[t2][0][j], f), g);
+                for (int j = 0; j < X; ++j) g = mfma_16x16x32(a[j], i4_frag(w[0][j], f), g);
 #pragma unroll
-                for (int v = 0; v < 4; ++v) acc[t2][v] = __builtin_fmaf(sc, __builtin_fmaf(-z, xs[v], g[v]), acc[t2][v]);
+                for (int v = 0; v < 4; ++v) acc[t][v] = __builtin_fmaf(sc, __builtin_fmaf(-z, xs[v], g[v]), acc[t][v]);
             }
         }
-        __builtin_amdgcn_sched_barrier(0);
     };
-    for (int t = 0; t < n; t += 2) {
-        use(slot0[wave], t);
-        if (t + 1 < n) use(slot1[wave], t + 1);
-    }
 
-    // partial tiles to the wave's own place, then the first waves add them in order and finish
+    // A group's end: partial tiles to LDS, then some of the waves add them and finish. Its operands are loaded a group ahead.
+    uint32_t scale[P], bias[P];
+    const __amdgpu_buffer_rsrc_t scales = make_rsrc(reinterpret_cast<const float*>(p.meta) + (F == kFP8 ? row0 : 0),
+                                                    F == kFP8 ? (uint32_t)p.N * 4u : 0u);
+    const __amdgpu_buffer_rsrc_t biases = make_rsrc(p.bias != nullptr ? p.bias + row0 : p.x, p.bias != nullptr ? (uint32_t)p.N * 2u : 0u);
+    const auto operands = [&](int g) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < P; ++t) *reinterpret_cast<f32x4*>(slot0[wave] + t * 1024 + lane * 16) = acc[t];
-    __syncthreads();
-    constexpr int kOuts = GATED ? P / 2 : P;
-    for (int q = wave; q < kOuts; q += WAVES) {
-        f32x4 v[GATED ? 2 : 1];
-        const int col = c0 + q * kTileRows + ln;
-        if (col >= p.cols) continue;
-#pragma unroll
-        for (int h = 0; h < (GATED ? 2 : 1); ++h) {
-            const int t = GATED ? 2 * q + h : q;
-            const int64_t row = row0 + (GATED ? h * p.cols : 0) + col;
-            f32x4 sum = *reinterpret_cast<const f32x4*>(slot0[0] + t * 1024 + lane * 16);
-#pragma unroll
-            for (int w = 1; w < WAVES; ++w) sum += *reinterpret_cast<const f32x4*>(slot0[w] + t * 1024 + lane * 16);
-            const float scale = F == kFP8 ? reinterpret_cast<const float*>(p.meta)[row] : 1.0f;
-            const float bias = p.bias != nullptr ? bf16_to_f32(p.bias[row]) : 0.0f;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) v[h][c] = finish<F>(sum[c], scale, bias);
+        for (int t = 0; t < P; ++t) {
+            const uint32_t row = (uint32_t)(tile_row<GATED, P>(p, group0 + g, t) + ln);
+            if constexpr (F == kFP8) scale[t] = __builtin_amdgcn_raw_buffer_load_b32(scales, row * 4u, 0u, 0);
+            bias[t] = ld_u16(biases, row * 2u, 0u);
         }
+    };
+    operands(0);
+    const auto finish_group = [&](int g) __attribute__((always_inline)) {
+        __syncthreads();                             // the last group's sums have been read
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const int m = 4 * lh + c;
-            const int pair = m < u.held ? p.order[u.first + m] : -1;
-            if ((uint32_t)pair >= (uint32_t)p.R) continue;
-            const float o = GATED ? silu(v[0][c]) * v[GATED ? 1 : 0][c] : v[0][c];
-            p.out[(int64_t)pair * p.out_stride + col] = (uint16_t)f32_to_bf16_out(o);
+        for (int t = 0; t < P; ++t) {
+            part[wave][t][lane] = acc[t];
+            acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        __syncthreads();
+        const int first = g * kOuts % WAVES;         // the groups' finishes go round the waves
+#pragma unroll
+        for (int q = 0; q < kOuts; ++q) {
+            if (wave != (first + q) % WAVES) continue;
+            const int col = (group0 + g) * kOutCols + q * kTileRows + ln;
+            f32x4 v[GATED ? 2 : 1];
+#pragma unroll
+            for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+                const int t = GATED ? 2 * q + h : q;
+                f32x4 sum = part[0][t][lane];
+#pragma unroll
+                for (int w = 1; w < WAVES; ++w) sum += part[w][t][lane];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) v[h][c] = finish<F>(sum[c], F == kFP8 ? __uint_as_float(scale[t]) : 1.0f, bf16_to_f32(bias[t]));
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if ((uint32_t)pairs[c] >= (uint32_t)p.R || col >= p.cols) continue;
+                const float o = GATED ? silu(v[0][c]) * v[GATED ? 1 : 0][c] : v[0][c];
+                p.out[(int64_t)pairs[c] * p.out_stride + col] = (uint16_t)f32_to_bf16_out(o);
+            }
+        }
+        operands(g + 1);
+    };
+
+    if (n == 0) {
+        for (int g = 0; g < groups; ++g) finish_group(g);
+        return;
+    }
+    int g = 0, t = 0;                                // of the stage that is consumed next
+    const auto step = [&]() __attribute__((always_inline)) {
+        if (++t == n) finish_group(g), t = 0, ++g;
+    };
+    const int all = groups * n;
+    int f = 0;
+    wait_loads<0>();                                 // the loop's waits then count its own order of loads alone
+    for (; f + D < all; f += D) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            consume(buf[d], k0 + t);
+            const int ng = ig, nt = it;
+            issue_w(buf[d]);
+            issue_x(buf[d], ng, nt);
+            next();
+            __builtin_amdgcn_sched_barrier(0);
+            step();
         }
     }
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+        if (f + d < all) {
+            consume(buf[d], k0 + t);
+            step();
+        }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
 // More rows an expert: a block is BM pairs by 16 tiles of weight rows, its 8 waves 2 x 4 (or 1 x 8) parts of that. Two places
-// in LDS are filled straight from memory in turn: while one stage is multiplied the next is on its way, one barrier a stage.
+// in LDS are filled in turn, one barrier a stage. Up to 128 pairs, where reading the weights still counts, the stages come by
+// way of registers with D of them in flight; blocks of 256, whose sums take the registers, are filled straight from memory
+// while the stage before is multiplied.
 // ---------------------------------------------------------------------------------------------------------------
 template <int F, int BM>
 struct TileShape {
@@ -418,10 +461,13 @@ struct TileShape {
     static constexpr int kM = BM >= 128 ? 2 : 1, kN = 8 / kM;    // the waves' parts
     static constexpr int kTM = BM / 16 / kM, kTN = kTiles / kN;
     static constexpr int kWBytes = kTiles * kTileRows * kRowBytes, kXBytes = BM * kXRowBytes;
+    static constexpr bool kDirect = BM == 256 || (kI4F && BM == 128);
+    static constexpr int kAhead = 2;                             // stages in flight in registers
+    static constexpr int kWaves = kWBytes + kXBytes <= 40960 && !kDirect && !(kI4F && BM > 32) ? 4 : 2;    // a SIMD's: two blocks a CU, or one
 };
 
 template <int F, int BM, bool GATED>
-__global__ void __launch_bounds__(512) experts_tile_kernel(const ExpertsParams p)
+__global__ void __launch_bounds__(512, (TileShape<F, BM>::kWaves)) experts_tile_kernel(const ExpertsParams p)
 {
     using T = TileShape<F, BM>;
     constexpr bool I4 = T::kI4F;
@@ -461,31 +507,59 @@ __global__ void __launch_bounds__(512) experts_tile_kernel(const ExpertsParams p
 #pragma unroll
     for (int i = 0; i < XL; ++i) xp[i] = x_row(p, pair_at(p, u, (wave * XL + i) * XR + xr));
     const int stages = (p.K + C - 1) / C;
-    const auto issue = [&](uint8_t* slot, int s) {
+    // A stage's addresses; bytes past a row's end come from its last piece instead, and are cleared in the last stage.
+    const auto w_from = [&](int s, int i) { return wp[i] + (wo[i] + min((uint32_t)s * RB + wpiece, p.row_bytes - 16u)); };
+    const auto x_from = [&](int s, int i) {
+        const int r = (wave * XL + i) * XR + xr;
+        return xp[i] + min((uint32_t)s * XB + (uint32_t)((lane % XP) ^ (r & 7)) * 16u, (uint32_t)p.K * 2u - 16u);
+    };
+    const auto issue = [&](uint8_t* slot, int s) __attribute__((always_inline)) {
         if (s >= stages) return;
-        const uint32_t wc = min((uint32_t)s * RB + wpiece, p.row_bytes - 16u);
 #pragma unroll
-        for (int i = 0; i < WL; ++i) lds_copy16(slot + (wave * WL + i) * 1024, wp[i] + (wo[i] + wc));
+        for (int i = 0; i < WL; ++i) lds_copy16(slot + (wave * WL + i) * 1024, w_from(s, i));
         if (XW == 8 || wave < XW) {
 #pragma unroll
-            for (int i = 0; i < XL; ++i) {
-                const int r = (wave * XL + i) * XR + xr;
-                const uint32_t c = (uint32_t)s * XB + (uint32_t)((lane % XP) ^ (r & 7)) * 16u;
-                lds_copy16(slot + T::kWBytes + (wave * XL + i) * 1024, xp[i] + min(c, (uint32_t)p.K * 2u - 16u));
+            for (int i = 0; i < XL; ++i) lds_copy16(slot + T::kWBytes + (wave * XL + i) * 1024, x_from(s, i));
+        }
+    };
+    struct Stage {
+        u32x4 w[WL], x[XL];
+    };
+    // Unconditional: past the last stage it reads that one again, waves without a part of x their neighbours' rows.
+    const auto load = [&](Stage& B, int s) __attribute__((always_inline)) {
+        s = min(s, stages - 1);
+#pragma unroll
+        for (int i = 0; i < WL; ++i) B.w[i] = *reinterpret_cast<const u32x4*>(w_from(s, i));
+#pragma unroll
+        for (int i = 0; i < XL; ++i) B.x[i] = *reinterpret_cast<const u32x4*>(x_from(s, i));
+    };
+    const auto store = [&](uint8_t* slot, const Stage& B) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < WL; ++i) *reinterpret_cast<u32x4*>(slot + (wave * WL + i) * 1024 + lane * 16) = B.w[i];
+        if (XW == 8 || wave < XW) {
+#pragma unroll
+            for (int i = 0; i < XL; ++i)
+                *reinterpret_cast<u32x4*>(slot + T::kWBytes + (wave * XL + i) * 1024 + lane * 16) = B.x[i];
+        }
+    };
+    // INT4: scale and zero point of the stage's group for the wave's columns, as they are stored, a stage ahead
+    struct Meta {
+        uint32_t s[I4 ? TN : 1], z[F == kI4ZP ? TN : 1];
+    };
+    Meta meta, ahead;
+    const auto meta_load = [&](Meta& m, int g) __attribute__((always_inline)) {
+        if constexpr (I4) {
+            g = min(g, p.G - 1);
+#pragma unroll
+            for (int t = 0; t < TN; ++t) {
+                const int i = wn * TN + t, rows = max(1, tile_rows<GATED, T::kTiles>(p, u.tile, i));
+                const int64_t first = row0 + min(tile_row<GATED, T::kTiles>(p, u.tile, i), p.N - 1);
+                const uint32_t r = (uint32_t)min(ln, rows - 1);
+                m.s[t] = *reinterpret_cast<const uint16_t*>(p.meta + first * p.G * 2 + (r * (uint32_t)p.G + (uint32_t)g) * 2u);
+                if constexpr (F == kI4ZP) m.z[t] = p.zeros[first * p.zbytes + (r * p.zbytes + (uint32_t)(g >> 1))];
             }
         }
     };
-    // INT4: the words of the stage's group for the wave's columns, a stage ahead
-    int64_t mrow[I4 ? TN : 1];
-    uint32_t word[I4 ? TN : 1];
-    if constexpr (I4) {
-#pragma unroll
-        for (int t = 0; t < TN; ++t) {
-            const int i = wn * TN + t, rows = max(1, tile_rows<GATED, T::kTiles>(p, u.tile, i));
-            mrow[t] = row0 + min(tile_row<GATED, T::kTiles>(p, u.tile, i), p.N - 1) + min(ln, rows - 1);
-            word[t] = i4_meta<F>(p, mrow[t], 0);
-        }
-    }
     const uint32_t one2 = (uint32_t)__builtin_amdgcn_readfirstlane((int)kI4Ones);
     const u32x4 ones = {one2, one2, one2, one2};
     f32x4 acc[TM][TN];
@@ -504,7 +578,7 @@ __global__ void __launch_bounds__(512) experts_tile_kernel(const ExpertsParams p
         const int r = (wn * TN + t) * 16 + ln;
         return *reinterpret_cast<const u32x4*>(slot + r * RB + (((4 * i + lh) ^ w_piece(r)) << 4));
     };
-    const auto use = [&](const uint8_t* slot) {
+    const auto use = [&](const uint8_t* slot, int group) __attribute__((always_inline)) {
         if constexpr (I4) {
             u32x4 a[TM][X], w[TN];
             f32x4 xs[TM];
@@ -522,7 +596,8 @@ __global__ void __launch_bounds__(512) experts_tile_kernel(const ExpertsParams p
             }
 #pragma unroll
             for (int t = 0; t < TN; ++t) {
-                const float f = i4_factor<F>(word[t]), sc = i4_scale<F>(word[t]), z = i4_zero<F>(word[t]);
+                const uint32_t m = i4_word_of<F>(meta.s[t], F == kI4ZP ? meta.z[F == kI4ZP ? t : 0] >> (4 * (group & 1)) & 15u : 8u);
+                const float f = i4_factor<F>(m), sc = i4_scale<F>(m), z = i4_zero<F>(m);
                 f32x4 g[TM];
 #pragma unroll
                 for (int i = 0; i < TM; ++i) g[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -562,7 +637,7 @@ __global__ void __launch_bounds__(512) experts_tile_kernel(const ExpertsParams p
         }
     };
     // The last stage of a K that is no multiple of its columns: what lies past the rows' ends is 0 in both operands.
-    const auto clear_past = [&](uint8_t* slot, int left) {
+    const auto clear_past = [&](uint8_t* slot, int left) __attribute__((always_inline)) {
         constexpr int kWCols = F == kFP8 ? 16 : 8;
         const u32x4 none = {0, 0, 0, 0};
         for (int e = (int)threadIdx.x; e < T::kTiles * kTileRows * WP; e += 512) {
@@ -575,26 +650,52 @@ __global__ void __launch_bounds__(512) experts_tile_kernel(const ExpertsParams p
         }
         __syncthreads();
     };
-    const auto stage = [&](uint8_t* mine, uint8_t* next, int s) {
-        wait_loads<0>();
-        __syncthreads();                             // this stage has arrived, the other place is read
-        issue(next, s + 1);
-        uint32_t ahead[I4 ? TN : 1];
-        if constexpr (I4) {
-#pragma unroll
-            for (int t = 0; t < TN; ++t) ahead[t] = i4_meta<F>(p, mrow[t], min(s + 1, p.G - 1));
-        }
-        if (!I4 && p.K - s * C < C) clear_past(mine, p.K - s * C);
-        if (busy) use(mine);
-        if constexpr (I4) {
-#pragma unroll
-            for (int t = 0; t < TN; ++t) word[t] = ahead[t];
-        }
+    const auto multiply = [&](uint8_t* slot, int s, bool last) __attribute__((always_inline)) {
+        if (!I4 && last && p.K - s * C < C) clear_past(slot, p.K - s * C);
+        if (busy) use(slot, s);
+        if constexpr (I4) meta = ahead;
     };
-    issue(slot0, 0);
-    for (int s = 0; s < stages; s += 2) {
-        stage(slot0, slot1, s);
-        if (s + 1 < stages) stage(slot1, slot0, s + 1);
+    meta_load(meta, 0);
+    if constexpr (T::kDirect) {
+        const auto stage = [&](uint8_t* mine, uint8_t* next, int s) __attribute__((always_inline)) {
+            wait_loads<0>();
+            __syncthreads();                         // this stage has arrived, the other place is read
+            issue(next, s + 1);
+            meta_load(ahead, s + 1);
+            multiply(mine, s, true);
+        };
+        issue(slot0, 0);
+        for (int s = 0; s < stages; s += 2) {
+            stage(slot0, slot1, s);
+            if (s + 1 < stages) stage(slot1, slot0, s + 1);
+        }
+    } else {
+        constexpr int D = T::kAhead;
+        static_assert(D % 2 == 0, "a buffer goes to the same place each time");
+        Stage buf[D];
+#pragma unroll
+        for (int d = 0; d < D; ++d) load(buf[d], d);
+        int s = 0;
+        for (; s + D < stages; s += D) {
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                uint8_t* slot = d & 1 ? slot1 : slot0;
+                store(slot, buf[d]);                 // what was there is read: two stages ago, before the last barrier
+                meta_load(ahead, s + d + 1);         // ahead of the loads that stay on their way
+                load(buf[d], s + d + D);
+                block_lds_order();
+                multiply(slot, s + d, false);
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+            if (s + d < stages) {
+                uint8_t* slot = d & 1 ? slot1 : slot0;
+                store(slot, buf[d]);
+                meta_load(ahead, s + d + 1);
+                block_lds_order();
+                multiply(slot, s + d, true);
+            }
     }
     if (!busy) return;
 
@@ -637,7 +738,7 @@ constexpr int kMostBlocks = 1 << 22;
 template <typename K>
 int launch_experts(K kernel, ExpertsParams p, int BM, int tiles_cols, int threads, hipStream_t st)
 {
-    p.tiles = (p.cols + tiles_cols - 1) / tiles_cols;
+    p.tiles = (int)(((int64_t)p.cols + tiles_cols - 1) / tiles_cols);
     p.by_tiles = Divisor((uint32_t)p.tiles);
     const int64_t bins = p.R < p.E + 1 ? p.R : p.E + 1;
     const int64_t most = ((int64_t)p.R + bins * (BM - 1)) / BM;
@@ -647,11 +748,13 @@ int launch_experts(K kernel, ExpertsParams p, int BM, int tiles_cols, int thread
     return (int)hipGetLastError();
 }
 template <int F, int MT, bool GATED>
-int launch_stream(const ExpertsParams& p, hipStream_t st)
+int launch_stream(ExpertsParams p, hipStream_t st)
 {
-    constexpr int P = 2, WAVES = 8;
-    return launch_experts(experts_stream_kernel<F, P, WAVES, MT, GATED>, p, MT, (GATED ? P / 2 : P) * kTileRows,
-                          WAVES * kWave, st);
+    constexpr int P = 2, WAVES = 8, D = 2, kCols = (GATED ? P / 2 : P) * kTileRows;
+    const int64_t groups = (p.cols + kCols - 1) / kCols, bins = p.R < p.E + 1 ? p.R : p.E + 1;
+    const int64_t most = ((int64_t)p.R + bins * (MT - 1)) / MT, aim = 2 * device_facts().cus;
+    p.span = (int)(groups * most > aim ? (groups * most + aim - 1) / aim : 1);
+    return launch_experts(experts_stream_kernel<F, P, WAVES, MT, D, GATED>, p, MT, kCols * p.span, WAVES * kWave, st);
 }
 template <int F, int BM, bool GATED>
 int launch_tiles(const ExpertsParams& p, hipStream_t st)
@@ -664,7 +767,7 @@ int launch_format(const ExpertsParams& p, hipStream_t st)
 {
     constexpr bool kI4F = F == kI4 || F == kI4ZP;
     const int64_t R = p.R, E = p.E;
-    if (R <= 12 * E && (!kI4F || p.G <= kStreamGroups)) {
+    if (R <= 12 * E && p.x_bytes != 0) {
         if (3 * R <= 4 * E) return launch_stream<F, 4, GATED>(p, st);
         if (3 * R <= 8 * E) return launch_stream<F, 8, GATED>(p, st);
         return launch_stream<F, 16, GATED>(p, st);
