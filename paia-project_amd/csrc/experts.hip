@@ -32,7 +32,7 @@ static int run_experts(int fmt, const ExpertOperands& o, hipStream_t st, Launch 
         (o.x_rows > 1 && o.x_stride < o.K) || o.out_stride < 0 || (o.pairs > 1 && o.out_stride < cols))
         return -2;
     ExpertsParams p;
-    p.tiles = p.most = p.span = 0;
+    p.tiles = p.most = 0;
     p.W = static_cast<const uint8_t*>(o.W);
     p.meta = static_cast<const uint8_t*>(o.meta);
     p.zeros = static_cast<const uint8_t*>(o.zeros);

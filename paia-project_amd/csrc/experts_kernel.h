@@ -28,7 +28,6 @@ struct ExpertsParams {
     int E, N, K, R;          // R: pairs
     int cols;                // outputs of a pair: N, or N / 2 where gated
     int tiles;               // units of columns
-    int span;                // groups of columns that a streaming unit takes one after the other
     uint32_t x_bytes;        // of x, first row's start to last row's end (streaming: below 2^31)
     int lane_experts;        // experts a lane counts: ceil(E / 64)
     int most;                // chunks that the launch has blocks for
@@ -54,50 +53,68 @@ __device__ __forceinline__ int wave_inclusive(int v)
     return v;
 }
 
-// The unit of this block, the same in every lane. Offsets are taken as they are but for their range: whatever they hold, first
-// and held stay within the pairs.
+// How many chunks of BM pairs the experts have, and which one is which; the same in every lane but `upto`. Offsets are taken as
+// they are but for their range: whatever they hold, the pairs of a chunk lie within the call's.
+template <int BM>
+struct Chunks {
+    int count, rest_at, rest;            // rest: chunks of the pairs without an expert, order[rest_at ..]
+    int upto, own;                       // chunks of the experts up to the lane's last, and of the lane's
+
+    __device__ __forceinline__ int place(const ExpertsParams& p, int e) const { return min(max(p.offsets[min(e, p.E)], 0), p.R); }
+    __device__ __forceinline__ explicit Chunks(const ExpertsParams& p)
+    {
+        const int e0 = lane_id() * p.lane_experts;
+        rest_at = place(p, p.E);
+        int from = place(p, e0);
+        own = 0;
+        for (int i = 1; i <= p.lane_experts; ++i) {
+            const int to = place(p, e0 + i);
+            own += (max(to - from, 0) + BM - 1) / BM;
+            from = to;
+        }
+        own = min(own, p.most);                  // no more than that in all, unless the offsets are not in order
+        upto = wave_inclusive(own);
+        count = min(__builtin_amdgcn_readlane(upto, 63), p.most);
+        rest = min((p.R - rest_at + BM - 1) / BM, p.most - count);
+    }
+    // The expert of chunk c < count, its pairs order[lo .. hi), and its chunks begin .. begin + n - 1.
+    struct Expert {
+        int expert, lo, hi, begin, n;
+    };
+    __device__ __forceinline__ Expert of(const ExpertsParams& p, int c) const
+    {
+        const int owner = __builtin_ctzll(__ballot(upto > c)), e0 = lane_id() * p.lane_experts;
+        int e = 0, begin = 0, lo = 0, hi = 0, n = 1, at = upto - own, from = place(p, e0);
+        for (int i = 1; i <= p.lane_experts; ++i) {
+            const int to = place(p, e0 + i), k = (max(to - from, 0) + BM - 1) / BM;
+            if (c >= at && c < at + k) e = e0 + i - 1, begin = at, lo = from, hi = to, n = k;
+            at += k;
+            from = to;
+        }
+        return {__builtin_amdgcn_readlane(e, owner), __builtin_amdgcn_readlane(lo, owner), __builtin_amdgcn_readlane(hi, owner),
+                __builtin_amdgcn_readlane(begin, owner), __builtin_amdgcn_readlane(n, owner)};
+    }
+};
+
+// Block b's place when each of the 8 XCDs, to which blocks are dealt in turn, takes a contiguous range of n.
+__device__ __forceinline__ int xcd_contiguous(int b, int n) { return b % 8 * (n / 8) + min(b % 8, n % 8) + b / 8; }
+
+// The unit of this block: units of one expert and tile follow each other.
 template <int BM>
 __device__ __forceinline__ ExpertUnit unit_of(const ExpertsParams& p)
 {
-    const int lane = lane_id(), e0 = lane * p.lane_experts;
-    const auto place = [&](int e) { return min(max(p.offsets[min(e, p.E)], 0), p.R); };
-    const int rest_at = place(p.E);
-    int from = place(e0), own = 0;
-    const int from0 = from;
-    for (int i = 1; i <= p.lane_experts; ++i) {
-        const int to = place(e0 + i);
-        own += (max(to - from, 0) + BM - 1) / BM;
-        from = to;
-    }
-    own = min(own, p.most);                  // no more than that in all, unless the offsets are not in order
-    const int upto = wave_inclusive(own);
-    const int chunks = min(__builtin_amdgcn_readlane(upto, 63), p.most);
-    const int units = min(chunks + (p.R - rest_at + BM - 1) / BM, p.most) * p.tiles;
-    int u = (int)blockIdx.x;
-    if (u >= units) return {-1, 0, 0, 0};
-    {
-        const int xcd = u % 8, per = units / 8, rem = units % 8;
-        u = xcd * per + min(xcd, rem) + u / 8;
-    }
+    const Chunks<BM> chunks(p);
+    const int units = (chunks.count + chunks.rest) * p.tiles;
+    if ((int)blockIdx.x >= units) return {-1, 0, 0, 0};
+    const int u = xcd_contiguous((int)blockIdx.x, units);
     const int c = (int)p.by_tiles.of((uint32_t)u);
-    if (c >= chunks) {
-        const int first = rest_at + (c - chunks) * BM;
+    if (c >= chunks.count) {
+        const int first = chunks.rest_at + (c - chunks.count) * BM;
         return {p.E, first, min(BM, p.R - first), u - c * p.tiles};
     }
-    const int owner = __builtin_ctzll(__ballot(upto > c));
-    int e = 0, begin = 0, lo = 0, hi = 0, n = 1, at = upto - own;
-    from = from0;
-    for (int i = 1; i <= p.lane_experts; ++i) {
-        const int to = place(e0 + i), k = (max(to - from, 0) + BM - 1) / BM;
-        if (c >= at && c < at + k) e = e0 + i - 1, begin = at, lo = from, hi = to, n = k;
-        at += k;
-        from = to;
-    }
-    e = __builtin_amdgcn_readlane(e, owner), begin = __builtin_amdgcn_readlane(begin, owner);
-    lo = __builtin_amdgcn_readlane(lo, owner), hi = __builtin_amdgcn_readlane(hi, owner);
-    n = __builtin_amdgcn_readlane(n, owner);
-    const int local = u - begin * p.tiles, tile = local / n, first = lo + (local - tile * n) * BM;
-    return {e, first, min(BM, hi - first), tile};
+    const auto x = chunks.of(p, c);
+    const int local = u - x.begin * p.tiles, tile = local / x.n, first = x.lo + (local - tile * x.n) * BM;
+    return {x.expert, first, min(BM, x.hi - first), tile};
 }
 
 __device__ __forceinline__ int pair_at(const ExpertsParams& p, const ExpertUnit& u, int i)
@@ -157,6 +174,13 @@ __device__ __forceinline__ u32x4 i4_frag(uint32_t v, float f)
     return u32x4{i4x2_to_bf16x2<false>(a, f), i4x2_to_bf16x2<true>(a, f), i4x2_to_bf16x2<false>(b, f),
                  i4x2_to_bf16x2<true>(b, f)};
 }
+// The same in the order of i4_pair_x's values: (k, k + 2), (k + 4, k + 6), (k + 1, k + 3), (k + 5, k + 7).
+__device__ __forceinline__ u32x4 i4_frag_paired(uint32_t v, float f)
+{
+    const uint32_t lo = v & 0x0F0F0F0Fu, hi = (v >> 4) & 0x0F0F0F0Fu;
+    return u32x4{i4x2_to_bf16x2<false>(lo, f), i4x2_to_bf16x2<true>(lo, f), i4x2_to_bf16x2<false>(hi, f),
+                 i4x2_to_bf16x2<true>(hi, f)};
+}
 __device__ __forceinline__ u32x4 fp8_frag(uint32_t d0, uint32_t d1)
 {
     return u32x4{fp8x2_to_bf16x2<false>(d0), fp8x2_to_bf16x2<true>(d0), fp8x2_to_bf16x2<false>(d1),
@@ -200,85 +224,91 @@ __device__ __forceinline__ int tile_rows(const ExpertsParams& p, int unit_tile, 
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Few rows an expert: bound by reading the weights. A unit is up to MT pairs and `span` groups of P tiles of 16 weight rows; the
-// WAVES waves of its block share K, a range each, and add their partial sums in LDS, in order, at the end of a group. A wave's
-// stages of all its groups are one stream with D stages of loads in flight in registers (they hold several times what LDS
-// could), which pass through wave-private LDS into the matrix layout: every load is row-contiguous, no barrier within a group.
+// Few rows an expert: bound by reading the weights. An item is up to MT pairs and P tiles of 16 weight rows; the items, chunk by
+// chunk, are shared out evenly among as many blocks as are resident, so that none waits for another's second round. The WAVES
+// waves of a block share K, a range each, and add their partial sums in LDS, in order, at an item's end. A wave's stages of all
+// items of a chunk are one stream with D stages of loads in flight in registers (they hold several times what LDS
+// could), which pass through wave-private LDS into the matrix layout: every load is row-contiguous, no barrier within an item.
 // ---------------------------------------------------------------------------------------------------------------
+constexpr int kStreamTiles = 2, kStreamWaves = 4, kStreamBlocks = 3;     // tiles of an item, waves of a block, blocks of a CU
 template <int F>
+constexpr int kStreamAhead = 2;
+
+template <int F, int MT>
 struct StreamFmt {
     static constexpr bool kI4F = F == kI4 || F == kI4ZP;
-    static constexpr int kCols = F == kBF16 ? 64 : 128;          // columns of a stage
-    static constexpr int kRowBytes = kI4F ? 64 : 128;            // weight bytes of a row and stage
-    static constexpr int kSteps = kCols / 32;
-    static constexpr int kXRowBytes = 2 * kCols;
+    static constexpr int kCols = F == kBF16 ? 64 : (kI4F && MT == 4 ? 256 : 128);          // columns of a stage
+    static constexpr int kRowBytes = F == kBF16 ? 2 * kCols : (F == kFP8 ? kCols : kCols / 2);      // its bytes of a weight row
+    static constexpr int kSteps = kCols / 32, kXRowBytes = 2 * kCols;
+    static constexpr int kXLoadRows = kWave * 16 / kXRowBytes, kXRows = MT > kXLoadRows ? MT : kXLoadRows;
+    static constexpr int kWBytes = kStreamTiles * kTileRows * kRowBytes, kWaveBytes = kWBytes + kXRows * kXRowBytes;
+};
+template <int F, int MT>
+struct StreamSpace {
+    __attribute__((aligned(16))) uint8_t place[kStreamWaves][StreamFmt<F, MT>::kWaveBytes];
+    f32x4 part[kStreamWaves][kStreamTiles][kWave];
 };
 
-template <int F, int P, int WAVES, int MT, int D, bool GATED>
-__global__ void __launch_bounds__(WAVES * kWave, 4) experts_stream_kernel(const ExpertsParams p)
+// `groups` items from column group `group0` on, of the pairs order[first .. first + held) of one expert.
+template <int F, int MT, bool GATED>
+__device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace<F, MT>& space, int expert, int first, int held,
+                                             int group0, int groups)
 {
-    using T = StreamFmt<F>;
+    using T = StreamFmt<F, MT>;
     constexpr bool I4 = T::kI4F;
+    constexpr int P = kStreamTiles, WAVES = kStreamWaves, D = kStreamAhead<F>;
     constexpr int C = T::kCols, RB = T::kRowBytes, X = T::kSteps, L = RB * kTileRows / kChunkBytes;
-    constexpr int WP = RB / 16, WR = kWave / WP, XP = T::kXRowBytes / 16, XR = kWave / XP;
-    constexpr int kXRows = MT > XR ? MT : XR, XL = kXRows / XR;
-    constexpr int kWBytes = P * kTileRows * RB, kWaveBytes = kWBytes + kXRows * T::kXRowBytes;
+    constexpr int H = I4 ? C / 128 : 1;               // INT4: groups of a stage
+    constexpr int WP = RB / 16, WR = kWave / WP, XP = T::kXRowBytes / 16, XR = T::kXLoadRows, XL = T::kXRows / XR;
     constexpr int kOuts = GATED ? P / 2 : P, kOutCols = kOuts * kTileRows;
-    __shared__ __attribute__((aligned(16))) uint8_t place[WAVES][kWaveBytes];
-    __shared__ f32x4 part[WAVES][P][kWave];
 
-    const ExpertUnit u = unit_of<MT>(p);
-    if (u.expert < 0) return;
     const int lane = lane_id(), wave = wave_id(), ln = lane & 15, lh = lane >> 4;
-    const int all_groups = (p.cols + kOutCols - 1) / kOutCols;
-    const int group0 = u.tile * p.span, groups = min(p.span, all_groups - group0);
-    if (u.expert == p.E) {
-        zero_rows(p, u, group0 * kOutCols, min((group0 + groups) * kOutCols, p.cols));
-        return;
-    }
-    const int64_t row0 = (int64_t)u.expert * p.N;
-    const int stages = (p.K + C - 1) / C;
-    const int k0 = stages * wave / WAVES, n = stages * (wave + 1) / WAVES - k0;      // this wave's stages
+    const int stages = (p.K + C - 1) / C, k0 = stages * wave / WAVES;                 // this wave's stages; where there are
+    const int mine_n = stages * (wave + 1) / WAVES - k0, n = max(1, mine_n);          // none, one that reads nothing
+    const int columns = mine_n > 0 ? p.K : 0;
+    const int64_t row0 = (int64_t)expert * p.N;
+    uint8_t* mine = space.place[wave];
 
-    // the stream's next stage: stage `it` of group `ig`, the descriptors of whose tiles end with their rows
+    struct Stage {
+        u32x4 w[P][L], x[XL];
+        uint32_t m[I4 ? P : 1][H], z[F == kI4ZP ? P : 1];
+    };
+    // the stream's next stage: stage `it` of item `ig`, the descriptors of whose tiles end with their rows
     int ig = 0, it = 0;
-    __amdgpu_buffer_rsrc_t rw[P];
+    __amdgpu_buffer_rsrc_t rw[P], rm[I4 ? P : 1], rz[F == kI4ZP ? P : 1];
     const auto aim = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < P; ++t) {
             const int rows = ig < groups ? max(0, tile_rows<GATED, P>(p, group0 + ig, t)) : 0;
+            const uint32_t in = (uint32_t)__builtin_amdgcn_readfirstlane(rows);
             const int64_t row = row0 + (rows ? tile_row<GATED, P>(p, group0 + ig, t) : 0);
-            rw[t] = make_rsrc(p.W + row * p.row_bytes, (uint32_t)__builtin_amdgcn_readfirstlane(rows) * p.row_bytes);
+            rw[t] = make_rsrc(p.W + row * p.row_bytes, in * p.row_bytes);
+            if constexpr (I4) rm[t] = make_rsrc(p.meta + row * p.G * 2, in * (uint32_t)p.G * 2u);
+            if constexpr (F == kI4ZP) rz[t] = make_rsrc(p.zeros + row * p.zbytes, in * p.zbytes);
         }
     };
+    // Unconditional loads (under a branch the compiler would wait for all that are on their way), out of range past the end.
     const uint32_t lw = (uint32_t)(lane / WP) * p.row_bytes + (uint32_t)(lane % WP) * 16u, wstep = (uint32_t)WR * p.row_bytes;
     const int cw = (lane % WP) * (C / WP), cx = (lane % XP) * 8;     // first column of the lane's 16 bytes
-    struct Stage {
-        u32x4 w[P][L], x[XL];
-        uint32_t m[I4 ? P : 1], z[F == kI4ZP ? P : 1];
-    };
-    // Unconditional loads (under a branch the compiler would wait for all that are on their way), out of range past the end.
     const auto issue_w = [&](Stage& B) __attribute__((always_inline)) {
-        const int kb = k0 + it, left = ig < groups ? p.K - kb * C : 0;
+        const int kb = k0 + it, left = ig < groups ? columns - kb * C : 0;
         const uint32_t wo = cw < left ? lw + (uint32_t)kb * (uint32_t)RB : kOOB;
 #pragma unroll
-        for (int t = 0; t < P; ++t)
+        for (int t = 0; t < P; ++t) {
 #pragma unroll
             for (int i = 0; i < L; ++i) B.w[t][i] = ld16<2>(rw[t], wo + wstep * (uint32_t)i, 0u);
-        if constexpr (I4) {
-            const int last = p.N - 1;
+            if constexpr (I4) {
+                const uint32_t lm = (uint32_t)ln * (uint32_t)p.G * 2u;
 #pragma unroll
-            for (int t = 0; t < P; ++t) {
-                const int64_t row = row0 + min(tile_row<GATED, P>(p, group0 + min(ig, groups - 1), t) + ln, last);
-                B.m[t] = reinterpret_cast<const uint16_t*>(p.meta)[row * p.G + min(kb, p.G - 1)];
-                if constexpr (F == kI4ZP) B.z[t] = p.zeros[row * p.zbytes + (min(kb, p.G - 1) >> 1)];
+                for (int h = 0; h < H; ++h) B.m[t][h] = ld_u16(rm[t], kb * H + h < p.G ? lm : kOOB, (uint32_t)(kb * H + h) * 2u);
+                if constexpr (F == kI4ZP) B.z[t] = ld_u8(rz[t], (uint32_t)ln * p.zbytes, (uint32_t)(kb * H >> 1));
             }
         }
     };
     uint32_t xo[XL];
     const __amdgpu_buffer_rsrc_t xrs = make_rsrc(p.x, p.x_bytes);
     const auto issue_x = [&](Stage& B, int g, int t) __attribute__((always_inline)) {
-        const int kb = k0 + t, left = g < groups ? p.K - kb * C : 0;
+        const int kb = k0 + t, left = g < groups ? columns - kb * C : 0;
 #pragma unroll
         for (int i = 0; i < XL; ++i) B.x[i] = ld16<0>(xrs, cx < left ? xo[i] + (uint32_t)kb * (2u * C) : kOOB, 0u);
     };
@@ -290,88 +320,91 @@ __global__ void __launch_bounds__(WAVES * kWave, 4) experts_stream_kernel(const 
     Stage buf[D];
     int pg[D], pt[D];
     aim();
-    if (n == 0) ig = groups;
 #pragma unroll
     for (int d = 0; d < D; ++d) {
         pg[d] = ig, pt[d] = it;
         issue_w(buf[d]);
-        if (n > 0) next();
+        next();
     }
 #pragma unroll
     for (int i = 0; i < XL; ++i) {
-        const int r = i * XR + lane / XP, pair = pair_at(p, u, r);
-        const bool held = r < u.held && (uint32_t)pair < (uint32_t)p.R;
-        xo[i] = held ? p.by_pairs.of((uint32_t)pair) * (uint32_t)(p.x_stride * 2) + (uint32_t)(lane % XP) * 16u : kOOB;
+        const int r = i * XR + lane / XP, pair = p.order[first + min(r, held - 1)];
+        const bool in = r < held && (uint32_t)pair < (uint32_t)p.R;
+        xo[i] = in ? p.by_pairs.of((uint32_t)pair) * (uint32_t)(p.x_stride * 2) + (uint32_t)(lane % XP) * 16u : kOOB;
     }
-    int pairs[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) pairs[c] = 4 * lh + c < u.held ? p.order[u.first + 4 * lh + c] : -1;
 #pragma unroll
     for (int d = 0; d < D; ++d) issue_x(buf[d], pg[d], pt[d]);
+    const int pairs = ln < held ? p.order[first + ln] : -1;
 
-    uint8_t* mine = place[wave];
     const auto w_at = [](int row, int piece) {
         return RB == 128 ? row * 128 + ((piece ^ (row & 7)) << 4) : row * 64 + ((piece ^ (row >> 1 & 3)) << 4);
     };
-    const auto x_at = [](int row, int piece) { return kWBytes + row * T::kXRowBytes + ((piece ^ (row & 7)) << 4); };
+    const auto x_at = [](int row, int piece) { return T::kWBytes + row * T::kXRowBytes + ((piece ^ (row & 7)) << 4); };
     const uint32_t one2 = (uint32_t)__builtin_amdgcn_readfirstlane((int)kI4Ones);
     const u32x4 ones = {one2, one2, one2, one2};
     f32x4 acc[P];
 #pragma unroll
     for (int t = 0; t < P; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
     const auto consume = [&](const Stage& B, int kb) __attribute__((always_inline)) {
         wave_lds_order();
 #pragma unroll
-        for (int i = 0; i < XL; ++i) *reinterpret_cast<u32x4*>(mine + x_at(i * XR + lane / XP, lane % XP)) = B.x[i];
+        for (int i = 0; i < XL; ++i)
+            *reinterpret_cast<u32x4*>(mine + x_at(i * XR + lane / XP, lane % XP)) = I4 ? i4_pair_x(B.x[i]) : B.x[i];
 #pragma unroll
         for (int t = 0; t < P; ++t)
 #pragma unroll
             for (int i = 0; i < L; ++i)
                 *reinterpret_cast<u32x4*>(mine + t * kTileRows * RB + w_at(i * WR + lane / WP, lane % WP)) = B.w[t][i];
         wave_lds_order();
-        u32x4 a[X];
-#pragma unroll
-        for (int j = 0; j < X; ++j) {
-            const int piece = F == kBF16 ? 4 * j + lh : (F == kFP8 ? 8 * (j >> 1) + 2 * lh + (j & 1) : 4 * lh + j);
-            a[j] = *reinterpret_cast<const u32x4*>(mine + x_at(ln & (kXRows - 1), piece));
-        }
-        f32x4 xs = {0.0f, 0.0f, 0.0f, 0.0f};
+        const auto x_piece = [&](int piece) { return *reinterpret_cast<const u32x4*>(mine + x_at(ln & (T::kXRows - 1), piece)); };
+        const auto w_piece = [&](int t, int piece) { return *reinterpret_cast<const u32x4*>(mine + t * kTileRows * RB + w_at(ln, piece)); };
         if constexpr (I4) {
 #pragma unroll
-            for (int j = 0; j < X; ++j) xs = mfma_16x16x32(a[j], ones, xs);
-        }
+            for (int h = 0; h < H; ++h) {
+                u32x4 a[4];
+                f32x4 xs = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int t = 0; t < P; ++t) {
-            u32x4 w[L];
+                for (int j = 0; j < 4; ++j) a[j] = x_piece(16 * h + 4 * lh + j);
 #pragma unroll
-            for (int i = 0; i < L; ++i) w[i] = *reinterpret_cast<const u32x4*>(mine + t * kTileRows * RB + w_at(ln, 4 * i + lh));
-            if constexpr (F == kBF16) {
+                for (int j = 0; j < 4; ++j) xs = mfma_16x16x32(a[j], ones, xs);
 #pragma unroll
-                for (int j = 0; j < X; ++j) acc[t] = mfma_16x16x32(a[j], w[j], acc[t]);
-            } else if constexpr (F == kFP8) {
+                for (int t = 0; t < P; ++t) {
+                    const u32x4 w = w_piece(t, 4 * h + lh);
+                    const uint32_t zero = F == kI4ZP ? B.z[F == kI4ZP ? t : 0] >> (4 * ((kb * H + h) & 1)) & 15u : 8u;
+                    const uint32_t m = i4_word_of<F>(B.m[t][h], zero);
+                    const float f = i4_factor<F>(m), sc = i4_scale<F>(m), z = i4_zero<F>(m);
+                    f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) g = mfma_16x16x32(a[j], i4_frag_paired(w[j], f), g);
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) acc[t][v] = __builtin_fmaf(sc, __builtin_fmaf(-z, xs[v], g[v]), acc[t][v]);
+                }
+                if (h + 1 < H) __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            u32x4 a[X];
+#pragma unroll
+            for (int j = 0; j < X; ++j) a[j] = x_piece(F == kBF16 ? 4 * j + lh : 8 * (j >> 1) + 2 * lh + (j & 1));
+#pragma unroll
+            for (int t = 0; t < P; ++t) {
+                u32x4 w[L];
+#pragma unroll
+                for (int i = 0; i < L; ++i) w[i] = w_piece(t, 4 * i + lh);
 #pragma unroll
                 for (int j = 0; j < X; ++j) {
-                    const u32x4 v = w[j >> 1];
-                    acc[t] = mfma_16x16x32(a[j], j & 1 ? fp8_frag(v.z, v.w) : fp8_frag(v.x, v.y), acc[t]);
+                    const u32x4 v = w[F == kFP8 ? j >> 1 : j];
+                    acc[t] = mfma_16x16x32(a[j], F == kBF16 ? v : (j & 1 ? fp8_frag(v.z, v.w) : fp8_frag(v.x, v.y)), acc[t]);
                 }
-            } else {
-                const uint32_t m = i4_word_of<F>(B.m[t], F == kI4ZP ? B.z[F == kI4ZP ? t : 0] >> (4 * (kb & 1)) & 15u : 8u);
-                const float f = i4_factor<F>(m), sc = i4_scale<F>(m), z = i4_zero<F>(m);
-                f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int j = 0; j < X; ++j) g = mfma_16x16x32(a[j], i4_frag(w[0][j], f), g);
-#pragma unroll
-                for (int v = 0; v < 4; ++v) acc[t][v] = __builtin_fmaf(sc, __builtin_fmaf(-z, xs[v], g[v]), acc[t][v]);
             }
         }
     };
 
-    // A group's end: partial tiles to LDS, then some of the waves add them and finish. Its operands are loaded a group ahead.
+    // An item's end: partial tiles to LDS, then some of the waves add them and finish. Its operands are loaded an item ahead.
     uint32_t scale[P], bias[P];
     const __amdgpu_buffer_rsrc_t scales = make_rsrc(reinterpret_cast<const float*>(p.meta) + (F == kFP8 ? row0 : 0),
                                                     F == kFP8 ? (uint32_t)p.N * 4u : 0u);
-    const __amdgpu_buffer_rsrc_t biases = make_rsrc(p.bias != nullptr ? p.bias + row0 : p.x, p.bias != nullptr ? (uint32_t)p.N * 2u : 0u);
+    const __amdgpu_buffer_rsrc_t biases = make_rsrc(p.bias != nullptr ? p.bias + row0 : p.x,
+                                                    p.bias != nullptr ? (uint32_t)p.N * 2u : 0u);
     const auto operands = [&](int g) __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < P; ++t) {
@@ -381,51 +414,44 @@ __global__ void __launch_bounds__(WAVES * kWave, 4) experts_stream_kernel(const 
         }
     };
     operands(0);
-    const auto finish_group = [&](int g) __attribute__((always_inline)) {
-        __syncthreads();                             // the last group's sums have been read
+    const auto finish_item = [&](int g) __attribute__((always_inline)) {
+        __syncthreads();                             // the last item's sums have been read
 #pragma unroll
         for (int t = 0; t < P; ++t) {
-            part[wave][t][lane] = acc[t];
+            space.part[wave][t][lane] = acc[t];
             acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
         __syncthreads();
-        const int first = g * kOuts % WAVES;         // the groups' finishes go round the waves
+        const int from = g * kOuts % WAVES;          // the items' finishes go round the waves
 #pragma unroll
         for (int q = 0; q < kOuts; ++q) {
-            if (wave != (first + q) % WAVES) continue;
+            if (wave != (from + q) % WAVES) continue;
             const int col = (group0 + g) * kOutCols + q * kTileRows + ln;
             f32x4 v[GATED ? 2 : 1];
 #pragma unroll
             for (int h = 0; h < (GATED ? 2 : 1); ++h) {
                 const int t = GATED ? 2 * q + h : q;
-                f32x4 sum = part[0][t][lane];
-#pragma unroll
-                for (int w = 1; w < WAVES; ++w) sum += part[w][t][lane];
+                f32x4 sum = space.part[0][t][lane];
+#pragma unroll 2
+                for (int w = 1; w < WAVES; ++w) sum += space.part[w][t][lane];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) v[h][c] = finish<F>(sum[c], F == kFP8 ? __uint_as_float(scale[t]) : 1.0f, bf16_to_f32(bias[t]));
             }
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                if ((uint32_t)pairs[c] >= (uint32_t)p.R || col >= p.cols) continue;
+                const int pair = __shfl(pairs, 4 * lh + c, kWave);
                 const float o = GATED ? silu(v[0][c]) * v[GATED ? 1 : 0][c] : v[0][c];
-                p.out[(int64_t)pairs[c] * p.out_stride + col] = (uint16_t)f32_to_bf16_out(o);
+                if ((uint32_t)pair < (uint32_t)p.R && col < p.cols)
+                    p.out[(int64_t)pair * p.out_stride + col] = (uint16_t)f32_to_bf16_out(o);
             }
         }
         operands(g + 1);
     };
 
-    if (n == 0) {
-        for (int g = 0; g < groups; ++g) finish_group(g);
-        return;
-    }
-    int g = 0, t = 0;                                // of the stage that is consumed next
-    const auto step = [&]() __attribute__((always_inline)) {
-        if (++t == n) finish_group(g), t = 0, ++g;
-    };
     const int all = groups * n;
-    int f = 0;
+    int g = 0, t = 0;                                // of the stage that is consumed next
     wait_loads<0>();                                 // the loop's waits then count its own order of loads alone
-    for (; f + D < all; f += D) {
+    for (int f = 0; f < all; f += D) {               // past the last stage the sums take zeros
 #pragma unroll
         for (int d = 0; d < D; ++d) {
             consume(buf[d], k0 + t);
@@ -434,15 +460,32 @@ __global__ void __launch_bounds__(WAVES * kWave, 4) experts_stream_kernel(const 
             issue_x(buf[d], ng, nt);
             next();
             __builtin_amdgcn_sched_barrier(0);
-            step();
+            if (++t == n && f + d < all) finish_item(g), t = 0, ++g;
         }
     }
-#pragma unroll
-    for (int d = 0; d < D; ++d)
-        if (f + d < all) {
-            consume(buf[d], k0 + t);
-            step();
-        }
+}
+
+template <int F, int MT, bool GATED>
+__global__ void __launch_bounds__(kStreamWaves * kWave, kStreamBlocks * kStreamWaves / 4) experts_stream_kernel(const ExpertsParams p)
+{
+    __shared__ StreamSpace<F, MT> space;
+    const Chunks<MT> chunks(p);
+    // below 2^32: at most kMostBlocks items, and fewer than 2^10 blocks
+    const uint32_t block = (uint32_t)xcd_contiguous((int)blockIdx.x, (int)gridDim.x), blocks = gridDim.x;
+    const uint32_t items = (uint32_t)(chunks.count * p.tiles), end = items * (block + 1) / blocks;
+    for (uint32_t item = items * block / blocks; item < end;) {
+        const int chunk = (int)p.by_tiles.of(item), group0 = (int)item - chunk * p.tiles;
+        const int groups = min(p.tiles - group0, (int)(end - item));
+        const auto x = chunks.of(p, chunk);
+        const int first = x.lo + (chunk - x.begin) * MT;
+        stream_items<F, MT, GATED>(p, space, x.expert, first, min(MT, x.hi - first), group0, groups);
+        item += (uint32_t)groups;
+    }
+    const uint32_t rest = (uint32_t)chunks.rest, rest_end = (uint32_t)((uint64_t)rest * (block + 1) / blocks);
+    for (uint32_t i = (uint32_t)((uint64_t)rest * block / blocks); i < rest_end; ++i) {
+        const int first = chunks.rest_at + (int)i * MT;
+        zero_rows(p, {p.E, first, min(MT, p.R - first), 0}, 0, p.cols);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -732,35 +775,35 @@ __global__ void __launch_bounds__(512, (TileShape<F, BM>::kWaves)) experts_tile_
 // host side
 // ---------------------------------------------------------------------------------------------------------------
 
-// Launches of a format's kernels; p as the entry point fills it but for tiles and most. 0, -2 (more blocks than a launch has)
-// or a hipError_t.
+// Launches of a format's kernels; p as the entry point fills it. 0, -2 (more blocks than a launch has) or a hipError_t.
 constexpr int kMostBlocks = 1 << 22;
-template <typename K>
-int launch_experts(K kernel, ExpertsParams p, int BM, int tiles_cols, int threads, hipStream_t st)
+// Sets what depends on the kernel's shape; the units, at most kMostBlocks, or -2.
+inline int64_t plan_experts(ExpertsParams& p, int BM, int unit_cols)
 {
-    p.tiles = (int)(((int64_t)p.cols + tiles_cols - 1) / tiles_cols);
+    p.tiles = (int)(((int64_t)p.cols + unit_cols - 1) / unit_cols);
     p.by_tiles = Divisor((uint32_t)p.tiles);
-    const int64_t bins = p.R < p.E + 1 ? p.R : p.E + 1;
-    const int64_t most = ((int64_t)p.R + bins * (BM - 1)) / BM;
-    if (most * p.tiles > kMostBlocks) return -2;
+    const int64_t bins = p.R < p.E + 1 ? p.R : p.E + 1, most = ((int64_t)p.R + bins * (BM - 1)) / BM;
     p.most = (int)most;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)(most * p.tiles)), dim3((uint32_t)threads), 0, st, p);
-    return (int)hipGetLastError();
+    return most * p.tiles <= kMostBlocks ? most * p.tiles : -2;
 }
 template <int F, int MT, bool GATED>
 int launch_stream(ExpertsParams p, hipStream_t st)
 {
-    constexpr int P = 2, WAVES = 8, D = 2, kCols = (GATED ? P / 2 : P) * kTileRows;
-    const int64_t groups = (p.cols + kCols - 1) / kCols, bins = p.R < p.E + 1 ? p.R : p.E + 1;
-    const int64_t most = ((int64_t)p.R + bins * (MT - 1)) / MT, aim = 2 * device_facts().cus;
-    p.span = (int)(groups * most > aim ? (groups * most + aim - 1) / aim : 1);
-    return launch_experts(experts_stream_kernel<F, P, WAVES, MT, D, GATED>, p, MT, kCols * p.span, WAVES * kWave, st);
+    const int64_t items = plan_experts(p, MT, (GATED ? kStreamTiles / 2 : kStreamTiles) * kTileRows);
+    if (items < 0) return -2;
+    const int64_t resident = kStreamBlocks * device_facts().cus;
+    hipLaunchKernelGGL((experts_stream_kernel<F, MT, GATED>), dim3((uint32_t)(items < resident ? items : resident)),
+                       dim3(kStreamWaves * kWave), 0, st, p);
+    return (int)hipGetLastError();
 }
 template <int F, int BM, bool GATED>
-int launch_tiles(const ExpertsParams& p, hipStream_t st)
+int launch_tiles(ExpertsParams p, hipStream_t st)
 {
     using T = TileShape<F, BM>;
-    return launch_experts(experts_tile_kernel<F, BM, GATED>, p, BM, (GATED ? T::kTiles / 2 : T::kTiles) * kTileRows, 512, st);
+    const int64_t units = plan_experts(p, BM, (GATED ? T::kTiles / 2 : T::kTiles) * kTileRows);
+    if (units < 0) return -2;
+    hipLaunchKernelGGL((experts_tile_kernel<F, BM, GATED>), dim3((uint32_t)units), dim3(512), 0, st, p);
+    return (int)hipGetLastError();
 }
 template <int F, bool GATED>
 int launch_format(const ExpertsParams& p, hipStream_t st)
@@ -768,8 +811,8 @@ int launch_format(const ExpertsParams& p, hipStream_t st)
     constexpr bool kI4F = F == kI4 || F == kI4ZP;
     const int64_t R = p.R, E = p.E;
     if (R <= 12 * E && p.x_bytes != 0) {
-        if (3 * R <= 4 * E) return launch_stream<F, 4, GATED>(p, st);
-        if (3 * R <= 8 * E) return launch_stream<F, 8, GATED>(p, st);
+        if (R <= E) return launch_stream<F, 4, GATED>(p, st);
+        if (R <= 4 * E) return launch_stream<F, 8, GATED>(p, st);
         return launch_stream<F, 16, GATED>(p, st);
     }
     if (R <= 32 * E) return launch_tiles<F, 32, GATED>(p, st);
