@@ -230,48 +230,50 @@ __device__ __forceinline__ int tile_rows(const ExpertsParams& p, int unit_tile, 
 // items of a chunk are one stream with D stages of loads in flight in registers (they hold several times what LDS
 // could), which pass through wave-private LDS into the matrix layout: every load is row-contiguous, no barrier within an item.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int kStreamTiles = 2, kStreamWaves = 4, kStreamBlocks = 3;     // tiles of an item, waves of a block, blocks of a CU
-template <int F>
-constexpr int kStreamAhead = 2;
-
-template <int F, int MT>
-struct StreamFmt {
+// WIDE (INT4 of an even number of groups): stages of 256 columns, whole 128-byte lines of the weights.
+template <int F, int MT, bool WIDE>
+struct StreamShape {
     static constexpr bool kI4F = F == kI4 || F == kI4ZP;
-    static constexpr int kCols = F == kBF16 ? 64 : (kI4F && MT == 4 ? 256 : 128);          // columns of a stage
+    static constexpr int kTiles = 2;                             // P
+    static constexpr int kWaves = 4, kBlocks = kI4F && MT == 16 ? 2 : 3;    // of a block, of a CU (more would spill)
+    static constexpr int kAhead = 2;                             // D
+    static constexpr int kCols = F == kBF16 ? 64 : (WIDE ? 256 : 128);          // columns of a stage
     static constexpr int kRowBytes = F == kBF16 ? 2 * kCols : (F == kFP8 ? kCols : kCols / 2);      // its bytes of a weight row
     static constexpr int kSteps = kCols / 32, kXRowBytes = 2 * kCols;
     static constexpr int kXLoadRows = kWave * 16 / kXRowBytes, kXRows = MT > kXLoadRows ? MT : kXLoadRows;
-    static constexpr int kWBytes = kStreamTiles * kTileRows * kRowBytes, kWaveBytes = kWBytes + kXRows * kXRowBytes;
+    static constexpr int kWBytes = kTiles * kTileRows * kRowBytes, kWaveBytes = kWBytes + kXRows * kXRowBytes;
 };
-template <int F, int MT>
+template <int F, int MT, bool WIDE>
 struct StreamSpace {
-    __attribute__((aligned(16))) uint8_t place[kStreamWaves][StreamFmt<F, MT>::kWaveBytes];
-    f32x4 part[kStreamWaves][kStreamTiles][kWave];
+    using T = StreamShape<F, MT, WIDE>;
+    __attribute__((aligned(16))) uint8_t place[T::kWaves][T::kWaveBytes];
+    f32x4 part[T::kWaves][T::kTiles][kWave];
 };
 
 // `groups` items from column group `group0` on, of the pairs order[first .. first + held) of one expert.
-template <int F, int MT, bool GATED>
-__device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace<F, MT>& space, int expert, int first, int held,
+template <int F, int MT, bool WIDE, bool SPLIT, bool GATED>
+__device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace<F, MT, WIDE>& space, int expert, int first, int held,
                                              int group0, int groups)
 {
-    using T = StreamFmt<F, MT>;
+    using T = StreamShape<F, MT, WIDE>;
     constexpr bool I4 = T::kI4F;
-    constexpr int P = kStreamTiles, WAVES = kStreamWaves, D = kStreamAhead<F>;
+    constexpr int P = T::kTiles, WAVES = T::kWaves, D = T::kAhead;
     constexpr int C = T::kCols, RB = T::kRowBytes, X = T::kSteps, L = RB * kTileRows / kChunkBytes;
     constexpr int H = I4 ? C / 128 : 1;               // INT4: groups of a stage
     constexpr int WP = RB / 16, WR = kWave / WP, XP = T::kXRowBytes / 16, XR = T::kXLoadRows, XL = T::kXRows / XR;
     constexpr int kOuts = GATED ? P / 2 : P, kOutCols = kOuts * kTileRows;
 
     const int lane = lane_id(), wave = wave_id(), ln = lane & 15, lh = lane >> 4;
-    const int stages = (p.K + C - 1) / C, k0 = stages * wave / WAVES;                 // this wave's stages; where there are
-    const int mine_n = stages * (wave + 1) / WAVES - k0, n = max(1, mine_n);          // none, one that reads nothing
+    const int stages = (p.K + C - 1) / C, k0 = SPLIT ? stages * wave / WAVES : 0;     // this wave's stages; where there are
+    const int mine_n = SPLIT ? stages * (wave + 1) / WAVES - k0 : stages;            // none, one that reads nothing
+    const int n = max(1, mine_n);
     const int columns = mine_n > 0 ? p.K : 0;
     const int64_t row0 = (int64_t)expert * p.N;
     uint8_t* mine = space.place[wave];
 
     struct Stage {
         u32x4 w[P][L], x[XL];
-        uint32_t m[I4 ? P : 1][H], z[F == kI4ZP ? P : 1];
+        uint32_t m[I4 ? P : 1], z[F == kI4ZP ? P : 1];       // INT4: scales (WIDE: two), zero points
     };
     // the stream's next stage: stage `it` of item `ig`, the descriptors of whose tiles end with their rows
     int ig = 0, it = 0;
@@ -298,9 +300,9 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
 #pragma unroll
             for (int i = 0; i < L; ++i) B.w[t][i] = ld16<2>(rw[t], wo + wstep * (uint32_t)i, 0u);
             if constexpr (I4) {
-                const uint32_t lm = (uint32_t)ln * (uint32_t)p.G * 2u;
-#pragma unroll
-                for (int h = 0; h < H; ++h) B.m[t][h] = ld_u16(rm[t], kb * H + h < p.G ? lm : kOOB, (uint32_t)(kb * H + h) * 2u);
+                const uint32_t lm = kb * H < p.G ? (uint32_t)ln * (uint32_t)p.G * 2u : kOOB;
+                if constexpr (WIDE) B.m[t] = __builtin_amdgcn_raw_buffer_load_b32(rm[t], lm, (uint32_t)kb * 4u, 0);
+                else B.m[t] = ld_u16(rm[t], lm, (uint32_t)kb * 2u);
                 if constexpr (F == kI4ZP) B.z[t] = ld_u8(rz[t], (uint32_t)ln * p.zbytes, (uint32_t)(kb * H >> 1));
             }
         }
@@ -371,7 +373,7 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
                 for (int t = 0; t < P; ++t) {
                     const u32x4 w = w_piece(t, 4 * h + lh);
                     const uint32_t zero = F == kI4ZP ? B.z[F == kI4ZP ? t : 0] >> (4 * ((kb * H + h) & 1)) & 15u : 8u;
-                    const uint32_t m = i4_word_of<F>(B.m[t][h], zero);
+                    const uint32_t m = i4_word_of<F>(WIDE && h ? B.m[t] >> 16 : B.m[t] & 0xFFFFu, zero);
                     const float f = i4_factor<F>(m), sc = i4_scale<F>(m), z = i4_zero<F>(m);
                     f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -414,37 +416,54 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
         }
     };
     operands(0);
-    const auto finish_item = [&](int g) __attribute__((always_inline)) {
-        __syncthreads();                             // the last item's sums have been read
+    // column tile q of item g out of its finished sums
+    const auto put = [&](int g, int q, const f32x4 (&sum)[GATED ? 2 : 1]) __attribute__((always_inline)) {
+        const int col = (group0 + g) * kOutCols + q * kTileRows + ln;
 #pragma unroll
-        for (int t = 0; t < P; ++t) {
-            space.part[wave][t][lane] = acc[t];
-            acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
-        __syncthreads();
-        const int from = g * kOuts % WAVES;          // the items' finishes go round the waves
-#pragma unroll
-        for (int q = 0; q < kOuts; ++q) {
-            if (wave != (from + q) % WAVES) continue;
-            const int col = (group0 + g) * kOutCols + q * kTileRows + ln;
-            f32x4 v[GATED ? 2 : 1];
+        for (int c = 0; c < 4; ++c) {
+            const int pair = __shfl(pairs, 4 * lh + c, kWave);
+            float v[GATED ? 2 : 1];
 #pragma unroll
             for (int h = 0; h < (GATED ? 2 : 1); ++h) {
                 const int t = GATED ? 2 * q + h : q;
-                f32x4 sum = space.part[0][t][lane];
-#pragma unroll 2
-                for (int w = 1; w < WAVES; ++w) sum += space.part[w][t][lane];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) v[h][c] = finish<F>(sum[c], F == kFP8 ? __uint_as_float(scale[t]) : 1.0f, bf16_to_f32(bias[t]));
+                v[h] = finish<F>(sum[h][c], F == kFP8 ? __uint_as_float(scale[t]) : 1.0f, bf16_to_f32(bias[t]));
             }
+            const float o = GATED ? silu(v[0]) * v[GATED ? 1 : 0] : v[0];
+            if ((uint32_t)pair < (uint32_t)p.R && col < p.cols)
+                p.out[(int64_t)pair * p.out_stride + col] = (uint16_t)f32_to_bf16_out(o);
+        }
+    };
+    const auto finish_item = [&](int g) __attribute__((always_inline)) {
+        if constexpr (SPLIT) {
+            __syncthreads();                         // the last item's sums have been read
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int pair = __shfl(pairs, 4 * lh + c, kWave);
-                const float o = GATED ? silu(v[0][c]) * v[GATED ? 1 : 0][c] : v[0][c];
-                if ((uint32_t)pair < (uint32_t)p.R && col < p.cols)
-                    p.out[(int64_t)pair * p.out_stride + col] = (uint16_t)f32_to_bf16_out(o);
+            for (int t = 0; t < P; ++t) space.part[wave][t][lane] = acc[t];
+            __syncthreads();
+            const int from = g * kOuts % WAVES;      // the items' finishes go round the waves
+#pragma unroll
+            for (int q = 0; q < kOuts; ++q) {
+                if (wave != (from + q) % WAVES) continue;
+                f32x4 sum[GATED ? 2 : 1];
+#pragma unroll
+                for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+                    const int t = GATED ? 2 * q + h : q;
+                    sum[h] = space.part[0][t][lane];
+#pragma unroll
+                    for (int w = 1; w < WAVES; ++w) sum[h] += space.part[w][t][lane];
+                }
+                put(g, q, sum);
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < kOuts; ++q) {
+                f32x4 sum[GATED ? 2 : 1];
+#pragma unroll
+                for (int h = 0; h < (GATED ? 2 : 1); ++h) sum[h] = acc[GATED ? 2 * q + h : q];
+                put(g, q, sum);
             }
         }
+#pragma unroll
+        for (int t = 0; t < P; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         operands(g + 1);
     };
 
@@ -465,20 +484,24 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
     }
 }
 
-template <int F, int MT, bool GATED>
-__global__ void __launch_bounds__(kStreamWaves * kWave, kStreamBlocks * kStreamWaves / 4) experts_stream_kernel(const ExpertsParams p)
+template <int F, int MT, bool WIDE, bool SPLIT, bool GATED>
+__global__ void __launch_bounds__((StreamShape<F, MT, WIDE>::kWaves * kWave),
+                                  (StreamShape<F, MT, WIDE>::kBlocks * StreamShape<F, MT, WIDE>::kWaves / 4))
+experts_stream_kernel(const ExpertsParams p)
 {
-    __shared__ StreamSpace<F, MT> space;
+    __shared__ StreamSpace<F, MT, WIDE> space;
     const Chunks<MT> chunks(p);
-    // below 2^32: at most kMostBlocks items, and fewer than 2^10 blocks
+    // the takers of items: blocks, or their waves, each for itself. Below 2^32: at most kMostItems, and fewer than 2^12 takers
+    constexpr uint32_t kEach = SPLIT ? 1 : StreamShape<F, MT, WIDE>::kWaves;
     const uint32_t block = (uint32_t)xcd_contiguous((int)blockIdx.x, (int)gridDim.x), blocks = gridDim.x;
-    const uint32_t items = (uint32_t)(chunks.count * p.tiles), end = items * (block + 1) / blocks;
-    for (uint32_t item = items * block / blocks; item < end;) {
+    const uint32_t taker = block * kEach + (SPLIT ? 0u : (uint32_t)wave_id()), takers = blocks * kEach;
+    const uint32_t items = (uint32_t)(chunks.count * p.tiles), end = items * (taker + 1) / takers;
+    for (uint32_t item = items * taker / takers; item < end;) {
         const int chunk = (int)p.by_tiles.of(item), group0 = (int)item - chunk * p.tiles;
         const int groups = min(p.tiles - group0, (int)(end - item));
         const auto x = chunks.of(p, chunk);
         const int first = x.lo + (chunk - x.begin) * MT;
-        stream_items<F, MT, GATED>(p, space, x.expert, first, min(MT, x.hi - first), group0, groups);
+        stream_items<F, MT, WIDE, SPLIT, GATED>(p, space, x.expert, first, min(MT, x.hi - first), group0, groups);
         item += (uint32_t)groups;
     }
     const uint32_t rest = (uint32_t)chunks.rest, rest_end = (uint32_t)((uint64_t)rest * (block + 1) / blocks);
@@ -786,14 +809,17 @@ inline int64_t plan_experts(ExpertsParams& p, int BM, int unit_cols)
     p.most = (int)most;
     return most * p.tiles <= kMostBlocks ? most * p.tiles : -2;
 }
-template <int F, int MT, bool GATED>
+constexpr int kMostItems = 1 << 20, kSplitBelow = 4;
+template <int F, int MT, bool WIDE, bool GATED>
 int launch_stream(ExpertsParams p, hipStream_t st)
 {
-    const int64_t items = plan_experts(p, MT, (GATED ? kStreamTiles / 2 : kStreamTiles) * kTileRows);
-    if (items < 0) return -2;
-    const int64_t resident = kStreamBlocks * device_facts().cus;
-    hipLaunchKernelGGL((experts_stream_kernel<F, MT, GATED>), dim3((uint32_t)(items < resident ? items : resident)),
-                       dim3(kStreamWaves * kWave), 0, st, p);
+    using T = StreamShape<F, MT, WIDE>;
+    const int64_t items = plan_experts(p, MT, (GATED ? T::kTiles / 2 : T::kTiles) * kTileRows);
+    if (items < 0 || items > kMostItems) return -2;
+    const int64_t resident = T::kBlocks * device_facts().cus;
+    const dim3 grid((uint32_t)(items < resident ? items : resident)), block(T::kWaves * kWave);
+    if (items < kSplitBelow * resident) hipLaunchKernelGGL((experts_stream_kernel<F, MT, WIDE, true, GATED>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((experts_stream_kernel<F, MT, WIDE, false, GATED>), grid, block, 0, st, p);
     return (int)hipGetLastError();
 }
 template <int F, int BM, bool GATED>
@@ -811,9 +837,15 @@ int launch_format(const ExpertsParams& p, hipStream_t st)
     constexpr bool kI4F = F == kI4 || F == kI4ZP;
     const int64_t R = p.R, E = p.E;
     if (R <= 12 * E && p.x_bytes != 0) {
-        if (R <= E) return launch_stream<F, 4, GATED>(p, st);
-        if (R <= 4 * E) return launch_stream<F, 8, GATED>(p, st);
-        return launch_stream<F, 16, GATED>(p, st);
+        const auto go = [&](auto wide) {
+            constexpr bool WIDE = decltype(wide)::value;
+            if (R <= E) return launch_stream<F, 4, WIDE, GATED>(p, st);
+            if (R <= 4 * E) return launch_stream<F, 8, WIDE, GATED>(p, st);
+            return launch_stream<F, 16, WIDE, GATED>(p, st);
+        };
+        if constexpr (kI4F)
+            if (p.G % 2 == 0 && aligned(p.meta, 4)) return go(std::true_type{});
+        return go(std::false_type{});
     }
     if (R <= 32 * E) return launch_tiles<F, 32, GATED>(p, st);
     if (R <= 64 * E) return launch_tiles<F, 64, GATED>(p, st);
