@@ -512,172 +512,152 @@ experts_stream_kernel(const ExpertsParams p)
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// More rows an expert: a block is BM pairs by 16 tiles of weight rows, its 8 waves 2 x 4 (or 1 x 8) parts of that. Two places
-// in LDS are filled in turn, one barrier a stage. Up to 128 pairs, where reading the weights still counts, the stages come by
-// way of registers with D of them in flight; blocks of 256, whose sums take the registers, are filled straight from memory
-// while the stage before is multiplied.
+// More rows an expert: a block is BM pairs by 8 or 16 tiles of weight rows, its 4 or 8 waves 1 x 4 or 2 x 4 parts of that. Two
+// places in LDS are filled in turn, one barrier a stage. Up to 128 pairs, where reading the weights still counts, the stages
+// come by way of registers with two of them in flight; larger blocks, whose sums take the registers, are filled straight from
+// memory while the stage before is multiplied. A block is a unit, and chunks of one expert and columns are neighbours, so that
+// they read the weights once: blocks that took several units, chunk by chunk, were slower (us, 64 tokens and two of 8 experts
+// 28672x4096 e4m3 169 -> 190).
 // ---------------------------------------------------------------------------------------------------------------
-template <int F, int BM>
+template <int F, int BM, bool WIDE>
 struct TileShape {
     static constexpr bool kI4F = F == kI4 || F == kI4ZP;
-    static constexpr int kCols = F == kBF16 || (F == kFP8 && BM == 256) ? 64 : 128;
+    static constexpr int kCols = F == kBF16 || (F == kFP8 && BM == 256) ? 64 : (WIDE ? 256 : 128);
     static constexpr int kRowBytes = F == kBF16 ? 2 * kCols : (F == kFP8 ? kCols : kCols / 2);
     static constexpr int kXRowBytes = 2 * kCols, kSteps = kCols / 32;
-    static constexpr int kTiles = 16;                            // of 16 weight rows
-    static constexpr int kM = BM >= 128 ? 2 : 1, kN = 8 / kM;    // the waves' parts
+    static constexpr int kWaves = BM >= 128 ? 8 : 4, kTiles = 2 * kWaves;        // of a block; its tiles of 16 weight rows
+    static constexpr int kM = BM >= 128 ? 2 : 1, kN = kWaves / kM;               // the waves' parts
     static constexpr int kTM = BM / 16 / kM, kTN = kTiles / kN;
     static constexpr int kWBytes = kTiles * kTileRows * kRowBytes, kXBytes = BM * kXRowBytes;
     static constexpr bool kDirect = BM == 256 || (kI4F && BM == 128);
-    static constexpr int kAhead = 2;                             // stages in flight in registers
-    static constexpr int kWaves = kWBytes + kXBytes <= 40960 && !kDirect && !(kI4F && BM > 32) ? 4 : 2;    // a SIMD's: two blocks a CU, or one
+    static constexpr int kBlocks = BM >= 128 ? 1 : (BM == 64 || WIDE ? 2 : 3);   // of a CU
 };
 
-template <int F, int BM, bool GATED>
-__global__ void __launch_bounds__(512, (TileShape<F, BM>::kWaves)) experts_tile_kernel(const ExpertsParams p)
+template <int F, int BM, bool WIDE, bool GATED>
+__global__ void __launch_bounds__((TileShape<F, BM, WIDE>::kWaves * kWave),
+                                  (TileShape<F, BM, WIDE>::kBlocks * TileShape<F, BM, WIDE>::kWaves / 4))
+experts_tile_kernel(const ExpertsParams p)
 {
-    using T = TileShape<F, BM>;
+    using T = TileShape<F, BM, WIDE>;
     constexpr bool I4 = T::kI4F;
     constexpr int C = T::kCols, RB = T::kRowBytes, XB = T::kXRowBytes, X = T::kSteps, TM = T::kTM, TN = T::kTN;
-    constexpr int WP = RB / 16, WR = kWave / WP, WL = T::kWBytes / 8192, XP = XB / 16, XR = kWave / XP;
-    constexpr int XL = (T::kXBytes + 8191) / 8192, XW = T::kXBytes / 1024 < 8 ? T::kXBytes / 1024 : 8;   // XW: waves that load x
+    constexpr int H = I4 ? C / 128 : 1;               // INT4: groups of a stage
+    constexpr int WAVES = T::kWaves, WP = RB / 16, WR = kWave / WP, WL = T::kWBytes / (1024 * WAVES), XP = XB / 16, XR = kWave / XP;
+    constexpr int XL = (T::kXBytes / 1024 + WAVES - 1) / WAVES;
+    constexpr int XW = T::kXBytes / 1024 < WAVES ? T::kXBytes / 1024 : WAVES;    // waves that load x
+    constexpr int kOutCols = (GATED ? T::kTiles / 2 : T::kTiles) * kTileRows;
     __shared__ __attribute__((aligned(16))) uint8_t slot0[T::kWBytes + T::kXBytes];
     __shared__ __attribute__((aligned(16))) uint8_t slot1[T::kWBytes + T::kXBytes];
 
-    const ExpertUnit u = unit_of<BM>(p);
-    if (u.expert < 0) return;
     const int lane = lane_id(), wave = wave_id(), ln = lane & 15, lh = lane >> 4;
     const int wm = wave / T::kN, wn = wave % T::kN;
-    constexpr int kOutCols = (GATED ? T::kTiles / 2 : T::kTiles) * kTileRows;
+    const int stages = (p.K + C - 1) / C;
+    const auto w_piece = [](int r) { return RB == 128 ? r & 7 : r >> 1 & 3; };
+    const int wr = lane / WP, xr = lane / XP;
+    const uint32_t wpiece = (uint32_t)((lane % WP) ^ w_piece(wr)) * 16u;         // a load's first row is a multiple of 8
+    const uint32_t one2 = (uint32_t)__builtin_amdgcn_readfirstlane((int)kI4Ones);
+    const u32x4 ones = {one2, one2, one2, one2};
+
+    const ExpertUnit u = unit_of<BM>(p);
+    if (u.expert < 0) return;
     const int c0 = u.tile * kOutCols;
     if (u.expert == p.E) {
         zero_rows(p, u, c0, min(c0 + kOutCols, p.cols));
         return;
     }
     const int64_t row0 = (int64_t)u.expert * p.N;
-    const uint8_t* We = p.W + row0 * p.row_bytes;
-
+    const bool busy = wm * TM * 16 < u.held;         // a part without pairs waits at the barriers only
     // A load of weights lies within a 16-row tile: its base is the wave's, an offset the lane's. x has an address a row.
-    const auto w_piece = [](int r) { return RB == 128 ? r & 7 : r >> 1 & 3; };
-    const uint8_t* wp[WL];
+    const uint8_t *wp[WL], *xp[XL];
     uint32_t wo[WL];
-    const int wr = lane / WP, xr = lane / XP;
-    const uint32_t wpiece = (uint32_t)((lane % WP) ^ w_piece(wr)) * 16u;         // a load's first row is a multiple of 8
 #pragma unroll
     for (int i = 0; i < WL; ++i) {
         const int r0 = (wave * WL + i) * WR, t = r0 / kTileRows;
         const int rows = max(1, tile_rows<GATED, T::kTiles>(p, u.tile, t));
-        wp[i] = We + (int64_t)min(tile_row<GATED, T::kTiles>(p, u.tile, t), p.N - 1) * p.row_bytes;
+        wp[i] = p.W + (row0 + min(tile_row<GATED, T::kTiles>(p, u.tile, t), p.N - 1)) * p.row_bytes;
         wo[i] = (uint32_t)min(r0 % kTileRows + wr, rows - 1) * p.row_bytes;
     }
-    const uint8_t* xp[XL];
 #pragma unroll
     for (int i = 0; i < XL; ++i) xp[i] = x_row(p, pair_at(p, u, (wave * XL + i) * XR + xr));
-    const int stages = (p.K + C - 1) / C;
     // A stage's addresses; bytes past a row's end come from its last piece instead, and are cleared in the last stage.
     const auto w_from = [&](int s, int i) { return wp[i] + (wo[i] + min((uint32_t)s * RB + wpiece, p.row_bytes - 16u)); };
     const auto x_from = [&](int s, int i) {
         const int r = (wave * XL + i) * XR + xr;
         return xp[i] + min((uint32_t)s * XB + (uint32_t)((lane % XP) ^ (r & 7)) * 16u, (uint32_t)p.K * 2u - 16u);
     };
-    const auto issue = [&](uint8_t* slot, int s) __attribute__((always_inline)) {
-        if (s >= stages) return;
-#pragma unroll
-        for (int i = 0; i < WL; ++i) lds_copy16(slot + (wave * WL + i) * 1024, w_from(s, i));
-        if (XW == 8 || wave < XW) {
-#pragma unroll
-            for (int i = 0; i < XL; ++i) lds_copy16(slot + T::kWBytes + (wave * XL + i) * 1024, x_from(s, i));
-        }
-    };
-    struct Stage {
-        u32x4 w[WL], x[XL];
-    };
-    // Unconditional: past the last stage it reads that one again, waves without a part of x their neighbours' rows.
-    const auto load = [&](Stage& B, int s) __attribute__((always_inline)) {
-        s = min(s, stages - 1);
-#pragma unroll
-        for (int i = 0; i < WL; ++i) B.w[i] = *reinterpret_cast<const u32x4*>(w_from(s, i));
-#pragma unroll
-        for (int i = 0; i < XL; ++i) B.x[i] = *reinterpret_cast<const u32x4*>(x_from(s, i));
-    };
-    const auto store = [&](uint8_t* slot, const Stage& B) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < WL; ++i) *reinterpret_cast<u32x4*>(slot + (wave * WL + i) * 1024 + lane * 16) = B.w[i];
-        if (XW == 8 || wave < XW) {
-#pragma unroll
-            for (int i = 0; i < XL; ++i)
-                *reinterpret_cast<u32x4*>(slot + T::kWBytes + (wave * XL + i) * 1024 + lane * 16) = B.x[i];
-        }
-    };
-    // INT4: scale and zero point of the stage's group for the wave's columns, as they are stored, a stage ahead
+    // INT4: scales (WIDE: two) and zero points of a stage's groups for the wave's columns, as they are stored
     struct Meta {
         uint32_t s[I4 ? TN : 1], z[F == kI4ZP ? TN : 1];
     };
     Meta meta, ahead;
-    const auto meta_load = [&](Meta& m, int g) __attribute__((always_inline)) {
+    const auto meta_load = [&](Meta& m, int s) __attribute__((always_inline)) {
         if constexpr (I4) {
-            g = min(g, p.G - 1);
+            s = min(s, stages - 1);
 #pragma unroll
             for (int t = 0; t < TN; ++t) {
                 const int i = wn * TN + t, rows = max(1, tile_rows<GATED, T::kTiles>(p, u.tile, i));
                 const int64_t first = row0 + min(tile_row<GATED, T::kTiles>(p, u.tile, i), p.N - 1);
                 const uint32_t r = (uint32_t)min(ln, rows - 1);
-                m.s[t] = *reinterpret_cast<const uint16_t*>(p.meta + first * p.G * 2 + (r * (uint32_t)p.G + (uint32_t)g) * 2u);
-                if constexpr (F == kI4ZP) m.z[t] = p.zeros[first * p.zbytes + (r * p.zbytes + (uint32_t)(g >> 1))];
+                const uint8_t* at = p.meta + first * p.G * 2 + (r * (uint32_t)p.G + (uint32_t)(s * H)) * 2u;
+                if constexpr (WIDE) m.s[t] = *reinterpret_cast<const uint32_t*>(at);
+                else m.s[t] = *reinterpret_cast<const uint16_t*>(at);
+                if constexpr (F == kI4ZP) m.z[t] = p.zeros[first * p.zbytes + (r * p.zbytes + (uint32_t)(s * H >> 1))];
             }
         }
     };
-    const uint32_t one2 = (uint32_t)__builtin_amdgcn_readfirstlane((int)kI4Ones);
-    const u32x4 ones = {one2, one2, one2, one2};
     f32x4 acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int t = 0; t < TN; ++t) acc[i][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const bool busy = wm * TM * 16 < u.held;         // a part without pairs waits at the barriers only
-
     const auto get_x = [&](const uint8_t* slot, int i, int j) {
         const int r = (wm * TM + i) * 16 + ln;
-        const int piece = F == kBF16 ? 4 * j + lh : (F == kFP8 ? 8 * (j >> 1) + 2 * lh + (j & 1) : 4 * lh + j);
+        const int piece = F == kBF16 ? 4 * j + lh : (F == kFP8 ? 8 * (j >> 1) + 2 * lh + (j & 1) : 16 * (j >> 2) + 4 * lh + (j & 3));
         return *reinterpret_cast<const u32x4*>(slot + T::kWBytes + r * XB + ((piece ^ (r & 7)) << 4));
     };
     const auto get_w = [&](const uint8_t* slot, int t, int i) {
         const int r = (wn * TN + t) * 16 + ln;
         return *reinterpret_cast<const u32x4*>(slot + r * RB + (((4 * i + lh) ^ w_piece(r)) << 4));
     };
-    const auto use = [&](const uint8_t* slot, int group) __attribute__((always_inline)) {
+    const auto use = [&](const uint8_t* slot, int s) __attribute__((always_inline)) {
         if constexpr (I4) {
-            u32x4 a[TM][X], w[TN];
-            f32x4 xs[TM];
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < X; ++j) a[i][j] = get_x(slot, i, j);
-#pragma unroll
-            for (int t = 0; t < TN; ++t) w[t] = get_w(slot, t, 0);
-#pragma unroll
-            for (int i = 0; i < TM; ++i) {
-                xs[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int j = 0; j < X; ++j) xs[i] = mfma_16x16x32(a[i][j], ones, xs[i]);
-            }
-#pragma unroll
-            for (int t = 0; t < TN; ++t) {
-                const uint32_t m = i4_word_of<F>(meta.s[t], F == kI4ZP ? meta.z[F == kI4ZP ? t : 0] >> (4 * (group & 1)) & 15u : 8u);
-                const float f = i4_factor<F>(m), sc = i4_scale<F>(m), z = i4_zero<F>(m);
-                f32x4 g[TM];
-#pragma unroll
-                for (int i = 0; i < TM; ++i) g[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int j = 0; j < X; ++j) {
-                    const u32x4 b = i4_frag(w[t][j], f);
-#pragma unroll
-                    for (int i = 0; i < TM; ++i) g[i] = mfma_16x16x32(a[i][j], b, g[i]);
-                }
+            for (int h = 0; h < H; ++h) {
+                u32x4 a[TM][4], w[TN];
+                f32x4 xs[TM];
 #pragma unroll
                 for (int i = 0; i < TM; ++i)
 #pragma unroll
-                    for (int v = 0; v < 4; ++v)
-                        acc[i][t][v] = __builtin_fmaf(sc, __builtin_fmaf(-z, xs[i][v], g[i][v]), acc[i][t][v]);
+                    for (int j = 0; j < 4; ++j) a[i][j] = get_x(slot, i, 4 * h + j);
+#pragma unroll
+                for (int t = 0; t < TN; ++t) w[t] = get_w(slot, t, h);
+#pragma unroll
+                for (int i = 0; i < TM; ++i) {
+                    xs[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) xs[i] = mfma_16x16x32(a[i][j], ones, xs[i]);
+                }
+#pragma unroll
+                for (int t = 0; t < TN; ++t) {
+                    const uint32_t zero = F == kI4ZP ? meta.z[F == kI4ZP ? t : 0] >> (4 * ((s * H + h) & 1)) & 15u : 8u;
+                    const uint32_t m = i4_word_of<F>(WIDE && h ? meta.s[t] >> 16 : meta.s[t] & 0xFFFFu, zero);
+                    const float f = i4_factor<F>(m), sc = i4_scale<F>(m), z = i4_zero<F>(m);
+                    f32x4 g[TM];
+#pragma unroll
+                    for (int i = 0; i < TM; ++i) g[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const u32x4 b = i4_frag(w[t][j], f);
+#pragma unroll
+                        for (int i = 0; i < TM; ++i) g[i] = mfma_16x16x32(a[i][j], b, g[i]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int v = 0; v < 4; ++v)
+                            acc[i][t][v] = __builtin_fmaf(sc, __builtin_fmaf(-z, xs[i][v], g[i][v]), acc[i][t][v]);
+                }
+                if (h + 1 < H) __builtin_amdgcn_sched_barrier(0);
             }
         } else {
             constexpr int kWSteps = F == kFP8 ? 2 : 1;     // steps that a 16-byte piece of a weight row holds
@@ -702,15 +682,16 @@ __global__ void __launch_bounds__(512, (TileShape<F, BM>::kWaves)) experts_tile_
             }
         }
     };
-    // The last stage of a K that is no multiple of its columns: what lies past the rows' ends is 0 in both operands.
+    // The last stage of a K that is no multiple of its columns: what lies past the rows' ends is 0 in both operands. (INT4
+    // WIDE has whole stages.)
     const auto clear_past = [&](uint8_t* slot, int left) __attribute__((always_inline)) {
         constexpr int kWCols = F == kFP8 ? 16 : 8;
         const u32x4 none = {0, 0, 0, 0};
-        for (int e = (int)threadIdx.x; e < T::kTiles * kTileRows * WP; e += 512) {
+        for (int e = (int)threadIdx.x; e < T::kTiles * kTileRows * WP; e += WAVES * kWave) {
             const int r = e / WP, at = e % WP;
             if ((at ^ w_piece(r)) * kWCols >= left) *reinterpret_cast<u32x4*>(slot + r * RB + at * 16) = none;
         }
-        for (int e = (int)threadIdx.x; e < BM * XP; e += 512) {
+        for (int e = (int)threadIdx.x; e < BM * XP; e += WAVES * kWave) {
             const int r = e / XP, at = e % XP;
             if ((at ^ (r & 7)) * 8 >= left) *reinterpret_cast<u32x4*>(slot + T::kWBytes + r * XB + at * 16) = none;
         }
@@ -721,8 +702,17 @@ __global__ void __launch_bounds__(512, (TileShape<F, BM>::kWaves)) experts_tile_
         if (busy) use(slot, s);
         if constexpr (I4) meta = ahead;
     };
+
     meta_load(meta, 0);
     if constexpr (T::kDirect) {
+        static_assert(!T::kDirect || XW == WAVES, "every wave has a part of x");
+        const auto issue = [&](uint8_t* slot, int s) __attribute__((always_inline)) {
+            if (s >= stages) return;
+#pragma unroll
+            for (int i = 0; i < WL; ++i) lds_copy16(slot + (wave * WL + i) * 1024, w_from(s, i));
+#pragma unroll
+            for (int i = 0; i < XL; ++i) lds_copy16(slot + T::kWBytes + (wave * XL + i) * 1024, x_from(s, i));
+        };
         const auto stage = [&](uint8_t* mine, uint8_t* next, int s) __attribute__((always_inline)) {
             wait_loads<0>();
             __syncthreads();                         // this stage has arrived, the other place is read
@@ -736,27 +726,46 @@ __global__ void __launch_bounds__(512, (TileShape<F, BM>::kWaves)) experts_tile_
             if (s + 1 < stages) stage(slot1, slot0, s + 1);
         }
     } else {
-        constexpr int D = T::kAhead;
-        static_assert(D % 2 == 0, "a buffer goes to the same place each time");
-        Stage buf[D];
+        struct Stage {
+            u32x4 w[WL], x[XL];
+        };
+        // Unconditional: past the last stage it reads that one again, waves without a part of x their neighbours' rows.
+        const auto load = [&](Stage& B, int s) __attribute__((always_inline)) {
+            s = min(s, stages - 1);
 #pragma unroll
-        for (int d = 0; d < D; ++d) load(buf[d], d);
+            for (int i = 0; i < WL; ++i) B.w[i] = *reinterpret_cast<const u32x4*>(w_from(s, i));
+#pragma unroll
+            for (int i = 0; i < XL; ++i) B.x[i] = *reinterpret_cast<const u32x4*>(x_from(s, i));
+        };
+        const auto store = [&](uint8_t* slot, const Stage& B) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < WL; ++i) *reinterpret_cast<u32x4*>(slot + (wave * WL + i) * 1024 + lane * 16) = B.w[i];
+            if (XW == WAVES || wave < XW) {
+#pragma unroll
+                for (int i = 0; i < XL; ++i)
+                    *reinterpret_cast<u32x4*>(slot + T::kWBytes + (wave * XL + i) * 1024 + lane * 16) = B.x[i];
+            }
+        };
+        Stage buf[2];
+        load(buf[0], 0);
+        load(buf[1], 1);
         int s = 0;
-        for (; s + D < stages; s += D) {
+        wait_loads<0>();                             // the loop's waits then count its own order of loads alone
+        for (; s + 2 < stages; s += 2) {
 #pragma unroll
-            for (int d = 0; d < D; ++d) {
-                uint8_t* slot = d & 1 ? slot1 : slot0;
+            for (int d = 0; d < 2; ++d) {
+                uint8_t* slot = d ? slot1 : slot0;
                 store(slot, buf[d]);                 // what was there is read: two stages ago, before the last barrier
                 meta_load(ahead, s + d + 1);         // ahead of the loads that stay on their way
-                load(buf[d], s + d + D);
+                load(buf[d], s + d + 2);
                 block_lds_order();
                 multiply(slot, s + d, false);
             }
         }
 #pragma unroll
-        for (int d = 0; d < D; ++d)
+        for (int d = 0; d < 2; ++d)
             if (s + d < stages) {
-                uint8_t* slot = d & 1 ? slot1 : slot0;
+                uint8_t* slot = d ? slot1 : slot0;
                 store(slot, buf[d]);
                 meta_load(ahead, s + d + 1);
                 block_lds_order();
@@ -765,6 +774,13 @@ __global__ void __launch_bounds__(512, (TileShape<F, BM>::kWaves)) experts_tile_
     }
     if (!busy) return;
 
+    // out: the pairs of the wave's rows, the columns' scales and biases
+    int pairs[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const int m = (wm * TM + i) * 16 + ln;
+        pairs[i] = m < u.held ? p.order[u.first + m] : -1;
+    }
     float scale[TN], bias[TN];
 #pragma unroll
     for (int t = 0; t < TN; ++t) {
@@ -777,8 +793,7 @@ __global__ void __launch_bounds__(512, (TileShape<F, BM>::kWaves)) experts_tile_
     for (int i = 0; i < TM; ++i) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            const int m = (wm * TM + i) * 16 + 4 * lh + c;
-            const int pair = m < u.held ? p.order[u.first + m] : -1;
+            const int pair = __shfl(pairs[i], 4 * lh + c, kWave);
             if ((uint32_t)pair >= (uint32_t)p.R) continue;
             uint16_t* out = p.out + (int64_t)pair * p.out_stride;
 #pragma unroll
@@ -822,13 +837,13 @@ int launch_stream(ExpertsParams p, hipStream_t st)
     else hipLaunchKernelGGL((experts_stream_kernel<F, MT, WIDE, false, GATED>), grid, block, 0, st, p);
     return (int)hipGetLastError();
 }
-template <int F, int BM, bool GATED>
+template <int F, int BM, bool WIDE, bool GATED>
 int launch_tiles(ExpertsParams p, hipStream_t st)
 {
-    using T = TileShape<F, BM>;
+    using T = TileShape<F, BM, WIDE>;
     const int64_t units = plan_experts(p, BM, (GATED ? T::kTiles / 2 : T::kTiles) * kTileRows);
     if (units < 0) return -2;
-    hipLaunchKernelGGL((experts_tile_kernel<F, BM, GATED>), dim3((uint32_t)units), dim3(512), 0, st, p);
+    hipLaunchKernelGGL((experts_tile_kernel<F, BM, WIDE, GATED>), dim3((uint32_t)units), dim3(T::kWaves * kWave), 0, st, p);
     return (int)hipGetLastError();
 }
 template <int F, bool GATED>
@@ -836,21 +851,21 @@ int launch_format(const ExpertsParams& p, hipStream_t st)
 {
     constexpr bool kI4F = F == kI4 || F == kI4ZP;
     const int64_t R = p.R, E = p.E;
-    if (R <= 12 * E && p.x_bytes != 0) {
-        const auto go = [&](auto wide) {
-            constexpr bool WIDE = decltype(wide)::value;
+    const auto go = [&](auto wide) {
+        constexpr bool WIDE = decltype(wide)::value;
+        if (R <= 12 * E && p.x_bytes != 0) {
             if (R <= E) return launch_stream<F, 4, WIDE, GATED>(p, st);
             if (R <= 4 * E) return launch_stream<F, 8, WIDE, GATED>(p, st);
             return launch_stream<F, 16, WIDE, GATED>(p, st);
-        };
-        if constexpr (kI4F)
-            if (p.G % 2 == 0 && aligned(p.meta, 4)) return go(std::true_type{});
-        return go(std::false_type{});
-    }
-    if (R <= 32 * E) return launch_tiles<F, 32, GATED>(p, st);
-    if (R <= 64 * E) return launch_tiles<F, 64, GATED>(p, st);
-    if (kI4F || R <= 160 * E) return launch_tiles<F, 128, GATED>(p, st);
-    return launch_tiles<F, kI4F ? 128 : 256, GATED>(p, st);
+        }
+        if (R <= 32 * E) return launch_tiles<F, 32, WIDE, GATED>(p, st);
+        if (R <= 64 * E) return launch_tiles<F, 64, false, GATED>(p, st);
+        if (kI4F || R <= 160 * E) return launch_tiles<F, 128, false, GATED>(p, st);
+        return launch_tiles<F, kI4F ? 128 : 256, false, GATED>(p, st);
+    };
+    if constexpr (kI4F)
+        if (p.G % 2 == 0 && aligned(p.meta, 4)) return go(std::true_type{});
+    return go(std::false_type{});
 }
 template <int F>
 int launch_experts_format(const ExpertsParams& p, bool gated, hipStream_t st)
