@@ -235,7 +235,7 @@ template <int F, int MT, bool WIDE>
 struct StreamShape {
     static constexpr bool kI4F = F == kI4 || F == kI4ZP;
     static constexpr int kTiles = 2;                             // P
-    static constexpr int kWaves = 4, kBlocks = kI4F && MT == 16 ? 2 : 3;    // of a block, of a CU (more would spill)
+    static constexpr int kWaves = 4, kBlocks = 3;                // of a block, of a CU
     static constexpr int kAhead = 2;                             // D
     static constexpr int kCols = F == kBF16 ? 64 : (WIDE ? 256 : 128);          // columns of a stage
     static constexpr int kRowBytes = F == kBF16 ? 2 * kCols : (F == kFP8 ? kCols : kCols / 2);      // its bytes of a weight row
@@ -522,15 +522,15 @@ experts_stream_kernel(const ExpertsParams p)
 template <int F, int BM, bool WIDE>
 struct TileShape {
     static constexpr bool kI4F = F == kI4 || F == kI4ZP;
-    static constexpr int kCols = F == kBF16 || (F == kFP8 && BM == 256) ? 64 : (WIDE ? 256 : 128);
+    static constexpr int kCols = F == kBF16 || (F == kFP8 && BM >= 128) ? 64 : (WIDE ? 256 : 128);
     static constexpr int kRowBytes = F == kBF16 ? 2 * kCols : (F == kFP8 ? kCols : kCols / 2);
     static constexpr int kXRowBytes = 2 * kCols, kSteps = kCols / 32;
-    static constexpr int kWaves = BM >= 128 ? 8 : 4, kTiles = 2 * kWaves;        // of a block; its tiles of 16 weight rows
+    static constexpr int kWaves = BM == 256 ? 8 : 4, kTiles = 2 * kWaves;     // of a block; its tiles of 16 weight rows
     static constexpr int kM = BM >= 128 ? 2 : 1, kN = kWaves / kM;               // the waves' parts
     static constexpr int kTM = BM / 16 / kM, kTN = kTiles / kN;
     static constexpr int kWBytes = kTiles * kTileRows * kRowBytes, kXBytes = BM * kXRowBytes;
-    static constexpr bool kDirect = BM == 256 || (kI4F && BM == 128);
-    static constexpr int kBlocks = BM >= 128 ? 1 : (BM == 64 || WIDE ? 2 : 3);   // of a CU
+    static constexpr bool kDirect = BM >= 128 || (kI4F && BM == 64);
+    static constexpr int kBlocks = kWaves == 8 ? 1 : (BM >= 64 || WIDE ? 2 : 3);                     // of a CU
 };
 
 template <int F, int BM, bool WIDE, bool GATED>
@@ -846,26 +846,50 @@ int launch_tiles(ExpertsParams p, hipStream_t st)
     hipLaunchKernelGGL((experts_tile_kernel<F, BM, WIDE, GATED>), dim3((uint32_t)units), dim3(T::kWaves * kWave), 0, st, p);
     return (int)hipGetLastError();
 }
+// The form of a call goes by the pairs an expert has on average, all that the host knows of them. Each side of a border measured
+// (us a call; e8: two of 8 experts 14336x4096 a token, e64: eight of 64, gated 2816x2048; the pairs an expert in front):
+//   E4M3  MT 4 / 8     0.5 e64 26.3/27.2, 2 e64 51.2/49.4        MT 8 / 16      2 e64 49.4/50.1, 4 e64 60.0/58.8 e8 86.4/86.7, 4096x14336 76/84
+//         MT 16 / 16   4 e64 58.8/63.6, 6 e8 106/89 e64 64/65    blocks 16 / 32 8 e64 64/67, 16 e64 74/73 e8 102/103
+//         32 / 128     24 e8 105/136, 48 e64 99/101 e8 131/148, 64 e64 116/114, 128 e8 234/189 (64: 235; 256: 222)
+//   BF16  MT 8 / 16    2 e64 100/100, 4 e64 123/116              MT 16 / 16     6 e64 122/131 e8 175/160, 8 e64 128/129
+//         16 / 32      8 e8 152/152, 16 e8 180/169               32 / 64        24 e64 138/144 e8 186/191, 32 e8 193/177
+//         64 / 256     64 e64 166/201 e8 203/229, 128 e64 210/208 e8 275/246, 512 e8 730/577 (128: 601)
+//   INT4  MT 4 / 16    0.25 e64 18.4/18.3 e8 20.2/22.0, 1 e64 24.0/26.9 e8 33.3/32.2, 2 e64 39.8/40.9 e8 62.8/58.0
+//   (zp)  16 / 32      12 e64 59/65, 16 e64 64/72 e8 86/79       32 / 64        32 e64 91/100 e8 127/116, 64 e64 138/130
+//         64 / 128     never (512 e8 816/953); without zero points 256 two of 8 gated 28672x4096 477/436, 512 1508/1307
 template <int F, bool GATED>
 int launch_format(const ExpertsParams& p, hipStream_t st)
 {
-    constexpr bool kI4F = F == kI4 || F == kI4ZP;
     const int64_t R = p.R, E = p.E;
-    const auto go = [&](auto wide) {
-        constexpr bool WIDE = decltype(wide)::value;
-        if (R <= 12 * E && p.x_bytes != 0) {
-            if (R <= E) return launch_stream<F, 4, WIDE, GATED>(p, st);
-            if (R <= 4 * E) return launch_stream<F, 8, WIDE, GATED>(p, st);
-            return launch_stream<F, 16, WIDE, GATED>(p, st);
+    if constexpr (F == kI4 || F == kI4ZP) {
+        const auto few = [&](auto wide) {
+            constexpr bool WIDE = decltype(wide)::value;
+            if (R <= E && p.x_bytes != 0) return launch_stream<F, 4, WIDE, GATED>(p, st);
+            if (R <= 14 * E) return launch_tiles<F, 16, WIDE, GATED>(p, st);
+            return launch_tiles<F, 32, WIDE, GATED>(p, st);
+        };
+        if (R <= 32 * E) return p.G % 2 == 0 && aligned(p.meta, 4) ? few(std::true_type{}) : few(std::false_type{});
+        if (F == kI4ZP || R <= 192 * E) return launch_tiles<F, 64, false, GATED>(p, st);
+        return launch_tiles<F, F == kI4 ? 128 : 64, false, GATED>(p, st);
+    } else if constexpr (F == kFP8) {
+        if (p.x_bytes != 0) {
+            if (R <= E) return launch_stream<F, 4, false, GATED>(p, st);
+            if (R <= 4 * E) return launch_stream<F, 8, false, GATED>(p, st);
+            if (R <= 5 * E) return launch_stream<F, 16, false, GATED>(p, st);
         }
-        if (R <= 32 * E) return launch_tiles<F, 32, WIDE, GATED>(p, st);
-        if (R <= 64 * E) return launch_tiles<F, 64, false, GATED>(p, st);
-        if (kI4F || R <= 160 * E) return launch_tiles<F, 128, false, GATED>(p, st);
-        return launch_tiles<F, kI4F ? 128 : 256, false, GATED>(p, st);
-    };
-    if constexpr (kI4F)
-        if (p.G % 2 == 0 && aligned(p.meta, 4)) return go(std::true_type{});
-    return go(std::false_type{});
+        if (R <= 12 * E) return launch_tiles<F, 16, false, GATED>(p, st);
+        if (R <= 56 * E) return launch_tiles<F, 32, false, GATED>(p, st);
+        return launch_tiles<F, 128, false, GATED>(p, st);
+    } else {
+        if (p.x_bytes != 0) {
+            if (R <= 3 * E) return launch_stream<F, 8, false, GATED>(p, st);
+            if (R <= 6 * E) return launch_stream<F, 16, false, GATED>(p, st);
+        }
+        if (R <= 8 * E) return launch_tiles<F, 16, false, GATED>(p, st);
+        if (R <= 28 * E) return launch_tiles<F, 32, false, GATED>(p, st);
+        if (R <= 112 * E) return launch_tiles<F, 64, false, GATED>(p, st);
+        return launch_tiles<F, 256, false, GATED>(p, st);
+    }
 }
 template <int F>
 int launch_experts_format(const ExpertsParams& p, bool gated, hipStream_t st)
