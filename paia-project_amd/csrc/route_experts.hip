@@ -32,9 +32,10 @@ struct RouteParams {
     const float* bias;                   // [E] or null
     int32_t *ids, *order, *offsets;
     float* weights;
-    int32_t* counts;                     // workspace: [block][E + 1]
+    int32_t* counts;                     // workspace: [block][count_stride], E + 1 of them used
     int64_t stride;                      // elements
     int M, E, k, tokens;                 // tokens: of a block
+    int count_stride;                    // E + 1 rounded up to 4
     int id_bits;
     bool fp32, renormalize;
     float scale;
@@ -52,42 +53,56 @@ __device__ __forceinline__ uint64_t sortable(double v)
     return b >> 63 ? ~b : b | 1ull << 63;
 }
 
+// The sum over the wave in every lane, by the steps of wave_sum.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ double dpp_add(double v)
+{
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROW_MASK, 0xF, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROW_MASK, 0xF, false);
+    return v + __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
 __device__ __forceinline__ double wave_add(double v)
 {
-#pragma unroll
-    for (int i = 1; i < kWave; i *= 2) v += __shfl_xor(v, i, kWave);
-    return v;
+    v = dpp_add<0xB1, 0xF>(v);
+    v = dpp_add<0x4E, 0xF>(v);
+    v = dpp_add<0x124, 0xF>(v);
+    v = dpp_add<0x128, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);
+    v = dpp_add<0x143, 0xC>(v);
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, 63);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), 63);
+    return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
 }
 
-// The largest key of the wave and its lowest index (lane + 64 i); false where all are 0. The key found is set to 0.
+// The largest key of the wave: its lowest index (lane + 64 i), -1 where all keys are 0. The key found is set to 0.
 template <int NE>
-__device__ __forceinline__ bool take_largest(uint32_t (&key)[NE], int* index)
+__device__ __forceinline__ int take_largest(uint32_t (&key)[NE])
 {
     uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < NE; ++i) most = max(most, key[i]);
     most = wave_max_u32(most);
-    if (most == 0) return false;
     int at = -1;
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
+    for (int i = NE - 1; i >= 0; --i) {
         const uint64_t here = __ballot(key[i] == most);
-        if (at < 0 && here != 0) at = 64 * i + __builtin_ctzll(here);
+        if (here != 0) at = 64 * i + __builtin_ctzll(here);
     }
-    *index = at;
+    if (most == 0) at = -1;
 #pragma unroll
     for (int i = 0; i < NE; ++i)
         if (at == 64 * i + lane_id()) key[i] = 0;
-    return true;
+    return at;
 }
 template <int NE>
-__device__ __forceinline__ bool take_largest(uint64_t (&key)[NE], int* index)
+__device__ __forceinline__ int take_largest(uint64_t (&key)[NE])
 {
-    uint32_t high = 0, low = 0;
+    uint32_t high = 0, low = 0;          // open keys are sums above -2^1024: their upper halves are not 0
 #pragma unroll
     for (int i = 0; i < NE; ++i) high = max(high, (uint32_t)(key[i] >> 32));
     high = wave_max_u32(high);
-    if (high == 0) return false;         // open keys are finite sums above -2^1024: their upper halves are not 0
 #pragma unroll
     for (int i = 0; i < NE; ++i)
         if ((uint32_t)(key[i] >> 32) == high) low = max(low, (uint32_t)key[i]);
@@ -95,76 +110,91 @@ __device__ __forceinline__ bool take_largest(uint64_t (&key)[NE], int* index)
     const uint64_t most = (uint64_t)high << 32 | low;
     int at = -1;
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
+    for (int i = NE - 1; i >= 0; --i) {
         const uint64_t here = __ballot(key[i] == most);
-        if (at < 0 && here != 0) at = 64 * i + __builtin_ctzll(here);
+        if (here != 0) at = 64 * i + __builtin_ctzll(here);
     }
-    *index = at;
+    if (high == 0) at = -1;
 #pragma unroll
     for (int i = 0; i < NE; ++i)
         if (at == 64 * i + lane_id()) key[i] = 0;
-    return true;
+    return at;
 }
 
-// The choice of one token by one wave; the lanes j < k hold (id, weight) j afterwards.
-template <int NE, bool SIGMOID>
-__device__ __forceinline__ void choose(const RouteParams& p, int m, int* id, float* weight)
+// The choices of T tokens m, m + step, .. by one wave, whose chains of dependent steps overlap. The lanes j < k write them.
+template <int NE, bool SIGMOID, int T>
+__device__ __forceinline__ void choose(const RouteParams& p, int m, int step)
 {
     const int lane = lane_id();
-    float v[NE];
+    float v[T][NE];
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
-        const int e = lane + 64 * i;
-        v[i] = -__builtin_inff();
-        if (e < p.E) {
-            const int64_t at = m * p.stride + e;
-            v[i] = p.fp32 ? static_cast<const float*>(p.logits)[at] : bf16_to_f32(static_cast<const uint16_t*>(p.logits)[at]);
+    for (int u = 0; u < T; ++u)
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+            const int e = lane + 64 * i;
+            v[u][i] = -__builtin_inff();
+            if (e < p.E) {
+                const int64_t at = (int64_t)(m + u * step) * p.stride + e;
+                v[u][i] = p.fp32 ? static_cast<const float*>(p.logits)[at] : bf16_to_f32(static_cast<const uint16_t*>(p.logits)[at]);
+            }
         }
-    }
     using Key = typename std::conditional<SIGMOID, uint64_t, uint32_t>::type;
-    Key key[NE];
+    Key key[T][NE];
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-        const bool open = v[i] > -__builtin_inff();
-        if constexpr (SIGMOID) {
-            const double b = p.bias != nullptr && lane + 64 * i < p.E ? (double)p.bias[lane + 64 * i] : 0.0;
-            const bool both = open && b > -__builtin_inf();
-            key[i] = both ? sortable(1.0 / (1.0 + exp(-(double)v[i])) + b) : 0;
-        } else {
-            key[i] = open ? sortable(v[i]) : 0;
+        double b = 0.0;
+        if constexpr (SIGMOID)
+            if (p.bias != nullptr && lane + 64 * i < p.E) b = (double)p.bias[lane + 64 * i];
+#pragma unroll
+        for (int u = 0; u < T; ++u) {
+            const bool open = v[u][i] > -__builtin_inff();
+            if constexpr (SIGMOID) {
+                key[u][i] = open && b > -__builtin_inf() ? sortable(1.0 / (1.0 + exp(-(double)v[u][i])) + b) : 0;
+            } else {
+                key[u][i] = open ? sortable(v[u][i]) : 0;
+            }
         }
     }
-    double all = 0.0;
-    float top = 0.0f;
-    bool first = true;
-    *id = -1;
-    float mine = 0.0f;                   // the logit of the lane's expert
-    for (int j = 0; j < p.k; ++j) {
-        int e;
-        if (!take_largest<NE>(key, &e)) break;
-        float logit = 0.0f;
+    int id[T];
+    float top[T], mine[T];               // the largest logit, and that of the lane's expert
 #pragma unroll
-        for (int i = 0; i < NE; ++i)
-            if (e >> 6 == i) logit = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v[i]), e & 63));
-        if (first) top = logit, first = false;
-        if (lane == j) *id = e, mine = logit;
-    }
-    double w = 0.0;
-    if constexpr (SIGMOID) {
-        if (*id >= 0) w = 1.0 / (1.0 + exp(-(double)mine));
-        all = p.renormalize ? wave_add(w) : 1.0;
-    } else {
-        if (*id >= 0) w = exp((double)mine - (double)top);
-        if (p.renormalize) {
-            all = wave_add(w);
-        } else {
+    for (int u = 0; u < T; ++u) id[u] = -1, top[u] = mine[u] = 0.0f;
+    for (int j = 0; j < p.k; ++j) {
+#pragma unroll
+        for (int u = 0; u < T; ++u) {
+            const int e = take_largest<NE>(key[u]);
+            float logit = 0.0f;
 #pragma unroll
             for (int i = 0; i < NE; ++i)
-                if (v[i] > -__builtin_inff()) all += exp((double)v[i] - (double)top);
-            all = wave_add(all);
+                if (e >> 6 == i) logit = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v[u][i]), e & 63));
+            if (j == 0) top[u] = logit;
+            if (lane == j) id[u] = e, mine[u] = logit;
         }
     }
-    *weight = (float)(all > 0.0 || all != all ? w / all * (double)p.scale : 0.0);
+#pragma unroll
+    for (int u = 0; u < T; ++u) {
+        double w = 0.0, all = 1.0;
+        if constexpr (SIGMOID) {
+            if (id[u] >= 0) w = 1.0 / (1.0 + exp(-(double)mine[u]));
+            if (p.renormalize) all = wave_add(w);
+        } else {
+            if (id[u] >= 0) w = exp((double)mine[u] - (double)top[u]);
+            if (p.renormalize) {
+                all = wave_add(w);
+            } else {
+                all = 0.0;
+#pragma unroll
+                for (int i = 0; i < NE; ++i)
+                    if (v[u][i] > -__builtin_inff()) all += exp((double)v[u][i] - (double)top[u]);
+                all = wave_add(all);
+            }
+        }
+        if (lane < p.k) {
+            const int at = (m + u * step) * p.k + lane;
+            p.ids[at] = id[u];
+            p.weights[at] = (float)(all > 0.0 || all != all ? w / all * (double)p.scale : 0.0);
+        }
+    }
 }
 
 __device__ __forceinline__ int inclusive(int v)
@@ -239,15 +269,10 @@ __global__ void __launch_bounds__(kRouteBlock) route_kernel(const RouteParams p)
     const int wave = wave_id(), t = (int)threadIdx.x;
     const int m0 = (int)blockIdx.x * p.tokens, m1 = min(p.M, m0 + p.tokens);
     if constexpr (SELECT) {
-        for (int m = m0 + wave; m < m1; m += kRouteWaves) {
-            int id;
-            float weight;
-            choose<NE, SIGMOID>(p, m, &id, &weight);
-            if (lane_id() < p.k) {
-                p.ids[m * p.k + lane_id()] = id;
-                p.weights[m * p.k + lane_id()] = weight;
-            }
-        }
+        int m = m0 + wave;
+        if constexpr (NE <= 4)
+            for (; m + kRouteWaves < m1; m += 2 * kRouteWaves) choose<NE, SIGMOID, 2>(p, m, kRouteWaves);
+        for (; m < m1; m += kRouteWaves) choose<NE, SIGMOID, 1>(p, m, kRouteWaves);
     }
     for (int e = t; e <= p.E; e += kRouteBlock)
 #pragma unroll
@@ -259,11 +284,12 @@ __global__ void __launch_bounds__(kRouteBlock) route_kernel(const RouteParams p)
     walk<false>(p, s.at[wave], from, to);
     __syncthreads();
     if constexpr (!ONE) {
-        for (int e = t; e <= p.E; e += kRouteBlock) {
+        for (int e = t; e < p.count_stride; e += kRouteBlock) {
             int sum = 0;
+            if (e <= p.E)
 #pragma unroll
-            for (int w = 0; w < kRouteWaves; ++w) sum += s.at[w][e];
-            p.counts[(int64_t)blockIdx.x * (p.E + 1) + e] = sum;
+                for (int w = 0; w < kRouteWaves; ++w) sum += s.at[w][e];
+            p.counts[(int64_t)blockIdx.x * p.count_stride + e] = sum;
         }
     } else {
         int own = 0, total;
@@ -286,44 +312,47 @@ __global__ void __launch_bounds__(kRouteBlock) route_kernel(const RouteParams p)
     }
 }
 
-// The second launch: block b's places follow from all blocks' counts.
+// The second launch: block b's places follow from all blocks' counts, four experts a thread and load; where there are fewer
+// such quads than threads, groups of threads share the blocks.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 __global__ void __launch_bounds__(kRouteBlock) route_order_kernel(const RouteParams p)
 {
     __shared__ SortSpace s;
+    __shared__ i32x4 sum[2][kRouteBlock];            // [before this block, in all][group][quad]
     const int wave = wave_id(), t = (int)threadIdx.x, bins = p.E + 1;
     const int m0 = (int)blockIdx.x * p.tokens, m1 = min(p.M, m0 + p.tokens);
+    const int quads = p.count_stride / 4, groups = kRouteBlock / quads, group = t / quads, quad = t - group * quads;
+    i32x4 before = {0, 0, 0, 0}, all = {0, 0, 0, 0};
+    if (group < groups) {
+        const i32x4* counts = reinterpret_cast<const i32x4*>(p.counts) + quad;
+        const int last = (int)gridDim.x - 1, own = (int)blockIdx.x;
+        constexpr int kAhead = 8;
+        for (int b = group; b <= last; b += kAhead * groups) {
+            i32x4 n[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) n[i] = counts[(int64_t)min(b + i * groups, last) * quads];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                if (b + i * groups <= last) all += n[i];
+                if (b + i * groups < own) before += n[i];
+            }
+        }
+        sum[0][t] = before, sum[1][t] = all;
+    }
     for (int b = t; b < bins; b += kRouteBlock)
 #pragma unroll
         for (int w = 0; w < kRouteWaves; ++w) s.at[w][b] = 0;
-    // counts of expert t before this block, and in all; with few experts several threads share one
-    int width = kWave;
-    while (width < bins) width *= 2;
-    const int groups = max(1, kRouteBlock / width), e = t % width, g = t / width;
-    int before = 0, all = 0, none_before = 0;
-    if (e < bins && g < groups) {
-        for (int b = g; b < (int)gridDim.x; b += groups) {
-            const int n = p.counts[(int64_t)b * bins + e];
-            all += n;
-            before += b < (int)blockIdx.x ? n : 0;
-        }
-    }
-    if (width > kRouteBlock) {           // 1024 experts: the last bin has no thread of its own
-        if (t == 0)
-            for (int b = 0; b < (int)blockIdx.x; ++b) none_before += p.counts[(int64_t)b * bins + p.E];
-    }
-    __shared__ int32_t sum[2][kRouteBlock];
-    sum[0][t] = before, sum[1][t] = all;
     __syncthreads();
     int from, to;
     wave_range(m0 * p.k, m1 * p.k, &from, &to);
     walk<false>(p, s.at[wave], from, to);
-    before = all = 0;
-    if (t < min(width, kRouteBlock))
-        for (int i = 0; i < groups; ++i) before += sum[0][i * width + t], all += sum[1][i * width + t];
-    if (width <= kRouteBlock && t == 0)
-        for (int i = 0; i < groups; ++i) none_before += sum[0][i * width + p.E];
+    const auto total_of = [&](int what, int bin) {
+        int n = 0;
+        for (int g = 0; g < groups; ++g) n += reinterpret_cast<const int32_t*>(sum[what])[g * p.count_stride + bin];
+        return n;
+    };
     int total;
-    const int at = block_scan(t < p.E ? all : 0, s.sums, &total);
+    const int at = block_scan(t < p.E ? total_of(1, t) : 0, s.sums, &total);
     __syncthreads();
     const auto places = [&](int bin, int place) {
 #pragma unroll
@@ -335,11 +364,11 @@ __global__ void __launch_bounds__(kRouteBlock) route_order_kernel(const RoutePar
     };
     if (t < p.E) {
         if (blockIdx.x == 0) p.offsets[t] = at;
-        places(t, at + before);
+        places(t, at + total_of(0, t));
     }
     if (t == 0) {
         if (blockIdx.x == 0) p.offsets[p.E] = total;
-        places(p.E, total + none_before);
+        places(p.E, total + total_of(0, p.E));
     }
     __syncthreads();
     walk<true>(p, s.at[wave], from, to);
@@ -359,7 +388,7 @@ static bool route_sizes(int M, int E, int k)
 static int64_t route_workspace(int M, int E)
 {
     int tokens;
-    return M <= kRouteTokens ? 0 : (int64_t)route_blocks(M, &tokens) * (E + 1) * (int64_t)sizeof(int32_t);
+    return M <= kRouteTokens ? 0 : (int64_t)route_blocks(M, &tokens) * ((E + 4) / 4 * 4) * (int64_t)sizeof(int32_t);
 }
 
 template <bool SIGMOID, bool SELECT, bool ONE>
@@ -378,6 +407,7 @@ static int run_route(RouteParams& p, bool select, bool sigmoid, void* workspace,
     const int64_t need = route_workspace(p.M, p.E);
     if (need > 0 && (workspace == nullptr || !aligned(workspace, 16) || bytes < need)) return -2;
     p.counts = static_cast<int32_t*>(workspace);
+    p.count_stride = (p.E + 4) / 4 * 4;
     p.id_bits = 0;
     while (p.E >> p.id_bits) ++p.id_bits;        // ids 0 .. E
     const int blocks = route_blocks(p.M, &p.tokens);
