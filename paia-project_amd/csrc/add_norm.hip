@@ -12,6 +12,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "gemv_kernel.h"
 #include "paia_gemv.h"
 
@@ -52,8 +54,8 @@ __device__ __forceinline__ u32x4 pack8(const float f[8])
     return u32x4{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
 }
 
-// NV: 16-byte pieces of a row that a thread holds. R32: the residual is fp32.
-template <int NV, bool R32>
+// NV: 16-byte pieces of a row that a thread holds. R32: the residual is fp32. PAIRS: x has pairs.
+template <int NV, bool R32, bool PAIRS>
 __global__ void __launch_bounds__(1024) add_norm_kernel(const AddNormParams p)
 {
     __shared__ float part[2][kNormMaxWaves];
@@ -63,12 +65,25 @@ __global__ void __launch_bounds__(1024) add_norm_kernel(const AddNormParams p)
     const auto load = [&](const uint16_t* row, int c) { return c < p.pieces ? reinterpret_cast<const u32x4*>(row)[c] : none; };
 
     // the loads that nothing has to be known for
-    u32x4 in[NV], gate[NV], post[NV], norm[NV], res[NV][R32 ? 2 : 1];
+    constexpr int kAhead = PAIRS ? 8 / NV : 1;       // rows of x whose loads are on their way together
+    const int rows = PAIRS ? p.pairs : 1;
     const uint16_t* x = p.x + m * p.x_stride;
+    u32x4 in[kAhead][NV], gate[NV], post[NV], norm[NV], res[NV][R32 ? 2 : 1];
+    float w[kAhead];
+    const auto load_rows = [&](int j) {
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+            if (j + a < rows) {
+                w[a] = PAIRS ? p.weights[m * p.pairs + j + a] : 1.0f;
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    in[a][i] = load(x + (j + a) * p.pair_stride, (int)(threadIdx.x + i * blockDim.x));
+            }
+    };
+    load_rows(0);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (int)(threadIdx.x + i * blockDim.x);
-        in[i] = load(x, c);
         res[i][0] = none;
         if constexpr (R32) {
             res[i][1] = none;
@@ -84,38 +99,24 @@ __global__ void __launch_bounds__(1024) add_norm_kernel(const AddNormParams p)
 
     float y[NV][8];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) unpack8(in[i], y[i]);
-    if (p.pairs > 0) {
-        const float* weights = p.weights + m * p.pairs;
-        const float w0 = weights[0];
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int e = 0; e < 8; ++e) y[i][e] = 0.0f;
+    for (int j = 0;;) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[i][e] = w0 != 0.0f ? w0 * y[i][e] : 0.0f;
-        constexpr int kAhead = NV == 1 ? 4 : (NV == 2 ? 2 : 1);
-        for (int j = 1; j < p.pairs; j += kAhead) {
-            u32x4 v[kAhead][NV];
-            float w[kAhead];
+        for (int a = 0; a < kAhead; ++a) {
+            if (j + a >= rows || w[a] == 0.0f) continue;     // a pair of weight 0 adds nothing, whatever its row holds
 #pragma unroll
-            for (int a = 0; a < kAhead; ++a) {
-                const bool in_row = j + a < p.pairs;
-                w[a] = in_row ? weights[j + a] : 0.0f;
+            for (int i = 0; i < NV; ++i) {
+                float f[8];
+                unpack8(in[a][i], f);
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
-                    v[a][i] = in_row ? load(x + (j + a) * p.pair_stride, (int)(threadIdx.x + i * blockDim.x)) : none;
-            }
-#pragma unroll
-            for (int a = 0; a < kAhead; ++a) {
-                if (w[a] == 0.0f) continue;          // a pair of weight 0 adds nothing, whatever its row holds
-#pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    float f[8];
-                    unpack8(v[a][i], f);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[i][e] = __builtin_fmaf(w[a], f[e], y[i][e]);
-                }
+                for (int e = 0; e < 8; ++e) y[i][e] = __builtin_fmaf(w[a], f[e], y[i][e]);
             }
         }
+        j += kAhead;
+        if (j >= rows) break;
+        load_rows(j);
     }
     const auto squares = [&]() {
         float s = 0.0f;
@@ -224,9 +225,14 @@ int paia_add_norm(const void* x, long long x_stride, const void* weights, long l
         p.r = residual_out != nullptr ? static_cast<uint8_t*>(residual_out) + m * residual_out_stride * width : nullptr;
         const dim3 grid((uint32_t)(M - m < rows ? M - m : rows)), block((uint32_t)threads);
         auto go = [&](auto narrow, auto wide) { hipLaunchKernelGGL(residual_fp32 ? wide : narrow, grid, block, 0, st, p); };
-        if (nv == 1) go(add_norm_kernel<1, false>, add_norm_kernel<1, true>);
-        else if (nv == 2) go(add_norm_kernel<2, false>, add_norm_kernel<2, true>);
-        else go(add_norm_kernel<4, false>, add_norm_kernel<4, true>);
+        const auto go_nv = [&](auto n) {
+            constexpr int NV = decltype(n)::value;
+            if (pairs > 0) go(add_norm_kernel<NV, false, true>, add_norm_kernel<NV, true, true>);
+            else go(add_norm_kernel<NV, false, false>, add_norm_kernel<NV, true, false>);
+        };
+        if (nv == 1) go_nv(std::integral_constant<int, 1>{});
+        else if (nv == 2) go_nv(std::integral_constant<int, 2>{});
+        else go_nv(std::integral_constant<int, 4>{});
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return (int)e;
         if (M - m <= rows) break;
     }

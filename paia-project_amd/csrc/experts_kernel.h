@@ -59,18 +59,21 @@ template <int BM>
 struct Chunks {
     int count, rest_at, rest;            // rest: chunks of the pairs without an expert, order[rest_at ..]
     int upto, own;                       // chunks of the experts up to the lane's last, and of the lane's
+    int from, to;                        // where the pairs of the lane's first expert begin, and of its last one end
+    int order;                           // of up to 64 pairs the lane's, loaded beside the offsets
 
     __device__ __forceinline__ int place(const ExpertsParams& p, int e) const { return min(max(p.offsets[min(e, p.E)], 0), p.R); }
     __device__ __forceinline__ explicit Chunks(const ExpertsParams& p)
     {
         const int e0 = lane_id() * p.lane_experts;
+        order = p.order[min(lane_id(), p.R - 1)];
         rest_at = place(p, p.E);
-        int from = place(p, e0);
+        from = place(p, e0);
         own = 0;
-        for (int i = 1; i <= p.lane_experts; ++i) {
-            const int to = place(p, e0 + i);
-            own += (max(to - from, 0) + BM - 1) / BM;
-            from = to;
+        for (int i = 1, begin = from; i <= p.lane_experts; ++i) {
+            to = place(p, e0 + i);
+            own += (max(to - begin, 0) + BM - 1) / BM;
+            begin = to;
         }
         own = min(own, p.most);                  // no more than that in all, unless the offsets are not in order
         upto = wave_inclusive(own);
@@ -84,12 +87,15 @@ struct Chunks {
     __device__ __forceinline__ Expert of(const ExpertsParams& p, int c) const
     {
         const int owner = __builtin_ctzll(__ballot(upto > c)), e0 = lane_id() * p.lane_experts;
-        int e = 0, begin = 0, lo = 0, hi = 0, n = 1, at = upto - own, from = place(p, e0);
-        for (int i = 1; i <= p.lane_experts; ++i) {
-            const int to = place(p, e0 + i), k = (max(to - from, 0) + BM - 1) / BM;
-            if (c >= at && c < at + k) e = e0 + i - 1, begin = at, lo = from, hi = to, n = k;
-            at += k;
-            from = to;
+        int e = lane_id(), begin = upto - own, lo = from, hi = to, n = own;
+        if (p.lane_experts > 1) {
+            int at = begin, a = from;
+            for (int i = 1; i <= p.lane_experts; ++i) {
+                const int b = place(p, e0 + i), k = (max(b - a, 0) + BM - 1) / BM;
+                if (c >= at && c < at + k) e = e0 + i - 1, begin = at, lo = a, hi = b, n = k;
+                at += k;
+                a = b;
+            }
         }
         return {__builtin_amdgcn_readlane(e, owner), __builtin_amdgcn_readlane(lo, owner), __builtin_amdgcn_readlane(hi, owner),
                 __builtin_amdgcn_readlane(begin, owner), __builtin_amdgcn_readlane(n, owner)};
@@ -253,7 +259,7 @@ struct StreamSpace {
 // `groups` items from column group `group0` on, of the pairs order[first .. first + held) of one expert.
 template <int F, int MT, bool WIDE, bool SPLIT, bool GATED>
 __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace<F, MT, WIDE>& space, int expert, int first, int held,
-                                             int group0, int groups)
+                                             int order, int group0, int groups)
 {
     using T = StreamShape<F, MT, WIDE>;
     constexpr bool I4 = T::kI4F;
@@ -318,6 +324,7 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
         if (++it == n) it = 0, ++ig, aim();
     };
 
+    const auto pair_of = [&](int i) { return p.R <= kWave ? __shfl(order, first + i, kWave) : p.order[first + i]; };
     // the weights' first loads go ahead of the chain order -> rows of x
     Stage buf[D];
     int pg[D], pt[D];
@@ -330,13 +337,13 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
     }
 #pragma unroll
     for (int i = 0; i < XL; ++i) {
-        const int r = i * XR + lane / XP, pair = p.order[first + min(r, held - 1)];
+        const int r = i * XR + lane / XP, pair = pair_of(min(r, held - 1));
         const bool in = r < held && (uint32_t)pair < (uint32_t)p.R;
         xo[i] = in ? p.by_pairs.of((uint32_t)pair) * (uint32_t)(p.x_stride * 2) + (uint32_t)(lane % XP) * 16u : kOOB;
     }
 #pragma unroll
     for (int d = 0; d < D; ++d) issue_x(buf[d], pg[d], pt[d]);
-    const int pairs = ln < held ? p.order[first + ln] : -1;
+    const int last = pair_of(min(ln, held - 1)), pairs = ln < held ? last : -1;
 
     const auto w_at = [](int row, int piece) {
         return RB == 128 ? row * 128 + ((piece ^ (row & 7)) << 4) : row * 64 + ((piece ^ (row >> 1 & 3)) << 4);
@@ -501,7 +508,8 @@ experts_stream_kernel(const ExpertsParams p)
         const int groups = min(p.tiles - group0, (int)(end - item));
         const auto x = chunks.of(p, chunk);
         const int first = x.lo + (chunk - x.begin) * MT;
-        stream_items<F, MT, WIDE, SPLIT, GATED>(p, space, x.expert, first, min(MT, x.hi - first), group0, groups);
+        stream_items<F, MT, WIDE, SPLIT, GATED>(p, space, x.expert, first, min(MT, x.hi - first), chunks.order,
+                                                 group0, groups);
         item += (uint32_t)groups;
     }
     const uint32_t rest = (uint32_t)chunks.rest, rest_end = (uint32_t)((uint64_t)rest * (block + 1) / blocks);

@@ -25,7 +25,7 @@ namespace paia {
 constexpr int kRouteBlock = 1024, kRouteWaves = kRouteBlock / kWave;
 constexpr int kRouteExperts = 1024;      // experts at most: a thread each in the scan
 constexpr int kRouteBlocks = 256;        // blocks at most that share the tokens
-constexpr int kRouteTokens = 32;         // tokens up to which one block does all of it
+constexpr int kRouteTokens = 32;          // tokens up to which one block does all of it (61 at a block: 11.8 us, in two launches 9.1)
 
 struct RouteParams {
     const void* logits;                  // bf16 or fp32 [M][E]
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kRouteBlock) route_order_kernel(const RoutePar
     __shared__ i32x4 sum[2][kRouteBlock];            // [before this block, in all][group][quad]
     const int wave = wave_id(), t = (int)threadIdx.x, bins = p.E + 1;
     const int m0 = (int)blockIdx.x * p.tokens, m1 = min(p.M, m0 + p.tokens);
-    const int quads = p.count_stride / 4, groups = kRouteBlock / quads, group = t / quads, quad = t - group * quads;
+    const int quads = p.count_stride / 4, groups = min(kRouteBlock / quads, 16), group = t / quads, quad = t - group * quads;
     i32x4 before = {0, 0, 0, 0}, all = {0, 0, 0, 0};
     if (group < groups) {
         const i32x4* counts = reinterpret_cast<const i32x4*>(p.counts) + quad;

@@ -1,6 +1,7 @@
 // torch.library custom ops of the feed-forward half of a layer with experts: residual and norms, each token's experts, the
 // experts' products. Same conduct as torch_ops.cpp: tensors are checked here, the C ABI is called on torch's current HIP
 // stream of the operands' device, Meta kernels give shapes.
+#include <ATen/hip/EmptyTensor.h>
 #include <torch/library.h>
 
 #include <cstdint>
@@ -14,6 +15,13 @@
 namespace {
 
 using OptTensor = std::optional<at::Tensor>;
+
+// A new tensor beside `like`; on a GPU straight from its allocator (through the dispatcher each took as long as a launch).
+at::Tensor new_like(const at::Tensor& like, at::IntArrayRef sizes, at::ScalarType type)
+{
+    if (like.is_cuda()) return at::Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
+    return at::empty(sizes, like.options().dtype(type));
+}
 
 bool is_bf16(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16; }
 
@@ -64,9 +72,8 @@ void add_norm_out(const at::Tensor& x, const OptTensor& residual, const at::Tens
 std::tuple<at::Tensor, at::Tensor> add_norm_new(const at::Tensor& x, const OptTensor& residual)
 {
     TORCH_CHECK(x.dim() == 2 || x.dim() == 3, "x must be [M, D] or [M, pairs, D]");
-    const auto options = x.options().dtype(at::kBFloat16);
-    return {at::empty({x.size(0), x.size(-1)}, options),
-            at::empty({x.size(0), x.size(-1)}, residual.has_value() ? options.dtype(residual->scalar_type()) : options)};
+    return {new_like(x, {x.size(0), x.size(-1)}, at::kBFloat16),
+            new_like(x, {x.size(0), x.size(-1)}, residual.has_value() ? residual->scalar_type() : at::kBFloat16)};
 }
 std::tuple<at::Tensor, at::Tensor> add_norm(const at::Tensor& x, const OptTensor& residual, const at::Tensor& norm,
                                             const OptTensor& post_norm, const OptTensor& gate, const OptTensor& weights,
@@ -95,9 +102,8 @@ Route route_new(const at::Tensor& logits, int64_t k)
 {
     TORCH_CHECK(logits.dim() == 2 && k > 0, "logits must be [M, experts], k positive");
     const int64_t M = logits.size(0);
-    const auto whole = logits.options().dtype(at::kInt);
-    return {at::empty({M, k}, whole), at::empty({M, k}, whole.dtype(at::kFloat)), at::empty({M * k}, whole),
-            at::empty({logits.size(1) + 1}, whole)};
+    return {new_like(logits, {M, k}, at::kInt), new_like(logits, {M, k}, at::kFloat), new_like(logits, {M * k}, at::kInt),
+            new_like(logits, {logits.size(1) + 1}, at::kInt)};
 }
 Route route_experts(const at::Tensor& logits, int64_t k, const OptTensor& bias, c10::string_view scoring, bool renormalize,
                     double scale, const OptTensor& workspace)
@@ -126,7 +132,7 @@ using Order = std::tuple<at::Tensor, at::Tensor>;
 Order order_new(const at::Tensor& ids, int64_t experts)
 {
     TORCH_CHECK(ids.dim() == 2 && experts > 0, "ids must be [M, k], experts positive");
-    return {at::empty({ids.numel()}, ids.options()), at::empty({experts + 1}, ids.options())};
+    return {new_like(ids, {ids.numel()}, at::kInt), new_like(ids, {experts + 1}, at::kInt)};
 }
 Order expert_order(const at::Tensor& ids, int64_t experts, const OptTensor& workspace)
 {
@@ -184,7 +190,7 @@ void check_meta(const at::Tensor& W, const at::Tensor& t, at::ScalarType type, i
 at::Tensor experts_new(const at::Tensor& W, const at::Tensor& x, const at::Tensor& order, bool gated)
 {
     TORCH_CHECK(W.dim() == 3 && order.dim() == 1, "W must be [experts, N, ...], order one row of pairs");
-    return at::empty({order.size(0), gated ? W.size(1) / 2 : W.size(1)}, x.options());
+    return new_like(x, {order.size(0), gated ? W.size(1) / 2 : W.size(1)}, at::kBFloat16);
 }
 
 void experts_bf16_out(const at::Tensor& W, const at::Tensor& x, const at::Tensor& order, const at::Tensor& offsets,

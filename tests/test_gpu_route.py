@@ -26,7 +26,7 @@ def random_logits(M, E, dtype, seed=0, dev="cuda"):
 
 
 @pytest.mark.parametrize("E", [1, 2, 7, 60, 64, 65, 128, 160, 256, 257, 512, 1000, 1023, 1024])
-@pytest.mark.parametrize("M", [1, 31, 32, 33, 200])
+@pytest.mark.parametrize("M", [1, 31, 32, 33, 64, 200])
 def test_sizes(cuda, E, M):
     for dtype in (torch.bfloat16, torch.float32):
         for k in {1, min(E, 4), min(E, 8), min(E, 64)}:
