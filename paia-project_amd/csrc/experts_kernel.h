@@ -538,7 +538,7 @@ struct TileShape {
     static constexpr int kTM = BM / 16 / kM, kTN = kTiles / kN;
     static constexpr int kWBytes = kTiles * kTileRows * kRowBytes, kXBytes = BM * kXRowBytes;
     static constexpr bool kDirect = BM >= 128 || (kI4F && BM == 64);
-    static constexpr int kBlocks = kWaves == 8 ? 1 : (BM >= 64 || WIDE ? 2 : 3);                     // of a CU
+    static constexpr int kBlocks = kWaves == 8 ? 1 : (BM >= 64 || (WIDE && BM == 32) ? 2 : 3);                     // of a CU
 };
 
 template <int F, int BM, bool WIDE, bool GATED>
@@ -655,7 +655,7 @@ experts_tile_kernel(const ExpertsParams p)
                     for (int i = 0; i < TM; ++i) g[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const u32x4 b = i4_frag(w[t][j], f);
+                        const u32x4 b = T::kDirect ? i4_frag(w[t][j], f) : i4_frag_paired(w[t][j], f);     // x as it was stored
 #pragma unroll
                         for (int i = 0; i < TM; ++i) g[i] = mfma_16x16x32(a[i][j], b, g[i]);
                     }
@@ -751,7 +751,7 @@ experts_tile_kernel(const ExpertsParams p)
             if (XW == WAVES || wave < XW) {
 #pragma unroll
                 for (int i = 0; i < XL; ++i)
-                    *reinterpret_cast<u32x4*>(slot + T::kWBytes + (wave * XL + i) * 1024 + lane * 16) = B.x[i];
+                    *reinterpret_cast<u32x4*>(slot + T::kWBytes + (wave * XL + i) * 1024 + lane * 16) = I4 ? i4_pair_x(B.x[i]) : B.x[i];
             }
         };
         Stage buf[2];
