@@ -206,6 +206,29 @@ template <int F> __device__ __forceinline__ float i4_factor(uint32_t m) { return
 template <int F> __device__ __forceinline__ float i4_scale(uint32_t m) { return __uint_as_float(F == kI4 ? m : m & 0xFFFF0000u); }
 template <int F> __device__ __forceinline__ float i4_zero(uint32_t m) { return F == kI4 ? 8.0f : (float)(m & 0xFFu); }
 
+// Where piece (16 bytes, 8 columns) `piece` of a row of x of XB bytes lies among the row's, before the XOR with the row's lowest
+// three bits. A 16-byte read takes 16 lanes at a time: eight rows (all values of those bits) of one column group of the
+// matrix instruction and eight of the next one, which differ in the lowest bit of the lane group lh. Their places are
+// disjoint where that bit decides the half of the 256 bytes of a cycle's banks: through the row's parity for rows of 128
+// bytes (the place's bit 0), as bit 3 of the place for longer ones. E4M3 by plain pieces had 118 conflict cycles for 182 of reads.
+template <int F, int XB>
+__device__ __forceinline__ int x_place(int piece)
+{
+    if constexpr (F == kBF16) return piece;                                    // 4 j + lh
+    else if constexpr (F == kFP8 && XB == 128) return piece >> 1 | (piece & 1) << 2;      // 2 lh + j
+    else if constexpr (F == kFP8) return (piece >> 1 & 1) << 3 | (piece >> 3 & 1) << 2 | (piece >> 2 & 1) << 1 | (piece & 1);
+    else return (piece & ~12) | (piece >> 2 & 1) << 3 | (piece >> 3 & 1) << 2;            // 16 h + 4 lh + j
+}
+// The piece at a place.
+template <int F, int XB>
+__device__ __forceinline__ int x_piece_at(int at)
+{
+    if constexpr (F == kBF16) return at;
+    else if constexpr (F == kFP8 && XB == 128) return (at & 3) << 1 | at >> 2;
+    else if constexpr (F == kFP8) return (at >> 3 & 1) << 1 | (at >> 2 & 1) << 3 | (at >> 1 & 1) << 2 | (at & 1);
+    else return (at & ~12) | (at >> 2 & 1) << 3 | (at >> 3 & 1) << 2;
+}
+
 // The sum of a row and column on its way out: scale, bias.
 template <int F>
 __device__ __forceinline__ float finish(float v, float scale, float bias)
@@ -348,7 +371,9 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
     const auto w_at = [](int row, int piece) {
         return RB == 128 ? row * 128 + ((piece ^ (row & 7)) << 4) : row * 64 + ((piece ^ (row >> 1 & 3)) << 4);
     };
-    const auto x_at = [](int row, int piece) { return T::kWBytes + row * T::kXRowBytes + ((piece ^ (row & 7)) << 4); };
+    const auto x_at = [](int row, int piece) {
+        return T::kWBytes + row * T::kXRowBytes + ((x_place<F, T::kXRowBytes>(piece) ^ (row & 7)) << 4);
+    };
     const uint32_t one2 = (uint32_t)__builtin_amdgcn_readfirstlane((int)kI4Ones);
     const u32x4 ones = {one2, one2, one2, one2};
     f32x4 acc[P];
@@ -591,7 +616,7 @@ experts_tile_kernel(const ExpertsParams p)
     const auto w_from = [&](int s, int i) { return wp[i] + (wo[i] + min((uint32_t)s * RB + wpiece, p.row_bytes - 16u)); };
     const auto x_from = [&](int s, int i) {
         const int r = (wave * XL + i) * XR + xr;
-        return xp[i] + min((uint32_t)s * XB + (uint32_t)((lane % XP) ^ (r & 7)) * 16u, (uint32_t)p.K * 2u - 16u);
+        return xp[i] + min((uint32_t)s * XB + (uint32_t)x_piece_at<F, XB>((lane % XP) ^ (r & 7)) * 16u, (uint32_t)p.K * 2u - 16u);
     };
     // INT4: scales (WIDE: two) and zero points of a stage's groups for the wave's columns, as they are stored
     struct Meta {
@@ -621,7 +646,7 @@ experts_tile_kernel(const ExpertsParams p)
     const auto get_x = [&](const uint8_t* slot, int i, int j) {
         const int r = (wm * TM + i) * 16 + ln;
         const int piece = F == kBF16 ? 4 * j + lh : (F == kFP8 ? 8 * (j >> 1) + 2 * lh + (j & 1) : 16 * (j >> 2) + 4 * lh + (j & 3));
-        return *reinterpret_cast<const u32x4*>(slot + T::kWBytes + r * XB + ((piece ^ (r & 7)) << 4));
+        return *reinterpret_cast<const u32x4*>(slot + T::kWBytes + r * XB + ((x_place<F, XB>(piece) ^ (r & 7)) << 4));
     };
     const auto get_w = [&](const uint8_t* slot, int t, int i) {
         const int r = (wn * TN + t) * 16 + ln;
@@ -701,7 +726,7 @@ experts_tile_kernel(const ExpertsParams p)
         }
         for (int e = (int)threadIdx.x; e < BM * XP; e += WAVES * kWave) {
             const int r = e / XP, at = e % XP;
-            if ((at ^ (r & 7)) * 8 >= left) *reinterpret_cast<u32x4*>(slot + T::kWBytes + r * XB + at * 16) = none;
+            if (x_piece_at<F, XB>(at ^ (r & 7)) * 8 >= left) *reinterpret_cast<u32x4*>(slot + T::kWBytes + r * XB + at * 16) = none;
         }
         __syncthreads();
     };
