@@ -280,7 +280,7 @@ struct StreamSpace {
 };
 
 // `groups` items from column group `group0` on, of the pairs order[first .. first + held) of one expert.
-template <int F, int MT, bool WIDE, bool SPLIT, bool GATED>
+template <int F, int MT, bool WIDE, bool GATED>
 __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace<F, MT, WIDE>& space, int expert, int first, int held,
                                              int order, int group0, int groups)
 {
@@ -293,8 +293,8 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
     constexpr int kOuts = GATED ? P / 2 : P, kOutCols = kOuts * kTileRows;
 
     const int lane = lane_id(), wave = wave_id(), ln = lane & 15, lh = lane >> 4;
-    const int stages = (p.K + C - 1) / C, k0 = SPLIT ? stages * wave / WAVES : 0;     // this wave's stages; where there are
-    const int mine_n = SPLIT ? stages * (wave + 1) / WAVES - k0 : stages;            // none, one that reads nothing
+    const int stages = (p.K + C - 1) / C, k0 = stages * wave / WAVES;          // this wave's stages; where there are none,
+    const int mine_n = stages * (wave + 1) / WAVES - k0;                       // one that reads nothing
     const int n = max(1, mine_n);
     const int columns = mine_n > 0 ? p.K : 0;
     const int64_t row0 = (int64_t)expert * p.N;
@@ -302,7 +302,10 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
 
     struct Stage {
         u32x4 w[P][L], x[XL];
-        uint32_t m[I4 ? P : 1], z[F == kI4ZP ? P : 1];       // INT4: scales (WIDE: two), zero points
+        // INT4: scales (WIDE: two) and zero points. Lane group lh loads those of the lh-th of four stages, in the first of the
+        // four that the wave has: a stage of its own at a time brought the lines of 32 rows four times, most of them from
+        // beyond the L2 by then (us, 4 tokens, two of 8 experts 4096x14336: 28.9 -> 26.7).
+        uint32_t m[I4 ? P : 1], z[F == kI4ZP ? P : 1];
     };
     // the stream's next stage: stage `it` of item `ig`, the descriptors of whose tiles end with their rows
     int ig = 0, it = 0;
@@ -329,10 +332,12 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
 #pragma unroll
             for (int i = 0; i < L; ++i) B.w[t][i] = ld16<2>(rw[t], wo + wstep * (uint32_t)i, 0u);
             if constexpr (I4) {
-                const uint32_t lm = kb * H < p.G ? (uint32_t)ln * (uint32_t)p.G * 2u : kOOB;
-                if constexpr (WIDE) B.m[t] = __builtin_amdgcn_raw_buffer_load_b32(rm[t], lm, (uint32_t)kb * 4u, 0);
-                else B.m[t] = ld_u16(rm[t], lm, (uint32_t)kb * 2u);
-                if constexpr (F == kI4ZP) B.z[t] = ld_u8(rz[t], (uint32_t)ln * p.zbytes, (uint32_t)(kb * H >> 1));
+                const int at = ((kb & ~3) + lh) * H;
+                const bool in = (it == 0 || (kb & 3) == 0) && left > 0 && at < p.G;
+                const uint32_t lm = in ? ((uint32_t)ln * (uint32_t)p.G + (uint32_t)at) * 2u : kOOB;
+                if constexpr (WIDE) B.m[t] = __builtin_amdgcn_raw_buffer_load_b32(rm[t], lm, 0u, 0);
+                else B.m[t] = ld_u16(rm[t], lm, 0u);
+                if constexpr (F == kI4ZP) B.z[t] = ld_u8(rz[t], in ? (uint32_t)ln * p.zbytes + (uint32_t)(at >> 1) : kOOB, 0u);
             }
         }
     };
@@ -379,7 +384,8 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
     f32x4 acc[P];
 #pragma unroll
     for (int t = 0; t < P; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const auto consume = [&](const Stage& B, int kb) __attribute__((always_inline)) {
+    uint32_t four_m[I4 ? P : 1], four_z[F == kI4ZP ? P : 1];      // the four stages' scales and zero points
+    const auto consume = [&](const Stage& B, int kb, bool first_of_item) __attribute__((always_inline)) {
         wave_lds_order();
 #pragma unroll
         for (int i = 0; i < XL; ++i)
@@ -393,6 +399,18 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
         const auto x_piece = [&](int piece) { return *reinterpret_cast<const u32x4*>(mine + x_at(ln & (T::kXRows - 1), piece)); };
         const auto w_piece = [&](int t, int piece) { return *reinterpret_cast<const u32x4*>(mine + t * kTileRows * RB + w_at(ln, piece)); };
         if constexpr (I4) {
+            uint32_t scales2[P], zeros2[P];
+            const bool fresh = first_of_item || (kb & 3) == 0;
+            const int from = (kb & 3) * 16 + ln;
+#pragma unroll
+            for (int t = 0; t < P; ++t) {
+                four_m[t] = fresh ? B.m[t] : four_m[t];
+                scales2[t] = (uint32_t)__shfl((int)four_m[t], from, kWave);
+                if constexpr (F == kI4ZP) {
+                    four_z[t] = fresh ? B.z[t] : four_z[t];
+                    zeros2[t] = (uint32_t)__shfl((int)four_z[t], from, kWave);
+                }
+            }
 #pragma unroll
             for (int h = 0; h < H; ++h) {
                 u32x4 a[4];
@@ -404,8 +422,8 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
 #pragma unroll
                 for (int t = 0; t < P; ++t) {
                     const u32x4 w = w_piece(t, 4 * h + lh);
-                    const uint32_t zero = F == kI4ZP ? B.z[F == kI4ZP ? t : 0] >> (4 * ((kb * H + h) & 1)) & 15u : 8u;
-                    const uint32_t m = i4_word_of<F>(WIDE && h ? B.m[t] >> 16 : B.m[t] & 0xFFFFu, zero);
+                    const uint32_t zero = F == kI4ZP ? zeros2[t] >> (4 * ((kb * H + h) & 1)) & 15u : 8u;
+                    const uint32_t m = i4_word_of<F>(WIDE && h ? scales2[t] >> 16 : scales2[t] & 0xFFFFu, zero);
                     const float f = i4_factor<F>(m), sc = i4_scale<F>(m), z = i4_zero<F>(m);
                     f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -466,33 +484,23 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
         }
     };
     const auto finish_item = [&](int g) __attribute__((always_inline)) {
-        if constexpr (SPLIT) {
-            __syncthreads();                         // the last item's sums have been read
+        __syncthreads();                         // the last item's sums have been read
 #pragma unroll
-            for (int t = 0; t < P; ++t) space.part[wave][t][lane] = acc[t];
-            __syncthreads();
-            const int from = g * kOuts % WAVES;      // the items' finishes go round the waves
+        for (int t = 0; t < P; ++t) space.part[wave][t][lane] = acc[t];
+        __syncthreads();
+        const int from = g * kOuts % WAVES;      // the items' finishes go round the waves
 #pragma unroll
-            for (int q = 0; q < kOuts; ++q) {
-                if (wave != (from + q) % WAVES) continue;
-                f32x4 sum[GATED ? 2 : 1];
+        for (int q = 0; q < kOuts; ++q) {
+            if (wave != (from + q) % WAVES) continue;
+            f32x4 sum[GATED ? 2 : 1];
 #pragma unroll
-                for (int h = 0; h < (GATED ? 2 : 1); ++h) {
-                    const int t = GATED ? 2 * q + h : q;
-                    sum[h] = space.part[0][t][lane];
+            for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+                const int t = GATED ? 2 * q + h : q;
+                sum[h] = space.part[0][t][lane];
 #pragma unroll
-                    for (int w = 1; w < WAVES; ++w) sum[h] += space.part[w][t][lane];
-                }
-                put(g, q, sum);
+                for (int w = 1; w < WAVES; ++w) sum[h] += space.part[w][t][lane];
             }
-        } else {
-#pragma unroll
-            for (int q = 0; q < kOuts; ++q) {
-                f32x4 sum[GATED ? 2 : 1];
-#pragma unroll
-                for (int h = 0; h < (GATED ? 2 : 1); ++h) sum[h] = acc[GATED ? 2 * q + h : q];
-                put(g, q, sum);
-            }
+            put(g, q, sum);
         }
 #pragma unroll
         for (int t = 0; t < P; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -505,7 +513,7 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
     for (int f = 0; f < all; f += D) {               // past the last stage the sums take zeros
 #pragma unroll
         for (int d = 0; d < D; ++d) {
-            consume(buf[d], k0 + t);
+            consume(buf[d], k0 + t, t == 0);
             const int ng = ig, nt = it;
             issue_w(buf[d]);
             issue_x(buf[d], ng, nt);
@@ -516,24 +524,22 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
     }
 }
 
-template <int F, int MT, bool WIDE, bool SPLIT, bool GATED>
+template <int F, int MT, bool WIDE, bool GATED>
 __global__ void __launch_bounds__((StreamShape<F, MT, WIDE>::kWaves * kWave),
                                   (StreamShape<F, MT, WIDE>::kBlocks * StreamShape<F, MT, WIDE>::kWaves / 4))
 experts_stream_kernel(const ExpertsParams p)
 {
     __shared__ StreamSpace<F, MT, WIDE> space;
     const Chunks<MT> chunks(p);
-    // the takers of items: blocks, or their waves, each for itself. Below 2^32: at most kMostItems, and fewer than 2^12 takers
-    constexpr uint32_t kEach = SPLIT ? 1 : StreamShape<F, MT, WIDE>::kWaves;
+    // below 2^32: at most kMostItems, and fewer than 2^10 blocks
     const uint32_t block = (uint32_t)xcd_contiguous((int)blockIdx.x, (int)gridDim.x), blocks = gridDim.x;
-    const uint32_t taker = block * kEach + (SPLIT ? 0u : (uint32_t)wave_id()), takers = blocks * kEach;
-    const uint32_t items = (uint32_t)(chunks.count * p.tiles), end = items * (taker + 1) / takers;
-    for (uint32_t item = items * taker / takers; item < end;) {
+    const uint32_t items = (uint32_t)(chunks.count * p.tiles), end = items * (block + 1) / blocks;
+    for (uint32_t item = items * block / blocks; item < end;) {
         const int chunk = (int)p.by_tiles.of(item), group0 = (int)item - chunk * p.tiles;
         const int groups = min(p.tiles - group0, (int)(end - item));
         const auto x = chunks.of(p, chunk);
         const int first = x.lo + (chunk - x.begin) * MT;
-        stream_items<F, MT, WIDE, SPLIT, GATED>(p, space, x.expert, first, min(MT, x.hi - first), chunks.order,
+        stream_items<F, MT, WIDE, GATED>(p, space, x.expert, first, min(MT, x.hi - first), chunks.order,
                                                  group0, groups);
         item += (uint32_t)groups;
     }
@@ -618,14 +624,17 @@ experts_tile_kernel(const ExpertsParams p)
         const int r = (wave * XL + i) * XR + xr;
         return xp[i] + min((uint32_t)s * XB + (uint32_t)x_piece_at<F, XB>((lane % XP) ^ (r & 7)) * 16u, (uint32_t)p.K * 2u - 16u);
     };
-    // INT4: scales (WIDE: two) and zero points of a stage's groups for the wave's columns, as they are stored
+    // INT4: scales (WIDE: two) and zero points of four stages' groups for the wave's columns, as they are stored; lane group
+    // lh has those of the lh-th. Loaded a round of four ahead: a stage at a time, one ahead, they came too late and each line of
+    // theirs several times (us, zero points, two of 8 experts 4096x13696, 16 tokens 81.6 -> 62.7; 64 of 8 2048x1408, 32 tokens 27.6
+    // -> 25.2; large calls -3 to 2%).
     struct Meta {
         uint32_t s[I4 ? TN : 1], z[F == kI4ZP ? TN : 1];
     };
     Meta meta, ahead;
     const auto meta_load = [&](Meta& m, int s) __attribute__((always_inline)) {
         if constexpr (I4) {
-            s = min(s, stages - 1);
+            s = min(s + lh, stages - 1);
 #pragma unroll
             for (int t = 0; t < TN; ++t) {
                 const int i = wn * TN + t, rows = max(1, tile_rows<GATED, T::kTiles>(p, u.tile, i));
@@ -652,8 +661,14 @@ experts_tile_kernel(const ExpertsParams p)
         const int r = (wn * TN + t) * 16 + ln;
         return *reinterpret_cast<const u32x4*>(slot + r * RB + (((4 * i + lh) ^ w_piece(r)) << 4));
     };
-    const auto use = [&](const uint8_t* slot, int s) __attribute__((always_inline)) {
+    const auto use = [&](const uint8_t* slot, int s, int of_four) __attribute__((always_inline)) {
         if constexpr (I4) {
+            Meta now;
+#pragma unroll
+            for (int t = 0; t < TN; ++t) {
+                now.s[t] = (uint32_t)__shfl((int)meta.s[t], of_four * 16 + ln, kWave);
+                if constexpr (F == kI4ZP) now.z[t] = (uint32_t)__shfl((int)meta.z[t], of_four * 16 + ln, kWave);
+            }
 #pragma unroll
             for (int h = 0; h < H; ++h) {
                 u32x4 a[TM][4], w[TN];
@@ -672,8 +687,8 @@ experts_tile_kernel(const ExpertsParams p)
                 }
 #pragma unroll
                 for (int t = 0; t < TN; ++t) {
-                    const uint32_t zero = F == kI4ZP ? meta.z[F == kI4ZP ? t : 0] >> (4 * ((s * H + h) & 1)) & 15u : 8u;
-                    const uint32_t m = i4_word_of<F>(WIDE && h ? meta.s[t] >> 16 : meta.s[t] & 0xFFFFu, zero);
+                    const uint32_t zero = F == kI4ZP ? now.z[F == kI4ZP ? t : 0] >> (4 * ((s * H + h) & 1)) & 15u : 8u;
+                    const uint32_t m = i4_word_of<F>(WIDE && h ? now.s[t] >> 16 : now.s[t] & 0xFFFFu, zero);
                     const float f = i4_factor<F>(m), sc = i4_scale<F>(m), z = i4_zero<F>(m);
                     f32x4 g[TM];
 #pragma unroll
@@ -730,14 +745,15 @@ experts_tile_kernel(const ExpertsParams p)
         }
         __syncthreads();
     };
-    const auto multiply = [&](uint8_t* slot, int s, bool last) __attribute__((always_inline)) {
+    constexpr int kRound = I4 ? 4 : 2;               // stages of a round of the loops
+    const auto multiply = [&](uint8_t* slot, int s, int d, bool last) __attribute__((always_inline)) {
         if (!I4 && last && p.K - s * C < C) clear_past(slot, p.K - s * C);
         if (busy) {
             if constexpr (F == kFP8) __builtin_amdgcn_s_setprio(1);      // ahead of the blocks that fetch: 1674 -> 1646 us at 4001
-            use(slot, s);                                                // tokens; INT4 1% slower so, BF16 even
+            use(slot, s, d);                                             // tokens; INT4 1% slower so, BF16 even
             if constexpr (F == kFP8) __builtin_amdgcn_s_setprio(0);
         }
-        if constexpr (I4) meta = ahead;
+        if (I4 && d == kRound - 1) meta = ahead;
     };
 
     meta_load(meta, 0);
@@ -750,18 +766,18 @@ experts_tile_kernel(const ExpertsParams p)
 #pragma unroll
             for (int i = 0; i < XL; ++i) lds_copy16(slot + T::kWBytes + (wave * XL + i) * 1024, x_from(s, i));
         };
-        const auto stage = [&](uint8_t* mine, uint8_t* next, int s) __attribute__((always_inline)) {
+        const auto stage = [&](uint8_t* mine, uint8_t* next, int s, int d) __attribute__((always_inline)) {
             wait_loads<0>();
             __syncthreads();                         // this stage has arrived, the other place is read
             issue(next, s + 1);
-            meta_load(ahead, s + 1);
-            multiply(mine, s, true);
+            if (d == 0) meta_load(ahead, s + kRound);
+            multiply(mine, s, d, true);
         };
         issue(slot0, 0);
-        for (int s = 0; s < stages; s += 2) {
-            stage(slot0, slot1, s);
-            if (s + 1 < stages) stage(slot1, slot0, s + 1);
-        }
+        for (int s = 0; s < stages; s += kRound)
+#pragma unroll
+            for (int d = 0; d < kRound; ++d)
+                if (s + d < stages) stage(d & 1 ? slot1 : slot0, d & 1 ? slot0 : slot1, s + d, d);
     } else {
         struct Stage {
             u32x4 w[WL], x[XL];
@@ -788,25 +804,25 @@ experts_tile_kernel(const ExpertsParams p)
         load(buf[1], 1);
         int s = 0;
         wait_loads<0>();                             // the loop's waits then count its own order of loads alone
-        for (; s + 2 < stages; s += 2) {
+        for (; s + kRound < stages; s += kRound) {
 #pragma unroll
-            for (int d = 0; d < 2; ++d) {
-                uint8_t* slot = d ? slot1 : slot0;
-                store(slot, buf[d]);                 // what was there is read: two stages ago, before the last barrier
-                meta_load(ahead, s + d + 1);         // ahead of the loads that stay on their way
-                load(buf[d], s + d + 2);
+            for (int d = 0; d < kRound; ++d) {
+                uint8_t* slot = d & 1 ? slot1 : slot0;
+                store(slot, buf[d & 1]);             // what was there is read: two stages ago, before the last barrier
+                if (d == 0) meta_load(ahead, s + kRound);      // ahead of the loads that stay on their way
+                load(buf[d & 1], s + d + 2);
                 block_lds_order();
-                multiply(slot, s + d, false);
+                multiply(slot, s + d, d, false);
             }
         }
 #pragma unroll
-        for (int d = 0; d < 2; ++d)
+        for (int d = 0; d < kRound; ++d)
             if (s + d < stages) {
-                uint8_t* slot = d ? slot1 : slot0;
-                store(slot, buf[d]);
-                meta_load(ahead, s + d + 1);
+                uint8_t* slot = d & 1 ? slot1 : slot0;
+                store(slot, buf[d & 1]);
+                if (kRound > 2 && s + d + 2 < stages) load(buf[d & 1], s + d + 2);
                 block_lds_order();
-                multiply(slot, s + d, true);
+                multiply(slot, s + d, d, true);
             }
     }
     if (!busy) return;
@@ -861,7 +877,7 @@ inline int64_t plan_experts(ExpertsParams& p, int BM, int unit_cols)
     p.most = (int)most;
     return most * p.tiles <= kMostBlocks ? most * p.tiles : -2;
 }
-constexpr int kMostItems = 1 << 20, kSplitBelow = 4;
+constexpr int kMostItems = 1 << 20;
 template <int F, int MT, bool WIDE, bool GATED>
 int launch_stream(ExpertsParams p, hipStream_t st)
 {
@@ -870,8 +886,7 @@ int launch_stream(ExpertsParams p, hipStream_t st)
     if (items < 0 || items > kMostItems) return -2;
     const int64_t resident = T::kBlocks * device_facts().cus;
     const dim3 grid((uint32_t)(items < resident ? items : resident)), block(T::kWaves * kWave);
-    if (items < kSplitBelow * resident) hipLaunchKernelGGL((experts_stream_kernel<F, MT, WIDE, true, GATED>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((experts_stream_kernel<F, MT, WIDE, false, GATED>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((experts_stream_kernel<F, MT, WIDE, GATED>), grid, block, 0, st, p);
     return (int)hipGetLastError();
 }
 template <int F, int BM, bool WIDE, bool GATED>
