@@ -877,17 +877,24 @@ inline int64_t plan_experts(ExpertsParams& p, int BM, int unit_cols)
     p.most = (int)most;
     return most * p.tiles <= kMostBlocks ? most * p.tiles : -2;
 }
-constexpr int kMostItems = 1 << 20;
+// A share's bounds, items * (block + 1), lie below 2^32.
+constexpr int64_t kMostItems = 1 << 20;
 template <int F, int MT, bool WIDE, bool GATED>
 int launch_stream(ExpertsParams p, hipStream_t st)
 {
     using T = StreamShape<F, MT, WIDE>;
     const int64_t items = plan_experts(p, MT, (GATED ? T::kTiles / 2 : T::kTiles) * kTileRows);
-    if (items < 0 || items > kMostItems) return -2;
     const int64_t resident = T::kBlocks * device_facts().cus;
-    const dim3 grid((uint32_t)(items < resident ? items : resident)), block(T::kWaves * kWave);
-    hipLaunchKernelGGL((experts_stream_kernel<F, MT, WIDE, GATED>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((experts_stream_kernel<F, MT, WIDE, GATED>), dim3((uint32_t)(items < resident ? items : resident)),
+                       dim3(T::kWaves * kWave), 0, st, p);
     return (int)hipGetLastError();
+}
+// Where reading weights bounds a call: its items of two tiles fit the shares, a descriptor spans x, and a wave's quarter of a row
+// is two lines or more.
+inline bool streams(const ExpertsParams& p, int64_t pairs)
+{
+    const int64_t R = p.R, bins = R < p.E + 1 ? R : p.E + 1, chunks = (R + bins * 3) / 4;     // MT >= 4
+    return R <= pairs && p.x_bytes != 0 && p.row_bytes >= 1024 && chunks * ((p.cols + 15) / 16) <= kMostItems;
 }
 template <int F, int BM, bool WIDE, bool GATED>
 int launch_tiles(ExpertsParams p, hipStream_t st)
@@ -899,16 +906,19 @@ int launch_tiles(ExpertsParams p, hipStream_t st)
     return (int)hipGetLastError();
 }
 // The form of a call goes by the pairs an expert has on average, all that the host knows of them. Each side of a border measured
-// (us a call; e8: two of 8 experts 14336x4096 a token, e64: eight of 64, gated 2816x2048; the pairs an expert in front):
-//   E4M3  MT 4 / 8     0.5 e64 26.3/27.2, 2 e64 51.2/49.4        MT 8 / 16      2 e64 49.4/50.1, 4 e64 60.0/58.8 e8 86.4/86.7, 4096x14336 76/84
-//         MT 16 / 16   4 e64 58.8/63.6, 6 e8 106/89 e64 64/65    blocks 16 / 32 8 e64 64/67, 16 e64 74/73 e8 102/103
-//         32 / 128     24 e8 105/136, 48 e64 99/101 e8 131/148, 64 e64 116/114, 128 e8 234/189 (64: 235; 256: 222)
-//   BF16  MT 8 / 16    2 e64 100/100, 4 e64 123/116              MT 16 / 16     6 e64 122/131 e8 175/160, 8 e64 128/129
-//         16 / 32      8 e8 152/152, 16 e8 180/169               32 / 64        24 e64 138/144 e8 186/191, 32 e8 193/177
-//         64 / 256     64 e64 166/201 e8 203/229, 128 e64 210/208 e8 275/246, 512 e8 730/577 (128: 601)
-//   INT4  MT 4 / 16    0.25 e64 18.4/18.3 e8 20.2/22.0, 1 e64 24.0/26.9 e8 33.3/32.2, 2 e64 39.8/40.9 e8 62.8/58.0
-//   (zp)  16 / 32      12 e64 59/65, 16 e64 64/72 e8 86/79       32 / 64        32 e64 91/100 e8 127/116, 64 e64 138/130
-//         64 / 128     never (512 e8 816/953); without zero points 256 two of 8 gated 28672x4096 477/436, 512 1508/1307
+// (us a call; e8: two of 8 experts gated 28672x4096 a token, d8: 4096x14336, e64: eight of 64, gated 2816x2048, d64: 2048x1408; the
+// pairs an expert in front):
+//   E4M3  MT 4 / 16    0.5 e8 56.6/58.9 e64 26.2/28.0, 0.75 e8 75.0/72.6 e64 32.5/34.4, 1 e64 34.9/32.2
+//         MT 16 / 16   4 e8 143/162 d8 75/80 e64 59/64, 6 e8 177/161 d8 111/109 e64 66/65 d64 38/35
+//         16 / 32      8 e64 64/67, 16 e64 74/73                 32 / 128   48 e64 99/101, 64 e64 116/114
+//   BF16  MT 8 / 16    0.25 e64 18.2/18.7, 1 e64 56.9/56.7       MT 16 / 16 4 e8 285/309 e64 107/126, 6 e8 328/320, 8 e64 124/129
+//         16 / 32      8 e64 128/131, 16 e64 151/139             32 / 64    24 e64 138/144
+//         64 / 256     64 e64 166/201, 128 e64 210/208
+//   INT4  MT 4 / 16    0.5 e8 39.1/40.8 d8 24.0/56, 1 e8 47.7/53.0 e64 25.6/24.5, 2 e8 91.6/85.6 d8 50.9/54.4 e64 38.0/37.9
+//         16 / 32      20 e8 157/164 d8 88/114 d64 (zp) 38/39, 25 e64 73/72 d64 (zp) 43.6/39.5, 28 e8 189/191
+//         32 / 64      50 e8 240/259 e64 111/109, 64 e8 289/268 e64 128/123
+//         64 / 128     with zero points never; without 256 e8 477/436, 512 1508/1307
+//   rows of 512 bytes, MT 4 / 16: E4M3 1024x512 11.4/7.9; of 704: INT4 d64 14.4/9.0; of 1024: INT4 e64 above; BF16 1024x512 12.4/11.8
 template <int F, bool GATED>
 int launch_format(const ExpertsParams& p, hipStream_t st)
 {
@@ -916,27 +926,22 @@ int launch_format(const ExpertsParams& p, hipStream_t st)
     if constexpr (F == kI4 || F == kI4ZP) {
         const auto few = [&](auto wide) {
             constexpr bool WIDE = decltype(wide)::value;
-            if (R <= E && p.x_bytes != 0) return launch_stream<F, 4, WIDE, GATED>(p, st);
-            if (R <= 14 * E) return launch_tiles<F, 16, WIDE, GATED>(p, st);
+            if (streams(p, E)) return launch_stream<F, 4, WIDE, GATED>(p, st);
+            if (R <= 22 * E) return launch_tiles<F, 16, WIDE, GATED>(p, st);
             return launch_tiles<F, 32, WIDE, GATED>(p, st);
         };
-        if (R <= 32 * E) return p.G % 2 == 0 && aligned(p.meta, 4) ? few(std::true_type{}) : few(std::false_type{});
+        if (R <= 56 * E) return p.G % 2 == 0 && aligned(p.meta, 4) ? few(std::true_type{}) : few(std::false_type{});
         if (F == kI4ZP || R <= 192 * E) return launch_tiles<F, 64, false, GATED>(p, st);
         return launch_tiles<F, F == kI4 ? 128 : 64, false, GATED>(p, st);
     } else if constexpr (F == kFP8) {
-        if (p.x_bytes != 0) {
-            if (R <= E) return launch_stream<F, 4, false, GATED>(p, st);
-            if (R <= 4 * E) return launch_stream<F, 8, false, GATED>(p, st);
-            if (R <= 5 * E) return launch_stream<F, 16, false, GATED>(p, st);
-        }
+        if (streams(p, E * 3 / 4)) return launch_stream<F, 4, false, GATED>(p, st);
+        if (streams(p, 5 * E)) return launch_stream<F, 16, false, GATED>(p, st);
         if (R <= 12 * E) return launch_tiles<F, 16, false, GATED>(p, st);
         if (R <= 56 * E) return launch_tiles<F, 32, false, GATED>(p, st);
         return launch_tiles<F, 128, false, GATED>(p, st);
     } else {
-        if (p.x_bytes != 0) {
-            if (R <= 3 * E) return launch_stream<F, 8, false, GATED>(p, st);
-            if (R <= 6 * E) return launch_stream<F, 16, false, GATED>(p, st);
-        }
+        if (streams(p, E)) return launch_stream<F, 8, false, GATED>(p, st);
+        if (streams(p, 6 * E)) return launch_stream<F, 16, false, GATED>(p, st);
         if (R <= 8 * E) return launch_tiles<F, 16, false, GATED>(p, st);
         if (R <= 28 * E) return launch_tiles<F, 32, false, GATED>(p, st);
         if (R <= 112 * E) return launch_tiles<F, 64, false, GATED>(p, st);

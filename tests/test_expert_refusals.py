@@ -77,7 +77,8 @@ def test_experts_refusals(gemv_lib, fmt):
            dict(rows=3), dict(rows=-1), dict(order=None), dict(order=A + 2), dict(off=None), dict(off=A + 2), dict(out=None),
            dict(out=A + 1), dict(os=63), dict(os=-64), dict(E=0), dict(E=1025), dict(N=0), dict(K=0), dict(K=(1 << 25) + 128),
            dict(K={"bf16": 260, "fp8": 264}.get(fmt, 192)), dict(pairs=-1), dict(pairs=1 << 26, rows=1 << 26), dict(gated=2),
-           dict(gated=1, N=63), dict(N=2 ** 31 - 1, os=2 ** 31 - 1, pairs=1 << 20)]
+           dict(gated=1, N=63), dict(N=2 ** 31 - 1, os=2 ** 31 - 1, pairs=1 << 20),
+           dict(N=1 << 20, os=1 << 20, pairs=1 << 22, rows=1 << 22)]
     bad += [dict(meta=None), dict(meta=A + (2 if fmt == "fp8" else 1))] if fmt != "bf16" else []
     bad += [dict(zeros=None)] if fmt == "int4_zp" else []
     bad += [dict(bias=A + 1)] if fmt != "int4" else []

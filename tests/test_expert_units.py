@@ -92,3 +92,54 @@ def test_any_offsets_stay_within_the_pairs(seed):
             e, first, held, tile = u
             assert 0 <= e <= E and 0 <= tile < tiles, (offsets, u)
             assert 0 < held <= BM and 0 <= first and first + held <= R, (offsets, u)
+
+
+def shares(chunks, tiles, cus):
+    """What the blocks of the form for few rows take: runs of items (chunk, first tile, tiles), as the kernel cuts them."""
+    items = chunks * tiles
+    blocks = min(items, 3 * cus)
+    assert items * (blocks + 1) < 2 ** 32
+    for b in range(blocks):
+        block = b % 8 * (blocks // 8) + min(b % 8, blocks % 8) + b // 8
+        item, end = items * block // blocks, items * (block + 1) // blocks
+        while item < end:
+            chunk = item // tiles
+            at = item - chunk * tiles
+            n = min(tiles - at, end - item)
+            yield chunk, at, n
+            item += n
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_shares_cover_every_item_once(seed):
+    rng = random.Random(seed)
+    chunks, tiles, cus = rng.choice([1, 2, 7, 40, 300]), rng.choice([1, 3, 88, 896]), rng.choice([4, 80, 256])
+    seen = set()
+    for chunk, at, n in shares(chunks, tiles, cus):
+        assert chunk < chunks and n > 0 and at + n <= tiles
+        for i in range(at, at + n):
+            assert (chunk, i) not in seen
+            seen.add((chunk, i))
+    assert len(seen) == chunks * tiles
+
+
+def test_the_largest_share_bounds_fit():
+    assert 2 ** 20 * (3 * 256 + 1) < 2 ** 32
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_waves_share_stages(seed):
+    """The four waves' stages of a row: in order, all of them, and the scales of four stages at a time are there when first used."""
+    rng = random.Random(seed)
+    stages = rng.randint(1, 200)
+    at = 0
+    for wave in range(4):
+        k0, k1 = stages * wave // 4, stages * (wave + 1) // 4
+        assert k0 == at
+        at = k1
+        have = None
+        for kb in range(k0, k1):
+            if kb == k0 or kb % 4 == 0:
+                have = kb & ~3
+            assert have <= kb < have + 4
+    assert at == stages

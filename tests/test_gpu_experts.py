@@ -1,6 +1,6 @@
 """ops.experts_bf16/fp8/int4/int4_zp and GemvLib's against the definition in 64 bits; tolerances as expert_util.experts64 derives
-them. Row counts are chosen so that every form of the kernels runs: few rows an expert (up to 4, 8, 16 a block), and blocks of
-32, 64, 128 and 256."""
+them. Row counts are chosen so that every form of the kernels runs: blocks of 16, 32, 64, 128 and 256 rows, and, where rows of
+weights have 1024 bytes or more (DEEP), few rows an expert (up to 4, 8, 16 a block) whose K the waves of a block share."""
 import pytest
 import torch
 
@@ -12,6 +12,9 @@ from paia_gemv import load_lib, ops
 pytestmark = pytest.mark.gpu
 
 CALL = {"bf16": ops.experts_bf16, "fp8": ops.experts_fp8, "int4": ops.experts_int4, "int4zp": ops.experts_int4_zp}
+
+
+DEEP = {"bf16": 512, "fp8": 1024, "int4": 2048, "int4zp": 2048}
 
 
 def ids_of(counts, M, k, seed=0):
@@ -61,10 +64,48 @@ def test_row_counts(cuda, fmt, counts):
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("N", [1, 2, 15, 16, 17, 31, 33, 255, 256, 257, 511, 514])
 def test_columns(cuda, fmt, N):
-    for counts in ([2, 1], [40, 30], [200, 150]):
-        case(fmt, counts, N, 256, bias=True, seed=N)
+    for counts, K in (([2, 1], 256), ([40, 30], 256), ([200, 150], 256), ([1, 1, 0], DEEP[fmt]), ([2, 5], DEEP[fmt])):
+        case(fmt, counts, N, K, bias=True, seed=N)
         if N % 2 == 0:
-            case(fmt, counts, N, 256, gated=True, bias=True, seed=N)
+            case(fmt, counts, N, K, gated=True, bias=True, seed=N)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tail", [0, 1, 2, 5, 9, 16])
+def test_few_rows_share_k(cuda, fmt, tail):
+    """Waves with and without whole stages, INT4 of odd and even numbers of groups, from one pair to 16 of an expert."""
+    K = DEEP[fmt] + tail * STEP[fmt]
+    for i, counts in enumerate(([1], [0, 4], [1, 0, 2, 0, 0, 1, 0, 0], [3, 1, 0, 5, 2, 0, 1], [9, 0, 0, 16, 1, 0, 8, 2], [5, 17, 1, 0])):
+        case(fmt, counts, 70, K, k=1 + i % 3, gated=i % 2 == 0, bias=True, shared=True, bare=i % 4, seed=tail + i)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_more_items_than_blocks(cuda, fmt):
+    """Shares of several items, of several experts, of which some end within an expert."""
+    case(fmt, [1, 2, 1, 0, 1, 2, 0, 1], 8000, DEEP[fmt], bias=True)
+    case(fmt, [2] * 7, 4100, DEEP[fmt], gated=True)
+    case(fmt, [1, 0, 1, 1] * 25, 514, DEEP[fmt], gated=True, bare=9)
+
+
+@pytest.mark.parametrize("fmt", ["int4", "int4zp"])
+def test_infinite_scales(cuda, fmt):
+    """A group whose scale is infinite, all of its values one above the zero point: infinite outputs, from whichever wave and whether
+    the others have stages or none."""
+    for K in (256, 1024, 2048, 2048 + 128, 4096):
+        for counts in ([1, 1], [20, 3], [60, 50]):
+            W, _ = make_experts(fmt, 2, 40, K)
+            W = [w.clone() for w in W]
+            ids = ids_of(counts, sum(counts), 1)
+            order, offsets = order64(ids, 2)
+            x = torch.rand(sum(counts), K, generator=torch.Generator().manual_seed(5)).bfloat16() + 0.5
+            codes, group = W[0].view(torch.uint8), K // 128 - 1
+            codes[:, 7, group * 64:group * 64 + 64] = 0x99
+            W[1][:, 7, group] = float("inf")
+            if fmt == "int4zp":
+                W[2][:, 7, group // 2] = 0x88
+            note(f"experts infinite scales {fmt} {K} {counts}")
+            got = run(fmt, W, None, x, order, offsets, cuda).cpu()
+            assert (got[:, 7] == float("inf")).all() and got[:, [i for i in range(40) if i != 7]].isfinite().all()
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -91,6 +132,8 @@ def test_shared_rows_and_bare_pairs(cuda, fmt, k):
     """A token's pairs share its row of x; pairs without an expert give zeros, all of them too."""
     for counts, bare in (([3, 0, 2, 4], 5), ([100, 60, 0, 90], 70), ([0, 0, 0, 0], 21), ([400, 300, 2], 11), ([0, 0, 0, 9], 0)):
         case(fmt, counts, 66, 256, k=k, shared=True, bare=bare, gated=True, seed=k)
+    for counts, bare in (([0, 0, 0, 0], 3), ([0, 1, 0, 0], 2)):
+        case(fmt, counts, 66, DEEP[fmt], k=k, shared=True, bare=bare, gated=True, seed=k)
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -100,6 +143,7 @@ def test_many_experts(cuda, fmt, E):
     counts = torch.randint(0, 4, (E,), generator=g)
     counts[torch.randint(0, E, (3,), generator=g)] = 37
     case(fmt, counts.tolist(), 18, 128, bare=6, seed=E)
+    case(fmt, torch.randint(0, 2, (E,), generator=g).tolist(), 18, DEEP[fmt], bare=6, seed=E)
 
 
 def poison(fmt, W, e):
@@ -113,10 +157,10 @@ def poison(fmt, W, e):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("rows", [2, 20, 50, 140, 300])
-def test_not_finite_values_stay_where_they_are(cuda, fmt, rows):
+@pytest.mark.parametrize("rows,deep", [(2, False), (20, False), (50, False), (140, False), (300, False), (2, True), (7, True)])
+def test_not_finite_values_stay_where_they_are(cuda, fmt, rows, deep):
     """Experts of NaN that nobody chose beside the ones in use, rows of NaN and infinities in x: the others keep their bits."""
-    K = 3 * STEP[fmt] + (0 if "int4" in fmt else 64)
+    K = 3 * STEP[fmt] + (0 if "int4" in fmt else 64) + deep * DEEP[fmt]
     counts = [0, rows, 0, rows, 0]
     ids = ids_of(counts, 2 * rows, 1)
     order, offsets = order64(ids, 5)
@@ -134,9 +178,9 @@ def test_not_finite_values_stay_where_they_are(cuda, fmt, rows):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("rows", [3, 30, 300])
-def test_strided_rows_and_what_lies_between(cuda, fmt, rows):
-    K, N = 256, 37
+@pytest.mark.parametrize("rows,deep", [(3, False), (30, False), (300, False), (1, True), (3, True)])
+def test_strided_rows_and_what_lies_between(cuda, fmt, rows, deep):
+    K, N = DEEP[fmt] if deep else 256, 37
     ids = ids_of([rows, rows], 2 * rows, 1)
     order, offsets = order64(ids, 2)
     W, b = make_experts(fmt, 2, N, K, bias=True)
@@ -175,11 +219,12 @@ def test_weights_beyond_32_bits(cuda, fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-def test_orders_that_are_not_in_order(cuda, fmt):
+@pytest.mark.parametrize("E,K", [(3, 128), (40, 2048)])
+def test_orders_that_are_not_in_order(cuda, fmt, E, K):
     """Offsets and pairs outside their ranges are not followed: what is right beside them is right, nothing else is written."""
-    W, _ = make_experts(fmt, 3, 33, 128)
-    x = torch.randn(40, 128, generator=torch.Generator().manual_seed(3)).bfloat16()
-    order, offsets = order64(ids_of([13, 13, 14], 40, 1), 3)
+    W, _ = make_experts(fmt, E, 33, K)
+    x = torch.randn(40, K, generator=torch.Generator().manual_seed(3)).bfloat16()
+    order, offsets = order64(ids_of([13, 13, 14] if E == 3 else [1] * 40, 40, 1), E)
     want = run(fmt, W, None, x, order, offsets, cuda)
     bad = order.clone()
     bad[5], bad[20], bad[39] = -1, 40, 2 ** 31 - 1
@@ -191,17 +236,18 @@ def test_orders_that_are_not_in_order(cuda, fmt):
     assert torch.equal(bits(out[keep]), bits(want[keep])) and (out[lost] == 7.0).all()
     for off in ([0, 1000, -5, 40], [40, 13, 26, 0], [-2 ** 31, 2 ** 31 - 1, 0, 2 ** 31 - 1]):
         note(f"experts bad offsets {fmt} {off}")
-        run(fmt, W, None, x, order, torch.tensor(off, dtype=torch.int32), cuda, out=out)
+        run(fmt, W, None, x, order, torch.tensor(off + off[-1:] * (E - 3), dtype=torch.int32), cuda, out=out)
     torch.cuda.synchronize()
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("M", [6, 90])
-def test_graph_follows_the_order(cuda, fmt, M):
+@pytest.mark.parametrize("M,deep", [(6, False), (90, False), (2, True), (6, True)])
+def test_graph_follows_the_order(cuda, fmt, M, deep):
     """One captured call replayed over other choices, eager work between the replays; every replay equals the eager call."""
-    W, _ = make_experts(fmt, 4, 130, 256)
+    K = DEEP[fmt] if deep else 256
+    W, _ = make_experts(fmt, 4, 130, K)
     d = [w.to(cuda) for w in W]
-    x = torch.randn(M, 256, generator=torch.Generator().manual_seed(3)).bfloat16().to(cuda)
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(3)).bfloat16().to(cuda)
     order, offsets = (t.to(cuda) for t in order64(ids_of([M // 2] * 4, M, 2), 4))
     call = lambda: CALL[fmt](*d, x, order, offsets, gated=True)  # noqa: E731
     call()
@@ -209,7 +255,7 @@ def test_graph_follows_the_order(cuda, fmt, M):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         out = call()
-    for counts in ([2 * M, 0, 0, 0], [0, 0, 0, 0], [1, M, 2, M - 3], [M // 2] * 4):
+    for counts in ([2 * M, 0, 0, 0], [0, 0, 0, 0], [1, M, 0, M - 1], [M // 2] * 4):
         o, f = order64(ids_of(counts, M, 2, seed=counts[0]), 4)
         order.copy_(o), offsets.copy_(f)
         junk = torch.randn(1 << 20, device=cuda).mul_(2.0)
@@ -223,10 +269,11 @@ def test_graph_follows_the_order(cuda, fmt, M):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-def test_c_abi_and_another_stream(cuda, fmt):
-    W, b = make_experts(fmt, 3, 64, 256, bias=fmt != "int4")
-    x = torch.randn(10, 256, generator=torch.Generator().manual_seed(3)).bfloat16()
-    order, offsets = order64(ids_of([7, 8, 4], 10, 2), 3)
+@pytest.mark.parametrize("E,K", [(3, 256), (20, 2048)])
+def test_c_abi_and_another_stream(cuda, fmt, E, K):
+    W, b = make_experts(fmt, E, 64, K, bias=fmt != "int4")
+    x = torch.randn(10, K, generator=torch.Generator().manual_seed(3)).bfloat16()
+    order, offsets = order64(ids_of([7, 8, 4] if E == 3 else [1] * 19, 10, 2), E)
     want = run(fmt, W, b, x, order, offsets, cuda)
     d, o, f = [w.to(cuda) for w in W], order.to(cuda), offsets.to(cuda)
     bd = None if b is None else b.to(cuda)
@@ -237,9 +284,41 @@ def test_c_abi_and_another_stream(cuda, fmt):
         xd = (x.to(cuda).float() * 2.0).bfloat16().div_(2.0)
         call = {"bf16": lib.experts_bf16, "fp8": lib.experts_fp8, "int4": lib.experts_int4, "int4zp": lib.experts_int4_zp}[fmt]
         more = {} if fmt == "int4" else {"bias_ptr": bd.data_ptr()}
-        call(*[w.data_ptr() for w in d], xd.data_ptr(), 10, o.data_ptr(), f.data_ptr(), out.data_ptr(), 3, 64, 256, 20, **more)
+        call(*[w.data_ptr() for w in d], xd.data_ptr(), 10, o.data_ptr(), f.data_ptr(), out.data_ptr(), E, 64, K, 20, **more)
     st.synchronize()
     assert torch.equal(bits(out), bits(want))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_rows_of_x_beyond_2_gib(cuda, fmt):
+    """Few rows that no 32-bit byte offset spans."""
+    K = DEEP[fmt]
+    W, _ = make_experts(fmt, 4, 50, K)
+    x = torch.randn(2, K, generator=torch.Generator().manual_seed(3)).bfloat16()
+    order, offsets = order64(torch.tensor([[3], [1]], dtype=torch.int32), 4)
+    far = torch.empty(2 ** 30 + K + 8, dtype=torch.bfloat16, device=cuda).as_strided((2, K), (2 ** 30 + 8, 1))
+    far.copy_(x)
+    note(f"experts far rows {fmt}")
+    out = CALL[fmt](*[w.to(cuda) for w in W], far, order.to(cuda), offsets.to(cuda))
+    check(out, fmt, W, None, x, order, offsets, False)
+
+
+def test_more_columns_than_shares(cuda):
+    """One expert of 16 GiB, either side of the most columns that few rows take item by item."""
+    N, K = 2 ** 24 + 64, 512
+    W = torch.zeros(1, N, K, dtype=torch.bfloat16, device=cuda)
+    x = torch.randn(1, K, generator=torch.Generator().manual_seed(3)).bfloat16()
+    order, offsets = torch.zeros(1, dtype=torch.int32), torch.tensor([0, 1], dtype=torch.int32)
+    for n in (N - 65, N):
+        some = torch.cat([torch.arange(50), torch.arange(n // 2 - 30, n // 2 + 30), torch.arange(n - 50, n)])
+        w = torch.randn(1, len(some), K, generator=torch.Generator().manual_seed(n)).bfloat16()
+        W[:, some.to(cuda)] = w.to(cuda)
+        note(f"experts columns {n}")
+        out = ops.experts_bf16(W[:, :n], x.to(cuda), order.to(cuda), offsets.to(cuda))
+        check(out[:, some.to(cuda)], "bf16", (w,), None, x, order, offsets, False)
+        some_zero = out.float().count_nonzero()
+        assert some_zero <= len(some)
+        W[:, some.to(cuda)] = 0
 
 
 def test_int32_and_uint8_views(cuda):
