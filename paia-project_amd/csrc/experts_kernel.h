@@ -202,6 +202,16 @@ __device__ __forceinline__ uint32_t i4_word_of(uint32_t scale, uint32_t zero)
     if constexpr (F == kI4) return __float_as_uint(up);
     return fabsf(up) > kF32Max ? i4zp_word_big(s, zero) : i4zp_word(up, zero);
 }
+// The words of a stage's H groups, the stage's number as odd as `stage`, from scales (two where H is 2) and zero points as stored.
+template <int F, int H>
+__device__ __forceinline__ void i4_words_of(uint32_t scales, uint32_t zeros, int stage, uint32_t (&word)[H])
+{
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        const uint32_t zero = F == kI4ZP ? zeros >> (4 * ((stage * H + h) & 1)) & 15u : 8u;
+        word[h] = i4_word_of<F>(h ? scales >> 16 : scales & 0xFFFFu, zero);
+    }
+}
 template <int F> __device__ __forceinline__ float i4_factor(uint32_t m) { return __uint_as_float(F == kI4 ? kI4Exp << 23 : (m & 0xFF00u) << 15); }
 template <int F> __device__ __forceinline__ float i4_scale(uint32_t m) { return __uint_as_float(F == kI4 ? m : m & 0xFFFF0000u); }
 template <int F> __device__ __forceinline__ float i4_zero(uint32_t m) { return F == kI4 ? 8.0f : (float)(m & 0xFFu); }
@@ -384,7 +394,7 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
     f32x4 acc[P];
 #pragma unroll
     for (int t = 0; t < P; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    uint32_t four_m[I4 ? P : 1], four_z[F == kI4ZP ? P : 1];      // the four stages' scales and zero points
+    uint32_t four[I4 ? P : 1][H];                    // the lane group's words of the four stages
     const auto consume = [&](const Stage& B, int kb, bool first_of_item) __attribute__((always_inline)) {
         wave_lds_order();
 #pragma unroll
@@ -399,18 +409,10 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
         const auto x_piece = [&](int piece) { return *reinterpret_cast<const u32x4*>(mine + x_at(ln & (T::kXRows - 1), piece)); };
         const auto w_piece = [&](int t, int piece) { return *reinterpret_cast<const u32x4*>(mine + t * kTileRows * RB + w_at(ln, piece)); };
         if constexpr (I4) {
-            uint32_t scales2[P], zeros2[P];
-            const bool fresh = first_of_item || (kb & 3) == 0;
-            const int from = (kb & 3) * 16 + ln;
+            if (first_of_item || (kb & 3) == 0)
 #pragma unroll
-            for (int t = 0; t < P; ++t) {
-                four_m[t] = fresh ? B.m[t] : four_m[t];
-                scales2[t] = (uint32_t)__shfl((int)four_m[t], from, kWave);
-                if constexpr (F == kI4ZP) {
-                    four_z[t] = fresh ? B.z[t] : four_z[t];
-                    zeros2[t] = (uint32_t)__shfl((int)four_z[t], from, kWave);
-                }
-            }
+                for (int t = 0; t < P; ++t) i4_words_of<F, H>(B.m[t], F == kI4ZP ? B.z[F == kI4ZP ? t : 0] : 0u, lh, four[t]);
+            const int from = (kb & 3) * 16 + ln;
 #pragma unroll
             for (int h = 0; h < H; ++h) {
                 u32x4 a[4];
@@ -422,8 +424,7 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
 #pragma unroll
                 for (int t = 0; t < P; ++t) {
                     const u32x4 w = w_piece(t, 4 * h + lh);
-                    const uint32_t zero = F == kI4ZP ? zeros2[t] >> (4 * ((kb * H + h) & 1)) & 15u : 8u;
-                    const uint32_t m = i4_word_of<F>(WIDE && h ? scales2[t] >> 16 : scales2[t] & 0xFFFFu, zero);
+                    const uint32_t m = (uint32_t)__shfl((int)four[t][h], from, kWave);
                     const float f = i4_factor<F>(m), sc = i4_scale<F>(m), z = i4_zero<F>(m);
                     f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -631,7 +632,12 @@ experts_tile_kernel(const ExpertsParams p)
     struct Meta {
         uint32_t s[I4 ? TN : 1], z[F == kI4ZP ? TN : 1];
     };
-    Meta meta, ahead;
+    Meta ahead;
+    // The lane group's words of the four stages; where there are no zero points scales as stored, cheaper to make words of again
+    // and again than to keep and hand on two of them (us, 200 tokens, four of 60 experts 1003x3584: 34.0, 36.9 as words; with
+    // zero points, words 39.7, as stored 41.0).
+    constexpr int kWords = F == kI4ZP ? H : 1;
+    uint32_t four[I4 ? TN : 1][kWords];
     const auto meta_load = [&](Meta& m, int s) __attribute__((always_inline)) {
         if constexpr (I4) {
             s = min(s + lh, stages - 1);
@@ -647,6 +653,14 @@ experts_tile_kernel(const ExpertsParams p)
             }
         }
     };
+    const auto take_meta = [&]() __attribute__((always_inline)) {
+        if constexpr (I4)
+#pragma unroll
+            for (int t = 0; t < TN; ++t) {
+                if constexpr (F == kI4ZP) i4_words_of<F, H>(ahead.s[t], ahead.z[t], lh, four[t]);
+                else four[t][0] = ahead.s[t];
+            }
+    };
     f32x4 acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
@@ -661,14 +675,8 @@ experts_tile_kernel(const ExpertsParams p)
         const int r = (wn * TN + t) * 16 + ln;
         return *reinterpret_cast<const u32x4*>(slot + r * RB + (((4 * i + lh) ^ w_piece(r)) << 4));
     };
-    const auto use = [&](const uint8_t* slot, int s, int of_four) __attribute__((always_inline)) {
+    const auto use = [&](const uint8_t* slot, int of_four) __attribute__((always_inline)) {
         if constexpr (I4) {
-            Meta now;
-#pragma unroll
-            for (int t = 0; t < TN; ++t) {
-                now.s[t] = (uint32_t)__shfl((int)meta.s[t], of_four * 16 + ln, kWave);
-                if constexpr (F == kI4ZP) now.z[t] = (uint32_t)__shfl((int)meta.z[t], of_four * 16 + ln, kWave);
-            }
 #pragma unroll
             for (int h = 0; h < H; ++h) {
                 u32x4 a[TM][4], w[TN];
@@ -687,8 +695,8 @@ experts_tile_kernel(const ExpertsParams p)
                 }
 #pragma unroll
                 for (int t = 0; t < TN; ++t) {
-                    const uint32_t zero = F == kI4ZP ? now.z[F == kI4ZP ? t : 0] >> (4 * ((s * H + h) & 1)) & 15u : 8u;
-                    const uint32_t m = i4_word_of<F>(WIDE && h ? now.s[t] >> 16 : now.s[t] & 0xFFFFu, zero);
+                    uint32_t m = (uint32_t)__shfl((int)four[t][F == kI4ZP ? h : 0], of_four * 16 + ln, kWave);
+                    if constexpr (F == kI4) m = i4_word_of<F>(h ? m >> 16 : m & 0xFFFFu, 8u);
                     const float f = i4_factor<F>(m), sc = i4_scale<F>(m), z = i4_zero<F>(m);
                     f32x4 g[TM];
 #pragma unroll
@@ -750,13 +758,14 @@ experts_tile_kernel(const ExpertsParams p)
         if (!I4 && last && p.K - s * C < C) clear_past(slot, p.K - s * C);
         if (busy) {
             if constexpr (F == kFP8) __builtin_amdgcn_s_setprio(1);      // ahead of the blocks that fetch: 1674 -> 1646 us at 4001
-            use(slot, s, d);                                             // tokens; INT4 1% slower so, BF16 even
+            use(slot, d);                                                // tokens; INT4 1% slower so, BF16 even
             if constexpr (F == kFP8) __builtin_amdgcn_s_setprio(0);
         }
-        if (I4 && d == kRound - 1) meta = ahead;
+        if (I4 && d == kRound - 1) take_meta();
     };
 
-    meta_load(meta, 0);
+    meta_load(ahead, 0);
+    take_meta();
     if constexpr (T::kDirect) {
         static_assert(!T::kDirect || XW == WAVES, "every wave has a part of x");
         const auto issue = [&](uint8_t* slot, int s) __attribute__((always_inline)) {
