@@ -559,26 +559,30 @@ experts_stream_kernel(const ExpertsParams p)
 // they read the weights once: blocks that took several units, chunk by chunk, were slower (us, 64 tokens and two of 8 experts
 // 28672x4096 e4m3 169 -> 190).
 // ---------------------------------------------------------------------------------------------------------------
-template <int F, int BM, bool WIDE>
+// SPLIT: two waves a part, which share the K of each stage. An INT4 wave has some 250 instructions a stage, as long as the stage's
+// bytes take: alone on its SIMD, as where there are few blocks, it kept the loads waiting (us, 16 tokens, two of 8 experts
+// 4096x14336: 57.3, two a part 48.2, without any products 43.4).
+template <int F, int BM, bool WIDE, bool SPLIT>
 struct TileShape {
     static constexpr bool kI4F = F == kI4 || F == kI4ZP;
     static constexpr int kCols = F == kBF16 || (F == kFP8 && BM >= 128) ? 64 : (WIDE ? 256 : 128);
     static constexpr int kRowBytes = F == kBF16 ? 2 * kCols : (F == kFP8 ? kCols : kCols / 2);
     static constexpr int kXRowBytes = 2 * kCols, kSteps = kCols / 32;
-    static constexpr int kWaves = BM == 256 ? 8 : 4, kTiles = 2 * kWaves;     // of a block; its tiles of 16 weight rows
-    static constexpr int kM = BM >= 128 ? 2 : 1, kN = kWaves / kM;               // the waves' parts
+    static constexpr int kParts = BM == 256 ? 8 : 4, kTiles = 2 * kParts;     // of a block; its tiles of 16 weight rows
+    static constexpr int kM = BM >= 128 ? 2 : 1, kN = kParts / kM;               // the parts' rows and columns
+    static constexpr int kHalves = SPLIT ? 2 : 1, kWaves = kParts * kHalves;      // waves of a part, of a block
     static constexpr int kTM = BM / 16 / kM, kTN = kTiles / kN;
     static constexpr int kWBytes = kTiles * kTileRows * kRowBytes, kXBytes = BM * kXRowBytes;
     static constexpr bool kDirect = BM >= 128 || (kI4F && BM == 64);
-    static constexpr int kBlocks = kWaves == 8 ? 1 : (BM >= 64 || (WIDE && BM == 32) ? 2 : 3);                     // of a CU
+    static constexpr int kBlocks = kParts == 8 ? 1 : SPLIT ? (BM == 16 ? 2 : 1) : (BM >= 64 || (WIDE && BM == 32) ? 2 : 3);                     // of a CU
 };
 
-template <int F, int BM, bool WIDE, bool GATED>
-__global__ void __launch_bounds__((TileShape<F, BM, WIDE>::kWaves * kWave),
-                                  (TileShape<F, BM, WIDE>::kBlocks * TileShape<F, BM, WIDE>::kWaves / 4))
+template <int F, int BM, bool WIDE, bool SPLIT, bool GATED>
+__global__ void __launch_bounds__((TileShape<F, BM, WIDE, SPLIT>::kWaves * kWave),
+                                  (TileShape<F, BM, WIDE, SPLIT>::kBlocks * TileShape<F, BM, WIDE, SPLIT>::kWaves / 4))
 experts_tile_kernel(const ExpertsParams p)
 {
-    using T = TileShape<F, BM, WIDE>;
+    using T = TileShape<F, BM, WIDE, SPLIT>;
     constexpr bool I4 = T::kI4F;
     constexpr int C = T::kCols, RB = T::kRowBytes, XB = T::kXRowBytes, X = T::kSteps, TM = T::kTM, TN = T::kTN;
     constexpr int H = I4 ? C / 128 : 1;               // INT4: groups of a stage
@@ -590,7 +594,10 @@ experts_tile_kernel(const ExpertsParams p)
     __shared__ __attribute__((aligned(16))) uint8_t slot1[T::kWBytes + T::kXBytes];
 
     const int lane = lane_id(), wave = wave_id(), ln = lane & 15, lh = lane >> 4;
-    const int wm = wave / T::kN, wn = wave % T::kN;
+    constexpr int HALVES = T::kHalves, HW = H == 2 ? H / HALVES : 1;       // HW: groups of a stage that a wave has
+    constexpr int J = I4 && H == 1 ? 4 / HALVES : 4;                           // its steps of a group
+    const int half = wave / (WAVES / HALVES), part = wave % (WAVES / HALVES);
+    const int wm = part / T::kN, wn = part % T::kN;
     const int stages = (p.K + C - 1) / C;
     const auto w_piece = [](int r) { return RB == 128 ? r & 7 : r >> 1 & 3; };
     const int wr = lane / WP, xr = lane / XP;
@@ -636,7 +643,7 @@ experts_tile_kernel(const ExpertsParams p)
     // The lane group's words of the four stages; where there are no zero points scales as stored, cheaper to make words of again
     // and again than to keep and hand on two of them (us, 200 tokens, four of 60 experts 1003x3584: 34.0, 36.9 as words; with
     // zero points, words 39.7, as stored 41.0).
-    constexpr int kWords = F == kI4ZP ? H : 1;
+    constexpr int kWords = F == kI4ZP ? HW : 1;
     uint32_t four[I4 ? TN : 1][kWords];
     const auto meta_load = [&](Meta& m, int s) __attribute__((always_inline)) {
         if constexpr (I4) {
@@ -657,8 +664,9 @@ experts_tile_kernel(const ExpertsParams p)
         if constexpr (I4)
 #pragma unroll
             for (int t = 0; t < TN; ++t) {
-                if constexpr (F == kI4ZP) i4_words_of<F, H>(ahead.s[t], ahead.z[t], lh, four[t]);
-                else four[t][0] = ahead.s[t];
+                const int g = H == 2 && HW == 1 ? half : 0;      // the first of the wave's groups
+                if constexpr (F == kI4ZP) i4_words_of<F, HW>(ahead.s[t] >> 16 * g, ahead.z[t], lh * H + g, four[t]);
+                else four[t][0] = ahead.s[t] >> 16 * g;
             }
     };
     f32x4 acc[TM][TN];
@@ -671,27 +679,38 @@ experts_tile_kernel(const ExpertsParams p)
         const int piece = F == kBF16 ? 4 * j + lh : (F == kFP8 ? 8 * (j >> 1) + 2 * lh + (j & 1) : 16 * (j >> 2) + 4 * lh + (j & 3));
         return *reinterpret_cast<const u32x4*>(slot + T::kWBytes + r * XB + ((x_place<F, XB>(piece) ^ (r & 7)) << 4));
     };
-    const auto get_w = [&](const uint8_t* slot, int t, int i) {
+    const auto w_at = [&](const uint8_t* slot, int t, int i) {
         const int r = (wn * TN + t) * 16 + ln;
-        return *reinterpret_cast<const u32x4*>(slot + r * RB + (((4 * i + lh) ^ w_piece(r)) << 4));
+        return slot + r * RB + (((4 * i + lh) ^ w_piece(r)) << 4);
     };
+    const auto get_w = [&](const uint8_t* slot, int t, int i) { return *reinterpret_cast<const u32x4*>(w_at(slot, t, i)); };
     const auto use = [&](const uint8_t* slot, int of_four) __attribute__((always_inline)) {
         if constexpr (I4) {
 #pragma unroll
-            for (int h = 0; h < H; ++h) {
-                u32x4 a[TM][4], w[TN];
+            for (int h = 0; h < HW; ++h) {
+                const int hg = H == 2 && HW == 1 ? half : h, j0 = J < 4 ? J * half : 0;
+                u32x4 a[TM][J];
+                uint32_t w[TN][J];
                 f32x4 xs[TM];
 #pragma unroll
                 for (int i = 0; i < TM; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) a[i][j] = get_x(slot, i, 4 * h + j);
+                    for (int j = 0; j < J; ++j) a[i][j] = get_x(slot, i, 4 * hg + j0 + j);
 #pragma unroll
-                for (int t = 0; t < TN; ++t) w[t] = get_w(slot, t, h);
+                for (int t = 0; t < TN; ++t)
+                    if constexpr (J == 4) {
+                        const u32x4 v = get_w(slot, t, hg);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) w[t][j] = v[j];
+                    } else {
+                        const uint64_t v = *reinterpret_cast<const uint64_t*>(w_at(slot, t, hg) + 4 * j0);
+                        w[t][0] = (uint32_t)v, w[t][1] = (uint32_t)(v >> 32);
+                    }
 #pragma unroll
                 for (int i = 0; i < TM; ++i) {
                     xs[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) xs[i] = mfma_16x16x32(a[i][j], ones, xs[i]);
+                    for (int j = 0; j < J; ++j) xs[i] = mfma_16x16x32(a[i][j], ones, xs[i]);
                 }
 #pragma unroll
                 for (int t = 0; t < TN; ++t) {
@@ -702,7 +721,7 @@ experts_tile_kernel(const ExpertsParams p)
 #pragma unroll
                     for (int i = 0; i < TM; ++i) g[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < J; ++j) {
                         const u32x4 b = T::kDirect ? i4_frag(w[t][j], f) : i4_frag_paired(w[t][j], f);     // x as it was stored
 #pragma unroll
                         for (int i = 0; i < TM; ++i) g[i] = mfma_16x16x32(a[i][j], b, g[i]);
@@ -713,12 +732,13 @@ experts_tile_kernel(const ExpertsParams p)
                         for (int v = 0; v < 4; ++v)
                             acc[i][t][v] = __builtin_fmaf(sc, __builtin_fmaf(-z, xs[i][v], g[i][v]), acc[i][t][v]);
                 }
-                if (h + 1 < H) __builtin_amdgcn_sched_barrier(0);
+                if (h + 1 < HW) __builtin_amdgcn_sched_barrier(0);
             }
         } else {
             constexpr int kWSteps = F == kFP8 ? 2 : 1;     // steps that a 16-byte piece of a weight row holds
 #pragma unroll
-            for (int j0 = 0; j0 < X; j0 += kWSteps) {
+            for (int j1 = 0; j1 < X / HALVES; j1 += kWSteps) {
+                const int j0 = j1 + X / HALVES * half;
                 u32x4 w[TN];
 #pragma unroll
                 for (int t = 0; t < TN; ++t) w[t] = get_w(slot, t, j0 / kWSteps);
@@ -829,10 +849,26 @@ experts_tile_kernel(const ExpertsParams p)
             if (s + d < stages) {
                 uint8_t* slot = d & 1 ? slot1 : slot0;
                 store(slot, buf[d & 1]);
-                if (kRound > 2 && s + d + 2 < stages) load(buf[d & 1], s + d + 2);
+                if (d + 2 < kRound && s + d + 2 < stages) load(buf[d & 1], s + d + 2);
                 block_lds_order();
                 multiply(slot, s + d, d, true);
             }
+    }
+    if constexpr (HALVES == 2) {
+        // the second half's sums go to the first's, by way of the places in LDS
+        f32x4* sums = reinterpret_cast<f32x4*>(slot0) + part * (TM * TN * kWave) + lane;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int t = 0; t < TN; ++t)
+                if (half == 1) sums[(i * TN + t) * kWave] = acc[i][t];
+        __syncthreads();
+        if (half == 1) return;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int t = 0; t < TN; ++t) acc[i][t] += sums[(i * TN + t) * kWave];
     }
     if (!busy) return;
 
@@ -905,13 +941,19 @@ inline bool streams(const ExpertsParams& p, int64_t pairs)
     const int64_t R = p.R, bins = R < p.E + 1 ? R : p.E + 1, chunks = (R + bins * 3) / 4;     // MT >= 4
     return R <= pairs && p.x_bytes != 0 && p.row_bytes >= 1024 && chunks * ((p.cols + 15) / 16) <= kMostItems;
 }
-template <int F, int BM, bool WIDE, bool GATED>
+template <int F, int BM, bool WIDE, bool SPLIT, bool GATED>
+int64_t tile_units(ExpertsParams& p)
+{
+    using T = TileShape<F, BM, WIDE, SPLIT>;
+    return plan_experts(p, BM, (GATED ? T::kTiles / 2 : T::kTiles) * kTileRows);
+}
+template <int F, int BM, bool WIDE, bool SPLIT, bool GATED>
 int launch_tiles(ExpertsParams p, hipStream_t st)
 {
-    using T = TileShape<F, BM, WIDE>;
-    const int64_t units = plan_experts(p, BM, (GATED ? T::kTiles / 2 : T::kTiles) * kTileRows);
+    using T = TileShape<F, BM, WIDE, SPLIT>;
+    const int64_t units = tile_units<F, BM, WIDE, SPLIT, GATED>(p);
     if (units < 0) return -2;
-    hipLaunchKernelGGL((experts_tile_kernel<F, BM, WIDE, GATED>), dim3((uint32_t)units), dim3(T::kWaves * kWave), 0, st, p);
+    hipLaunchKernelGGL((experts_tile_kernel<F, BM, WIDE, SPLIT, GATED>), dim3((uint32_t)units), dim3(T::kWaves * kWave), 0, st, p);
     return (int)hipGetLastError();
 }
 // The form of a call goes by the pairs an expert has on average, all that the host knows of them. Each side of a border measured
@@ -926,35 +968,42 @@ int launch_tiles(ExpertsParams p, hipStream_t st)
 //   INT4  MT 4 / 16    0.5 e8 39.1/40.8 d8 24.0/56, 1 e8 47.7/53.0 e64 25.6/24.5, 2 e8 91.6/85.6 d8 50.9/54.4 e64 38.0/37.9
 //         16 / 32      20 e8 157/164 d8 88/114 d64 (zp) 38/39, 25 e64 73/72 d64 (zp) 43.6/39.5, 28 e8 189/191
 //         32 / 64      50 e8 240/259 e64 111/109, 64 e8 289/268 e64 128/123
+//         blocks of 16, waves alone / two a part: d8 4 57.3/48.2, 13 of 60 1003x3584 33.7/32.6 (zp 39.5/34.6), 4096x3584 105/111 (zp
+//                      121/115), 4 e8 89/91 (zp 98/95), 8 e64 42.3/43.8 (zp 48.6/45.4)
 //         64 / 128     with zero points never; without 256 e8 477/436, 512 1508/1307
 //   rows of 512 bytes, MT 4 / 16: E4M3 1024x512 11.4/7.9; of 704: INT4 d64 14.4/9.0; of 1024: INT4 e64 above; BF16 1024x512 12.4/11.8
 template <int F, bool GATED>
-int launch_format(const ExpertsParams& p, hipStream_t st)
+int launch_format(ExpertsParams p, hipStream_t st)
 {
     const int64_t R = p.R, E = p.E;
     if constexpr (F == kI4 || F == kI4ZP) {
         const auto few = [&](auto wide) {
             constexpr bool WIDE = decltype(wide)::value;
             if (streams(p, E)) return launch_stream<F, 4, WIDE, GATED>(p, st);
-            if (R <= 22 * E) return launch_tiles<F, 16, WIDE, GATED>(p, st);
-            return launch_tiles<F, 32, WIDE, GATED>(p, st);
+            if constexpr (WIDE) {
+                const bool split = F == kI4ZP || tile_units<F, 16, true, true, GATED>(p) <= 3 * device_facts().cus;
+                if (R <= 22 * E && split) return launch_tiles<F, 16, true, true, GATED>(p, st);
+            }
+            if constexpr (!WIDE || F == kI4)
+                if (R <= 22 * E) return launch_tiles<F, 16, WIDE, false, GATED>(p, st);
+            return launch_tiles<F, 32, WIDE, false, GATED>(p, st);
         };
         if (R <= 56 * E) return p.G % 2 == 0 && aligned(p.meta, 4) ? few(std::true_type{}) : few(std::false_type{});
-        if (F == kI4ZP || R <= 192 * E) return launch_tiles<F, 64, false, GATED>(p, st);
-        return launch_tiles<F, F == kI4 ? 128 : 64, false, GATED>(p, st);
+        if (F == kI4ZP || R <= 192 * E) return launch_tiles<F, 64, false, false, GATED>(p, st);
+        return launch_tiles<F, F == kI4 ? 128 : 64, false, false, GATED>(p, st);
     } else if constexpr (F == kFP8) {
         if (streams(p, E * 3 / 4)) return launch_stream<F, 4, false, GATED>(p, st);
         if (streams(p, 5 * E)) return launch_stream<F, 16, false, GATED>(p, st);
-        if (R <= 12 * E) return launch_tiles<F, 16, false, GATED>(p, st);
-        if (R <= 56 * E) return launch_tiles<F, 32, false, GATED>(p, st);
-        return launch_tiles<F, 128, false, GATED>(p, st);
+        if (R <= 12 * E) return launch_tiles<F, 16, false, false, GATED>(p, st);
+        if (R <= 56 * E) return launch_tiles<F, 32, false, false, GATED>(p, st);
+        return launch_tiles<F, 128, false, false, GATED>(p, st);
     } else {
         if (streams(p, E)) return launch_stream<F, 8, false, GATED>(p, st);
         if (streams(p, 6 * E)) return launch_stream<F, 16, false, GATED>(p, st);
-        if (R <= 8 * E) return launch_tiles<F, 16, false, GATED>(p, st);
-        if (R <= 28 * E) return launch_tiles<F, 32, false, GATED>(p, st);
-        if (R <= 112 * E) return launch_tiles<F, 64, false, GATED>(p, st);
-        return launch_tiles<F, 256, false, GATED>(p, st);
+        if (R <= 8 * E) return launch_tiles<F, 16, false, false, GATED>(p, st);
+        if (R <= 28 * E) return launch_tiles<F, 32, false, false, GATED>(p, st);
+        if (R <= 112 * E) return launch_tiles<F, 64, false, false, GATED>(p, st);
+        return launch_tiles<F, 256, false, false, GATED>(p, st);
     }
 }
 template <int F>

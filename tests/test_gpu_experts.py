@@ -85,6 +85,7 @@ def test_more_items_than_blocks(cuda, fmt):
     case(fmt, [1, 2, 1, 0, 1, 2, 0, 1], 8000, DEEP[fmt], bias=True)
     case(fmt, [2] * 7, 4100, DEEP[fmt], gated=True)
     case(fmt, [1, 0, 1, 1] * 25, 514, DEEP[fmt], gated=True, bare=9)
+    case(fmt, [5] * 8, 10300, 256, bias=True)          # blocks of 16, more than the chip holds at a time
 
 
 @pytest.mark.parametrize("fmt", ["int4", "int4zp"])
