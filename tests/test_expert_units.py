@@ -33,8 +33,8 @@ def units(offsets, R, E, BM, tiles):
         if b >= total:
             out.append(None)
             continue
-        xcd = b % 8
-        u = xcd * (total // 8) + min(xcd, total % 8) + b // 8
+        xcd, real = b % 8, chunks * tiles
+        u = xcd * (real // 8) + min(xcd, real % 8) + b // 8 if b < real else b
         c = u // tiles
         if c >= chunks:
             first = rest + (c - chunks) * BM
@@ -143,3 +143,18 @@ def test_waves_share_stages(seed):
                 have = kb & ~3
             assert have <= kb < have + 4
     assert at == stages
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_rows_without_an_expert_are_all_cleared(seed):
+    rng = random.Random(seed)
+    rest, cols, blocks = rng.choice([0, 1, 4, 300]), rng.choice([1, 255, 256, 257, 5000]), rng.choice([1, 7, 88, 768])
+    pieces, seen = -(-cols // 256), set()
+    for block in range(blocks):
+        for i in range(rest * pieces * block // blocks, rest * pieces * (block + 1) // blocks):
+            r, at = divmod(i, pieces)
+            for thread in range(256):
+                if at * 256 + thread < cols:
+                    assert (r, at * 256 + thread) not in seen
+                    seen.add((r, at * 256 + thread))
+    assert len(seen) == rest * cols
