@@ -213,9 +213,12 @@ __device__ __forceinline__ void i4_words_of(uint32_t scales, uint32_t zeros, int
         word[h] = i4_word_of<F>(h ? scales >> 16 : scales & 0xFFFFu, zero);
     }
 }
+// Two bf16 whose products with x sum up to what a group's zero points take: -8 in the nibbles' scale, so that the group's sum begins
+// with it; with zero points of their own 1, and each row takes its multiple (8 of 200 instructions of a stage more).
+template <int F> constexpr uint32_t kI4Take = F == kI4 ? (kI4Ones + 0x01800180u) | 0x80008000u : kI4Ones;
 template <int F> __device__ __forceinline__ float i4_factor(uint32_t m) { return __uint_as_float(F == kI4 ? kI4Exp << 23 : (m & 0xFF00u) << 15); }
 template <int F> __device__ __forceinline__ float i4_scale(uint32_t m) { return __uint_as_float(F == kI4 ? m : m & 0xFFFF0000u); }
-template <int F> __device__ __forceinline__ float i4_zero(uint32_t m) { return F == kI4 ? 8.0f : (float)(m & 0xFFu); }
+template <int F> __device__ __forceinline__ float i4_zero(uint32_t m) { return (float)(m & 0xFFu); }
 
 // Where piece (16 bytes, 8 columns) `piece` of a row of x of XB bytes lies among the row's, before the XOR with the row's lowest
 // three bits. A 16-byte read takes 16 lanes at a time: eight rows (all values of those bits) of one column group of the
@@ -393,7 +396,7 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
     const auto x_at = [](int row, int piece) {
         return T::kWBytes + row * T::kXRowBytes + ((x_place<F, T::kXRowBytes>(piece) ^ (row & 7)) << 4);
     };
-    const uint32_t one2 = (uint32_t)__builtin_amdgcn_readfirstlane((int)kI4Ones);
+    const uint32_t one2 = (uint32_t)__builtin_amdgcn_readfirstlane((int)kI4Take<F>);
     const u32x4 ones = {one2, one2, one2, one2};
     f32x4 acc[P];
 #pragma unroll
@@ -430,11 +433,11 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
                     const u32x4 w = w_piece(t, 4 * h + lh);
                     const uint32_t m = (uint32_t)__shfl((int)four[t][h], from, kWave);
                     const float f = i4_factor<F>(m), sc = i4_scale<F>(m), z = i4_zero<F>(m);
-                    f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f};
+                    f32x4 g = F == kI4 ? xs : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) g = mfma_16x16x32(a[j], i4_frag_paired(w[j], f), g);
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) acc[t][v] = __builtin_fmaf(sc, __builtin_fmaf(-z, xs[v], g[v]), acc[t][v]);
+                    for (int v = 0; v < 4; ++v) acc[t][v] = __builtin_fmaf(sc, F == kI4 ? g[v] : __builtin_fmaf(-z, xs[v], g[v]), acc[t][v]);
                 }
                 if (h + 1 < H) __builtin_amdgcn_sched_barrier(0);
             }
@@ -613,7 +616,7 @@ experts_tile_kernel(const ExpertsParams p)
     const auto w_piece = [](int r) { return RB == 128 ? r & 7 : r >> 1 & 3; };
     const int wr = lane / WP, xr = lane / XP;
     const uint32_t wpiece = (uint32_t)((lane % WP) ^ w_piece(wr)) * 16u;         // a load's first row is a multiple of 8
-    const uint32_t one2 = (uint32_t)__builtin_amdgcn_readfirstlane((int)kI4Ones);
+    const uint32_t one2 = (uint32_t)__builtin_amdgcn_readfirstlane((int)kI4Take<F>);
     const u32x4 ones = {one2, one2, one2, one2};
 
     const ExpertUnit u = unit_of<BM>(p);
@@ -730,7 +733,7 @@ experts_tile_kernel(const ExpertsParams p)
                     const float f = i4_factor<F>(m), sc = i4_scale<F>(m), z = i4_zero<F>(m);
                     f32x4 g[TM];
 #pragma unroll
-                    for (int i = 0; i < TM; ++i) g[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int i = 0; i < TM; ++i) g[i] = F == kI4 ? xs[i] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int j = 0; j < J; ++j) {
                         const u32x4 b = T::kDirect ? i4_frag(w[t][j], f) : i4_frag_paired(w[t][j], f);     // x as it was stored
@@ -741,7 +744,7 @@ experts_tile_kernel(const ExpertsParams p)
                     for (int i = 0; i < TM; ++i)
 #pragma unroll
                         for (int v = 0; v < 4; ++v)
-                            acc[i][t][v] = __builtin_fmaf(sc, __builtin_fmaf(-z, xs[i][v], g[i][v]), acc[i][t][v]);
+                            acc[i][t][v] = __builtin_fmaf(sc, F == kI4 ? g[i][v] : __builtin_fmaf(-z, xs[i][v], g[i][v]), acc[i][t][v]);
                 }
                 if (h + 1 < HW) __builtin_amdgcn_sched_barrier(0);
             }
