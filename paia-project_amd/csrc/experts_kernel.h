@@ -11,6 +11,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "divisor.h"
 #include "gemv_tile.h"
 
@@ -39,6 +41,7 @@ struct ExpertsParams {
 struct ExpertUnit {
     int expert;              // E: pairs without an expert; -1: no unit
     int first, held, tile;   // its pairs are order[first .. first + held)
+    int chunks;              // of its expert
 };
 
 __device__ __forceinline__ int wave_inclusive(int v)
@@ -111,17 +114,17 @@ __device__ __forceinline__ ExpertUnit unit_of(const ExpertsParams& p)
 {
     const Chunks<BM> chunks(p);
     const int units = chunks.count * p.tiles, b = (int)blockIdx.x;
-    if (b >= units + chunks.rest * p.tiles) return {-1, 0, 0, 0};
+    if (b >= units + chunks.rest * p.tiles) return {-1, 0, 0, 0, 0};
     // units without an expert come last: dealt out with the others they left one XCD almost nothing to do
     const int u = b < units ? xcd_contiguous(b, units) : b;
     const int c = (int)p.by_tiles.of((uint32_t)u);
     if (c >= chunks.count) {
         const int first = chunks.rest_at + (c - chunks.count) * BM;
-        return {p.E, first, min(BM, p.R - first), u - c * p.tiles};
+        return {p.E, first, min(BM, p.R - first), u - c * p.tiles, 0};
     }
     const auto x = chunks.of(p, c);
     const int local = u - x.begin * p.tiles, tile = local / x.n, first = x.lo + (local - tile * x.n) * BM;
-    return {x.expert, first, min(BM, x.hi - first), tile};
+    return {x.expert, first, min(BM, x.hi - first), tile, x.n};
 }
 
 __device__ __forceinline__ int pair_at(const ExpertsParams& p, const ExpertUnit& u, int i)
@@ -297,7 +300,7 @@ struct StreamSpace {
 };
 
 // `groups` items from column group `group0` on, of the pairs order[first .. first + held) of one expert.
-template <int F, int MT, bool WIDE, bool GATED>
+template <int F, int MT, bool WIDE, bool PAST, bool GATED>
 __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace<F, MT, WIDE>& space, int expert, int first, int held,
                                              int order, int group0, int groups)
 {
@@ -347,7 +350,7 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
 #pragma unroll
         for (int t = 0; t < P; ++t) {
 #pragma unroll
-            for (int i = 0; i < L; ++i) B.w[t][i] = ld16<2>(rw[t], wo + wstep * (uint32_t)i, 0u);
+            for (int i = 0; i < L; ++i) B.w[t][i] = ld16<PAST ? 2 : 0>(rw[t], wo + wstep * (uint32_t)i, 0u);
             if constexpr (I4) {
                 const int at = ((kb & ~3) + lh) * H;
                 const bool in = (it == 0 || (kb & 3) == 0) && left > 0 && at < p.G;
@@ -532,7 +535,7 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
     }
 }
 
-template <int F, int MT, bool WIDE, bool GATED>
+template <int F, int MT, bool WIDE, bool PAST, bool GATED>
 __global__ void __launch_bounds__((StreamShape<F, MT, WIDE>::kWaves * kWave),
                                   (StreamShape<F, MT, WIDE>::kBlocks * StreamShape<F, MT, WIDE>::kWaves / 4))
 experts_stream_kernel(const ExpertsParams p)
@@ -547,7 +550,7 @@ experts_stream_kernel(const ExpertsParams p)
         const int groups = min(p.tiles - group0, (int)(end - item));
         const auto x = chunks.of(p, chunk);
         const int first = x.lo + (chunk - x.begin) * MT;
-        stream_items<F, MT, WIDE, GATED>(p, space, x.expert, first, min(MT, x.hi - first), chunks.order,
+        stream_items<F, MT, WIDE, PAST, GATED>(p, space, x.expert, first, min(MT, x.hi - first), chunks.order,
                                                  group0, groups);
         item += (uint32_t)groups;
     }
@@ -591,7 +594,7 @@ struct TileShape {
     static constexpr int kBlocks = kParts == 8 ? 1 : (SPLIT || BM >= 64 || (WIDE && BM == 32) ? 2 : 3);      // of a CU
 };
 
-template <int F, int BM, bool WIDE, bool SPLIT, bool GATED>
+template <int F, int BM, bool WIDE, bool SPLIT, bool PAST, bool GATED>
 __global__ void __launch_bounds__((TileShape<F, BM, WIDE, SPLIT>::kWaves * kWave),
                                   (TileShape<F, BM, WIDE, SPLIT>::kBlocks * TileShape<F, BM, WIDE, SPLIT>::kWaves / 4))
 experts_tile_kernel(const ExpertsParams p)
@@ -826,10 +829,13 @@ experts_tile_kernel(const ExpertsParams p)
             u32x4 w[WL], x[XL];
         };
         // Unconditional: past the last stage it reads that one again, waves without a part of x their neighbours' rows.
-        const auto load = [&](Stage& B, int s) __attribute__((always_inline)) {
+        const auto load = [&](auto once, Stage& B, int s) __attribute__((always_inline)) {
             s = min(s, stages - 1);
 #pragma unroll
-            for (int i = 0; i < WL; ++i) B.w[i] = *reinterpret_cast<const u32x4*>(w_from(s, i));
+            for (int i = 0; i < WL; ++i) {
+                const u32x4* from = reinterpret_cast<const u32x4*>(w_from(s, i));
+                B.w[i] = decltype(once)::value ? __builtin_nontemporal_load(from) : *from;
+            }
 #pragma unroll
             for (int i = 0; i < XL; ++i) B.x[i] = *reinterpret_cast<const u32x4*>(x_from(s, i));
         };
@@ -842,31 +848,39 @@ experts_tile_kernel(const ExpertsParams p)
                     *reinterpret_cast<u32x4*>(slot + T::kWBytes + (wave * XL + i) * 1024 + lane * 16) = I4 ? i4_pair_x(B.x[i]) : B.x[i];
             }
         };
-        Stage buf[2];
-        load(buf[0], 0);
-        load(buf[1], 1);
-        int s = 0;
-        wait_loads<0>();                             // the loop's waits then count its own order of loads alone
-        for (; s + kRound < stages; s += kRound) {
+        const auto run = [&](auto once) __attribute__((always_inline)) {
+            asm volatile("" ::"i"((int)decltype(once)::value) : "memory");
+            Stage buf[2];
+            load(once, buf[0], 0);
+            load(once, buf[1], 1);
+            int s = 0;
+            wait_loads<0>();                             // the loop's waits then count its own order of loads alone
+            for (; s + kRound < stages; s += kRound) {
 #pragma unroll
-            for (int d = 0; d < kRound; ++d) {
-                uint8_t* slot = d & 1 ? slot1 : slot0;
-                store(slot, buf[d & 1]);             // what was there is read: two stages ago, before the last barrier
-                if (d == 0) meta_load(ahead, s + kRound);      // ahead of the loads that stay on their way
-                load(buf[d & 1], s + d + 2);
-                block_lds_order();
-                multiply(slot, s + d, d, false);
+                for (int d = 0; d < kRound; ++d) {
+                    uint8_t* slot = d & 1 ? slot1 : slot0;
+                    store(slot, buf[d & 1]);             // what was there is read: two stages ago, before the last barrier
+                    if (d == 0) meta_load(ahead, s + kRound);      // ahead of the loads that stay on their way
+                    load(once, buf[d & 1], s + d + 2);
+                    block_lds_order();
+                    multiply(slot, s + d, d, false);
+                }
             }
-        }
 #pragma unroll
-        for (int d = 0; d < kRound; ++d)
-            if (s + d < stages) {
-                uint8_t* slot = d & 1 ? slot1 : slot0;
-                store(slot, buf[d & 1]);
-                if (d + 2 < kRound && s + d + 2 < stages) load(buf[d & 1], s + d + 2);
-                block_lds_order();
-                multiply(slot, s + d, d, true);
-            }
+            for (int d = 0; d < kRound; ++d)
+                if (s + d < stages) {
+                    uint8_t* slot = d & 1 ? slot1 : slot0;
+                    store(slot, buf[d & 1]);
+                    if (d + 2 < kRound && s + d + 2 < stages) load(once, buf[d & 1], s + d + 2);
+                    block_lds_order();
+                    multiply(slot, s + d, d, true);
+                }
+        };
+        // Weights that no other block reads pass by the caches (us, two of 8 experts 28672x4096, 64 tokens bf16 323 -> 293, 48 e4m3
+        // 170 -> 152; 509 tokens, four of 64 experts 2816x2048 bf16 145 -> 128), those of several chunks do not: bf16, 300 tokens
+        // 429, past the caches 527. Nor do rows whose lines two stages share (d64 INT4 of 11 groups 24.7 -> 26.0). For INT4 the host decides (PAST): two loops would share too few registers.
+        if (I4 ? PAST : __builtin_amdgcn_readfirstlane(u.chunks) == 1 && p.row_bytes % 128 == 0) run(std::true_type{});
+        else run(std::false_type{});
     }
     if constexpr (HALVES == 2) {
         // the second half's sums go to the first's, by way of the places in LDS
@@ -944,9 +958,15 @@ int launch_stream(ExpertsParams p, hipStream_t st)
     using T = StreamShape<F, MT, WIDE>;
     const int64_t items = plan_experts(p, MT, (GATED ? T::kTiles / 2 : T::kTiles) * kTileRows);
     const int64_t resident = T::kBlocks * device_facts().cus;
-    hipLaunchKernelGGL((experts_stream_kernel<F, MT, WIDE, GATED>), dim3((uint32_t)(items < resident ? items : resident)),
-                       dim3(T::kWaves * kWave), 0, st, p);
-    return (int)hipGetLastError();
+    // Weights pass by the caches where a stage has whole lines; lines that two stages share are kept for the second (us, 4 tokens, two
+    // of 8 experts 28672x4112 e4m3 96, past the caches 120; 28672x4096 83 and 76; INT4 of 33 groups 62 and 69).
+    const auto go = [&](auto past) {
+        hipLaunchKernelGGL((experts_stream_kernel<F, MT, WIDE, decltype(past)::value, GATED>),
+                           dim3((uint32_t)(items < resident ? items : resident)), dim3(T::kWaves * kWave), 0, st, p);
+        return (int)hipGetLastError();
+    };
+    if constexpr (T::kI4F) return go(std::bool_constant<WIDE>{});
+    else return p.row_bytes % 128 == 0 ? go(std::true_type{}) : go(std::false_type{});
 }
 // Where reading weights bounds a call: its items of two tiles fit the shares, a descriptor spans x, and a wave's quarter of a row
 // is two lines or more.
@@ -961,13 +981,13 @@ int64_t tile_units(ExpertsParams& p)
     using T = TileShape<F, BM, WIDE, SPLIT>;
     return plan_experts(p, BM, (GATED ? T::kTiles / 2 : T::kTiles) * kTileRows);
 }
-template <int F, int BM, bool WIDE, bool SPLIT, bool GATED>
+template <int F, int BM, bool WIDE, bool SPLIT, bool GATED, bool PAST = false>
 int launch_tiles(ExpertsParams p, hipStream_t st)
 {
     using T = TileShape<F, BM, WIDE, SPLIT>;
     const int64_t units = tile_units<F, BM, WIDE, SPLIT, GATED>(p);
     if (units < 0) return -2;
-    hipLaunchKernelGGL((experts_tile_kernel<F, BM, WIDE, SPLIT, GATED>), dim3((uint32_t)units), dim3(T::kWaves * kWave), 0, st, p);
+    hipLaunchKernelGGL((experts_tile_kernel<F, BM, WIDE, SPLIT, PAST, GATED>), dim3((uint32_t)units), dim3(T::kWaves * kWave), 0, st, p);
     return (int)hipGetLastError();
 }
 // The form of a call goes by the pairs an expert has on average, all that the host knows of them. Each side of a border measured
@@ -986,6 +1006,8 @@ int launch_tiles(ExpertsParams p, hipStream_t st)
 //         32 / 64      50 e8 240/259 e64 111/109, 64 e8 289/268 e64 128/123
 //         blocks of 16, waves alone / two a part: d8 4 57.3/48.2, 13 of 60 1003x3584 33.7/32.6 (zp 39.5/34.6), 4096x3584 105/111 (zp
 //                      121/115), 4 e8 89/91 (zp 98/95), 8 e64 42.3/43.8 (zp 48.6/45.4)
+//         16, weights kept / past the caches: 4 e8 88/82 d8 48/45, 8 e64 42/38 (zp 45/43), 13 of 60 1003x3584 (zp) 35.1/34.1,
+//                      20 e64 58/58 e8 143/149 d8 76/79
 //         64 / 128     with zero points never; without 256 e8 477/436, 512 1508/1307
 //   rows of 512 bytes, MT 4 / 16: E4M3 1024x512 11.4/7.9; of 704: INT4 d64 14.4/9.0; of 1024: INT4 e64 above; BF16 1024x512 12.4/11.8
 // Few units (no more than the chip holds at a time): an expert's second chunk is then another block on some of the CUs, and the call
@@ -998,12 +1020,17 @@ int launch_format(ExpertsParams p, hipStream_t st)
         const auto few = [&](auto wide) {
             constexpr bool WIDE = decltype(wide)::value;
             if (streams(p, E)) return launch_stream<F, 4, WIDE, GATED>(p, st);
+            const auto sixteen = [&](auto split) {
+                constexpr bool SPLIT = decltype(split)::value;
+                return WIDE && R <= 14 * E ? launch_tiles<F, 16, WIDE, SPLIT, GATED, WIDE>(p, st)
+                                           : launch_tiles<F, 16, WIDE, SPLIT, GATED>(p, st);
+            };
             if constexpr (WIDE) {
                 const bool split = F == kI4ZP || tile_units<F, 16, true, true, GATED>(p) <= few_units;
-                if (R <= 22 * E && split) return launch_tiles<F, 16, true, true, GATED>(p, st);
+                if (R <= 22 * E && split) return sixteen(std::true_type{});
             }
             if constexpr (!WIDE || F == kI4)
-                if (R <= 22 * E) return launch_tiles<F, 16, WIDE, false, GATED>(p, st);
+                if (R <= 22 * E) return sixteen(std::false_type{});
             return launch_tiles<F, 32, WIDE, false, GATED>(p, st);
         };
         if (R <= 56 * E) return p.G % 2 == 0 && aligned(p.meta, 4) ? few(std::true_type{}) : few(std::false_type{});
