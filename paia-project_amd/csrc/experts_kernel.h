@@ -993,13 +993,15 @@ int launch_tiles(ExpertsParams p, hipStream_t st)
 // The form of a call goes by the pairs an expert has on average, all that the host knows of them. Each side of a border measured
 // (us a call; e8: two of 8 experts gated 28672x4096 a token, d8: 4096x14336, e64: eight of 64, gated 2816x2048, d64: 2048x1408; the
 // pairs an expert in front):
-//   E4M3  MT 4 / 16    0.5 e8 56.6/58.9 e64 26.2/28.0, 0.75 e8 75.0/72.6 e64 32.5/34.4, 1 e64 34.9/32.2
-//         MT 16 / 32   4 e8 143/162 d8 75/80, 5 d8 75/72, 6 e8 177/163 d8 111/81 e64 66/66
-//         16 / 32      6 d64 35/39, 10 d64 38/41; longer rows: 6 e8 165/163 d8 109/81 e64 66/66, 12 e8 172/169 d8 114/83 e64 72/69
-//         32 / 64, few units: 16 d8 84/95, 20 121/98, 38 123/100, 50 120/152; many: 12 e64 69/78
+//   E4M3  MT 4 / 16    0.25 e8 37/42 d8 21/48 e64 17.7/17.9, 0.5 e8 56/54 d8 31/50 e64 25.7/27.1, 0.75 e64 32.6/30.0,
+//                      1 e8 72/79 d8 38/52 e64 34.6/29.6, 1.5 e8 91/96 d8 51/54, 2 e8 142/132 d8 75/62 e64 50/47
+//         16 / 32      4 d8 69/70 e64 55/56, 5 e8 129/130 d8 63/65, 6 d8 109/81 d64 31/35, 16 e8 164/148; d64 10 38/41
+//         32 / 64, few units: 16 d8 84/95, 20 121/98, 38 123/100, 50 120/152; many: 19 e64 65/74, 31 79/87
 //         32 / 128     48 e64 99/101, 64 e64 116/114
-//   BF16  MT 8 / 16    0.25 e64 18.2/18.7, 1 e64 56.9/56.7       MT 16 / 32 4 e8 285/309 e64 107/126, 6 e8 326/310 d8 191/171, 7 e64 121/131
-//         32 / 64      few units: 16 d8 173/175, 20 223/175, 25 210/171; many: 16 e8 313/315, 25 e8 336/325 d64 73/79
+//   BF16  MT 8 / 16    0.25 e64 18.2/18.7, 1 e64 56.9/56.7       MT 16 / 32 2 e64 90/96,
+//                      4 e8 281/284 d8 140/174 e64 109/122, 6 e8 328/285 d8 191/157 e64 120/115
+//         32 / 64      few units: 16 d8 173/175, 20 223/175, 25 210/171; many: 19 e64 119/124, 25 e8 317/300 d64 63/70,
+//                      31 e64 136/132
 //         64 / 256     64 e64 166/201, 128 e64 210/208
 //   INT4  MT 4 / 16    0.5 e8 39.1/40.8 d8 24.0/56, 1 e8 47.7/53.0 e64 25.6/24.5, 2 e8 91.6/85.6 d8 50.9/54.4 e64 38.0/37.9
 //         16 / 32      20 e8 157/164 d8 88/114 d64 (zp) 38/39, 25 e64 73/72 d64 (zp) 43.6/39.5, 28 e8 189/191
@@ -1009,7 +1011,8 @@ int launch_tiles(ExpertsParams p, hipStream_t st)
 //         16, weights kept / past the caches: 4 e8 88/82 d8 48/45, 8 e64 42/38 (zp 45/43), 13 of 60 1003x3584 (zp) 35.1/34.1,
 //                      20 e64 58/58 e8 143/149 d8 76/79
 //         64 / 128     with zero points never; without 256 e8 477/436, 512 1508/1307
-//   rows of 512 bytes, MT 4 / 16: E4M3 1024x512 11.4/7.9; of 704: INT4 d64 14.4/9.0; of 1024: INT4 e64 above; BF16 1024x512 12.4/11.8
+//   rows of 512 bytes, MT 4 / 16: E4M3 1024x512 11.4/7.9; of 704: INT4 d64 14.4/9.0; of 1024: INT4 e64 above; BF16 1024x512
+//   12.4/11.8; of 1408: E4M3 d64 14.2/9.7
 // Few units (no more than the chip holds at a time): an expert's second chunk is then another block on some of the CUs, and the call
 // takes as long as those. Many units even that out.
 template <int F, bool GATED>
@@ -1037,9 +1040,8 @@ int launch_format(ExpertsParams p, hipStream_t st)
         if (F == kI4ZP || R <= 192 * E) return launch_tiles<F, 64, false, false, GATED>(p, st);
         return launch_tiles<F, F == kI4 ? 128 : 64, false, false, GATED>(p, st);
     } else if constexpr (F == kFP8) {
-        if (streams(p, E * 3 / 4)) return launch_stream<F, 4, false, GATED>(p, st);
-        if (streams(p, 5 * E)) return launch_stream<F, 16, false, GATED>(p, st);
-        if (R <= 12 * E && p.row_bytes < 2048) return launch_tiles<F, 16, false, false, GATED>(p, st);
+        if (streams(p, p.row_bytes >= 4096 ? E * 3 / 2 : E / 2)) return launch_stream<F, 4, false, GATED>(p, st);
+        if (R <= (p.row_bytes < 2048 ? 12 : 5) * E) return launch_tiles<F, 16, false, false, GATED>(p, st);
         if (R <= 56 * E) {
             if (R > 16 * E && R <= 40 * E && tile_units<F, 64, false, false, GATED>(p) <= few_units)
                 return launch_tiles<F, 64, false, false, GATED>(p, st);
@@ -1048,7 +1050,7 @@ int launch_format(ExpertsParams p, hipStream_t st)
         return launch_tiles<F, 128, false, false, GATED>(p, st);
     } else {
         if (streams(p, E)) return launch_stream<F, 8, false, GATED>(p, st);
-        if (streams(p, 6 * E)) return launch_stream<F, 16, false, GATED>(p, st);
+        if (streams(p, 5 * E)) return launch_stream<F, 16, false, GATED>(p, st);
         const int64_t most32 = tile_units<F, 64, false, false, GATED>(p) <= few_units ? 16 : 28;
         if (R <= most32 * E) return launch_tiles<F, 32, false, false, GATED>(p, st);
         if (R <= 112 * E) return launch_tiles<F, 64, false, false, GATED>(p, st);
