@@ -108,7 +108,7 @@ struct Chunks {
 // Block b's place when each of the 8 XCDs, to which blocks are dealt in turn, takes a contiguous range of n.
 __device__ __forceinline__ int xcd_contiguous(int b, int n) { return b % 8 * (n / 8) + min(b % 8, n % 8) + b / 8; }
 
-// The unit of this block: units of one expert and tile follow each other.
+// The unit of this block: units of one expert and tile (or group of tiles) follow each other.
 template <int BM>
 __device__ __forceinline__ ExpertUnit unit_of(const ExpertsParams& p)
 {
@@ -123,7 +123,17 @@ __device__ __forceinline__ ExpertUnit unit_of(const ExpertsParams& p)
         return {p.E, first, min(BM, p.R - first), u - c * p.tiles, 0};
     }
     const auto x = chunks.of(p, c);
-    const int local = u - x.begin * p.tiles, tile = local / x.n, first = x.lo + (local - tile * x.n) * BM;
+    // eight tiles at a time through all of many chunks: of 8 tiles by 8 chunks, as an XCD holds at a time, rows and weights alike come
+    // once to its L2 (us, two of 8 experts 28672x4096 e4m3, 8001 tokens 3836 -> 3265, 4001 1738 -> 1681; fewer chunks +-1%)
+    const int local = u - x.begin * p.tiles;
+    int tile, chunk;
+    if (BM < 256 && x.n >= 6) {
+        const int g = local / (8 * x.n), in = local - g * 8 * x.n, wide = min(8, p.tiles - g * 8);
+        chunk = in / wide, tile = g * 8 + in - chunk * wide;
+    } else {
+        tile = local / x.n, chunk = local - tile * x.n;
+    }
+    const int first = x.lo + chunk * BM;
     return {x.expert, first, min(BM, x.hi - first), tile, x.n};
 }
 

@@ -49,9 +49,11 @@ def units(offsets, R, E, BM, tiles):
                 found = (lane * per + i - 1, at, start, to, k)
             at, start = at + k, to
         e, begin, lo, hi, n = found
-        local = u - begin * tiles
-        tile = local // n
-        first = lo + (local - tile * n) * BM
+        local, group = u - begin * tiles, 8 if BM < 256 and n >= 6 else 1
+        g = local // (group * n)
+        wide = min(group, tiles - g * group)
+        chunk, at = divmod(local - g * group * n, wide)
+        tile, first = g * group + at, lo + chunk * BM
         out.append((e, first, min(BM, hi - first), tile))
     return out
 
