@@ -621,8 +621,8 @@ experts_tile_kernel(const ExpertsParams p)
     __shared__ __attribute__((aligned(16))) uint8_t slot1[T::kWBytes + T::kXBytes];
 
     const int lane = lane_id(), wave = wave_id(), ln = lane & 15, lh = lane >> 4;
-    constexpr int HALVES = T::kHalves, HW = H == 2 ? H / HALVES : 1;       // HW: groups of a stage that a wave has
-    constexpr int J = I4 && H == 1 ? 4 / HALVES : 4;                           // its steps of a group
+    constexpr int HALVES = T::kHalves, HW = H / HALVES;       // HW: groups of a stage that a wave has
+    static_assert(!SPLIT || H == 2, "each half has a group");
     const int half = wave / (WAVES / HALVES), part = wave % (WAVES / HALVES);
     const int wm = part / T::kN, wn = part % T::kN;
     const int stages = (p.K + C - 1) / C;
@@ -691,7 +691,7 @@ experts_tile_kernel(const ExpertsParams p)
         if constexpr (I4)
 #pragma unroll
             for (int t = 0; t < TN; ++t) {
-                const int g = H == 2 && HW == 1 ? half : 0;      // the first of the wave's groups
+                const int g = SPLIT ? half : 0;                  // the first of the wave's groups
                 if constexpr (F == kI4ZP) i4_words_of<F, HW>(ahead.s[t] >> 16 * g, ahead.z[t], lh * H + g, four[t]);
                 else four[t][0] = ahead.s[t] >> 16 * g;
             }
@@ -706,38 +706,28 @@ experts_tile_kernel(const ExpertsParams p)
         const int piece = F == kBF16 ? 4 * j + lh : (F == kFP8 ? 8 * (j >> 1) + 2 * lh + (j & 1) : 16 * (j >> 2) + 4 * lh + (j & 3));
         return *reinterpret_cast<const u32x4*>(slot + T::kWBytes + r * XB + ((x_place<F, XB>(piece) ^ (r & 7)) << 4));
     };
-    const auto w_at = [&](const uint8_t* slot, int t, int i) {
+    const auto get_w = [&](const uint8_t* slot, int t, int i) {
         const int r = (wn * TN + t) * 16 + ln;
-        return slot + r * RB + (((4 * i + lh) ^ w_piece(r)) << 4);
+        return *reinterpret_cast<const u32x4*>(slot + r * RB + (((4 * i + lh) ^ w_piece(r)) << 4));
     };
-    const auto get_w = [&](const uint8_t* slot, int t, int i) { return *reinterpret_cast<const u32x4*>(w_at(slot, t, i)); };
     const auto use = [&](const uint8_t* slot, int of_four) __attribute__((always_inline)) {
         if constexpr (I4) {
 #pragma unroll
             for (int h = 0; h < HW; ++h) {
-                const int hg = H == 2 && HW == 1 ? half : h, j0 = J < 4 ? J * half : 0;
-                u32x4 a[TM][J];
-                uint32_t w[TN][J];
+                const int hg = SPLIT ? half : h;
+                u32x4 a[TM][4], w[TN];
                 f32x4 xs[TM];
 #pragma unroll
                 for (int i = 0; i < TM; ++i)
 #pragma unroll
-                    for (int j = 0; j < J; ++j) a[i][j] = get_x(slot, i, 4 * hg + j0 + j);
+                    for (int j = 0; j < 4; ++j) a[i][j] = get_x(slot, i, 4 * hg + j);
 #pragma unroll
-                for (int t = 0; t < TN; ++t)
-                    if constexpr (J == 4) {
-                        const u32x4 v = get_w(slot, t, hg);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) w[t][j] = v[j];
-                    } else {
-                        const uint64_t v = *reinterpret_cast<const uint64_t*>(w_at(slot, t, hg) + 4 * j0);
-                        w[t][0] = (uint32_t)v, w[t][1] = (uint32_t)(v >> 32);
-                    }
+                for (int t = 0; t < TN; ++t) w[t] = get_w(slot, t, hg);
 #pragma unroll
                 for (int i = 0; i < TM; ++i) {
                     xs[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int j = 0; j < J; ++j) xs[i] = mfma_16x16x32(a[i][j], ones, xs[i]);
+                    for (int j = 0; j < 4; ++j) xs[i] = mfma_16x16x32(a[i][j], ones, xs[i]);
                 }
 #pragma unroll
                 for (int t = 0; t < TN; ++t) {
@@ -748,7 +738,7 @@ experts_tile_kernel(const ExpertsParams p)
 #pragma unroll
                     for (int i = 0; i < TM; ++i) g[i] = F == kI4 ? xs[i] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int j = 0; j < J; ++j) {
+                    for (int j = 0; j < 4; ++j) {
                         const u32x4 b = T::kDirect ? i4_frag(w[t][j], f) : i4_frag_paired(w[t][j], f);     // x as it was stored
 #pragma unroll
                         for (int i = 0; i < TM; ++i) g[i] = mfma_16x16x32(a[i][j], b, g[i]);
@@ -764,8 +754,7 @@ experts_tile_kernel(const ExpertsParams p)
         } else {
             constexpr int kWSteps = F == kFP8 ? 2 : 1;     // steps that a 16-byte piece of a weight row holds
 #pragma unroll
-            for (int j1 = 0; j1 < X / HALVES; j1 += kWSteps) {
-                const int j0 = j1 + X / HALVES * half;
+            for (int j0 = 0; j0 < X; j0 += kWSteps) {
                 u32x4 w[TN];
 #pragma unroll
                 for (int t = 0; t < TN; ++t) w[t] = get_w(slot, t, j0 / kWSteps);
