@@ -287,7 +287,7 @@ __device__ __forceinline__ int tile_rows(const ExpertsParams& p, int unit_tile, 
 // could), which pass through wave-private LDS into the matrix layout: every load is row-contiguous, no barrier within an item.
 // Waves with items of their own, without the sums in LDS, were slower (us, 16 tokens, two of 8 experts 28672x4096 bf16 285 -> 316,
 // e4m3 145 -> 176). Measured (us, of the weights' bytes TB/s): 4 tokens, two of 8 experts 28672x4096 bf16 140, 6.7; e4m3 72, 6.5; INT4
-// 47, 5.2 (weights alone 39, the rest scales, x and decode); one token, eight of 64 experts 2816x2048 e4m3 8.8, 3.8.
+// 44.5, 5.4 (weights alone 39, the rest scales, x and decode); one token, eight of 64 experts 2816x2048 e4m3 8.8, 3.8.
 // ---------------------------------------------------------------------------------------------------------------
 // WIDE (INT4 of an even number of groups): stages of 256 columns, whole 128-byte lines of the weights.
 template <int F, int MT, bool WIDE>
@@ -577,18 +577,19 @@ experts_stream_kernel(const ExpertsParams p)
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// More rows an expert: a block is BM pairs by 8 or 16 tiles of weight rows, its 4 or 8 waves 1 x 4 or 2 x 4 parts of that. Two
-// places in LDS are filled in turn, one barrier a stage. Up to 128 pairs, where reading the weights still counts, the stages
-// come by way of registers with two of them in flight; larger blocks, whose sums take the registers, are filled straight from
-// memory while the stage before is multiplied. A block is a unit, and chunks of one expert and columns are neighbours, so that
-// they read the weights once: blocks that took several units, chunk by chunk, were slower (us, 64 tokens and two of 8 experts
-// 28672x4096 e4m3 169 -> 190). Measured: 4001 tokens, two of 8 experts 28672x4096 e4m3 1635 us, 1150 TFLOP/s, bf16 1028, INT4
-// 820, with zero points 670 (a library bf16 product of 1000x28672x4096: 1156); 509 tokens, four of 64 experts 2816x2048
-// bf16 143 us, 5.2 TB/s; 48 tokens, two of 8 experts 4096x14336 e4m3 83 us, 5.7 TB/s.
+// More rows an expert: a block is BM pairs by 8 or 16 tiles of weight rows, its 4 or 8 waves 1 x 4, 2 x 2 or 2 x 4 parts of that. Two
+// places in LDS are filled in turn, one barrier a stage. Up to 64 pairs (INT4 32), where reading the weights still counts, the
+// stages come by way of registers with two of them in flight; larger blocks, whose sums take the registers, are filled straight
+// from memory while the stage before is multiplied. A block is a unit, and chunks of one expert and columns are neighbours, so
+// that they read the weights once: blocks that took several units, chunk by chunk, were slower (us, 64 tokens and two of 8
+// experts 28672x4096 e4m3 169 -> 190). INT4 weights loaded by the lanes that use them, 64 bytes of a row at a time, without LDS
+// were slower (16 tokens 86 -> 101). Measured, two of 8 experts 28672x4096: 4001 tokens e4m3 1635 us, 1150 TFLOP/s, bf16 1055,
+// INT4 850, with zero points 670 (a library bf16 product of 1000x28672x4096: 1156); 48 tokens e4m3 152, 64 bf16 290 (6.2 and
+// 6.5 TB/s), 16 INT4 82 (5.9); 509 tokens, four of 64 experts 2816x2048 bf16 128 (5.8).
 // ---------------------------------------------------------------------------------------------------------------
 // SPLIT: two waves a part, which share the K of each stage. An INT4 wave has some 250 instructions a stage, as long as the stage's
 // bytes take: alone on its SIMD, as where there are few blocks, it kept the loads waiting (us, 16 tokens, two of 8 experts
-// 4096x14336: 57.3, two a part 48.2, without any products 43.4).
+// 4096x14336: 57.3, two a part 48.2, without any products 43.4; 44.5 since the weights pass by the caches).
 template <int F, int BM, bool WIDE, bool SPLIT>
 struct TileShape {
     static constexpr bool kI4F = F == kI4 || F == kI4ZP;
