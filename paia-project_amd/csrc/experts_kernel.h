@@ -997,12 +997,13 @@ int launch_tiles(ExpertsParams p, hipStream_t st)
 //                      1 e8 72/79 d8 38/52 e64 34.6/29.6, 1.5 e8 91/96 d8 51/54, 2 e8 142/132 d8 75/62 e64 50/47
 //         16 / 32      4 d8 69/70 e64 55/56, 5 e8 129/130 d8 63/65, 6 d8 109/81 d64 31/35, 16 e8 164/148; d64 10 38/41
 //         32 / 64, few units: 16 d8 84/95, 20 121/98, 38 123/100, 50 120/152; many: 19 e64 65/74, 31 79/87
-//         32 / 128     48 e64 99/101, 64 e64 116/114
+//         32 / 128     50 e64 99/97, 60 e8 260/265 d8 160/195, 64 e64 112/113, 75 e8 293/264, 88 e64 134/121
 //   BF16  MT 8 / 16    0.25 e64 18.2/18.7, 1 e64 56.9/56.7       MT 16 / 32 2 e64 90/96,
 //                      4 e8 281/284 d8 140/174 e64 109/122, 6 e8 328/285 d8 191/157 e64 120/115
 //         32 / 64      few units: 16 d8 173/175, 20 223/175, 25 210/171; many: 19 e64 119/124, 25 e8 317/300 d64 63/70,
 //                      31 e64 136/132
-//         64 / 256     64 e64 166/201, 128 e64 210/208
+//         64 / 128     62 e64 155/162, 75 e8 428/388 d8 240/281, 88 e64 182/182, 100 e8 480/428
+//         128 / 256    125 e64 199/211, 150 e8 539/483 d8 303/371, 187 e64 244/254, 250 e8 679/623
 //   INT4  MT 4 / 16    0.5 e8 39.1/40.8 d8 24.0/56, 1 e8 47.7/53.0 e64 25.6/24.5, 2 e8 91.6/85.6 d8 50.9/54.4 e64 38.0/37.9
 //         16 / 32      20 e8 157/164 d8 88/114 d64 (zp) 38/39, 25 e64 73/72 d64 (zp) 43.6/39.5, 28 e8 189/191
 //         32 / 64      50 e8 240/259 e64 111/109, 64 e8 289/268 e64 128/123
@@ -1042,7 +1043,7 @@ int launch_format(ExpertsParams p, hipStream_t st)
     } else if constexpr (F == kFP8) {
         if (streams(p, p.row_bytes >= 4096 ? E * 3 / 2 : E / 2)) return launch_stream<F, 4, false, GATED>(p, st);
         if (R <= (p.row_bytes < 2048 ? 12 : 5) * E) return launch_tiles<F, 16, false, false, GATED>(p, st);
-        if (R <= 56 * E) {
+        if (R <= 64 * E) {
             if (R > 16 * E && R <= 40 * E && tile_units<F, 64, false, false, GATED>(p) <= few_units)
                 return launch_tiles<F, 64, false, false, GATED>(p, st);
             return launch_tiles<F, 32, false, false, GATED>(p, st);
@@ -1053,7 +1054,8 @@ int launch_format(ExpertsParams p, hipStream_t st)
         if (streams(p, 5 * E)) return launch_stream<F, 16, false, GATED>(p, st);
         const int64_t most32 = tile_units<F, 64, false, false, GATED>(p) <= few_units ? 16 : 28;
         if (R <= most32 * E) return launch_tiles<F, 32, false, false, GATED>(p, st);
-        if (R <= 112 * E) return launch_tiles<F, 64, false, false, GATED>(p, st);
+        if (R <= 80 * E) return launch_tiles<F, 64, false, false, GATED>(p, st);
+        if (R <= 192 * E) return launch_tiles<F, 128, false, false, GATED>(p, st);
         return launch_tiles<F, 256, false, false, GATED>(p, st);
     }
 }
