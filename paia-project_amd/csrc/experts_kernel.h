@@ -584,7 +584,7 @@ experts_stream_kernel(const ExpertsParams p)
 // that they read the weights once: blocks that took several units, chunk by chunk, were slower (us, 64 tokens and two of 8
 // experts 28672x4096 e4m3 169 -> 190). INT4 weights loaded by the lanes that use them, 64 bytes of a row at a time, without LDS
 // were slower (16 tokens 86 -> 101). Measured, two of 8 experts 28672x4096: 4001 tokens e4m3 1635 us, 1150 TFLOP/s, bf16 1055,
-// INT4 850, with zero points 670 (a library bf16 product of 1000x28672x4096: 1156); 48 tokens e4m3 152, 64 bf16 290 (6.2 and
+// INT4 850, with zero points 770 (a library bf16 product of 1000x28672x4096: 1156); 48 tokens e4m3 152, 64 bf16 290 (6.2 and
 // 6.5 TB/s), 16 INT4 82 (5.9); 509 tokens, four of 64 experts 2816x2048 bf16 128 (5.8).
 // ---------------------------------------------------------------------------------------------------------------
 // SPLIT: two waves a part, which share the K of each stage. An INT4 wave has some 250 instructions a stage, as long as the stage's
@@ -1011,7 +1011,8 @@ int launch_tiles(ExpertsParams p, hipStream_t st)
 //                      121/115), 4 e8 89/91 (zp 98/95), 8 e64 42.3/43.8 (zp 48.6/45.4)
 //         16, weights kept / past the caches: 4 e8 88/82 d8 48/45, 8 e64 42/38 (zp 45/43), 13 of 60 1003x3584 (zp) 35.1/34.1,
 //                      20 e64 58/58 e8 143/149 d8 76/79
-//         64 / 128     with zero points never; without 256 e8 477/436, 512 1508/1307
+//         64 / 128     125 e8 418/433 e64 171/165 (zp 445/448, 188/175), 175 e8 533/546, 250 e8 746/706 d8 390/397 (zp 803/740,
+//                      428/422), 1000 e8 2659/2287 (zp 2891/2441)
 //   rows of 512 bytes, MT 4 / 16: E4M3 1024x512 11.4/7.9; of 704: INT4 d64 14.4/9.0; of 1024: INT4 e64 above; BF16 1024x512
 //   12.4/11.8; of 1408: E4M3 d64 14.2/9.7
 // Few units (no more than the chip holds at a time): an expert's second chunk is then another block on some of the CUs, and the call
@@ -1038,8 +1039,8 @@ int launch_format(ExpertsParams p, hipStream_t st)
             return launch_tiles<F, 32, WIDE, false, GATED>(p, st);
         };
         if (R <= 56 * E) return p.G % 2 == 0 && aligned(p.meta, 4) ? few(std::true_type{}) : few(std::false_type{});
-        if (F == kI4ZP || R <= 192 * E) return launch_tiles<F, 64, false, false, GATED>(p, st);
-        return launch_tiles<F, F == kI4 ? 128 : 64, false, false, GATED>(p, st);
+        if (R <= 192 * E) return launch_tiles<F, 64, false, false, GATED>(p, st);
+        return launch_tiles<F, 128, false, false, GATED>(p, st);
     } else if constexpr (F == kFP8) {
         if (streams(p, p.row_bytes >= 4096 ? E * 3 / 2 : E / 2)) return launch_stream<F, 4, false, GATED>(p, st);
         if (R <= (p.row_bytes < 2048 ? 12 : 5) * E) return launch_tiles<F, 16, false, false, GATED>(p, st);

@@ -51,7 +51,8 @@ def case(fmt, counts, N, K, k=1, gated=False, bias=False, shared=False, bare=0, 
 
 
 COUNTS = {"single": [1], "few": [1, 0, 2, 0, 0, 1, 0, 0], "eight": [3, 1, 0, 5, 2, 8, 1, 4], "sixteen": [16, 3, 0, 17, 9, 1],
-          "thirty": [33, 0, 31, 20], "sixty": [64, 65, 1, 50], "hundred": [129, 100, 0, 140], "many": [300, 257, 3]}
+          "thirty": [33, 0, 31, 20], "sixty": [64, 65, 1, 50], "hundred": [129, 100, 0, 140], "many": [300, 257, 3],
+          "more": [400, 310]}
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -64,7 +65,7 @@ def test_row_counts(cuda, fmt, counts):
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("N", [1, 2, 15, 16, 17, 31, 33, 255, 256, 257, 511, 514])
 def test_columns(cuda, fmt, N):
-    for counts, K in (([2, 1], 256), ([40, 30], 256), ([200, 150], 256), ([1, 1, 0], DEEP[fmt]), ([2, 5], DEEP[fmt])):
+    for counts, K in (([2, 1], 256), ([40, 30], 256), ([200, 150], 256), ([290, 200], 256), ([1, 1, 0], DEEP[fmt]), ([2, 5], DEEP[fmt])):
         case(fmt, counts, N, K, bias=True, seed=N)
         if N % 2 == 0:
             case(fmt, counts, N, K, gated=True, bias=True, seed=N)
@@ -86,6 +87,14 @@ def test_more_items_than_blocks(cuda, fmt):
     case(fmt, [2] * 7, 4100, DEEP[fmt], gated=True)
     case(fmt, [1, 0, 1, 1] * 25, 514, DEEP[fmt], gated=True, bare=9)
     case(fmt, [5] * 8, 10300, 256, bias=True)          # blocks of 16, more than the chip holds at a time
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_experts_of_many_chunks(cuda, fmt):
+    """Groups of eight columns of blocks through six chunks and more, the last group narrower, other experts beside them."""
+    case(fmt, [700, 30], 1300, 128, bias=True)
+    case(fmt, [3, 0, 210, 0, 1, 0, 0, 2], 1300, 128, bare=3)
+    case(fmt, [100, 7, 0, 0, 0, 0, 0, 0, 0, 0], 2050, 256, gated=True)
 
 
 @pytest.mark.parametrize("fmt", ["int4", "int4zp"])
