@@ -7,15 +7,15 @@
 //
 // Experts whose logit (or bias) is -inf or NaN are closed to the token; where fewer than k are open the rest of ids is -1, of
 // weight 0. A wave has a token, a lane every 64th expert of it: the largest key comes of one DPP maximum, its lowest index of
-// the lanes' ballots, k times. Keys that are computed (sigmoid), and all weights, are so in 64 bits: neighbouring keys decide
-// which experts run, and there are few of them.
+// the lanes' ballots, k times; a bf16 logit and its index are one key (8001 tokens, eight of 256 22.0 -> 19.4 us). Keys that are
+// computed (sigmoid), and all weights, are so in 64 bits: neighbouring keys decide which experts run, and there are few of them.
 //
 // order: the pairs m * k + j sorted by expert, in their own order within one, those without an expert at the end. A block counts
 // its pairs by wave and expert in LDS and gives each its place: the lanes with the same expert find each other by one ballot
 // a bit of the id. Few tokens are one launch of one block. Otherwise each block leaves its counts in the workspace and the second
 // launch's blocks add up those before their own (integers: the order of sums does not matter, nothing is atomic across blocks).
-// Bound by its dependent steps, k maxima and two walks over the pairs; two tokens a wave overlap theirs. Measured: one token, eight of 64
-// experts 4.4 us; 61 tokens, six of 160 by sigmoid 8.5 + 4.6; 8001 tokens, eight of 256 14.2 + 8.9, half of that VALU work.
+// Bound by its dependent steps, k maxima and two walks over the pairs; two tokens a wave overlap theirs. Measured: one token, eight
+// of 64 experts 4.2 us; 61 tokens, six of 160 by sigmoid 12.9; 8001 tokens, eight of 256 19.4, 9 of it the second launch.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -27,7 +27,7 @@ namespace paia {
 constexpr int kRouteBlock = 1024, kRouteWaves = kRouteBlock / kWave;
 constexpr int kRouteExperts = 1024;      // experts at most: a thread each in the scan
 constexpr int kRouteBlocks = 256;        // blocks at most that share the tokens
-constexpr int kRouteTokens = 32;          // tokens up to which one block does all of it (61 at a block: 11.8 us, in two launches 9.1)
+constexpr int kRouteTokens = 32;         // tokens up to which one block does all of it (61 at a block: 11.8 us, in two launches 9.1)
 
 struct RouteParams {
     const void* logits;                  // bf16 or fp32 [M][E]
@@ -123,8 +123,21 @@ __device__ __forceinline__ int take_largest(uint64_t (&key)[NE])
     return at;
 }
 
+// A bf16 logit's 16 sortable bits above its index from the far end: the largest is the largest logit at its lowest index, all that
+// a choice by softmax needs to know. 0: closed.
+__device__ __forceinline__ uint32_t packed_key(uint32_t b, int e)
+{
+    if ((b & 0x7FFFu) > 0x7F80u || b == 0xFF80u) return 0;       // NaN, -inf
+    if (b == 0x8000u) b = 0;
+    return (b >> 15 ? ~b & 0xFFFFu : b | 0x8000u) << 16 | (0xFFFFu - (uint32_t)e);
+}
+__device__ __forceinline__ float packed_logit(uint32_t key)
+{
+    return __uint_as_float(key >> 31 ? (key & 0x7FFF0000u) : ~key & 0xFFFF0000u);
+}
+
 // The choices of T tokens m, m + step, .. by one wave, whose chains of dependent steps overlap. The lanes j < k write them.
-template <int NE, bool SIGMOID, int T>
+template <int NE, bool SIGMOID, bool PACKED, int T>
 __device__ __forceinline__ void choose(const RouteParams& p, int m, int step)
 {
     const int lane = lane_id();
@@ -137,40 +150,69 @@ __device__ __forceinline__ void choose(const RouteParams& p, int m, int step)
             v[u][i] = -__builtin_inff();
             if (e < p.E) {
                 const int64_t at = (int64_t)(m + u * step) * p.stride + e;
-                v[u][i] = p.fp32 ? static_cast<const float*>(p.logits)[at] : bf16_to_f32(static_cast<const uint16_t*>(p.logits)[at]);
+                v[u][i] = !PACKED && p.fp32 ? static_cast<const float*>(p.logits)[at] : bf16_to_f32(static_cast<const uint16_t*>(p.logits)[at]);
             }
         }
-    using Key = typename std::conditional<SIGMOID, uint64_t, uint32_t>::type;
-    Key key[T][NE];
-#pragma unroll
-    for (int i = 0; i < NE; ++i) {
-        double b = 0.0;
-        if constexpr (SIGMOID)
-            if (p.bias != nullptr && lane + 64 * i < p.E) b = (double)p.bias[lane + 64 * i];
-#pragma unroll
-        for (int u = 0; u < T; ++u) {
-            const bool open = v[u][i] > -__builtin_inff();
-            if constexpr (SIGMOID) {
-                key[u][i] = open && b > -__builtin_inf() ? sortable(1.0 / (1.0 + exp(-(double)v[u][i])) + b) : 0;
-            } else {
-                key[u][i] = open ? sortable(v[u][i]) : 0;
-            }
-        }
-    }
     int id[T];
     float top[T], mine[T];               // the largest logit, and that of the lane's expert
 #pragma unroll
     for (int u = 0; u < T; ++u) id[u] = -1, top[u] = mine[u] = 0.0f;
-    for (int j = 0; j < p.k; ++j) {
+    if constexpr (PACKED) {
+        uint32_t key[T][NE], first[T], own[T];
 #pragma unroll
         for (int u = 0; u < T; ++u) {
-            const int e = take_largest<NE>(key[u]);
-            float logit = 0.0f;
+            first[u] = own[u] = 0;
 #pragma unroll
-            for (int i = 0; i < NE; ++i)
-                if (e >> 6 == i) logit = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v[u][i]), e & 63));
-            if (j == 0) top[u] = logit;
-            if (lane == j) id[u] = e, mine[u] = logit;
+            for (int i = 0; i < NE; ++i) key[u][i] = packed_key(__float_as_uint(v[u][i]) >> 16, lane + 64 * i);
+        }
+        for (int j = 0; j < p.k; ++j) {
+#pragma unroll
+            for (int u = 0; u < T; ++u) {
+                uint32_t most = 0;
+#pragma unroll
+                for (int i = 0; i < NE; ++i) most = max(most, key[u][i]);
+                most = wave_max_u32(most);
+#pragma unroll
+                for (int i = 0; i < NE; ++i) key[u][i] = key[u][i] == most ? 0u : key[u][i];
+                if (j == 0) first[u] = most;
+                if (lane == j) own[u] = most;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < T; ++u)
+            if (own[u] != 0) id[u] = (int)(0xFFFFu - (own[u] & 0xFFFFu)), mine[u] = packed_logit(own[u]);
+#pragma unroll
+        for (int u = 0; u < T; ++u)
+            if (first[u] != 0) top[u] = packed_logit(first[u]);
+    } else {
+        using Key = typename std::conditional<SIGMOID, uint64_t, uint32_t>::type;
+        Key key[T][NE];
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+            double b = 0.0;
+            if constexpr (SIGMOID)
+                if (p.bias != nullptr && lane + 64 * i < p.E) b = (double)p.bias[lane + 64 * i];
+#pragma unroll
+            for (int u = 0; u < T; ++u) {
+                const bool open = v[u][i] > -__builtin_inff();
+                if constexpr (SIGMOID) {
+                    key[u][i] = open && b > -__builtin_inf() ? sortable(1.0 / (1.0 + exp(-(double)v[u][i])) + b) : 0;
+                } else {
+                    key[u][i] = open ? sortable(v[u][i]) : 0;
+                }
+            }
+        }
+        for (int j = 0; j < p.k; ++j) {
+#pragma unroll
+            for (int u = 0; u < T; ++u) {
+                const int e = take_largest<NE>(key[u]);
+                float logit = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NE; ++i)
+                    if (e >> 6 == i) logit = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v[u][i]), e & 63));
+                if (j == 0) top[u] = logit;
+                if (lane == j) id[u] = e, mine[u] = logit;
+            }
         }
     }
 #pragma unroll
@@ -271,10 +313,15 @@ __global__ void __launch_bounds__(kRouteBlock) route_kernel(const RouteParams p)
     const int wave = wave_id(), t = (int)threadIdx.x;
     const int m0 = (int)blockIdx.x * p.tokens, m1 = min(p.M, m0 + p.tokens);
     if constexpr (SELECT) {
-        int m = m0 + wave;
-        if constexpr (NE <= 4)
-            for (; m + kRouteWaves < m1; m += 2 * kRouteWaves) choose<NE, SIGMOID, 2>(p, m, kRouteWaves);
-        for (; m < m1; m += kRouteWaves) choose<NE, SIGMOID, 1>(p, m, kRouteWaves);
+        const auto all = [&](auto packed) __attribute__((always_inline)) {
+            constexpr bool PACKED = decltype(packed)::value;
+            int m = m0 + wave;
+            if constexpr (NE <= 4)
+                for (; m + kRouteWaves < m1; m += 2 * kRouteWaves) choose<NE, SIGMOID, PACKED, 2>(p, m, kRouteWaves);
+            for (; m < m1; m += kRouteWaves) choose<NE, SIGMOID, PACKED, 1>(p, m, kRouteWaves);
+        };
+        if (SIGMOID || p.fp32) all(std::false_type{});
+        else all(std::bool_constant<!SIGMOID>{});
     }
     for (int e = t; e <= p.E; e += kRouteBlock)
 #pragma unroll

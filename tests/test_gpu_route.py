@@ -51,15 +51,20 @@ def test_many_tokens(cuda, M):
         order, offsets = order64(want.cpu(), E)
         assert torch.equal(got[2].cpu(), order) and torch.equal(got[3].cpu(), offsets)
         check(x[:50], k, ops.route_experts(x[:50], k))
+        x = x.bfloat16()                                 # ties in many rows
+        got = ops.route_experts(x, k)
+        assert torch.equal(got[0], torch.sort(x.float(), dim=1, descending=True, stable=True).indices[:, :k].int())
 
 
-def test_ties_go_to_the_lower_index(cuda):
-    for E in (64, 200):
-        x = torch.zeros(5, E, device=cuda)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_ties_go_to_the_lower_index(cuda, dtype):
+    for E in (64, 200, 1024):
+        x = torch.zeros(5, E, device=cuda, dtype=dtype)
         x[1, ::2] = -0.0
         x[2, 3::5] = 1.0
         x[3] = torch.arange(E, device=cuda) % 3
         x[4] = -7.0
+        x[4, 1::3] = -7.03125
         for scoring in ("softmax", "sigmoid"):
             note(f"route ties E={E} {scoring}")
             check(x, 8, ops.route_experts(x, 8, scoring=scoring), scoring=scoring)
@@ -88,9 +93,10 @@ def test_closed_experts(cuda, scoring):
                   renormalize=renormalize)
 
 
-def test_infinite_logits(cuda):
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_infinite_logits(cuda, dtype):
     """An infinite logit is chosen first; its softmax is NaN, as inf - inf is."""
-    x = random_logits(2, 64, torch.float32)
+    x = random_logits(2, 64, dtype)
     x[0, 9] = math.inf
     note("route infinite")
     ids, w, _, _ = ops.route_experts(x, 4)
