@@ -121,3 +121,39 @@ def test_command(cuda, capsys):
     for bad in (["--batch", "17"], ["--chosen", "9"], ["--chosen", "0"]):
         with pytest.raises(SystemExit):
             main(bad)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int4"])
+def test_two_steps_at_once(cuda, fmt):
+    """Steps of two sizes on two streams, over and over, each as alone."""
+    block = ExpertBlock(1024, 512, 16, 4, fmt, seed=6)
+    g = torch.Generator().manual_seed(7)
+    sizes = (2, 16)
+    rows = [[torch.randn(n, 1024, generator=g).bfloat16().to(cuda) for _ in range(2)] for n in sizes]
+    want = [[t.clone() for t in block.step(*r)] for r in rows]
+    streams = [torch.cuda.Stream() for _ in sizes]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    note(f"expert block on two streams {fmt}")
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(block.step(*rows[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(bits(a), bits(b)) for step in got[i] for a, b in zip(step, want[i]))
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "fp8", "int4", "int4zp"])
+def test_the_same_expert_twice(cuda, fmt):
+    """Ids that name an expert more than once, or one that is not there: pairs of their own, and zeros."""
+    block = ExpertBlock(2048, 128, 6, 3, fmt, seed=8)
+    ids = torch.tensor([[4, 4, 4], [1, 9, 1], [-1, -1, -1], [0, 5, 4]], dtype=torch.int32, device=cuda)
+    x = torch.randn(4, 2048, generator=torch.Generator().manual_seed(9)).bfloat16().to(cuda)
+    note(f"the same expert twice {fmt}")
+    order, offsets = ops.expert_order(ids, 6)
+    out = block.gate_up(x, order, offsets, gated=True).view(4, 3, -1)
+    check_experts(block.gate_up, out.view(12, -1), x, order, offsets, True)
+    assert torch.equal(bits(out[0, 0]), bits(out[0, 1])) and torch.equal(bits(out[0, 0]), bits(out[0, 2]))
+    assert torch.equal(bits(out[1, 0]), bits(out[1, 2])) and not bits(out[1, 1]).any() and not bits(out[2]).any()
