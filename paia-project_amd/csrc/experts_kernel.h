@@ -878,7 +878,8 @@ experts_tile_kernel(const ExpertsParams p)
         };
         // Weights that no other block reads pass by the caches (us, two of 8 experts 28672x4096, 64 tokens bf16 323 -> 293, 48 e4m3
         // 170 -> 152; 509 tokens, four of 64 experts 2816x2048 bf16 145 -> 128), those of several chunks do not: bf16, 300 tokens
-        // 429, past the caches 527. Nor do rows whose lines two stages share (d64 INT4 of 11 groups 24.7 -> 26.0). For INT4 the host decides (PAST): two loops would share too few registers.
+        // 429, past the caches 527. Nor do rows whose lines two stages share (INT4 of 11 groups, 32 tokens, eight of 64 experts
+        // 2048x1408 24.7 -> 26.0). For INT4 the host decides (PAST): two loops would share too few registers.
         if (I4 ? PAST : __builtin_amdgcn_readfirstlane(u.chunks) == 1 && p.row_bytes % 128 == 0) run(std::true_type{});
         else run(std::false_type{});
     }
