@@ -942,14 +942,14 @@ experts_tile_kernel(const ExpertsParams p)
 
 // Launches of a format's kernels; p as the entry point fills it. 0, -2 (more blocks than a launch has) or a hipError_t.
 constexpr int kMostBlocks = 1 << 22;
-// Sets what depends on the kernel's shape; the units, at most kMostBlocks, or -2.
+// Sets what depends on the kernel's shape; the units that these sizes can need.
 inline int64_t plan_experts(ExpertsParams& p, int BM, int unit_cols)
 {
     p.tiles = (int)(((int64_t)p.cols + unit_cols - 1) / unit_cols);
     p.by_tiles = Divisor((uint32_t)p.tiles);
     const int64_t bins = p.R < p.E + 1 ? p.R : p.E + 1, most = ((int64_t)p.R + bins * (BM - 1)) / BM;
     p.most = (int)most;
-    return most * p.tiles <= kMostBlocks ? most * p.tiles : -2;
+    return most * p.tiles;
 }
 // A share's bounds, items * (block + 1), lie below 2^32.
 constexpr int64_t kMostItems = 1 << 20;
@@ -987,7 +987,12 @@ int launch_tiles(ExpertsParams p, hipStream_t st)
 {
     using T = TileShape<F, BM, WIDE, SPLIT>;
     const int64_t units = tile_units<F, BM, WIDE, SPLIT, GATED>(p);
-    if (units < 0) return -2;
+    if (units > kMostBlocks) {
+        // the format's largest blocks, of which there are the fewest, are what the contract counts
+        constexpr int kLargest = F == kBF16 ? 256 : 128;
+        if constexpr (BM < kLargest) return launch_tiles<F, kLargest, false, false, GATED>(p, st);
+        return -2;
+    }
     hipLaunchKernelGGL((experts_tile_kernel<F, BM, WIDE, SPLIT, PAST, GATED>), dim3((uint32_t)units), dim3(T::kWaves * kWave), 0, st, p);
     return (int)hipGetLastError();
 }
