@@ -5,8 +5,8 @@
 // The pairs come ordered by expert (`order`, `offsets`), as many each as the tokens happened to choose; what a call has to do
 // is known on the device alone. So the host launches the most blocks that these sizes can need, and a block finds from the
 // offsets which expert, which of its chunks of at most BM pairs and which columns are its own, or that there is nothing left
-// (unit_of: one load a lane and a scan, no list has to be made beforehand). Units of one expert and columns follow each
-// other, and each of the 8 XCDs takes a contiguous range of them: its chunks read the weights from one L2.
+// (unit_of: one load a lane and a scan, no list has to be made beforehand; the arithmetic is in expert_units.h). Units of one
+// expert and columns follow each other, and each of the 8 XCDs takes a contiguous range of them: its chunks read the weights from one L2.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -14,6 +14,7 @@
 #include <type_traits>
 
 #include "divisor.h"
+#include "expert_units.h"
 #include "gemv_tile.h"
 
 namespace paia {
@@ -38,12 +39,6 @@ struct ExpertsParams {
     Divisor by_tiles, by_pairs;      // by `tiles`; by the pairs that share a row of x
 };
 
-struct ExpertUnit {
-    int expert;              // E: pairs without an expert; -1: no unit
-    int first, held, tile;   // its pairs are order[first .. first + held)
-    int chunks;              // of its expert
-};
-
 __device__ __forceinline__ int wave_inclusive(int v)
 {
     // row-wise shifts, then the row ends carried on: lane 63 holds the sum
@@ -56,59 +51,35 @@ __device__ __forceinline__ int wave_inclusive(int v)
     return v;
 }
 
-// How many chunks of BM pairs the experts have, and which one is which; the same in every lane but `upto`. Offsets are taken as
-// they are but for their range: whatever they hold, the pairs of a chunk lie within the call's.
+// How many chunks of BM pairs the experts have, and which one is which; the same in every lane but `upto` and `mine`. What a
+// lane does by itself is in expert_units.h.
 template <int BM>
 struct Chunks {
     int count, rest_at, rest;            // rest: chunks of the pairs without an expert, order[rest_at ..]
-    int upto, own;                       // chunks of the experts up to the lane's last, and of the lane's
-    int from, to;                        // where the pairs of the lane's first expert begin, and of its last one end
+    int upto;                            // chunks of the experts up to the lane's last
+    LaneChunks mine;
     int order;                           // of up to 64 pairs the lane's, loaded beside the offsets
 
-    __device__ __forceinline__ int place(const ExpertsParams& p, int e) const { return min(max(p.offsets[min(e, p.E)], 0), p.R); }
     __device__ __forceinline__ explicit Chunks(const ExpertsParams& p)
     {
-        const int e0 = lane_id() * p.lane_experts;
         order = p.order[min(lane_id(), p.R - 1)];
-        rest_at = place(p, p.E);
-        from = place(p, e0);
-        own = 0;
-        for (int i = 1, begin = from; i <= p.lane_experts; ++i) {
-            to = place(p, e0 + i);
-            own += (max(to - begin, 0) + BM - 1) / BM;
-            begin = to;
-        }
-        own = min(own, p.most);                  // no more than that in all, unless the offsets are not in order
-        upto = wave_inclusive(own);
+        rest_at = pairs_begin(p.offsets, p.E, p.E, p.R);
+        mine = lane_chunks(p.offsets, p.E, p.R, BM, lane_id() * p.lane_experts, p.lane_experts, p.most);
+        upto = wave_inclusive(mine.own);
         count = min(__builtin_amdgcn_readlane(upto, 63), p.most);
-        rest = min((p.R - rest_at + BM - 1) / BM, p.most - count);
+        rest = min(chunks_of(p.R - rest_at, BM), p.most - count);
     }
-    // The expert of chunk c < count, its pairs order[lo .. hi), and its chunks begin .. begin + n - 1.
-    struct Expert {
-        int expert, lo, hi, begin, n;
-    };
-    __device__ __forceinline__ Expert of(const ExpertsParams& p, int c) const
+    // That of chunk c < count.
+    __device__ __forceinline__ ChunkExpert of(const ExpertsParams& p, int c) const
     {
-        const int owner = __builtin_ctzll(__ballot(upto > c)), e0 = lane_id() * p.lane_experts;
-        int e = lane_id(), begin = upto - own, lo = from, hi = to, n = own;
-        if (p.lane_experts > 1) {
-            int at = begin, a = from;
-            for (int i = 1; i <= p.lane_experts; ++i) {
-                const int b = place(p, e0 + i), k = (max(b - a, 0) + BM - 1) / BM;
-                if (c >= at && c < at + k) e = e0 + i - 1, begin = at, lo = a, hi = b, n = k;
-                at += k;
-                a = b;
-            }
-        }
-        return {__builtin_amdgcn_readlane(e, owner), __builtin_amdgcn_readlane(lo, owner), __builtin_amdgcn_readlane(hi, owner),
-                __builtin_amdgcn_readlane(begin, owner), __builtin_amdgcn_readlane(n, owner)};
+        const int owner = __builtin_ctzll(__ballot(upto > c));
+        const ChunkExpert x = expert_of(p.offsets, p.E, p.R, BM, lane_id() * p.lane_experts, p.lane_experts, mine, upto - mine.own, c);
+        return {__builtin_amdgcn_readlane(x.expert, owner), __builtin_amdgcn_readlane(x.lo, owner), __builtin_amdgcn_readlane(x.hi, owner),
+                __builtin_amdgcn_readlane(x.begin, owner), __builtin_amdgcn_readlane(x.n, owner)};
     }
 };
 
-// Block b's place when each of the 8 XCDs, to which blocks are dealt in turn, takes a contiguous range of n.
-__device__ __forceinline__ int xcd_contiguous(int b, int n) { return b % 8 * (n / 8) + min(b % 8, n % 8) + b / 8; }
-
-// The unit of this block: units of one expert and tile (or group of tiles) follow each other.
+// The unit of this block.
 template <int BM>
 __device__ __forceinline__ ExpertUnit unit_of(const ExpertsParams& p)
 {
@@ -118,23 +89,8 @@ __device__ __forceinline__ ExpertUnit unit_of(const ExpertsParams& p)
     // units without an expert come last: dealt out with the others they left one XCD almost nothing to do
     const int u = b < units ? xcd_contiguous(b, units) : b;
     const int c = (int)p.by_tiles.of((uint32_t)u);
-    if (c >= chunks.count) {
-        const int first = chunks.rest_at + (c - chunks.count) * BM;
-        return {p.E, first, min(BM, p.R - first), u - c * p.tiles, 0};
-    }
-    const auto x = chunks.of(p, c);
-    // eight tiles at a time through all of many chunks: of 8 tiles by 8 chunks, as an XCD holds at a time, rows and weights alike come
-    // once to its L2 (us, two of 8 experts 28672x4096 e4m3, 8001 tokens 3836 -> 3265, 4001 1738 -> 1681; fewer chunks +-1%)
-    const int local = u - x.begin * p.tiles;
-    int tile, chunk;
-    if (BM < 256 && x.n >= 6) {
-        const int g = local / (8 * x.n), in = local - g * 8 * x.n, wide = min(8, p.tiles - g * 8);
-        chunk = in / wide, tile = g * 8 + in - chunk * wide;
-    } else {
-        tile = local / x.n, chunk = local - tile * x.n;
-    }
-    const int first = x.lo + chunk * BM;
-    return {x.expert, first, min(BM, x.hi - first), tile, x.n};
+    if (c >= chunks.count) return unit_without<BM>(p.E, p.R, chunks.rest_at, c - chunks.count, u - c * p.tiles);
+    return unit_in<BM>(chunks.of(p, c), u, p.tiles);
 }
 
 __device__ __forceinline__ int pair_at(const ExpertsParams& p, const ExpertUnit& u, int i)
@@ -323,8 +279,8 @@ __device__ __forceinline__ void stream_items(const ExpertsParams& p, StreamSpace
     constexpr int kOuts = GATED ? P / 2 : P, kOutCols = kOuts * kTileRows;
 
     const int lane = lane_id(), wave = wave_id(), ln = lane & 15, lh = lane >> 4;
-    const int stages = (p.K + C - 1) / C, k0 = stages * wave / WAVES;          // this wave's stages; where there are none,
-    const int mine_n = stages * (wave + 1) / WAVES - k0;                       // one that reads nothing
+    const int stages = (p.K + C - 1) / C, k0 = wave_begin(stages, wave, WAVES);      // this wave's stages; where there are none,
+    const int mine_n = wave_begin(stages, wave + 1, WAVES) - k0;                     // one that reads nothing
     const int n = max(1, mine_n);
     const int columns = mine_n > 0 ? p.K : 0;
     const int64_t row0 = (int64_t)expert * p.N;
@@ -552,10 +508,10 @@ experts_stream_kernel(const ExpertsParams p)
 {
     __shared__ StreamSpace<F, MT, WIDE> space;
     const Chunks<MT> chunks(p);
-    // below 2^32: at most kMostItems, and fewer than 2^10 blocks
+    // below 2^32: at most kMostItems, and fewer than 2^12 blocks
     const uint32_t block = (uint32_t)xcd_contiguous((int)blockIdx.x, (int)gridDim.x), blocks = gridDim.x;
-    const uint32_t items = (uint32_t)(chunks.count * p.tiles), end = items * (block + 1) / blocks;
-    for (uint32_t item = items * block / blocks; item < end;) {
+    const uint32_t items = (uint32_t)(chunks.count * p.tiles), end = share_begin(items, block + 1, blocks);
+    for (uint32_t item = share_begin(items, block, blocks); item < end;) {
         const int chunk = (int)p.by_tiles.of(item), group0 = (int)item - chunk * p.tiles;
         const int groups = min(p.tiles - group0, (int)(end - item));
         const auto x = chunks.of(p, chunk);
@@ -568,8 +524,8 @@ experts_stream_kernel(const ExpertsParams p)
     // four such pairs of 16 tokens were 10 of 85 us)
     const uint32_t width = StreamShape<F, MT, WIDE>::kWaves * kWave, pieces = ((uint32_t)p.cols + width - 1) / width;
     const uint64_t all = (uint64_t)(uint32_t)(p.R - chunks.rest_at) * pieces;
-    const uint64_t last = all * (block + 1) / blocks;
-    for (uint64_t i = all * block / blocks; i < last; ++i) {
+    const uint64_t last = share_begin<uint64_t>(all, block + 1, blocks);
+    for (uint64_t i = share_begin<uint64_t>(all, block, blocks); i < last; ++i) {
         const uint32_t r = (uint32_t)i / pieces, col = ((uint32_t)i - r * pieces) * width + threadIdx.x;
         const int pair = p.order[chunks.rest_at + (int)r];
         if ((uint32_t)pair < (uint32_t)p.R && col < (uint32_t)p.cols) p.out[(int64_t)pair * p.out_stride + col] = 0;
@@ -941,18 +897,15 @@ experts_tile_kernel(const ExpertsParams p)
 // ---------------------------------------------------------------------------------------------------------------
 
 // Launches of a format's kernels; p as the entry point fills it. 0, -2 (more blocks than a launch has) or a hipError_t.
-constexpr int kMostBlocks = 1 << 22;
 // Sets what depends on the kernel's shape; the units that these sizes can need.
 inline int64_t plan_experts(ExpertsParams& p, int BM, int unit_cols)
 {
     p.tiles = (int)(((int64_t)p.cols + unit_cols - 1) / unit_cols);
     p.by_tiles = Divisor((uint32_t)p.tiles);
-    const int64_t bins = p.R < p.E + 1 ? p.R : p.E + 1, most = ((int64_t)p.R + bins * (BM - 1)) / BM;
+    const int64_t most = most_chunks(p.R, p.E, BM);
     p.most = (int)most;
     return most * p.tiles;
 }
-// A share's bounds, items * (block + 1), lie below 2^32.
-constexpr int64_t kMostItems = 1 << 20;
 template <int F, int MT, bool WIDE, bool GATED>
 int launch_stream(ExpertsParams p, hipStream_t st)
 {
@@ -973,8 +926,7 @@ int launch_stream(ExpertsParams p, hipStream_t st)
 // is two lines or more.
 inline bool streams(const ExpertsParams& p, int64_t pairs)
 {
-    const int64_t R = p.R, bins = R < p.E + 1 ? R : p.E + 1, chunks = (R + bins * 3) / 4;     // MT >= 4
-    return R <= pairs && p.x_bytes != 0 && p.row_bytes >= 1024 && chunks * ((p.cols + 15) / 16) <= kMostItems;
+    return p.R <= pairs && p.x_bytes != 0 && p.row_bytes >= 1024 && most_chunks(p.R, p.E, 4) * ((p.cols + 15) / 16) <= kMostItems;
 }
 template <int F, int BM, bool WIDE, bool SPLIT, bool GATED>
 int64_t tile_units(ExpertsParams& p)
