@@ -444,11 +444,15 @@ template <bool SIGMOID, bool SELECT, bool ONE>
 static void launch_route(const RouteParams& p, int blocks, hipStream_t st)
 {
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(kRouteBlock), 0, st, p); };
-    if (!SELECT || p.E <= 64) go(route_kernel<1, SIGMOID, SELECT, ONE>);
-    else if (p.E <= 128) go(route_kernel<2, SIGMOID, SELECT, ONE>);
-    else if (p.E <= 256) go(route_kernel<4, SIGMOID, SELECT, ONE>);
-    else if (p.E <= 512) go(route_kernel<8, SIGMOID, SELECT, ONE>);
-    else go(route_kernel<16, SIGMOID, SELECT, ONE>);
+    if constexpr (!SELECT) {
+        go(route_kernel<1, SIGMOID, SELECT, ONE>);           // holds no logits
+    } else {
+        if (p.E <= 64) go(route_kernel<1, SIGMOID, SELECT, ONE>);
+        else if (p.E <= 128) go(route_kernel<2, SIGMOID, SELECT, ONE>);
+        else if (p.E <= 256) go(route_kernel<4, SIGMOID, SELECT, ONE>);
+        else if (p.E <= 512) go(route_kernel<8, SIGMOID, SELECT, ONE>);
+        else go(route_kernel<16, SIGMOID, SELECT, ONE>);
+    }
 }
 
 static int run_route(RouteParams& p, bool select, bool sigmoid, void* workspace, long long bytes, hipStream_t st)
