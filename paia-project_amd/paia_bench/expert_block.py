@@ -4,12 +4,12 @@
     experts -> their gate and up projections (silu(gate) * up) -> their down projections -> sum by the router's weights,
     residual and the next layer's norm
 
-for a batch of tokens, one of each sequence. Rows without a token (a captured batch that is not full) are marked in `absent`: they
-choose no experts. Weights are random (seeded), every expert of the size of the model's feed-forward block.
+for a batch of tokens, one of each sequence, or a prompt's. Rows without a token (a captured batch that is not full) are marked in
+`absent`: they choose no experts. Weights are random (seeded), every expert of the size of the model's feed-forward block.
 
     python -m paia_bench.expert_block --model llama31_8b --fmt fp8 --experts 8 --chosen 2 --batch 8
 
-times a step. The layer's experts together can exceed the 256 MiB last-level cache by far while the chosen ones lie in it whole, so
+times a step of a decode batch. The layer's experts together can exceed the 256 MiB last-level cache by far while the chosen ones lie in it whole, so
 the command steps as many blocks in turn (`copies`) as keep any of them from being found there when it is next used.
 """
 from __future__ import annotations
@@ -63,8 +63,18 @@ class ExpertBlock:
         self.norm, self.next_norm = bf16(hidden, by=0.1) + 1.0, bf16(hidden, by=0.1) + 1.0
         self.post_norm = bf16(hidden, by=0.1) + 1.0 if post_norm else None
 
+    def logits(self, x):
+        """The router's product with x [tokens, hidden], bf16 [tokens, experts]: up to 16 rows as a small batch, more as the product
+        with the one expert that all of them have chosen."""
+        tokens = len(x)
+        if tokens <= 16:
+            return ops.gemv_bf16(self.router, x)
+        order = torch.arange(tokens, dtype=torch.int32, device=x.device)
+        offsets = torch.arange(0, tokens + 1, tokens, dtype=torch.int32, device=x.device)
+        return ops.experts_bf16(self.router[None], x, order, offsets)
+
     def route(self, x, absent=None):
-        logits = ops.gemv_bf16(self.router, x)
+        logits = self.logits(x)
         if absent is not None:
             logits = logits.masked_fill(absent[:, None], float("-inf"))
         return ops.route_experts(logits, self.chosen)
@@ -93,7 +103,7 @@ def main(argv=None):
     ap.add_argument("--steps", type=int, default=32)
     a = ap.parse_args(argv)
     if not 1 <= a.batch <= 16:
-        ap.error("--batch: the router's projection takes 1 to 16 rows")
+        ap.error("--batch: 1 to 16 sequences")
     if not 1 <= a.chosen <= a.experts:
         ap.error("--chosen: 1 to --experts")
     _, hidden, down = next(shape for shape in LAYER[a.model] if shape[0] == "down")
