@@ -262,7 +262,8 @@ PAIA_API int paia_expert_order(const void* ids, void* order, void* offsets, int 
  * offsets[experts] on) are 0. fp32 sums, one rounding at the end; W, scale(s), zeros and bias as [experts] times the
  * operands of the M = 1 entry point of the format, same alignment and rules for K. x and its rows 16-byte aligned, out
  * bf16, its rows anywhere; strides in elements. out overlaps nothing. order and offsets are read on the device (a captured
- * call follows them); entries outside their ranges are not followed. experts <= 1024, pairs < 2^26, N and K <= 2^25, and at most
+ * call follows them); entries outside their ranges are not followed. The kernel is chosen by pairs / experts, pairs without an
+ * expert included. INT4: a row of x with an infinity in it gives NaN (a group's sums of q x and of x are taken apart). experts <= 1024, pairs < 2^26, N and K <= 2^25, and at most
  * 2^22 blocks of 128 pairs of an expert by 128 rows (BF16 of 256 by 256): (pairs + min(pairs, experts + 1) * 127) / 128 times
  * ceil(N / 128), -2 beyond; pairs = 0 does nothing. */
 PAIA_API int paia_experts_bf16(const void* W, const void* x, long long x_stride, int x_rows, const void* order,

@@ -9,7 +9,8 @@
 // threads hold the row's values in registers from the first load to the last store. Bound by bytes where there are many rows
 // and by latency (the loads, then one or two sums over the block) where there is one: every load is on its way ahead of the
 // first sum. Measured: 8001 tokens of two pairs of 4096 56 to 58 us (5.7 TB/s; a copy moves 4.9), 13 tokens of eight pairs of 3584 with
-// a norm behind the block 4.5, one token 2.6, of which the launch is 1.6.
+// a norm behind the block 5.0, one token 2.7, of which the launch is 1.6. Four pieces a thread with pairs (D beyond 16384) keep 46 and more
+// registers in memory: 2000 tokens of two pairs of 18944 143 us (2.6 TB/s), of 16384 68 (4.8), of 18944 without pairs 58 (5.2).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

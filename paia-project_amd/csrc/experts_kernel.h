@@ -243,7 +243,7 @@ __device__ __forceinline__ int tile_rows(const ExpertsParams& p, int unit_tile, 
 // could), which pass through wave-private LDS into the matrix layout: every load is row-contiguous, no barrier within an item.
 // Waves with items of their own, without the sums in LDS, were slower (us, 16 tokens, two of 8 experts 28672x4096 bf16 285 -> 316,
 // e4m3 145 -> 176). Measured (us, of the weights' bytes TB/s): 4 tokens, two of 8 experts 28672x4096 bf16 140, 6.7; e4m3 72, 6.5; INT4
-// 44.5, 5.4 (weights alone 39, the rest scales, x and decode); one token, eight of 64 experts 2816x2048 e4m3 8.8, 3.8.
+// 44.5, 5.4 (weights alone 39, the rest scales, x and decode); one token, eight of 64 experts 2048x2048 e4m3 8.8, 3.8.
 // ---------------------------------------------------------------------------------------------------------------
 // WIDE (INT4 of an even number of groups): stages of 256 columns, whole 128-byte lines of the weights.
 template <int F, int MT, bool WIDE>
@@ -539,8 +539,8 @@ experts_stream_kernel(const ExpertsParams p)
 // from memory while the stage before is multiplied. A block is a unit, and chunks of one expert and columns are neighbours, so
 // that they read the weights once: blocks that took several units, chunk by chunk, were slower (us, 64 tokens and two of 8
 // experts 28672x4096 e4m3 169 -> 190). INT4 weights loaded by the lanes that use them, 64 bytes of a row at a time, without LDS
-// were slower (16 tokens 86 -> 101). Measured, two of 8 experts 28672x4096: 4001 tokens e4m3 1635 us, 1150 TFLOP/s, bf16 1055,
-// INT4 850, with zero points 770 (a library bf16 product of 1000x28672x4096: 1156); 48 tokens e4m3 152, 64 bf16 290 (6.2 and
+// were slower (16 tokens 86 -> 101). Measured, two of 8 experts 28672x4096: 4001 tokens e4m3 1635 us, 1150 TFLOP/s, bf16 1015 to 1055,
+// INT4 840, with zero points 790 (a library bf16 product of 1000x28672x4096: 1156); 48 tokens e4m3 152, 64 bf16 290 (6.2 and
 // 6.5 TB/s), 16 INT4 82 (5.9); 509 tokens, four of 64 experts 2816x2048 bf16 128 (5.8).
 // ---------------------------------------------------------------------------------------------------------------
 // SPLIT: two waves a part, which share the K of each stage. An INT4 wave has some 250 instructions a stage, as long as the stage's
@@ -913,7 +913,10 @@ int launch_stream(ExpertsParams p, hipStream_t st)
     const int64_t items = plan_experts(p, MT, (GATED ? T::kTiles / 2 : T::kTiles) * kTileRows);
     const int64_t resident = T::kBlocks * device_facts().cus;
     // Weights pass by the caches where a stage has whole lines; lines that two stages share are kept for the second (us, 4 tokens, two
-    // of 8 experts 28672x4112 e4m3 96, past the caches 120; 28672x4096 83 and 76; INT4 of 33 groups 62 and 69).
+    // of 8 experts 28672x4112 e4m3 96, past the caches 120; 28672x4096 83 and 76; INT4 of 33 groups 62 and 69). That an expert has
+    // several chunks, which read its matrix again, the host cannot know; then kept lines are the better choice (us, kept / past: 12
+    // pairs of one of 8 experts e4m3 28672x4096 55/62, 4096x14336 35/41; 40 of one bf16 100/116 and 71/98; 8 of one INT4 28.5/28.6 and
+    // 17.2/17.5; spread evenly e4m3 167/146 and 83/73, bf16 318/278 and 157/139, INT4 92/81 and 44.3/44.1).
     const auto go = [&](auto past) {
         hipLaunchKernelGGL((experts_stream_kernel<F, MT, WIDE, decltype(past)::value, GATED>),
                            dim3((uint32_t)(items < resident ? items : resident)), dim3(T::kWaves * kWave), 0, st, p);
@@ -948,7 +951,11 @@ int launch_tiles(ExpertsParams p, hipStream_t st)
     hipLaunchKernelGGL((experts_tile_kernel<F, BM, WIDE, SPLIT, PAST, GATED>), dim3((uint32_t)units), dim3(T::kWaves * kWave), 0, st, p);
     return (int)hipGetLastError();
 }
-// The form of a call goes by the pairs an expert has on average, all that the host knows of them. Each side of a border measured
+// The form of a call goes by the pairs an expert has on average, all that the host knows of them: it counts pairs without an expert
+// too, and a call most of whose pairs are such (experts that lie on several GPUs) takes blocks that are too large for it (us, 8 experts
+// of 32 pairs each, alone / beside seven times as many without one: e4m3 28672x4096 153/240, 4096x14336 96/190; bf16 299/441, 156/321;
+// INT4 134/290, 65/160, with zero points 143/306, 79/169; of 4 pairs each e4m3 143/146, 69/94; bf16 288/289, 145/165; INT4 89/123,
+// 51/64). Each side of a border measured, on these matrices alone
 // (us a call; e8: two of 8 experts gated 28672x4096 a token, d8: 4096x14336, e64: eight of 64, gated 2816x2048, d64: 2048x1408; the
 // pairs an expert in front):
 //   E4M3  MT 4 / 16    0.25 e8 37/42 d8 21/48 e64 17.7/17.9, 0.5 e8 56/54 d8 31/50 e64 25.7/27.1, 0.75 e64 32.6/30.0,
@@ -973,8 +980,9 @@ int launch_tiles(ExpertsParams p, hipStream_t st)
 //                      428/422), 1000 e8 2659/2287 (zp 2891/2441)
 //   rows of 512 bytes, MT 4 / 16: E4M3 1024x512 11.4/7.9; of 704: INT4 d64 14.4/9.0; of 1024: INT4 e64 above; BF16 1024x512
 //   12.4/11.8; of 1408: E4M3 d64 14.2/9.7
-// Few units (no more than the chip holds at a time): an expert's second chunk is then another block on some of the CUs, and the call
-// takes as long as those. Many units even that out.
+// Few units: three a CU or fewer by the most that these sizes can need, of which a usual call has one or two a CU, as many as
+// blocks of 64 fit. An expert's second chunk is then another block on some of the CUs, and the call takes as long as those. Many units
+// even that out.
 template <int F, bool GATED>
 int launch_format(ExpertsParams p, hipStream_t st)
 {
